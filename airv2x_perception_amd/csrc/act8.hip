@@ -1,0 +1,537 @@
+// Saved activations in 8 bits and the backward passes that read them.
+//
+//   x8 = q s,  s = max|x| / 127 per row and group of 128 channels,  q = clamp(rint(x (127 / max(max|x|, 1e-30))), -127, 127)
+//   (all three one correctly rounded fp32 operation each, so a stored byte does not depend on who computes it; a group that holds an
+//   infinity or a NaN gets s = NaN: what was lost in the forward shows in the gradients)
+//
+//   act8_pack / act8_unpack          x -> (q, s), (q, s) -> x8                                                              HBM-bound
+//   act8_layernorm                   y = (x - mean) rstd gamma + beta, (q, s) of x, (mean, rstd)   one pass over x          HBM-bound
+//   act8_layernorm_backward          u = (x8 - mean) rstd, a = g gamma: dx = rstd (a - mean(a) - u mean(a u)), dgamma, dbeta  HBM-bound
+//   act8_gelu / act8_gelu_backward   h = gelu(z) and (q, s) of z; dz = dh gelu'(z8)                                          HBM-bound
+//   act8_wgrad                       dW = dY^T X over the rows, db = sum dY, X = x8 | u gamma + beta | gelu(x8)             matrix cores / HBM
+//
+// The weight gradient is where the bytes pay twice: an integer up to 127 is exact in bf16, so the scale moves to dY's side
+// (dY s, split into three bf16 terms: exact to 2^-24) and a product costs three MFMAs where two fp32 operands cost six.
+// LayerNorm's affine leaves the sum:  dW[o, i] = gamma_i (sum (dY s rstd)[r, o] q[r, i] - sum dY[r, o] mean_r rstd_r) + beta_i db_o.
+#include <type_traits>
+
+#include "token_common.hpp"
+
+namespace {
+
+constexpr int kGroup = 128;           // channels of one scale = columns of one weight-gradient tile
+constexpr float kTiny = 1e-30f;
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ float gelu8_f(float v) { return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f)); }
+__device__ __forceinline__ float gelu8_df(float v) {
+    return 0.5f * (1.0f + erff(v * 0.70710678118654752f)) + v * 0.3989422804014327f * expf(-0.5f * v * v);
+}
+
+// the 32 lanes of a group agree on its scale and quantise their four channels each
+__device__ __forceinline__ unsigned pack4(f32x4 v, bool in, float* scale_out, int lane) {
+    float m = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+    int bad = !(m < INFINITY) || v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w;      // fmaxf skips a NaN
+    if (!in) { m = 0.f; bad = 0; }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        m = fmaxf(m, __shfl_xor(m, o));
+        bad |= __shfl_xor(bad, o);
+    }
+    const float r = 127.0f / fmaxf(m, kTiny);
+    if (scale_out && (lane & 31) == 0) *scale_out = bad ? __builtin_nanf("") : m / 127.0f;
+    auto q = [&](float x) { return (unsigned)(unsigned char)(signed char)(int)fminf(fmaxf(rintf(x * r), -127.f), 127.f); };
+    return q(v.x) | q(v.y) << 8 | q(v.z) << 16 | q(v.w) << 24;
+}
+
+__device__ __forceinline__ f32x4 unpack4(unsigned w, float s) {
+    return f32x4{(float)(signed char)(w & 0xff) * s, (float)(signed char)(w >> 8 & 0xff) * s, (float)(signed char)(w >> 16 & 0xff) * s,
+                 (float)(signed char)(w >> 24) * s};
+}
+
+// One half wave per (row, group).  MODE 0: pack.  1: out = gelu(x) too.  2: unpack.  3: out = dy gelu'(x8).
+template <int MODE>
+__global__ __launch_bounds__(256) void act8_elementwise_kernel(const float* __restrict__ x, const float* __restrict__ dy, unsigned* __restrict__ q,
+                                                               float* __restrict__ s, float* __restrict__ out, long long rows, int c) {
+    const int groups = (c + kGroup - 1) / kGroup, lane = threadIdx.x & 63, l = lane & 31;
+    const long long total = rows * groups, step = (long long)gridDim.x * 8;
+    for (long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); i < total; i += step) {      // a half wave leaves as one
+        const long long row = i / groups;
+        const int g = (int)(i - row * groups), ch = g * kGroup + l * 4;
+        const bool in = ch < c;
+        const size_t at = (size_t)row * c + ch;
+        if constexpr (MODE <= 1) {
+            f32x4 v{0.f, 0.f, 0.f, 0.f};
+            if (in) v = *reinterpret_cast<const f32x4*>(x + at);
+            const unsigned w = pack4(v, in, s + i, lane);
+            if (in) {
+                q[at / 4] = w;
+                if constexpr (MODE == 1) *reinterpret_cast<f32x4*>(out + at) = f32x4{gelu8_f(v.x), gelu8_f(v.y), gelu8_f(v.z), gelu8_f(v.w)};
+            }
+        } else if (in) {
+            f32x4 v = unpack4(q[at / 4], s[i]);
+            if constexpr (MODE == 3) {
+                const f32x4 d = *reinterpret_cast<const f32x4*>(dy + at);
+                v = f32x4{d.x * gelu8_df(v.x), d.y * gelu8_df(v.y), d.z * gelu8_df(v.z), d.w * gelu8_df(v.w)};
+            }
+            *reinterpret_cast<f32x4*>(out + at) = v;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------ LayerNorm
+// one wave per row, 256 CK channels at most; channel k * 256 + lane * 4: the two half waves of a step are two groups
+template <int CK>
+__global__ __launch_bounds__(256) void act8_layernorm_kernel(const float* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta,
+                                                             float* __restrict__ y, unsigned* __restrict__ q, float* __restrict__ s,
+                                                             f32x2* __restrict__ stats, long long rows, int c, float eps) {
+    const int lane = threadIdx.x & 63, groups = (c + kGroup - 1) / kGroup;
+    for (long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += (long long)gridDim.x * 4) {
+        f32x4 v[CK];
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < CK; ++k) {
+            const int ch = k * 256 + lane * 4;
+            v[k] = ch < c ? *reinterpret_cast<const f32x4*>(x + (size_t)row * c + ch) : f32x4{0.f, 0.f, 0.f, 0.f};
+            sum += (v[k].x + v[k].y) + (v[k].z + v[k].w);
+        }
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
+        const float mean = sum / (float)c;
+        float sq = 0.f;
+#pragma unroll
+        for (int k = 0; k < CK; ++k) {
+            if (k * 256 + lane * 4 < c) {
+                const f32x4 d = v[k] - mean;
+                sq += (d.x * d.x + d.y * d.y) + (d.z * d.z + d.w * d.w);
+            }
+        }
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) sq += __shfl_xor(sq, o);
+        const float rstd = 1.0f / sqrtf(sq / (float)c + eps);
+        if (lane == 0) stats[row] = f32x2{mean, rstd};
+#pragma unroll
+        for (int k = 0; k < CK; ++k) {
+            const int ch = k * 256 + lane * 4, g = ch / kGroup;
+            const bool in = ch < c;
+            const unsigned w = pack4(v[k], in, in ? s + row * groups + g : nullptr, lane);
+            if (in) {
+                const size_t at = (size_t)row * c + ch;
+                q[at / 4] = w;
+                *reinterpret_cast<f32x4*>(y + at) = (v[k] - mean) * rstd * *reinterpret_cast<const f32x4*>(gamma + ch) + *reinterpret_cast<const f32x4*>(beta + ch);
+            }
+        }
+    }
+}
+
+constexpr int kLnGroups = 1024;       // workgroups of the backward pass = rows of its dgamma / dbeta partials
+
+template <int CK>
+__global__ __launch_bounds__(256) void act8_layernorm_backward_kernel(const unsigned* __restrict__ q, const float* __restrict__ s,
+                                                                      const f32x2* __restrict__ stats, const float* __restrict__ gamma,
+                                                                      const float* __restrict__ dy, float* __restrict__ dx, float* __restrict__ partial,
+                                                                      long long rows, int c) {
+    __shared__ f32x4 red[2][4][64 * CK];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, groups = (c + kGroup - 1) / kGroup;
+    f32x4 gm[CK], dg[CK], db[CK];
+#pragma unroll
+    for (int k = 0; k < CK; ++k) {
+        const int ch = k * 256 + lane * 4;
+        gm[k] = ch < c ? *reinterpret_cast<const f32x4*>(gamma + ch) : f32x4{0.f, 0.f, 0.f, 0.f};
+        dg[k] = db[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (long long row = (long long)blockIdx.x * 4 + wave; row < rows; row += (long long)gridDim.x * 4) {
+        const f32x2 st = stats[row];
+        f32x4 u[CK], d[CK];
+        float sa = 0.f, sb = 0.f;
+#pragma unroll
+        for (int k = 0; k < CK; ++k) {
+            const int ch = k * 256 + lane * 4;
+            u[k] = d[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (ch < c) {
+                const size_t at = (size_t)row * c + ch;
+                u[k] = (unpack4(q[at / 4], s[row * groups + ch / kGroup]) - st.x) * st.y;
+                d[k] = *reinterpret_cast<const f32x4*>(dy + at);
+            }
+            dg[k] += d[k] * u[k];
+            db[k] += d[k];
+            d[k] *= gm[k];
+            sa += (d[k].x + d[k].y) + (d[k].z + d[k].w);
+            sb += (d[k].x * u[k].x + d[k].y * u[k].y) + (d[k].z * u[k].z + d[k].w * u[k].w);
+        }
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) { sa += __shfl_xor(sa, o); sb += __shfl_xor(sb, o); }
+        const float ma = sa / (float)c, mb = sb / (float)c;
+#pragma unroll
+        for (int k = 0; k < CK; ++k) {
+            const int ch = k * 256 + lane * 4;
+            if (ch < c) *reinterpret_cast<f32x4*>(dx + (size_t)row * c + ch) = (d[k] - ma - u[k] * mb) * st.y;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < CK; ++k) { red[0][wave][k * 64 + lane] = dg[k]; red[1][wave][k * 64 + lane] = db[k]; }
+    __syncthreads();
+    if (wave < 2) {
+#pragma unroll
+        for (int k = 0; k < CK; ++k) {
+            const int ch = k * 256 + lane * 4;
+            const f32x4 t = (red[wave][0][k * 64 + lane] + red[wave][1][k * 64 + lane]) + (red[wave][2][k * 64 + lane] + red[wave][3][k * 64 + lane]);
+            if (ch < c) *reinterpret_cast<f32x4*>(partial + ((size_t)wave * gridDim.x + blockIdx.x) * c + ch) = t;
+        }
+    }
+}
+
+// out[c] = sum over n rows of partial[which][row][c]: 32 channels x 8 rows a workgroup, a fixed order
+__global__ __launch_bounds__(256) void act8_colsum_kernel(const float* __restrict__ partial, int n, int c, float* out0, float* out1) {
+    __shared__ float red[8][33];
+    const int ch = blockIdx.x * 32 + (threadIdx.x & 31), r = threadIdx.x >> 5;
+    float t = 0.f;
+    if (ch < c)
+        for (int i = r; i < n; i += 8) t += partial[((size_t)blockIdx.y * n + i) * c + ch];
+    red[r][threadIdx.x & 31] = t;
+    __syncthreads();
+    if (r == 0 && ch < c) {
+        t = 0.f;
+        for (int i = 0; i < 8; ++i) t += red[i][threadIdx.x];
+        float* o = blockIdx.y ? out1 : out0;
+        if (o) o[ch] = t;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------ weight gradient
+// Tile 128 outputs x 128 inputs (one scale group) x 64 rows, four waves of 64 x 64; a workgroup walks its share of the rows and writes a
+// slab; act8_wgrad_reduce_kernel adds the slabs in order.  The 64 x 128 pieces of dY and q are transposed on the way to LDS: a thread
+// loads eight rows of four columns and writes, per column, the eight rows as one 16-byte fragment of an MFMA operand.  A column's eight
+// 16-byte fragments are rotated by its index (swz) so that sixteen lanes reading neighbouring columns meet all 64 banks once.
+enum { kPlain = 0, kNorm = 1, kGelu = 2 };
+constexpr int kRows = 64;
+
+__device__ __forceinline__ int swz(int col, int chunk) { return col * 64 + ((chunk ^ (col >> 1)) & 7) * 8; }      // element offset, 64 rows a column
+
+__device__ __forceinline__ void split3(const float (&v)[8], bf16x8& hi, bf16x8& mid, bf16x8& lo) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        f32x2 a{v[i], v[i + 1]};
+        const bf16x2 h = __builtin_convertvector(a, bf16x2);
+        const f32x2 hf = __builtin_convertvector(h, f32x2);
+        a.x -= hf.x; a.y -= hf.y;
+        const bf16x2 m = __builtin_convertvector(a, bf16x2);
+        const f32x2 mf = __builtin_convertvector(m, f32x2);
+        a.x -= mf.x; a.y -= mf.y;
+        const bf16x2 l = __builtin_convertvector(a, bf16x2);
+        hi[i] = h[0]; hi[i + 1] = h[1];
+        mid[i] = m[0]; mid[i + 1] = m[1];
+        lo[i] = l[0]; lo[i + 1] = l[1];
+    }
+}
+
+template <int KIND>
+__global__ __launch_bounds__(256, 2) void act8_wgrad_kernel(const float* __restrict__ dy, const unsigned* __restrict__ q, const float* __restrict__ s,
+                                                         const f32x2* __restrict__ stats, float* __restrict__ slabs, float* __restrict__ extra,
+                                                         long long rows, int co, int ci, int tiles_o, int tiles_i, long long rows_per) {
+    constexpr int XP = KIND == kGelu ? 3 : 1;                        // bf16 terms of X
+    extern __shared__ __align__(16) char smem[];
+    __bf16* la = reinterpret_cast<__bf16*>(smem);                    // [3][128][64]
+    __bf16* lb = la + 3 * 128 * 64;                                  // [XP][128][64]
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tile = blockIdx.x % (tiles_o * tiles_i), split = blockIdx.x / (tiles_o * tiles_i);
+    const int o0 = tile / tiles_i * 128, g = tile % tiles_i, i0 = g * 128, groups = tiles_i;
+    const long long r0 = split * rows_per, r1 = min(rows, r0 + rows_per);
+    const int cg = tid & 31, rc = tid >> 5;                          // four columns, eight rows
+    const int oc = o0 + cg * 4, ic = i0 + cg * 4;
+    const bool oin = oc < co, iin = ic < ci;
+    const int wo = (wave >> 1) * 64, wi = (wave & 1) * 64;
+    f32x16 acc[2][2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
+    f32x4 sum{0.f, 0.f, 0.f, 0.f}, sumu{0.f, 0.f, 0.f, 0.f};
+    f32x4 pd[8];
+    unsigned pq[8];
+    auto fetch = [&](long long r) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const long long row = r + rc * 8 + j;
+            const bool rin = row < r1;
+            pd[j] = rin && oin ? *reinterpret_cast<const f32x4*>(dy + (size_t)row * co + oc) : f32x4{0.f, 0.f, 0.f, 0.f};
+            pq[j] = rin && iin ? q[((size_t)row * ci + ic) / 4] : 0u;
+        }
+    };
+    fetch(r0);
+    for (long long r = r0; r < r1; r += kRows) {
+        float sc[8], mu[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const long long row = min(r + rc * 8 + j, r1 - 1);
+            sc[j] = s[row * groups + g];
+            mu[j] = 0.f;
+            if constexpr (KIND == kNorm) {
+                const f32x2 st = stats[row];
+                sc[j] *= st.y;
+                mu[j] = st.x * st.y;
+            }
+        }
+        if constexpr (KIND == kNorm) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sumu += pd[j] * mu[j];
+        }
+        // pairwise: the rows of one step, then the running sum
+        sum += ((pd[0] + pd[1]) + (pd[2] + pd[3])) + ((pd[4] + pd[5]) + (pd[6] + pd[7]));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float v[8], x[8];
+            bf16x8 t[3];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = KIND == kGelu ? pd[j][e] : pd[j][e] * sc[j];
+                x[j] = (float)(signed char)(pq[j] >> (8 * e) & 0xff);
+            }
+            split3(v, t[0], t[1], t[2]);
+            const int at = swz(cg * 4 + e, rc);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(la + p * 128 * 64 + at) = t[p];
+            if constexpr (KIND == kGelu) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = gelu8_f(x[j] * sc[j]);
+                split3(x, t[0], t[1], t[2]);
+#pragma unroll
+                for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(lb + p * 128 * 64 + at) = t[p];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    const bf16x2 h = __builtin_convertvector((f32x2{x[j], x[j + 1]}), bf16x2);     // |x| <= 127: exact
+                    t[0][j] = h[0]; t[0][j + 1] = h[1];
+                }
+                *reinterpret_cast<bf16x8*>(lb + at) = t[0];
+            }
+        }
+        __syncthreads();
+        if (r + kRows < r1) fetch(r + kRows);                        // in flight under the products
+#pragma unroll
+        for (int ks = 0; ks < kRows / 16; ++ks) {
+            const int chunk = ks * 2 + (lane >> 5);
+            bf16x8 A[2][3], B[2][XP];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+#pragma unroll
+                for (int p = 0; p < 3; ++p) A[m][p] = *reinterpret_cast<const bf16x8*>(la + p * 128 * 64 + swz(wo + m * 32 + (lane & 31), chunk));
+#pragma unroll
+                for (int p = 0; p < XP; ++p) B[m][p] = *reinterpret_cast<const bf16x8*>(lb + p * 128 * 64 + swz(wi + m * 32 + (lane & 31), chunk));
+            }
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    if constexpr (KIND == kGelu) {                   // smallest first
+                        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[a][2], B[b][0], acc[a][b], 0, 0, 0);
+                        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[a][0], B[b][2], acc[a][b], 0, 0, 0);
+                        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[a][1], B[b][1], acc[a][b], 0, 0, 0);
+                        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[a][1], B[b][0], acc[a][b], 0, 0, 0);
+                        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[a][0], B[b][1], acc[a][b], 0, 0, 0);
+                    } else {
+                        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[a][2], B[b][0], acc[a][b], 0, 0, 0);
+                        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[a][1], B[b][0], acc[a][b], 0, 0, 0);
+                    }
+                    acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[a][0], B[b][0], acc[a][b], 0, 0, 0);
+                }
+        }
+        __syncthreads();
+    }
+    float* slab = slabs + (size_t)split * co * ci;
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int o = o0 + wo + a * 32 + 8 * (e / 4) + 4 * (lane >> 5) + (e & 3), i = i0 + wi + b * 32 + (lane & 31);
+                if (o < co && i < ci) slab[(size_t)o * ci + i] = acc[a][b][e];
+            }
+    if (g == 0) {                                                    // sums over the rows: once per output tile
+        f32x4* red = reinterpret_cast<f32x4*>(smem);                 // [2][8][32]
+        red[rc * 32 + cg] = sum;
+        red[256 + rc * 32 + cg] = sumu;
+        __syncthreads();
+        if (tid < 64) {
+            const int which = tid >> 5;
+            f32x4 t = red[which * 256 + cg];
+            for (int j = 1; j < 8; ++j) t += red[which * 256 + j * 32 + cg];
+            if (oin) *reinterpret_cast<f32x4*>(extra + ((size_t)split * 2 + which) * co + oc) = t;
+        }
+    }
+}
+
+// dW of one output row and up to 256 inputs: four waves take every fourth slab each
+template <int KIND>
+__global__ __launch_bounds__(256) void act8_wgrad_reduce_kernel(const float* __restrict__ slabs, const float* __restrict__ extra, int splits, int co, int ci,
+                                                                const float* __restrict__ gamma, const float* __restrict__ beta, float* __restrict__ dw,
+                                                                float* __restrict__ db) {
+    __shared__ f32x4 red[4][64];
+    __shared__ float rs[2][4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, o = blockIdx.y, i = blockIdx.x * 256 + lane * 4;
+    f32x4 t{0.f, 0.f, 0.f, 0.f};
+    if (i < ci)
+        for (int sp = wave; sp < splits; sp += 4) t += *reinterpret_cast<const f32x4*>(slabs + ((size_t)sp * co + o) * ci + i);
+    red[wave][lane] = t;
+    float e0 = 0.f, e1 = 0.f;
+    for (int sp = threadIdx.x; sp < splits; sp += 256) {
+        e0 += extra[((size_t)sp * 2) * co + o];
+        e1 += extra[((size_t)sp * 2 + 1) * co + o];
+    }
+#pragma unroll
+    for (int k = 32; k >= 1; k >>= 1) { e0 += __shfl_xor(e0, k); e1 += __shfl_xor(e1, k); }
+    if (lane == 0) { rs[0][wave] = e0; rs[1][wave] = e1; }
+    __syncthreads();
+    if (wave == 0) {
+        const float d = (rs[0][0] + rs[0][1]) + (rs[0][2] + rs[0][3]), u = (rs[1][0] + rs[1][1]) + (rs[1][2] + rs[1][3]);
+        if (i < ci && dw) {
+            t = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+            if constexpr (KIND == kNorm) t = (t - u) * *reinterpret_cast<const f32x4*>(gamma + i) + *reinterpret_cast<const f32x4*>(beta + i) * d;
+            *reinterpret_cast<f32x4*>(dw + (size_t)o * ci + i) = t;
+        }
+        if (blockIdx.x == 0 && lane == 0 && db) db[o] = d;
+    }
+}
+
+int act8_check(const char* what, const void* const* ptrs, int n, int64_t rows, int32_t c, int32_t most) {
+    if (rows < 0 || rows > (1ll << 40)) return av2x::fail("%s: rows %lld", what, (long long)rows);
+    if (c < 4 || c % 4 || c > most) return av2x::fail("%s: %d channels (a multiple of 4, at most %d)", what, c, most);
+    for (int i = 0; i < n; ++i) {
+        if (!ptrs[i]) return av2x::fail("%s: null tensor", what);
+        if (!tok_aligned(ptrs[i], 16)) return av2x::fail("%s: tensors must be aligned to 16 bytes", what);
+    }
+    return 0;
+}
+
+unsigned act8_grid(int64_t half_waves) {
+    const int64_t g = (half_waves + 7) / 8;
+    return (unsigned)(g < 1 ? 1 : g > 16384 ? 16384 : g);
+}
+
+constexpr int kMaxC = 1 << 20;
+
+struct WgradPlan { int tiles_o, tiles_i, splits; int64_t rows_per; };
+WgradPlan wgrad_plan(int64_t rows, int co, int ci) {
+    WgradPlan p{(co + 127) / 128, (ci + 127) / 128, 1, kRows};
+    // two workgroups a CU; at least one step of rows each
+    int64_t want = 512 / ((int64_t)p.tiles_o * p.tiles_i);
+    const int64_t steps = (rows + kRows - 1) / kRows;
+    if (want > steps) want = steps;
+    if (want < 1) want = 1;
+    p.rows_per = (steps + want - 1) / want * kRows;
+    if (p.rows_per < kRows) p.rows_per = kRows;
+    p.splits = (int)((rows + p.rows_per - 1) / p.rows_per);
+    if (p.splits < 1) p.splits = 1;
+    return p;
+}
+
+}  // namespace
+
+extern "C" int av2x_act8_pack(const float* x, int8_t* q, float* scale, int64_t rows, int32_t c, av2x_stream_t stream) {
+    const void* p[] = {x, q, scale};
+    if (rows == 0) return 0;
+    if (int rc = act8_check("av2x_act8_pack", p, 3, rows, c, kMaxC)) return rc;
+    act8_elementwise_kernel<0><<<act8_grid(rows * ((c + 127) / 128)), 256, 0, av2x::as_stream(stream)>>>(x, nullptr, (unsigned*)q, scale, nullptr, rows, c);
+    return av2x::check_launch("av2x_act8_pack");
+}
+
+extern "C" int av2x_act8_unpack(const int8_t* q, const float* scale, float* out, int64_t rows, int32_t c, av2x_stream_t stream) {
+    const void* p[] = {q, scale, out};
+    if (rows == 0) return 0;
+    if (int rc = act8_check("av2x_act8_unpack", p, 3, rows, c, kMaxC)) return rc;
+    act8_elementwise_kernel<2><<<act8_grid(rows * ((c + 127) / 128)), 256, 0, av2x::as_stream(stream)>>>(nullptr, nullptr, (unsigned*)q, (float*)scale, out, rows, c);
+    return av2x::check_launch("av2x_act8_unpack");
+}
+
+extern "C" int av2x_act8_gelu(const float* z, float* h, int8_t* q, float* scale, int64_t rows, int32_t c, av2x_stream_t stream) {
+    const void* p[] = {z, h, q, scale};
+    if (rows == 0) return 0;
+    if (int rc = act8_check("av2x_act8_gelu", p, 4, rows, c, kMaxC)) return rc;
+    act8_elementwise_kernel<1><<<act8_grid(rows * ((c + 127) / 128)), 256, 0, av2x::as_stream(stream)>>>(z, nullptr, (unsigned*)q, scale, h, rows, c);
+    return av2x::check_launch("av2x_act8_gelu");
+}
+
+extern "C" int av2x_act8_gelu_backward(const int8_t* q, const float* scale, const float* dh, float* dz, int64_t rows, int32_t c, av2x_stream_t stream) {
+    const void* p[] = {q, scale, dh, dz};
+    if (rows == 0) return 0;
+    if (int rc = act8_check("av2x_act8_gelu_backward", p, 4, rows, c, kMaxC)) return rc;
+    act8_elementwise_kernel<3><<<act8_grid(rows * ((c + 127) / 128)), 256, 0, av2x::as_stream(stream)>>>(nullptr, dh, (unsigned*)q, (float*)scale, dz, rows, c);
+    return av2x::check_launch("av2x_act8_gelu_backward");
+}
+
+extern "C" int av2x_act8_layernorm(const float* x, const float* gamma, const float* beta, float* y, int8_t* q, float* scale, float* stats, int64_t rows,
+                                   int32_t c, float eps, av2x_stream_t stream) {
+    const void* p[] = {x, gamma, beta, y, q, scale, stats};
+    if (rows == 0) return 0;
+    if (int rc = act8_check("av2x_act8_layernorm", p, 7, rows, c, 1024)) return rc;
+    const unsigned grid = (unsigned)((rows + 3) / 4 < 8192 ? (rows + 3) / 4 : 8192);
+    auto go = [&](auto ck) {
+        act8_layernorm_kernel<decltype(ck)::value><<<grid, 256, 0, av2x::as_stream(stream)>>>(x, gamma, beta, y, (unsigned*)q, scale, (f32x2*)stats, rows, c, eps);
+    };
+    if (c <= 256) go(std::integral_constant<int, 1>{});
+    else if (c <= 512) go(std::integral_constant<int, 2>{});
+    else go(std::integral_constant<int, 4>{});
+    return av2x::check_launch("av2x_act8_layernorm");
+}
+
+extern "C" uint64_t av2x_act8_layernorm_backward_workspace_bytes(int32_t c) { return (uint64_t)2 * kLnGroups * (c > 0 ? c : 0) * 4; }
+
+extern "C" int av2x_act8_layernorm_backward(const int8_t* q, const float* scale, const float* stats, const float* gamma, const float* dy, float* dx,
+                                            float* dgamma, float* dbeta, int64_t rows, int32_t c, void* workspace, av2x_stream_t stream) {
+    const void* p[] = {gamma, workspace, q, scale, stats, dy, dx};
+    if (int rc = act8_check("av2x_act8_layernorm_backward", p, rows ? 7 : 2, rows, c, 1024)) return rc;
+    const unsigned grid = (unsigned)((rows + 3) / 4 < 1 ? 1 : (rows + 3) / 4 < kLnGroups ? (rows + 3) / 4 : kLnGroups);
+    float* partial = static_cast<float*>(workspace);
+    auto go = [&](auto ck) {
+        act8_layernorm_backward_kernel<decltype(ck)::value><<<grid, 256, 0, av2x::as_stream(stream)>>>((const unsigned*)q, scale, (const f32x2*)stats, gamma, dy, dx,
+                                                                                                  partial, rows, c);
+    };
+    if (c <= 256) go(std::integral_constant<int, 1>{});
+    else if (c <= 512) go(std::integral_constant<int, 2>{});
+    else go(std::integral_constant<int, 4>{});
+    if (int rc = av2x::check_launch("av2x_act8_layernorm_backward")) return rc;
+    if (!dgamma && !dbeta) return 0;
+    act8_colsum_kernel<<<dim3((c + 31) / 32, 2), 256, 0, av2x::as_stream(stream)>>>(partial, (int)grid, c, dgamma, dbeta);
+    return av2x::check_launch("av2x_act8_layernorm_backward: sums");
+}
+
+extern "C" uint64_t av2x_act8_wgrad_workspace_bytes(int64_t rows, int32_t cout, int32_t cin) {
+    if (rows < 0 || cout < 1 || cin < 1) return 0;
+    const WgradPlan p = wgrad_plan(rows, cout, cin);
+    return (uint64_t)p.splits * ((uint64_t)cout * cin + 2ull * cout) * 4;
+}
+
+extern "C" int av2x_act8_wgrad(const float* dy, const int8_t* q, const float* scale, const float* stats, const float* gamma, const float* beta, int32_t kind,
+                               int64_t rows, int32_t cout, int32_t cin, float* dw, float* db, void* workspace, av2x_stream_t stream) {
+    const char* what = "av2x_act8_wgrad";
+    const void* p[] = {workspace, dy, q, scale};
+    if (kind < 0 || kind > 2) return av2x::fail("%s: kind %d", what, kind);
+    if (int rc = act8_check(what, p, rows ? 4 : 1, rows, cin, 65536)) return rc;
+    if (cout < 4 || cout % 4 || cout > 65536) return av2x::fail("%s: %d outputs (a multiple of 4, at most 65536)", what, cout);
+    if (kind == kNorm && (!gamma || !beta || (rows && !stats))) return av2x::fail("%s: LayerNorm's statistics and parameters are needed", what);
+    if (!tok_aligned(gamma, 16) || !tok_aligned(beta, 16) || !tok_aligned(dw, 16) || !tok_aligned(stats, 8)) return av2x::fail("%s: tensors must be aligned to 16 bytes", what);
+    const WgradPlan pl = wgrad_plan(rows, cout, cin);
+    float* slabs = static_cast<float*>(workspace);
+    float* extra = slabs + (size_t)pl.splits * cout * cin;
+    const int64_t grid = (int64_t)pl.tiles_o * pl.tiles_i * pl.splits;
+    if (grid > 0x7fffffff) return av2x::fail("%s: too large", what);
+    auto go = [&](auto kd) {
+        constexpr int K = decltype(kd)::value;
+        constexpr size_t lds = (size_t)(3 + (K == kGelu ? 3 : 1)) * 128 * 64 * 2;
+        static av2x::LdsLimit lim;
+        lim.ensure((const void*)act8_wgrad_kernel<K>, lds);
+        act8_wgrad_kernel<K><<<(unsigned)grid, 256, lds, av2x::as_stream(stream)>>>(dy, (const unsigned*)q, scale, (const f32x2*)stats, slabs, extra, rows, cout, cin,
+                                                                             pl.tiles_o, pl.tiles_i, pl.rows_per);
+        if (int rc = av2x::check_launch(what)) return rc;
+        act8_wgrad_reduce_kernel<K><<<dim3((cin + 255) / 256, cout), 256, 0, av2x::as_stream(stream)>>>(slabs, extra, pl.splits, cout, cin, gamma, beta, dw, db);
+        return av2x::check_launch("av2x_act8_wgrad: sums");
+    };
+    if (kind == kPlain) return go(std::integral_constant<int, kPlain>{});
+    if (kind == kNorm) return go(std::integral_constant<int, kNorm>{});
+    return go(std::integral_constant<int, kGelu>{});
+}

@@ -1,0 +1,1145 @@
+// Attention over blocks of 64 keys that a cheap score selects for each query, forward and backward.
+//
+//   bounds    per block and kv head: upper / lower bound of every channel over the visible keys, as integers U, L (fp16) times one scale s_j
+//   score     sum_g sum_d (q_d > 0 ? q_d U_d : q_d L_d) s_j,  q as integers up to 127: an upper bound of q . k in the block.  Every partial
+//             sum is an integer below 2^24 (G D 127^2 with G D <= 1024): the fp16 matrix instruction adds it without rounding, so the
+//             choice is the same whoever computes it
+//   select    the n largest scores, ties to the lowest block, ascending
+//   attend    softmax over the visible keys of a query's blocks; a query with none gets zeros
+//
+// Each query has blocks of its own, so a tile of neighbouring queries shares none: read query by query, K and V would cross the L2 once per
+// (query, block).  With many queries the work is turned round: the mentions of a block are listed (a counting sort that keeps their order),
+// one workgroup holds the block's K and V in LDS and takes the queries that named it through matrix instructions, 32 per wave; every mention
+// writes its (o, max, sum) to a place of its own and a second pass joins the n places of a query.  No atomics: dK and dV of a block are summed
+// by the workgroups that hold it, in the order of its list.  With few queries one wave takes one mention and reads its block directly.
+#include <type_traits>
+
+#include "token_common.hpp"
+
+namespace {
+
+constexpr int kKeys = 64;                    // keys of a block
+constexpr int kMaxPick = 64;                 // blocks a query may have
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kTinyBs = 1e-30f;
+
+template <typename T> struct is_f32 : std::false_type {};
+template <> struct is_f32<float> : std::true_type {};
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+struct BsArgs {
+    const void *q, *k, *v;
+    const uint8_t* mask;                     // (B, Nk) visible keys, or null
+    const int32_t* blocks;                   // (B, T, KV, n)
+    long long qb, qt, qh, kb, kt, kh, vb, vt, vh;      // element strides
+    int B, T, Nk, H, KV, G, NB, n;
+    float scale;
+    // lists
+    const int32_t* list;                     // (B KV, T n) mentions t * 64 + slot of block 0, 1, ..
+    const int32_t* start;                    // (B KV, NB + 1)
+    const int32_t* items;                    // (B KV, max_items) 2 x int32: block, first row
+    const int32_t* n_items;                  // (B KV)
+    int max_items;
+    // forward
+    float* part;                             // (B, T, H, n, D)
+    f32x2* ml;                               // (B, T, H, n) maximum (scaled, base 2) and sum
+    void* out;                               // (B, T, H, D)
+    float* lse;                              // (B, T, H) base 2, +inf: no key; may be null
+    // backward
+    const void* dout;
+    const f32x2* ld;                         // (B, T, H) log-sum-exp (base 2), sum dO O
+    float* slab;                             // (B KV, max_items, 2, 64, D)
+    void *dq, *dk, *dv;
+};
+
+// ------------------------------------------------------------------------------------------------------------ bounds
+// one wave per (block, kv head): D / 4 lanes a key, 256 / D keys a step
+template <typename T, int D>
+__global__ __launch_bounds__(256) void bs_bounds_kernel(const T* __restrict__ k, const uint8_t* __restrict__ mask, long long kb, long long kt, long long kh,
+                                                        int nk, int kv, int nb, int first, int count, _Float16* __restrict__ ints, float* __restrict__ scale,
+                                                        long long total) {
+    constexpr int LPK = D / 4, KPS = 64 / LPK;
+    const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (w >= total) return;
+    const int lane = threadIdx.x & 63, sub = lane % LPK;
+    const int h = (int)(w % kv), j = first + (int)(w / kv % count), b = (int)(w / kv / count);
+    f32x4 hi{-INFINITY, -INFINITY, -INFINITY, -INFINITY}, lo{INFINITY, INFINITY, INFINITY, INFINITY};
+    int some = 0;
+#pragma unroll
+    for (int s = 0; s < kKeys / KPS; ++s) {
+        const int t = j * kKeys + s * KPS + lane / LPK;
+        if (t < nk && (!mask || mask[(size_t)b * nk + t])) {
+            const f32x4 x = tok_load4(k + b * kb + t * kt + h * kh + sub * 4);
+            some = 1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { hi[i] = fmaxf(hi[i], x[i]); lo[i] = fminf(lo[i], x[i]); }
+        }
+    }
+#pragma unroll
+    for (int o = LPK; o < 64; o <<= 1) {
+        some |= __shfl_xor(some, o);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { hi[i] = fmaxf(hi[i], __shfl_xor(hi[i], o)); lo[i] = fminf(lo[i], __shfl_xor(lo[i], o)); }
+    }
+    if (!some) hi = lo = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = fmaxf(m, fmaxf(fabsf(hi[i]), fabsf(lo[i])));
+#pragma unroll
+    for (int o = 1; o < LPK; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    const float r = 127.0f / fmaxf(m, kTinyBs);
+    if (lane < LPK) {
+        const size_t at = ((size_t)b * kv + h) * nb + j;
+        typename tok_vec<_Float16>::v4 u, l;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            u[i] = (_Float16)fminf(fmaxf(rintf(hi[i] * r), -127.f), 127.f);
+            l[i] = (_Float16)fminf(fmaxf(rintf(lo[i] * r), -127.f), 127.f);
+        }
+        *reinterpret_cast<typename tok_vec<_Float16>::v4*>(ints + at * 2 * D + sub * 4) = u;
+        *reinterpret_cast<typename tok_vec<_Float16>::v4*>(ints + at * 2 * D + D + sub * 4) = l;
+        if (lane == 0) scale[at] = some ? m / 127.0f : -1.0f;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------ selection
+constexpr int kChunk = 512;                  // scores of 16 queries in LDS
+constexpr int kScPitch = kChunk + 4;         // 4 consecutive scores per store, 16 queries: all banks
+
+__device__ __forceinline__ unsigned order_key(float s) {       // unsigned order of floats; 0 = not a candidate
+    const int b = __builtin_bit_cast(int, s + 0.0f);
+    return (unsigned)(b < 0 ? b ^ 0x7fffffff : b) ^ 0x80000000u;
+}
+
+// n largest of {key (lane) , c[0], c[1], ..} (candidates in this order, lane by lane), 0 = none, ties to the earliest.  Returns how many; the
+// chosen ones land in key / idx of lanes 0, 1, .. in order.
+template <int E>
+__device__ __forceinline__ int keep_largest(unsigned& key, int& idx, const unsigned (&c)[E], int base, int n, unsigned* lk, int* li, int lane) {
+    unsigned t = 0;
+    bool exact = false;
+    for (int bit = 31; bit >= 0; --bit) {
+        const unsigned trial = t | 1u << bit;
+        int cnt = __popcll(__ballot(key >= trial));
+#pragma unroll
+        for (int e = 0; e < E; ++e) cnt += __popcll(__ballot(c[e] >= trial));
+        if (cnt >= n) t = trial;
+        if (cnt == n) { exact = true; break; }
+    }
+    // t: the n-th largest (0: fewer than n candidates), or a bound that exactly n reach
+    int above = 0;
+    if (!exact) {
+        above = __popcll(__ballot(key > t));
+#pragma unroll
+        for (int e = 0; e < E; ++e) above += __popcll(__ballot(c[e] > t));
+    }
+    int ties = exact || t == 0 ? 0 : n - above, out = 0;
+    const unsigned long long below = (1ull << lane) - 1;
+    auto put = [&](unsigned x, int i) {
+        const unsigned long long eq = __ballot(!exact && t != 0 && x == t);
+        const bool in = exact ? x >= t : x > t || (x == t && t != 0 && __popcll(eq & below) < ties);
+        const unsigned long long m = __ballot(in);
+        if (in) { lk[out + __popcll(m & below)] = x; li[out + __popcll(m & below)] = i; }
+        ties -= min(ties, __popcll(eq));
+        out += __popcll(m);
+    };
+    put(key, idx);
+#pragma unroll
+    for (int e = 0; e < E; ++e) put(c[e], base + e * 64 + lane);
+    __builtin_amdgcn_wave_barrier();
+    key = lane < out ? lk[lane] : 0u;
+    idx = lane < out ? li[lane] : -1;
+    __builtin_amdgcn_wave_barrier();
+    return out;
+}
+
+// 16 queries x 1 kv head a workgroup: integers of the queries, scores of 512 blocks at a time on the fp16 matrix cores, the n best kept in
+// a wave's registers (four queries a wave)
+template <typename T, int D>
+__global__ __launch_bounds__(256) void bs_select_kernel(const T* __restrict__ q, long long qb, long long qt, long long qh, const _Float16* __restrict__ ints,
+                                                        const float* __restrict__ scale, int B, int T_, int G, int KV, int NB, int n, int32_t* __restrict__ out) {
+    __shared__ __align__(16) unsigned sc[16 * kScPitch];
+    __shared__ __align__(16) _Float16 qi[16][2 * D + 8];
+    __shared__ unsigned lk[4][kMaxPick];
+    __shared__ int li[4][kMaxPick];
+    constexpr int CH = D / 16, KS = 2 * D / 32;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int t0 = blockIdx.x * 16, h = blockIdx.y, b = blockIdx.z;
+    {
+        const int row = tid >> 4, l = tid & 15, t = min(t0 + row, T_ - 1);
+        const T* p = q + b * qb + t * qt + (long long)h * G * qh + l * CH;
+        float m = 0.f;
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int c = 0; c < CH; ++c) m = fmaxf(m, fabsf((float)p[g * qh + c]));
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+        const float r = 127.0f / fmaxf(m, kTinyBs);
+        float up[CH], lo[CH];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) up[c] = lo[c] = 0.f;
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const float x = fminf(fmaxf(rintf((float)p[g * qh + c] * r), -127.f), 127.f);
+                up[c] += fmaxf(x, 0.f);
+                lo[c] += fminf(x, 0.f);
+            }
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {       // at most 127 G <= 2048: exact in fp16
+            qi[row][l * CH + c] = (_Float16)up[c];
+            qi[row][D + l * CH + c] = (_Float16)lo[c];
+        }
+    }
+    __syncthreads();
+    f16x8 bf[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) bf[s] = *reinterpret_cast<const f16x8*>(&qi[lane & 15][s * 32 + (lane >> 4) * 8]);
+    const _Float16* kp = ints + ((size_t)b * KV + h) * NB * 2 * D;
+    const float* sp = scale + ((size_t)b * KV + h) * NB;
+    unsigned key[4] = {0u, 0u, 0u, 0u};
+    int idx[4] = {-1, -1, -1, -1}, have[4] = {0, 0, 0, 0};
+    for (int j0 = 0; j0 < NB; j0 += kChunk) {
+        const int tiles = (min(kChunk, NB - j0) + 15) / 16;
+        for (int tl = wave; tl < kChunk / 16; tl += 4) {
+            const int jr = j0 + tl * 16;
+            f32x4 acc{0.f, 0.f, 0.f, 0.f};
+            if (tl < tiles) {
+                const int ja = min(jr + (lane & 15), NB - 1);
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    const f16x8 a = *reinterpret_cast<const f16x8*>(kp + (size_t)ja * 2 * D + s * 32 + (lane >> 4) * 8);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bf[s], acc, 0, 0, 0);
+                }
+            }
+            unsigned k4[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = jr + (lane >> 4) * 4 + i;
+                const float s = j < NB ? sp[j] : -1.0f;
+                k4[i] = s < 0.f ? 0u : order_key(acc[i] * s);
+            }
+            *reinterpret_cast<uint4*>(&sc[(lane & 15) * kScPitch + tl * 16 + (lane >> 4) * 4]) = make_uint4(k4[0], k4[1], k4[2], k4[3]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int row = wave * 4 + u;
+            unsigned c[kChunk / 64];
+            unsigned top = 0;
+#pragma unroll
+            for (int e = 0; e < kChunk / 64; ++e) { c[e] = sc[row * kScPitch + e * 64 + lane]; top = max(top, c[e]); }
+            // later blocks enter only above the smallest one kept (ties go to the earlier block)
+            unsigned least = have[u] == n ? key[u] : 0u;
+            if (have[u] == n) {
+                least = lane < n ? key[u] : 0xffffffffu;
+#pragma unroll
+                for (int o = 32; o >= 1; o >>= 1) least = min(least, (unsigned)__shfl_xor((int)least, o));
+            }
+            if (__ballot(top > least)) have[u] = keep_largest(key[u], idx[u], c, j0, n, lk[wave], li[wave], lane);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int t = t0 + wave * 4 + u;
+        if (t < T_ && lane < n) out[(((size_t)b * T_ + t) * KV + h) * n + lane] = lane < have[u] ? idx[u] : -1;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------ lists
+// Counting sort of the mentions of a (sample, kv head) by block.  One wave takes a run of mentions in order; equal blocks among the 64 lanes
+// are found with one ballot per bit of the block number, counters live in LDS.  Same lists whatever the timing.
+template <bool FILL>
+__global__ __launch_bounds__(64) void bs_list_kernel(const int32_t* __restrict__ blocks, int T_, int KV, int NB, int n, int runs, int run_len, int bits,
+                                                     int32_t* __restrict__ hist, const int32_t* __restrict__ start, int32_t* __restrict__ list) {
+    extern __shared__ int cnt[];
+    const int lane = threadIdx.x, run = blockIdx.x, bh = blockIdx.y, b = bh / KV, h = bh % KV;
+    int32_t* hp = hist + ((size_t)bh * runs + run) * NB;
+    for (int j = lane; j < NB; j += 64) cnt[j] = FILL ? hp[j] + start[(size_t)bh * (NB + 1) + j] : 0;
+    __syncthreads();
+    const long long total = (long long)T_ * n, e0 = (long long)run * run_len, e1 = min(total, e0 + run_len);
+    for (long long e = e0; e < e1; e += 64) {
+        const bool in = e + lane < e1;
+        int j = -1, t = 0, s = 0;
+        if (in) {
+            t = (int)((e + lane) / n);
+            s = (int)((e + lane) - (long long)t * n);
+            j = blocks[(((size_t)b * T_ + t) * KV + h) * n + s];
+        }
+        const bool ok = in && j >= 0 && j < NB;
+        unsigned long long same = __ballot(ok);
+        for (int bit = 0; bit < bits; ++bit) {
+            const unsigned long long m = __ballot(ok && (j >> bit & 1));
+            same &= (j >> bit & 1) ? m : ~m;
+        }
+        const int rank = __popcll(same & ((1ull << lane) - 1));
+        const int at = ok ? cnt[j] + rank : 0;
+        __syncthreads();
+        if (ok && rank == 0) cnt[j] += __popcll(same);
+        __syncthreads();
+        if constexpr (FILL) {
+            if (ok) list[(size_t)bh * total + at] = t * kMaxPick + s;
+        }
+    }
+    if constexpr (!FILL) {
+        __syncthreads();
+        for (int j = lane; j < NB; j += 64) hp[j] = cnt[j];
+    }
+}
+
+// one workgroup per (sample, kv head): counts of the runs -> places, starts of the lists, work items of at most `rows` rows
+__global__ __launch_bounds__(1024) void bs_scan_kernel(int32_t* __restrict__ hist, int runs, int NB, int G, int rows, int max_items, int32_t* __restrict__ start,
+                                                       int32_t* __restrict__ items, int32_t* __restrict__ n_items) {
+    __shared__ int ws[2][16];
+    __shared__ int carry[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bh = blockIdx.x;
+    int32_t* hp = hist + (size_t)bh * runs * NB;
+    if (tid < 2) carry[tid] = 0;
+    __syncthreads();
+    for (int j0 = 0; j0 < NB; j0 += 1024) {
+        const int j = j0 + tid;
+        int len = 0;
+        if (j < NB)
+            for (int r = 0; r < runs; ++r) {
+                const int c = hp[(size_t)r * NB + j];
+                hp[(size_t)r * NB + j] = len;
+                len += c;
+            }
+        const int its = (int)(((long long)len * G + rows - 1) / rows);
+        int a = len, c = its;          // inclusive scans over the workgroup
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_up(a, o), y = __shfl_up(c, o);
+            if (lane >= o) { a += x; c += y; }
+        }
+        if (lane == 63) { ws[0][wave] = a; ws[1][wave] = c; }
+        __syncthreads();
+        int pa = carry[0], pc = carry[1];
+        for (int w = 0; w < wave; ++w) { pa += ws[0][w]; pc += ws[1][w]; }
+        if (j < NB) {
+            start[(size_t)bh * (NB + 1) + j] = pa + a - len;
+            for (int i = 0; i < its; ++i) {
+                int32_t* it = items + ((size_t)bh * max_items + pc + c - its + i) * 2;
+                it[0] = j;
+                it[1] = i * rows;
+            }
+        }
+        __syncthreads();
+        if (tid == 1023) { carry[0] = pa + a; carry[1] = pc + c; }
+        __syncthreads();
+    }
+    if (tid == 0) { start[(size_t)bh * (NB + 1) + NB] = carry[0]; n_items[bh] = carry[1]; }
+}
+
+// ------------------------------------------------------------------------------------------------------------ tiles
+// Operands of the 32 x 32 matrix instructions.  16-bit types: k-step of 16, a lane holds eight consecutive k of its row; fp32: k-step of 2, a lane
+// holds one.  A contraction over d walks it in the order the lanes hold it: d = 16 s + 8 half + i (16 bit), d = half D / 2 + s (fp32).
+// Accumulators (both): column lane & 31, rows 8 (i / 4) + 4 half + i % 4.  A contraction over keys or queries takes that accumulator as the B operand as
+// it lies: step s of 16 covers rows 16 s + 4 half + {0..3, 8..11}, step s of 2 (fp32) row 8 (s / 4) + 4 half + s % 4.
+template <typename T> struct Op;
+template <> struct Op<__bf16> {
+    typedef __bf16 frag __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Op<_Float16> {
+    typedef _Float16 frag __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Op<float> {
+    typedef float frag;
+    static __device__ __forceinline__ f32x16 mma(float a, float b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
+};
+
+template <typename T, int D> struct Shape {
+    static constexpr bool F = is_f32<T>::value;
+    static constexpr int KS = F ? D / 2 : D / 16;               // k-steps over d
+    static constexpr int DT = (D + 31) / 32;                    // 32-wide tiles of d
+    static constexpr int P = F ? D + 1 : D + 8;                 // row pitch of a [row][d] tile: banks
+    static constexpr int PT = F ? 0 : kKeys + 4;                // row pitch of a [d][key] tile (16-bit types only)
+    static constexpr int kOver = F && D < 32 ? 32 : 0;          // a 32-wide read of the last row stays inside
+    static constexpr int kRowTile = kKeys * P + kOver;
+    static constexpr int kTransTile = DT * 32 * PT;             // d padded to 32 with zeros
+};
+
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = 0.f;
+    return z;
+}
+
+// rows [0, 64) of a block to LDS: [key][d], and (16-bit types) [d][key].  Keys behind the end or masked are zeros.
+template <typename T, int D, bool ROW, bool TRANS>
+__device__ __forceinline__ void load_block(const T* src, long long st, int t0, int nk, unsigned long long seen, T* row, T* tr) {
+    using S = Shape<T, D>;
+    constexpr int V = 16 / sizeof(T), CPR = D / V;
+    for (int i = threadIdx.x; i < kKeys * CPR; i += blockDim.x) {
+        const int key = i & 63, c = i >> 6;
+        typedef T vec __attribute__((ext_vector_type(V)));
+        vec x;
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[e] = (T)0.f;
+        if (seen >> key & 1) x = *reinterpret_cast<const vec*>(src + (long long)(t0 + key) * st + c * V);
+        if constexpr (ROW) {
+            if constexpr (S::F) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) row[key * S::P + c * V + e] = x[e];
+            } else {
+                *reinterpret_cast<vec*>(row + key * S::P + c * V) = x;
+            }
+        }
+        if constexpr (TRANS && !S::F) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) tr[(c * V + e) * S::PT + key] = x[e];
+        }
+    }
+    if constexpr (TRANS && !S::F && D < 32) {
+        for (int i = threadIdx.x; i < (32 - D) * S::PT; i += blockDim.x) tr[D * S::PT + i] = (T)0.f;
+    }
+}
+
+template <typename T, int D> __device__ __forceinline__ typename Op<T>::frag row_frag(const T* tile, int r, int s, int half) {
+    using S = Shape<T, D>;
+    if constexpr (S::F) return tile[r * S::P + half * (D / 2) + s];
+    else return *reinterpret_cast<const typename Op<T>::frag*>(tile + r * S::P + s * 16 + half * 8);
+}
+
+// a head vector as fragments, straight from global memory
+template <typename T, int D> __device__ __forceinline__ void global_frags(const T* p, bool in, int half, typename Op<T>::frag (&f)[Shape<T, D>::KS]) {
+    if constexpr (is_f32<T>::value) {
+#pragma unroll
+        for (int s = 0; s < D / 8; ++s) {
+            f32x4 x{0.f, 0.f, 0.f, 0.f};
+            if (in) x = *reinterpret_cast<const f32x4*>(p + half * (D / 2) + s * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[s * 4 + e] = x[e];
+        }
+    } else {
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+            typename Op<T>::frag x;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = (T)0.f;
+            if (in) x = *reinterpret_cast<const typename Op<T>::frag*>(p + s * 16 + half * 8);
+            f[s] = x;
+        }
+    }
+}
+
+// 32 x 32 accumulator rows (keys or queries) as B operands, in two terms for the 16-bit types: the product then has the precision of
+// fp32 probabilities and the result's own rounding is the only one that counts
+template <typename T> struct Split {
+    typename Op<T>::frag hi[2], lo[2];
+    __device__ __forceinline__ explicit Split(const f32x16& p) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float x = p[s * 8 + e];
+                const T h = (T)x;
+                hi[s][e] = h;
+                lo[s][e] = (T)(x - (float)h);
+            }
+    }
+};
+
+// acc (d x columns) += A^T (d x 32 rows) p (32 rows x columns): A in LDS, [row][d] for fp32 (pitch P) or [d][row] for 16-bit types (pitch PT)
+template <typename T>
+__device__ __forceinline__ f32x16 mma_rows(const T* a, int pitch, int lane, const f32x16& p, f32x16 acc) {
+    const int half = lane >> 5, m = lane & 31;
+    if constexpr (is_f32<T>::value) {
+#pragma unroll
+        for (int s = 0; s < 16; ++s) acc = Op<T>::mma(a[(8 * (s / 4) + 4 * half + (s & 3)) * pitch + m], p[s], acc);
+    } else {
+        typedef T v4 __attribute__((ext_vector_type(4)));
+        const Split<T> x(p);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const v4 u = *reinterpret_cast<const v4*>(a + m * pitch + s * 16 + half * 4), w = *reinterpret_cast<const v4*>(a + m * pitch + s * 16 + half * 4 + 8);
+            typename Op<T>::frag f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { f[e] = u[e]; f[4 + e] = w[e]; }
+            acc = Op<T>::mma(f, x.lo[s], acc);
+            acc = Op<T>::mma(f, x.hi[s], acc);
+        }
+    }
+    return acc;
+}
+
+// The backward's P and dS have no largest value to be relative to, and fp16 ends at 2^-24: a tile is brought to at most 1 by a power of two before it is
+// split, and its product brought back (gradients of a scaled or a small loss keep their precision).  bf16 and fp32 have the range.
+template <typename T> struct Ranged {
+    f32x16 p;
+    float back = 1.0f;
+    __device__ __forceinline__ explicit Ranged(const f32x16& x) : p(x) {
+        if constexpr (std::is_same<T, _Float16>::value) {
+            float m = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(x[i]));
+#pragma unroll
+            for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+            const int e = m > 1e-30f && m < INFINITY ? __builtin_amdgcn_frexp_expf(m) : 0;
+            back = ldexpf(1.0f, e);
+            const float to = ldexpf(1.0f, -e);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[i] *= to;
+        }
+    }
+};
+template <typename T> __device__ __forceinline__ f32x16 mma_rows(const T* a, int pitch, int lane, const Ranged<T>& x, f32x16 acc) {
+    if constexpr (std::is_same<T, _Float16>::value) {
+        const f32x16 t = mma_rows<T>(a, pitch, lane, x.p, zero16());
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] += t[i] * x.back;
+        return acc;
+    } else {
+        return mma_rows<T>(a, pitch, lane, x.p, acc);
+    }
+}
+
+__device__ __forceinline__ unsigned long long seen_keys(const BsArgs& a, int b, int j) {       // visible keys of a block, same in every lane
+    const int t = j * kKeys + (threadIdx.x & 63);
+    return __ballot(t < a.Nk && (!a.mask || a.mask[(size_t)b * a.Nk + t]));
+}
+
+// the mention a row stands for: row = mention * G + head of the group
+struct Row { bool in; int t, slot, head; };
+__device__ __forceinline__ Row row_of(const BsArgs& a, const int32_t* list, int len, int h, int r) {
+    Row x;
+    const int e = a.G == 1 ? r : r / a.G;
+    x.in = e < len;
+    const int m = x.in ? list[e] : 0;
+    x.t = m / kMaxPick;
+    x.slot = m % kMaxPick;
+    x.head = h * a.G + (a.G == 1 ? 0 : r - e * a.G);
+    return x;
+}
+
+constexpr int kItemRows = 512;               // rows (mentions x heads of the group) of a work item
+
+// ------------------------------------------------------------------------------------------------------------ attention, many queries
+template <typename T, int D>
+__global__ __launch_bounds__(256) void bs_forward_kernel(BsArgs a) {
+    using S = Shape<T, D>;
+    __shared__ __align__(16) T lk[S::kRowTile];
+    __shared__ __align__(16) T lv[S::F ? S::kRowTile : S::kTransTile];
+    const int bh = blockIdx.y, b = bh / a.KV, h = bh % a.KV;
+    if ((int)blockIdx.x >= a.n_items[bh]) return;
+    const int32_t* it = a.items + ((size_t)bh * a.max_items + blockIdx.x) * 2;
+    const int j = it[0], first = it[1];
+    const int32_t* st = a.start + (size_t)bh * (a.NB + 1) + j;
+    const int len = st[1] - st[0];
+    const int32_t* list = a.list + (size_t)bh * a.T * a.n + st[0];
+    const unsigned long long seen = seen_keys(a, b, j);
+    load_block<T, D, true, false>(static_cast<const T*>(a.k) + b * a.kb + h * a.kh, a.kt, j * kKeys, a.Nk, seen, lk, nullptr);
+    if constexpr (S::F) load_block<T, D, true, false>(static_cast<const T*>(a.v) + b * a.vb + h * a.vh, a.vt, j * kKeys, a.Nk, seen, lv, nullptr);
+    else load_block<T, D, false, true>(static_cast<const T*>(a.v) + b * a.vb + h * a.vh, a.vt, j * kKeys, a.Nk, seen, nullptr, lv);
+    __syncthreads();
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int last = min(first + kItemRows, len * a.G);
+    const float c2 = a.scale * kLog2e;
+    for (int r0 = first + wave * 32; r0 < last; r0 += 128) {
+        const Row r = row_of(a, list, len, h, r0 + (lane & 31));
+        typename Op<T>::frag qf[S::KS];
+        global_frags<T, D>(static_cast<const T*>(a.q) + b * a.qb + r.t * a.qt + r.head * a.qh, r.in, half, qf);
+        f32x16 s[2];
+        float m = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            s[kt] = zero16();
+#pragma unroll
+            for (int ks = 0; ks < S::KS; ++ks) s[kt] = Op<T>::mma(row_frag<T, D>(lk, kt * 32 + (lane & 31), ks, half), qf[ks], s[kt]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = kt * 32 + 8 * (i / 4) + 4 * half + (i & 3);
+                s[kt][i] = seen >> key & 1 ? s[kt][i] * c2 : -INFINITY;
+                m = fmaxf(m, s[kt][i]);
+            }
+        }
+        m = fmaxf(m, __shfl_xor(m, 32));
+        const float base = m == -INFINITY ? 0.f : m;
+        float l = 0.f;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[kt][i] = exp2f(s[kt][i] - base);
+                l += s[kt][i];
+            }
+        l += __shfl_xor(l, 32);
+        const size_t at = (((size_t)b * a.T + r.t) * a.H + r.head) * a.n + r.slot;
+#pragma unroll
+        for (int dt = 0; dt < S::DT; ++dt) {
+            f32x16 o = zero16();
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                if constexpr (S::F) o = mma_rows<T>(lv + kt * 32 * S::P + dt * 32, S::P, lane, s[kt], o);
+                else o = mma_rows<T>(lv + dt * 32 * S::PT + kt * 32, S::PT, lane, s[kt], o);
+            }
+            if (r.in) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int d = dt * 32 + 8 * i + 4 * half;
+                    if (d < D) *reinterpret_cast<f32x4*>(a.part + at * D + d) = f32x4{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]};
+                }
+            }
+        }
+        if (r.in && half == 0) a.ml[at] = f32x2{m, l};
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------ attention, few queries
+// one wave per mention, all heads of its group: a lane per key for the scores, D / 8 lanes per key for the values
+template <typename T, int D>
+__global__ __launch_bounds__(64) void bs_few_kernel(BsArgs a) {
+    __shared__ float lq[D];
+    __shared__ float lp[kKeys];
+    const int lane = threadIdx.x;
+    const long long w = blockIdx.x;                      // (b, t, kv head, slot)
+    const int slot = (int)(w % a.n), h = (int)(w / a.n % a.KV);
+    const long long bt = w / a.n / a.KV;
+    const int b = (int)(bt / a.T), t = (int)(bt - (long long)b * a.T);
+    const int j = a.blocks[w];
+    if (j < 0 || j >= a.NB) return;
+    const unsigned long long seen = seen_keys(a, b, j);
+    const bool mine = seen >> lane & 1;
+    const T* kp = static_cast<const T*>(a.k) + b * a.kb + h * a.kh + (long long)(j * kKeys + (mine ? lane : 0)) * a.kt;
+    constexpr int LPK = D / 8, KPS = 64 / LPK;
+    const int sub = lane % LPK, kq = lane / LPK;
+    const T* vp = static_cast<const T*>(a.v) + b * a.vb + h * a.vh + (long long)j * kKeys * a.vt + sub * 8;
+    for (int g = 0; g < a.G; ++g) {
+        const T* qp = static_cast<const T*>(a.q) + b * a.qb + (long long)t * a.qt + (long long)(h * a.G + g) * a.qh;
+        __syncthreads();
+        for (int d = lane; d < D; d += 64) lq[d] = (float)qp[d];
+        __syncthreads();
+        float s = -INFINITY;
+        if (mine) {
+            f32x4 acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int d = 0; d < D; d += 4) acc += tok_load4(kp + d) * *reinterpret_cast<const f32x4*>(lq + d);
+            s = ((acc.x + acc.y) + (acc.z + acc.w)) * (a.scale * kLog2e);
+        }
+        float m = s;
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        const float p = exp2f(s - (m == -INFINITY ? 0.f : m));
+        float l = p;
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o);
+        lp[lane] = p;
+        __syncthreads();
+        f32x4 o0{0.f, 0.f, 0.f, 0.f}, o1 = o0;
+#pragma unroll
+        for (int i = 0; i < kKeys / KPS; ++i) {
+            const int key = i * KPS + kq;
+            if (seen >> key & 1) {
+                const float x = lp[key];
+                o0 += tok_load4(vp + (long long)key * a.vt) * x;
+                o1 += tok_load4(vp + (long long)key * a.vt + 4) * x;
+            }
+        }
+#pragma unroll
+        for (int o = LPK; o < 64; o <<= 1)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { o0[e] += __shfl_xor(o0[e], o); o1[e] += __shfl_xor(o1[e], o); }
+        const size_t at = (((size_t)b * a.T + t) * a.H + h * a.G + g) * a.n + slot;
+        if (lane < LPK) {
+            *reinterpret_cast<f32x4*>(a.part + at * D + sub * 8) = o0;
+            *reinterpret_cast<f32x4*>(a.part + at * D + sub * 8 + 4) = o1;
+        }
+        if (lane == 0) a.ml[at] = f32x2{m, l};
+    }
+}
+
+// the n places of a query joined: D / 4 lanes a (query, head)
+template <typename T, int D>
+__global__ __launch_bounds__(256) void bs_join_kernel(BsArgs a, long long rows) {
+    constexpr int L = D / 4;
+    const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / L;
+    const int sub = threadIdx.x % L;
+    if (r >= rows) return;
+    const int hq = (int)(r % a.H);
+    const long long bt = r / a.H;
+    const int32_t* bl = a.blocks + (bt * a.KV + hq / a.G) * a.n;
+    const f32x2* ml = a.ml + r * a.n;
+    float m = -INFINITY;
+    for (int s = 0; s < a.n; ++s)
+        if (bl[s] >= 0 && bl[s] < a.NB) m = fmaxf(m, ml[s].x);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    f32x4 o{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.n; ++s)
+        if (bl[s] >= 0 && bl[s] < a.NB) {
+            const float w = exp2f(ml[s].x - base);
+            l += ml[s].y * w;
+            o += *reinterpret_cast<const f32x4*>(a.part + (r * a.n + s) * D + sub * 4) * w;
+        }
+    const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : __builtin_nanf(""));
+    tok_store4(static_cast<T*>(a.out) + r * D + sub * 4, o * inv);
+    if (a.lse && sub == 0) a.lse[r] = l == 0.f ? INFINITY : m + log2f(l);
+}
+
+// ------------------------------------------------------------------------------------------------------------ backward
+// (log-sum-exp, sum dO O) of every (query, head), next to each other: a mention reads both at once
+template <typename T, int D>
+__global__ __launch_bounds__(256) void bs_delta_kernel(const T* __restrict__ out, const T* __restrict__ dout, const float* __restrict__ lse, f32x2* __restrict__ ld,
+                                                       long long rows) {
+    constexpr int L = D / 4;
+    const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / L;
+    const int sub = threadIdx.x % L;
+    if (r >= rows) return;
+    const f32x4 p = tok_load4(out + r * D + sub * 4) * tok_load4(dout + r * D + sub * 4);
+    float s = (p.x + p.y) + (p.z + p.w);
+#pragma unroll
+    for (int o = 1; o < L; o <<= 1) s += __shfl_xor(s, o);
+    if (sub == 0) ld[r] = f32x2{lse[r], s};
+}
+
+// One workgroup per work item, four waves of 32 rows.  P and dP are computed twice, as keys x queries for dQ (a lane keeps a query) and as queries x
+// keys for dK, dV (a lane keeps a key): two more products instead of a transpose through LDS.  DA: the part of d whose dK, dV, dQ this workgroup
+// keeps (blockIdx.z-th).
+template <typename T, int D, int DA>
+__global__ __launch_bounds__(256, 1) void bs_backward_kernel(BsArgs a) {
+    using S = Shape<T, D>;
+    constexpr bool F = S::F;
+    constexpr int AT = (DA + 31) / 32;                                     // d tiles of this workgroup
+    constexpr int QP = F ? DA + 1 : 32 + 4;                                // per-wave tile of 32 rows: [row][d] fp32, [d][row] 16 bit
+    constexpr int kWaveTile = F ? 32 * QP + S::kOver : AT * 32 * QP;
+    __shared__ __align__(16) T lk[S::kRowTile], lv[S::kRowTile];
+    __shared__ __align__(16) T lkt[F ? 1 : S::kTransTile];
+    __shared__ __align__(16) T lq[4][kWaveTile], lo[4][kWaveTile];
+    __shared__ __align__(16) f32x2 lld[4][32];
+    const int bh = blockIdx.y, b = bh / a.KV, h = bh % a.KV, d0 = blockIdx.z * DA;
+    if ((int)blockIdx.x >= a.n_items[bh]) return;
+    const int32_t* it = a.items + ((size_t)bh * a.max_items + blockIdx.x) * 2;
+    const int j = it[0], first = it[1];
+    const int32_t* st = a.start + (size_t)bh * (a.NB + 1) + j;
+    const int len = st[1] - st[0];
+    const int32_t* list = a.list + (size_t)bh * a.T * a.n + st[0];
+    const unsigned long long seen = seen_keys(a, b, j);
+    load_block<T, D, true, true>(static_cast<const T*>(a.k) + b * a.kb + h * a.kh, a.kt, j * kKeys, a.Nk, seen, lk, lkt);
+    load_block<T, D, true, false>(static_cast<const T*>(a.v) + b * a.vb + h * a.vh, a.vt, j * kKeys, a.Nk, seen, lv, nullptr);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    if constexpr (!F && DA < 32) {                                         // channels behind D: zeros, once
+        for (int i = lane; i < (32 - DA) * QP; i += 64) lq[wave][DA * QP + i] = lo[wave][DA * QP + i] = (T)0.f;
+    }
+    __syncthreads();
+    const int last = min(first + kItemRows, len * a.G);
+    const float c2 = a.scale * kLog2e;
+    f32x16 dk[AT][2], dv[AT][2];
+#pragma unroll
+    for (int t = 0; t < AT; ++t) { dk[t][0] = zero16(); dk[t][1] = zero16(); dv[t][0] = zero16(); dv[t][1] = zero16(); }
+    for (int r0 = first + wave * 32; r0 < last; r0 += 128) {
+        const Row r = row_of(a, list, len, h, r0 + (lane & 31));
+        const size_t qrow = ((size_t)b * a.T + r.t) * a.H + r.head;
+        typename Op<T>::frag qf[S::KS], of[S::KS];
+        global_frags<T, D>(static_cast<const T*>(a.q) + b * a.qb + r.t * a.qt + r.head * a.qh, r.in, half, qf);
+        global_frags<T, D>(static_cast<const T*>(a.dout) + qrow * D, r.in, half, of);
+        const f32x2 ld = r.in ? a.ld[qrow] : f32x2{INFINITY, 0.f};         // rows that are not there: P = 0
+        if (half == 0) lld[wave][lane & 31] = ld;
+        if constexpr (F) {
+#pragma unroll
+            for (int s = 0; s < S::KS; ++s) {
+                const int d = half * (D / 2) + s - d0;
+                if (DA == D || (d >= 0 && d < DA)) {
+                    lq[wave][(lane & 31) * QP + d] = qf[s];
+                    lo[wave][(lane & 31) * QP + d] = of[s];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < S::KS; ++s)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int d = s * 16 + half * 8 + e - d0;
+                    if (DA == D || (d >= 0 && d < DA)) {
+                        lq[wave][d * QP + (lane & 31)] = qf[s][e];
+                        lo[wave][d * QP + (lane & 31)] = of[s][e];
+                    }
+                }
+        }
+        __builtin_amdgcn_wave_barrier();
+        f32x16 dq[AT];
+#pragma unroll
+        for (int t = 0; t < AT; ++t) dq[t] = zero16();
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            f32x16 s = zero16(), p = zero16();
+            // keys x queries
+#pragma unroll
+            for (int ks = 0; ks < S::KS; ++ks) {
+                s = Op<T>::mma(row_frag<T, D>(lk, kt * 32 + (lane & 31), ks, half), qf[ks], s);
+                p = Op<T>::mma(row_frag<T, D>(lv, kt * 32 + (lane & 31), ks, half), of[ks], p);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = kt * 32 + 8 * (i / 4) + 4 * half + (i & 3);
+                const float w = seen >> key & 1 ? exp2f(s[i] * c2 - ld.x) : 0.f;
+                p[i] = w * (p[i] - ld.y) * a.scale;
+            }
+            const Ranged<T> ds(p);
+#pragma unroll
+            for (int t = 0; t < AT; ++t) {
+                if constexpr (F) dq[t] = mma_rows<T>(lk + kt * 32 * S::P + d0 + t * 32, S::P, lane, ds, dq[t]);
+                else dq[t] = mma_rows<T>(lkt + (d0 + t * 32) * S::PT + kt * 32, S::PT, lane, ds, dq[t]);
+            }
+            // queries x keys
+            s = zero16();
+            p = zero16();
+#pragma unroll
+            for (int ks = 0; ks < S::KS; ++ks) {
+                s = Op<T>::mma(qf[ks], row_frag<T, D>(lk, kt * 32 + (lane & 31), ks, half), s);
+                p = Op<T>::mma(of[ks], row_frag<T, D>(lv, kt * 32 + (lane & 31), ks, half), p);
+            }
+            const bool vis = seen >> (kt * 32 + (lane & 31)) & 1;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const f32x2 x = lld[wave][8 * (i / 4) + 4 * half + (i & 3)];
+                s[i] = vis ? exp2f(s[i] * c2 - x.x) : 0.f;
+                p[i] = s[i] * (p[i] - x.y) * a.scale;
+            }
+            const Ranged<T> rp(s), rs(p);
+#pragma unroll
+            for (int t = 0; t < AT; ++t) {
+                constexpr int step = F ? 32 : 32 * QP;
+                dv[t][kt] = mma_rows<T>(lo[wave] + t * step, QP, lane, rp, dv[t][kt]);
+                dk[t][kt] = mma_rows<T>(lq[wave] + t * step, QP, lane, rs, dk[t][kt]);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+        if (r.in) {
+            float* dst = a.part + (qrow * a.n + r.slot) * D + d0;
+#pragma unroll
+            for (int t = 0; t < AT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int d = t * 32 + 8 * i + 4 * half;
+                    if (d < DA) *reinterpret_cast<f32x4*>(dst + d) = f32x4{dq[t][4 * i], dq[t][4 * i + 1], dq[t][4 * i + 2], dq[t][4 * i + 3]};
+                }
+        }
+    }
+    // the four waves' sums, in order, through LDS: 32 keys x 32 channels at a time
+    float* red = reinterpret_cast<float*>(&lq[0][0]);
+    static_assert(sizeof(T) * 4 * kWaveTile >= 4096, "one tile of 32 x 32 sums");
+    float* slab = a.slab + ((size_t)bh * a.max_items + blockIdx.x) * 2 * kKeys * D;
+#pragma unroll
+    for (int w2 = 0; w2 < 2; ++w2)
+#pragma unroll
+        for (int t = 0; t < AT; ++t)
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                const f32x16 x = w2 ? dv[t][kt] : dk[t][kt];
+                f32x16 y = x;
+                for (int w = 1; w < 4; ++w) {
+                    __syncthreads();
+                    if (wave == w) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) red[i * 64 + lane] = x[i];
+                    }
+                    __syncthreads();
+                    if (wave == 0) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) y[i] += red[i * 64 + lane];
+                    }
+                }
+                if (wave == 0) {
+                    const int key = kt * 32 + (lane & 31);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int d = t * 32 + 8 * i + 4 * half;
+                        if (d < DA) *reinterpret_cast<f32x4*>(slab + ((size_t)w2 * kKeys + key) * D + d0 + d) = f32x4{y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]};
+                    }
+                }
+            }
+}
+
+// dK, dV of a block: the slabs of its items, in order (none: zeros).  One workgroup per (block, sample, kv head).
+template <typename T, int D>
+__global__ __launch_bounds__(256) void bs_dkv_kernel(BsArgs a) {
+    const int j = blockIdx.x, bh = blockIdx.y, b = bh / a.KV, h = bh % a.KV;
+    // items are in the order of the blocks: the first one of block j
+    const int32_t* it = a.items + (size_t)bh * a.max_items * 2;
+    const int total = a.n_items[bh];
+    int lo = 0, hi = total;
+    while (lo < hi) {
+        const int m = (lo + hi) / 2;
+        if (it[2 * m] < j) lo = m + 1;
+        else hi = m;
+    }
+    int end = lo;
+    while (end < total && it[2 * end] == j) ++end;
+    for (int i = threadIdx.x; i < 2 * kKeys * D / 4; i += 256) {
+        const int which = i / (kKeys * D / 4), key = i % (kKeys * D / 4) / (D / 4), d = i % (D / 4) * 4, t = j * kKeys + key;
+        if (t >= a.Nk) continue;
+        f32x4 x{0.f, 0.f, 0.f, 0.f};
+        for (int e = lo; e < end; ++e) x += *reinterpret_cast<const f32x4*>(a.slab + ((size_t)bh * a.max_items + e) * 2 * kKeys * D + (size_t)i * 4);
+        T* dst = static_cast<T*>(which ? a.dv : a.dk);
+        if (dst) tok_store4(dst + (((size_t)b * a.Nk + t) * a.KV + h) * D + d, x);
+    }
+}
+
+// dQ: the n places of a query added
+template <typename T, int D>
+__global__ __launch_bounds__(256) void bs_dq_kernel(BsArgs a, long long rows) {
+    constexpr int L = D / 4;
+    const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / L;
+    const int sub = threadIdx.x % L;
+    if (r >= rows) return;
+    const int hq = (int)(r % a.H);
+    const int32_t* bl = a.blocks + (r / a.H * a.KV + hq / a.G) * a.n;
+    f32x4 o{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.n; ++s)
+        if (bl[s] >= 0 && bl[s] < a.NB) o += *reinterpret_cast<const f32x4*>(a.part + (r * a.n + s) * D + sub * 4);
+    tok_store4(static_cast<T*>(a.dq) + r * D + sub * 4, o);
+}
+
+// ------------------------------------------------------------------------------------------------------------ host
+constexpr int kMaxBlocks = 32768;            // LDS counters of the list kernels: 128 KB
+
+int bs_check(const char* what, int32_t B, int32_t T, int32_t Nk, int32_t H, int32_t KV, int32_t D, int32_t n, int32_t dtype) {
+    if (D != 16 && D != 32 && D != 64 && D != 128) return av2x::fail("%s: dim %d is not 16, 32, 64 or 128", what, D);
+    if (dtype < 0 || dtype > 2) return av2x::fail("%s: dtype %d", what, dtype);
+    if (B < 1 || T < 0 || Nk < 0 || H < 1 || KV < 1 || H % KV) return av2x::fail("%s: batch %d, queries %d, keys %d, heads %d over %d", what, B, T, Nk, H, KV);
+    if (H / KV > 16 || H / KV * D > 1024) return av2x::fail("%s: %d heads of %d channels share keys (at most 16, 1024 channels)", what, H / KV, D);
+    if (n < 1 || n > kMaxPick) return av2x::fail("%s: %d blocks a query (1 .. %d)", what, n, kMaxPick);
+    if ((Nk + kKeys - 1) / kKeys > kMaxBlocks) return av2x::fail("%s: %d keys (at most %d)", what, Nk, kMaxBlocks * kKeys);
+    if (T > (1 << 25) || (int64_t)T * n > 0x7fffffff || (int64_t)T * n * (H / KV) > 0x7fffffff || B > 65535 / KV) return av2x::fail("%s: too many queries", what);
+    return 0;
+}
+
+// rows are read in pieces of 16 bytes
+int bs_rows(const char* what, const void* p, const int64_t* s, int dtype) {
+    if (!p) return av2x::fail("%s: null tensor", what);
+    const int64_t v = 16 / (int64_t)tok_size(dtype);
+    if (!tok_aligned(p, 16) || s[0] % v || s[1] % v || s[2] % v) return av2x::fail("%s: tensors and strides must be aligned to 16 bytes", what);
+    return 0;
+}
+
+int bs_runs(int64_t bh, int64_t entries) {
+    int64_t r = 2048 / bh;
+    const int64_t most = (entries + 255) / 256;
+    if (r > most) r = most;
+    return (int)(r < 1 ? 1 : r);
+}
+
+struct Lists { int32_t *hist, *start, *list, *items, *n_items; int runs, max_items; size_t bytes; };
+Lists bs_lists(void* base, int32_t B, int32_t T, int32_t Nk, int32_t H, int32_t KV, int32_t n) {
+    Lists l{};
+    const int64_t bh = (int64_t)B * KV, NB = (Nk + kKeys - 1) / kKeys, entries = (int64_t)T * n, rows = entries * (H / KV);
+    l.runs = bs_runs(bh, entries);
+    l.max_items = (int)(rows / kItemRows + NB + 1);
+    int32_t* p = static_cast<int32_t*>(base);
+    size_t at = 0;
+    auto take = [&](int64_t count) { int32_t* r = p ? p + at : nullptr; at += (size_t)((count + 3) & ~3ll); return r; };
+    l.list = take(bh * entries);
+    l.start = take(bh * (NB + 1));
+    l.items = take(bh * l.max_items * 2);
+    l.n_items = take(bh);
+    l.hist = take(bh * l.runs * NB);
+    l.bytes = at * 4;
+    return l;
+}
+
+template <typename F> int bs_go(int dtype, int dim, F&& f) {
+    auto by_dim = [&](auto t) {
+        switch (dim) {
+            case 16: return f(t, std::integral_constant<int, 16>{});
+            case 32: return f(t, std::integral_constant<int, 32>{});
+            case 64: return f(t, std::integral_constant<int, 64>{});
+            default: return f(t, std::integral_constant<int, 128>{});
+        }
+    };
+    struct F32 { using type = float; };
+    struct B16 { using type = __bf16; };
+    struct H16 { using type = _Float16; };
+    return dtype == kTokF32 ? by_dim(F32{}) : dtype == kTokBF16 ? by_dim(B16{}) : by_dim(H16{});
+}
+
+}  // namespace
+
+extern "C" int av2x_block_bounds(const void* k, const uint8_t* mask, const int64_t* strides, int32_t batch, int32_t keys, int32_t kv_heads, int32_t dim, int32_t dtype,
+                                 int32_t first_block, int32_t n_blocks, uint16_t* ints, float* scale, av2x_stream_t stream) {
+    const char* what = "av2x_block_bounds";
+    if (int rc = bs_check(what, batch, 0, keys, kv_heads, kv_heads, dim, 1, dtype)) return rc;
+    const int NB = (keys + kKeys - 1) / kKeys;
+    if (first_block < 0 || n_blocks < 0 || first_block > NB - n_blocks) return av2x::fail("%s: blocks %d .. %d of %d", what, first_block, first_block + n_blocks, NB);
+    if (n_blocks == 0) return 0;
+    if (!k || !ints || !scale) return av2x::fail("%s: null tensor", what);
+    const size_t al = 4 * tok_size(dtype);
+    if (!tok_aligned(k, al) || strides[0] % 4 || strides[1] % 4 || strides[2] % 4 || !tok_aligned(ints, 8)) return av2x::fail("%s: tensors and strides must be aligned to four elements", what);
+    const long long total = (long long)batch * n_blocks * kv_heads;
+    return bs_go(dtype, dim, [&](auto t, auto d) {
+        using T = typename decltype(t)::type;
+        bs_bounds_kernel<T, decltype(d)::value><<<(unsigned)((total + 3) / 4), 256, 0, av2x::as_stream(stream)>>>(
+            static_cast<const T*>(k), mask, strides[0], strides[1], strides[2], keys, kv_heads, NB, first_block, n_blocks, reinterpret_cast<_Float16*>(ints), scale, total);
+        return av2x::check_launch(what);
+    });
+}
+
+extern "C" int av2x_select_blocks(const void* q, const int64_t* strides, const uint16_t* ints, const float* scale, int32_t batch, int32_t queries, int32_t keys,
+                                  int32_t heads, int32_t kv_heads, int32_t dim, int32_t n, int32_t dtype, int32_t* blocks, av2x_stream_t stream) {
+    const char* what = "av2x_select_blocks";
+    if (int rc = bs_check(what, batch, queries, keys, heads, kv_heads, dim, n, dtype)) return rc;
+    if (queries == 0) return 0;
+    const int NB = (keys + kKeys - 1) / kKeys;
+    if (!q || !blocks || (NB && (!ints || !scale))) return av2x::fail("%s: null tensor", what);
+    if (!tok_aligned(ints, 16)) return av2x::fail("%s: the bounds must be aligned to 16 bytes", what);
+    return bs_go(dtype, dim, [&](auto t, auto d) {
+        using T = typename decltype(t)::type;
+        bs_select_kernel<T, decltype(d)::value><<<dim3((queries + 15) / 16, kv_heads, batch), 256, 0, av2x::as_stream(stream)>>>(
+            static_cast<const T*>(q), strides[0], strides[1], strides[2], reinterpret_cast<const _Float16*>(ints), scale, batch, queries, heads / kv_heads, kv_heads, NB, n, blocks);
+        return av2x::check_launch(what);
+    });
+}
+
+extern "C" uint64_t av2x_block_lists_bytes(int32_t batch, int32_t queries, int32_t keys, int32_t heads, int32_t kv_heads, int32_t n) {
+    if (batch < 1 || queries < 0 || keys < 0 || kv_heads < 1 || heads < 1 || n < 1) return 0;
+    return bs_lists(nullptr, batch, queries, keys, heads, kv_heads, n).bytes;
+}
+
+extern "C" int av2x_block_lists(const int32_t* blocks, int32_t batch, int32_t queries, int32_t keys, int32_t heads, int32_t kv_heads, int32_t n, void* lists,
+                                av2x_stream_t stream) {
+    const char* what = "av2x_block_lists";
+    if (int rc = bs_check(what, batch, queries, keys, heads, kv_heads, 16, n, 0)) return rc;
+    const int NB = (keys + kKeys - 1) / kKeys, bh = batch * kv_heads, G = heads / kv_heads;
+    if (queries == 0 || NB == 0) return 0;
+    if (!blocks || !lists || !tok_aligned(lists, 16)) return av2x::fail("%s: null or unaligned tensor", what);
+    const Lists l = bs_lists(lists, batch, queries, keys, heads, kv_heads, n);
+    const int64_t entries = (int64_t)queries * n;
+    const int run_len = (int)(((entries + l.runs - 1) / l.runs + 63) / 64 * 64);
+    int bits = 1;
+    while (bits < 31 && NB > 1 << bits) ++bits;
+    const size_t lds = (size_t)NB * 4;
+    hipStream_t st = av2x::as_stream(stream);
+    static av2x::LdsLimit lim0, lim1;
+    lim0.ensure((const void*)bs_list_kernel<false>, lds);
+    lim1.ensure((const void*)bs_list_kernel<true>, lds);
+    bs_list_kernel<false><<<dim3(l.runs, bh), 64, lds, st>>>(blocks, queries, kv_heads, NB, n, l.runs, run_len, bits, l.hist, nullptr, nullptr);
+    if (int rc = av2x::check_launch(what)) return rc;
+    bs_scan_kernel<<<bh, 1024, 0, st>>>(l.hist, l.runs, NB, G, kItemRows, l.max_items, l.start, l.items, l.n_items);
+    if (int rc = av2x::check_launch(what)) return rc;
+    bs_list_kernel<true><<<dim3(l.runs, bh), 64, lds, st>>>(blocks, queries, kv_heads, NB, n, l.runs, run_len, bits, l.hist, l.start, l.list);
+    return av2x::check_launch(what);
+}
+
+namespace {
+
+size_t up16(size_t x) { return (x + 15) & ~(size_t)15; }
+
+struct Work { size_t part, ml, ld, slab, bytes; };       // byte offsets
+Work bs_work(int64_t B, int64_t T, int64_t Nk, int64_t H, int64_t KV, int64_t D, int64_t n, bool backward) {
+    Work w{};
+    const size_t rows = (size_t)(B * T * H);
+    w.part = 0;
+    size_t at = up16(rows * n * D * 4);
+    if (!backward) {
+        w.ml = at;
+        at += up16(rows * n * 8);
+    } else {
+        w.ld = at;
+        at += up16(rows * 8);
+        w.slab = at;
+        at += (size_t)bs_lists(nullptr, (int32_t)B, (int32_t)T, (int32_t)Nk, (int32_t)H, (int32_t)KV, (int32_t)n).max_items * B * KV * 2 * kKeys * D * 4;
+    }
+    w.bytes = at;
+    return w;
+}
+
+BsArgs bs_args(const void* q, const void* k, const void* v, const uint8_t* mask, const int32_t* blocks, const void* lists, const int64_t* s, float scale, int32_t B,
+               int32_t T, int32_t Nk, int32_t H, int32_t KV, int32_t n) {
+    BsArgs a{};
+    a.q = q; a.k = k; a.v = v; a.mask = mask; a.blocks = blocks;
+    a.qb = s[0]; a.qt = s[1]; a.qh = s[2]; a.kb = s[3]; a.kt = s[4]; a.kh = s[5]; a.vb = s[6]; a.vt = s[7]; a.vh = s[8];
+    a.B = B; a.T = T; a.Nk = Nk; a.H = H; a.KV = KV; a.G = H / KV; a.NB = (Nk + kKeys - 1) / kKeys; a.n = n;
+    a.scale = scale;
+    if (lists) {
+        const Lists l = bs_lists(const_cast<void*>(lists), B, T, Nk, H, KV, n);
+        a.list = l.list; a.start = l.start; a.items = l.items; a.n_items = l.n_items; a.max_items = l.max_items;
+    }
+    return a;
+}
+
+}  // namespace
+
+extern "C" uint64_t av2x_block_sparse_workspace_bytes(int32_t batch, int32_t queries, int32_t keys, int32_t heads, int32_t kv_heads, int32_t dim, int32_t n, int32_t backward) {
+    if (batch < 1 || queries < 0 || keys < 0 || kv_heads < 1 || heads < 1 || n < 1 || dim < 1) return 0;
+    return bs_work(batch, queries, keys, heads, kv_heads, dim, n, backward != 0).bytes;
+}
+
+extern "C" int av2x_block_sparse_attention(const void* q, const void* k, const void* v, const int64_t* strides, const uint8_t* mask, const int32_t* blocks,
+                                           const void* lists, int32_t batch, int32_t queries, int32_t keys, int32_t heads, int32_t kv_heads, int32_t dim, int32_t n,
+                                           int32_t dtype, float scale, void* out, float* lse, void* workspace, av2x_stream_t stream) {
+    const char* what = "av2x_block_sparse_attention";
+    if (int rc = bs_check(what, batch, queries, keys, heads, kv_heads, dim, n, dtype)) return rc;
+    if (queries == 0) return 0;
+    if (!out || !blocks || !workspace || !tok_aligned(out, 16) || !tok_aligned(workspace, 16) || !tok_aligned(lists, 16)) return av2x::fail("%s: null or unaligned tensor", what);
+    if (keys > 0) {
+        if (int rc = bs_rows(what, q, strides, dtype)) return rc;
+        if (int rc = bs_rows(what, k, strides + 3, dtype)) return rc;
+        if (int rc = bs_rows(what, v, strides + 6, dtype)) return rc;
+    }
+    const long long mentions = (long long)batch * queries * kv_heads * n;
+    if (!lists && mentions > 0x7fffffff) return av2x::fail("%s: so many queries need lists", what);
+    BsArgs a = bs_args(q, k, v, mask, blocks, lists, strides, scale, batch, queries, keys, heads, kv_heads, n);
+    const Work w = bs_work(batch, queries, keys, heads, kv_heads, dim, n, false);
+    char* ws = static_cast<char*>(workspace);
+    a.part = reinterpret_cast<float*>(ws + w.part);
+    a.ml = reinterpret_cast<f32x2*>(ws + w.ml);
+    a.out = out;
+    a.lse = lse;
+    hipStream_t st = av2x::as_stream(stream);
+    return bs_go(dtype, dim, [&](auto t, auto d) {
+        using T = typename decltype(t)::type;
+        constexpr int D = decltype(d)::value;
+        if (a.NB > 0) {
+            if (lists) bs_forward_kernel<T, D><<<dim3(a.max_items, batch * kv_heads), 256, 0, st>>>(a);
+            else bs_few_kernel<T, D><<<(unsigned)mentions, 64, 0, st>>>(a);
+            if (int rc = av2x::check_launch(what)) return rc;
+        }
+        const long long rows = (long long)batch * queries * heads;
+        bs_join_kernel<T, D><<<(unsigned)((rows * (D / 4) + 255) / 256), 256, 0, st>>>(a, rows);
+        return av2x::check_launch(what);
+    });
+}
+
+extern "C" int av2x_block_sparse_attention_backward(const void* q, const void* k, const void* v, const int64_t* strides, const uint8_t* mask, const int32_t* blocks,
+                                                    const void* lists, const void* out, const float* lse, const void* dout, int32_t batch, int32_t queries, int32_t keys,
+                                                    int32_t heads, int32_t kv_heads, int32_t dim, int32_t n, int32_t dtype, float scale, void* dq, void* dk, void* dv,
+                                                    void* workspace, av2x_stream_t stream) {
+    const char* what = "av2x_block_sparse_attention_backward";
+    if (int rc = bs_check(what, batch, queries, keys, heads, kv_heads, dim, n, dtype)) return rc;
+    if (queries == 0 || keys == 0) return av2x::fail("%s: no queries or no keys", what);
+    const void* ptrs[] = {blocks, lists, out, lse, dout, workspace, dq};
+    for (const void* p : ptrs)
+        if (!p || !tok_aligned(p, 16)) return av2x::fail("%s: null or unaligned tensor", what);
+    if (!tok_aligned(dk, 16) || !tok_aligned(dv, 16)) return av2x::fail("%s: unaligned tensor", what);
+    if (int rc = bs_rows(what, q, strides, dtype)) return rc;
+    if (int rc = bs_rows(what, k, strides + 3, dtype)) return rc;
+    if (int rc = bs_rows(what, v, strides + 6, dtype)) return rc;
+    BsArgs a = bs_args(q, k, v, mask, blocks, lists, strides, scale, batch, queries, keys, heads, kv_heads, n);
+    const Work w = bs_work(batch, queries, keys, heads, kv_heads, dim, n, true);
+    char* ws = static_cast<char*>(workspace);
+    f32x2* ld = reinterpret_cast<f32x2*>(ws + w.ld);
+    a.part = reinterpret_cast<float*>(ws + w.part);
+    a.slab = reinterpret_cast<float*>(ws + w.slab);
+    a.ld = ld;
+    a.dout = dout;
+    a.dq = dq; a.dk = dk; a.dv = dv;
+    hipStream_t st = av2x::as_stream(stream);
+    return bs_go(dtype, dim, [&](auto t, auto d) {
+        using T = typename decltype(t)::type;
+        constexpr int D = decltype(d)::value, DA = D > 64 ? 64 : D;
+        const long long rows = (long long)batch * queries * heads;
+        const unsigned by_row = (unsigned)((rows * (D / 4) + 255) / 256);
+        bs_delta_kernel<T, D><<<by_row, 256, 0, st>>>(static_cast<const T*>(out), static_cast<const T*>(dout), lse, ld, rows);
+        if (int rc = av2x::check_launch(what)) return rc;
+        bs_backward_kernel<T, D, DA><<<dim3(a.max_items, batch * kv_heads, D / DA), 256, 0, st>>>(a);
+        if (int rc = av2x::check_launch(what)) return rc;
+        bs_dq_kernel<T, D><<<by_row, 256, 0, st>>>(a, rows);
+        if (int rc = av2x::check_launch(what)) return rc;
+        if (!dk && !dv) return 0;
+        bs_dkv_kernel<T, D><<<dim3(a.NB, batch * kv_heads), 256, 0, st>>>(a);
+        return av2x::check_launch(what);
+    });
+}

@@ -954,6 +954,83 @@ int av2x_roiaware_pool3d_backward(const int32_t* pts_idx_of_voxels, const int32_
 int av2x_bbox_overlaps(const float* boxes, const float* query, int32_t n, int32_t k, float* out, int32_t intersections_only);
 int av2x_box_vote(const float* dets_nms, const float* dets_all, int32_t n, int32_t m, int32_t cols, float* out);
 
+/* ------------------------------------------------------------------------------------
+ * Token operators of the transformer fusions.  dtype: 0 = fp32, 1 = bf16, 2 = fp16 (tensors; all arithmetic in fp32); strides are in
+ * elements; dim = channels of a head in {16, 32, 64, 128}.
+ *
+ * av2x_qk_norm_rotate: per head x / sqrt(mean(x^2) + eps) * gamma, then its dim / 2 pairs turned by 2 pi pos freq.
+ *   q (rows, heads, dim), k (rows, kv_heads, dim) with the last axis contiguous, strides: HOST {q row, q head, k row, k head}, multiples of 4, as the
+ *   addresses are of 4 elements; kv_heads = 0: no keys.  positions (rows, axes) i32; freqs (dim / 2) f64 in turns per unit of position, pair i of axis
+ *   i / (dim / 2 / axes); interleaved: pair i = channels (2 i, 2 i + 1), else (i, i + dim / 2).  out_q, out_k contiguous.
+ * av2x_qk_norm_rotate_backward: dq, dk (strides of row and head in dstrides, HOST, {dq, dk, dv}) and the gammas' gradients (NULL: not wanted) from
+ *   dout_q, dout_k (contiguous; NULL: zeros).  dv non-NULL: dout_v (rows, kv_heads, dim; NULL: zeros) is copied there, which completes the gradient of
+ *   a fused [q | k | v] buffer.  Bit-reproducible.  workspace: av2x_qk_norm_rotate_backward_workspace_bytes(dim).
+ * ------------------------------------------------------------------------------------ */
+int av2x_qk_norm_rotate(const void* q, const void* k, const int64_t* strides, const float* gamma_q, const float* gamma_k, const int32_t* positions,
+                        const double* freqs, void* out_q, void* out_k, int64_t rows, int32_t heads, int32_t kv_heads, int32_t dim, int32_t axes,
+                        int32_t interleaved, int32_t dtype, float eps, av2x_stream_t stream);
+uint64_t av2x_qk_norm_rotate_backward_workspace_bytes(int32_t dim);
+int av2x_qk_norm_rotate_backward(const void* q, const void* k, const int64_t* strides, const float* gamma_q, const float* gamma_k, const int32_t* positions,
+                                 const double* freqs, const void* dout_q, const void* dout_k, const void* dout_v, void* dq, void* dk, void* dv,
+                                 const int64_t* dstrides, float* dgamma_q, float* dgamma_k, int64_t rows, int32_t heads, int32_t kv_heads, int32_t dim,
+                                 int32_t axes, int32_t interleaved, int32_t dtype, float eps, void* workspace, av2x_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * Saved activations in 8 bits: q (rows, c) i8, scale (rows, ceil(c / 128)) f32;  x8 = q scale, scale = max|x| / 127 over a row's 128 channels,
+ * q = clamp(rint(x (127 / max(max|x|, 1e-30))), -127, 127).  A group with an infinity or a NaN gets scale = NaN.  c % 4 == 0, 16-byte aligned.
+ * av2x_act8_pack / unpack      x -> (q, scale); (q, scale) -> x8
+ * av2x_act8_gelu               h = gelu(z) and (q, scale) of z;  av2x_act8_gelu_backward: dz = dh gelu'(z8)
+ * av2x_act8_layernorm          y = LayerNorm(x), (q, scale) of x, stats (rows, 2) = (mean, rstd); c <= 1024
+ * av2x_act8_layernorm_backward dx, dgamma, dbeta (NULL: not wanted) of LayerNorm at x8 with the forward's statistics
+ * av2x_act8_wgrad              dw (cout, cin) = dy^T X, db (cout) = sum dy over the rows (NULL: not wanted);  X = x8 (kind 0), (x8 - mean) rstd gamma +
+ *                              beta (kind 1: stats, gamma, beta), gelu(x8) (kind 2).  Products exact to 2^-24, fp32 sums, bit-reproducible.
+ * ------------------------------------------------------------------------------------ */
+int av2x_act8_pack(const float* x, int8_t* q, float* scale, int64_t rows, int32_t c, av2x_stream_t stream);
+int av2x_act8_unpack(const int8_t* q, const float* scale, float* out, int64_t rows, int32_t c, av2x_stream_t stream);
+int av2x_act8_gelu(const float* z, float* h, int8_t* q, float* scale, int64_t rows, int32_t c, av2x_stream_t stream);
+int av2x_act8_gelu_backward(const int8_t* q, const float* scale, const float* dh, float* dz, int64_t rows, int32_t c, av2x_stream_t stream);
+int av2x_act8_layernorm(const float* x, const float* gamma, const float* beta, float* y, int8_t* q, float* scale, float* stats, int64_t rows, int32_t c,
+                        float eps, av2x_stream_t stream);
+uint64_t av2x_act8_layernorm_backward_workspace_bytes(int32_t c);
+int av2x_act8_layernorm_backward(const int8_t* q, const float* scale, const float* stats, const float* gamma, const float* dy, float* dx, float* dgamma,
+                                 float* dbeta, int64_t rows, int32_t c, void* workspace, av2x_stream_t stream);
+uint64_t av2x_act8_wgrad_workspace_bytes(int64_t rows, int32_t cout, int32_t cin);
+int av2x_act8_wgrad(const float* dy, const int8_t* q, const float* scale, const float* stats, const float* gamma, const float* beta, int32_t kind,
+                    int64_t rows, int32_t cout, int32_t cin, float* dw, float* db, void* workspace, av2x_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * Attention over blocks of 64 keys that an integer score selects for each query.
+ *   q (batch, queries, heads, dim), k, v (batch, keys, kv_heads, dim), last axis contiguous; heads / kv_heads <= 16 heads share their keys (their channels
+ *   together <= 1024).  mask (batch, keys) u8: visible keys, or NULL.  n <= 64 blocks a query, NB = ceil(keys / 64) <= 32768.
+ * av2x_block_bounds   ints (batch, kv_heads, NB, 2, dim) fp16: upper, lower bound of every channel over the visible keys of a block as whole numbers;
+ *                     scale (batch, kv_heads, NB): ints * scale is the bound; -1: no visible key.  Only blocks first_block .. + n_blocks are written.
+ *                     strides: HOST {batch, token, head} of k.
+ * av2x_select_blocks  score of a block = sum over the group's channels of max(q U, q L), q as whole numbers up to 127 (one scale a group), times the
+ *                     block's scale: exact whatever the order of summation.  blocks (batch, queries, kv_heads, n) i32: the n best, ties to the lowest
+ *                     block, ascending, -1 behind the last.  strides: HOST {batch, token, head} of q.
+ * av2x_block_lists    the mentions of every block, for the two calls below: av2x_block_lists_bytes bytes of device memory, kept by the caller
+ * av2x_block_sparse_attention   out (batch, queries, heads, dim) = softmax(scale q k^T) v over the visible keys of a query's blocks (indices outside
+ *                     0 .. NB - 1 are none; one that is named twice counts twice; no key at all: zeros), lse (batch, queries, heads) or NULL: log-sum-exp to
+ *                     base 2.  lists NULL: one wave per mention (few queries).  strides: HOST {q, k, v} x {batch, token, head}; 16-byte rows.
+ * av2x_block_sparse_attention_backward   dq (as out), dk, dv (as k, v but contiguous; NULL: not wanted).  Bit-reproducible.
+ * workspace: av2x_block_sparse_workspace_bytes.
+ * ------------------------------------------------------------------------------------ */
+int av2x_block_bounds(const void* k, const uint8_t* mask, const int64_t* strides, int32_t batch, int32_t keys, int32_t kv_heads, int32_t dim, int32_t dtype,
+                      int32_t first_block, int32_t n_blocks, uint16_t* ints, float* scale, av2x_stream_t stream);
+int av2x_select_blocks(const void* q, const int64_t* strides, const uint16_t* ints, const float* scale, int32_t batch, int32_t queries, int32_t keys,
+                       int32_t heads, int32_t kv_heads, int32_t dim, int32_t n, int32_t dtype, int32_t* blocks, av2x_stream_t stream);
+uint64_t av2x_block_lists_bytes(int32_t batch, int32_t queries, int32_t keys, int32_t heads, int32_t kv_heads, int32_t n);
+int av2x_block_lists(const int32_t* blocks, int32_t batch, int32_t queries, int32_t keys, int32_t heads, int32_t kv_heads, int32_t n, void* lists,
+                     av2x_stream_t stream);
+uint64_t av2x_block_sparse_workspace_bytes(int32_t batch, int32_t queries, int32_t keys, int32_t heads, int32_t kv_heads, int32_t dim, int32_t n, int32_t backward);
+int av2x_block_sparse_attention(const void* q, const void* k, const void* v, const int64_t* strides, const uint8_t* mask, const int32_t* blocks, const void* lists,
+                                int32_t batch, int32_t queries, int32_t keys, int32_t heads, int32_t kv_heads, int32_t dim, int32_t n, int32_t dtype, float scale,
+                                void* out, float* lse, void* workspace, av2x_stream_t stream);
+int av2x_block_sparse_attention_backward(const void* q, const void* k, const void* v, const int64_t* strides, const uint8_t* mask, const int32_t* blocks,
+                                         const void* lists, const void* out, const float* lse, const void* dout, int32_t batch, int32_t queries, int32_t keys,
+                                         int32_t heads, int32_t kv_heads, int32_t dim, int32_t n, int32_t dtype, float scale, void* dq, void* dk, void* dv,
+                                         void* workspace, av2x_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

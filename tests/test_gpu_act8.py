@@ -1,0 +1,238 @@
+"""GPU: token layers with 8-bit saved activations (csrc/act8.hip, opencood_iface/act8_ops.py) against 64-bit formulas.
+
+The stored bytes are exact by definition (one correctly rounded fp32 operation each).  Everything else is fp32 arithmetic: a sum of N products is off by at
+most N 2^-24 of the sum of their sizes; with partial sums of blocks sqrt-like, 40 x 2^-24 of the sum of sizes covers every length used here (chains of at
+most 16 per matrix instruction step, the accumulation of up to 35 steps and of the slabs after it), plus the operands' own errors of a few steps.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def held(x):
+    """The definition, on the CPU in fp32."""
+    c = x.shape[-1]
+    f = torch.nn.functional.pad(x.reshape(-1, c), (0, -c % 128)).view(-1, (c + 127) // 128, 128)
+    big = f.abs().amax(-1)
+    m = torch.full_like(big, 127.0)
+    q = (f * (m / big.clamp_min(1e-30))[..., None]).round().clamp(-127, 127)
+    return q.flatten(1)[:, :c].to(torch.int8).view(x.shape), big / m
+
+
+def data(seed, rows, ci, co, lead=None):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, ci, generator=g) * torch.randn(rows, 1, generator=g).mul(0.4).exp() + 0.3 * torch.randn(1, ci, generator=g)
+    w, b = torch.randn(co, ci, generator=g) / math.sqrt(ci), 0.1 * torch.randn(co, generator=g)
+    res, dy = torch.randn(rows, co, generator=g), torch.randn(rows, co, generator=g)
+    return x, w, b, res, dy, 1 + 0.1 * torch.randn(ci, generator=g), 0.1 * torch.randn(ci, generator=g)
+
+
+def near(got, want, bound, what):
+    got, want, bound = got.detach().double().cpu(), want.detach().double(), bound.double()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    r = ((got - want).abs() / bound.clamp_min(1e-300)).max() if got.numel() else 0.0
+    assert float(r) <= 1.0, f"{what}: {float(r):.2f} x the bound"
+
+
+@pytest.mark.parametrize("shape", [(1, 4), (3, 128), (37, 132), (5, 7, 260), (1000, 256), (2, 3, 4, 1024), (0, 64)])
+def test_stored_bytes_are_the_definition(shape):
+    from airv2x_perception_amd.opencood_iface import act8_ops as A
+    x = torch.randn(*shape, generator=torch.Generator().manual_seed(sum(shape)))
+    if x.numel() > 64:
+        x.view(-1, shape[-1])[0] = 0                                  # a row of zeros
+        x.view(-1, shape[-1])[-1] *= 1e-38                             # below the smallest scale
+    p = A.pack(x.cuda())
+    q, s = held(x)
+    assert torch.equal(p.q.cpu(), q) and torch.equal(p.scale.cpu(), s)
+    full = s.repeat_interleave(128, 1)[:, :shape[-1]].view(x.shape)
+    assert torch.equal(A.unpack(p).cpu(), q.float() * full)
+
+
+def test_groups_with_infinities_and_nans_are_marked():
+    from airv2x_perception_amd.opencood_iface import act8_ops as A
+    x = torch.randn(6, 256)
+    x[1, 3], x[2, 200], x[3, 5], x[4] = float("inf"), float("nan"), -float("inf"), float("nan")
+    s = A.pack(x.cuda()).scale.cpu()
+    bad = torch.tensor([[0, 0], [1, 0], [0, 1], [1, 0], [1, 1], [0, 0]], dtype=torch.bool)
+    assert torch.equal(s.isnan(), bad) and torch.equal(s[~bad], held(x)[1][~bad])
+
+
+@pytest.mark.parametrize("rows,ci,co", [(1, 64, 32), (63, 256, 256), (65, 96, 100), (2200, 256, 256), (777, 320, 68), (129, 512, 4), (1500, 36, 132)])
+@pytest.mark.parametrize("kind", ["linear", "norm_linear", "gelu_linear"])
+def test_forward_and_gradients(kind, rows, ci, co):
+    from airv2x_perception_amd.opencood_iface import act8_ops as A
+    x, w, b, res, dy, gamma, beta = data(rows + ci, rows, ci, co)
+    q, s = held(x)
+    x8 = (q.double() * s.double().repeat_interleave(128, 1)[:, :ci])
+    D = lambda t: t.double()
+    src = D(dy) @ D(w)
+    srcb = (D(dy).abs() @ D(w).abs()) * 40 * U                        # bound of dY W
+    leaves = [t.cuda().requires_grad_() for t in (x, w, b)]
+    if ci % 32 or co % 32:                                            # the GEMM's limit: refused; the weight gradient itself takes any multiple of 4
+        with pytest.raises(ValueError, match="multiples of 32"):
+            A.norm_linear(leaves[0], gamma.cuda(), beta.cuda(), leaves[1]) if kind == "norm_linear" else (A.linear if kind == "linear" else A.gelu_linear)(*leaves)
+        from airv2x_perception_amd.opencood_iface.autograd import _runner
+        mean, sd = x.mean(1, keepdim=True), (x.var(1, unbiased=False, keepdim=True) + 1e-5).sqrt()
+        stats = torch.cat([mean, 1 / sd], 1)
+        mean, rs = D(stats[:, :1]), D(stats[:, 1:])
+        X = x8 if kind == "linear" else (x8 - mean) * rs * D(gamma) + D(beta) if kind == "norm_linear" else 0.5 * x8 * (1 + torch.erf(x8 / math.sqrt(2)))
+        size = X.abs() + (x8.abs() * 4 if kind == "gelu_linear" else 0) + ((x8.abs() + mean.abs()) * rs * D(gamma).abs() + D(beta).abs() if kind == "norm_linear" else 0)
+        p = A.pack(x.cuda())
+        dw, db = A._wgrad(_runner(dy.cuda().device), ["linear", "norm_linear", "gelu_linear"].index(kind), dy.cuda(), *p, ci, stats.cuda(), gamma.cuda(), beta.cuda())
+        near(dw, D(dy).t() @ X, D(dy).abs().t() @ size * 60 * U + 1e-12, "dW")
+        near(db, D(dy).sum(0), D(dy).abs().sum(0) * 40 * U + 1e-12, "db")
+        return
+    if kind == "norm_linear":
+        extra = [t.cuda().requires_grad_() for t in (gamma, beta)]
+        y = A.norm_linear(leaves[0], *extra, leaves[1], leaves[2])
+        mean = D(x).mean(1, keepdim=True)
+        sd = (D(x).var(1, unbiased=False, keepdim=True) + 1e-5).sqrt()
+        n = (D(x) - mean) / sd
+        fed, want = n * D(gamma) + D(beta), None
+        yb = ((n.abs() + (mean / sd).abs() + 1) * D(gamma).abs() + D(beta).abs()) @ D(w).abs().t() * 60 * U
+        u = (x8 - mean) / sd
+        ub = (u.abs() + (mean / sd).abs() * 2 + 1) * 24 * U           # mean, rstd: a tree over 64 lanes; the difference x8 - mean
+        X, Xb = u * D(gamma) + D(beta), ub * D(gamma).abs()
+    else:
+        extra = [res.cuda().requires_grad_()]
+        y = (A.linear if kind == "linear" else A.gelu_linear)(leaves[0], leaves[1], leaves[2], extra[0])
+        gl = lambda z: 0.5 * z * (1 + torch.erf(z / math.sqrt(2)))
+        fed = D(x) if kind == "linear" else gl(D(x))
+        yb = (fed.abs() + (0 if kind == "linear" else D(x).abs() * 4 * U)) @ D(w).abs().t() * 40 * U + D(res).abs() * 4 * U + 1e-9
+        X = x8 if kind == "linear" else gl(x8)
+        Xb = X.abs() * 0 + (0 if kind == "linear" else 1) * x8.abs() * 6 * U
+    yw = fed @ D(w).t() + D(b) + (0 if kind == "norm_linear" else D(res))
+    near(y, yw, yb + D(b).abs() * 4 * U + 1e-7, "y")
+    grads = torch.autograd.grad(y, leaves + extra, dy.cuda())
+    # LayerNorm's affine leaves the sum: its terms carry |mean| rstd as well
+    size = X.abs() if kind != "norm_linear" else (u.abs() + 2 * (mean / sd).abs()) * D(gamma).abs() + D(beta).abs()
+    near(grads[1], D(dy).t() @ X, D(dy).abs().t() @ (size * 60 * U + Xb) + 1e-12, "dW")
+    near(grads[2], D(dy).sum(0), D(dy).abs().sum(0) * 40 * U + 1e-12, "db")
+    if kind == "linear":
+        near(grads[0], src, srcb + 1e-12, "dx")
+    elif kind == "gelu_linear":
+        slope = 0.5 * (1 + torch.erf(x8 / math.sqrt(2))) + x8 * torch.exp(-x8 * x8 / 2) / math.sqrt(2 * math.pi)
+        near(grads[0], src * slope, srcb * slope.abs() + src.abs() * (1 + x8.abs() + x8 ** 2) * 8 * U + 1e-12, "dz")
+    else:
+        a = src * D(gamma)
+        ab = srcb * D(gamma).abs() + a.abs() * 2 * U
+        m1, m2 = a.mean(1, keepdim=True), (a * u).mean(1, keepdim=True)
+        dx = (a - m1 - u * m2) / sd
+        b1 = ab.mean(1, keepdim=True) + a.abs().mean(1, keepdim=True) * 16 * U
+        b2 = (ab * u.abs() + a.abs() * ub).mean(1, keepdim=True) + (a * u).abs().mean(1, keepdim=True) * 16 * U
+        near(grads[0], dx, (ab + b1 + u.abs() * b2 + ub * m2.abs()) / sd + (a.abs() + m1.abs() + (u * m2).abs()) / sd * 24 * U + 1e-12, "dx")
+        near(grads[3], (src * u).sum(0), (srcb * u.abs() + src.abs() * ub).sum(0) + (src * u).abs().sum(0) * 40 * U + 1e-12, "dgamma")
+        near(grads[4], src.sum(0), srcb.sum(0) + src.abs().sum(0) * 40 * U + 1e-12, "dbeta")
+    if kind != "norm_linear":
+        assert torch.equal(grads[3].cpu(), dy)
+    # the same call again: the same bits
+    again = torch.autograd.grad((A.norm_linear(leaves[0], *extra, leaves[1], leaves[2]) if kind == "norm_linear" else
+                                 (A.linear if kind == "linear" else A.gelu_linear)(leaves[0], leaves[1], leaves[2], extra[0])), leaves + extra, dy.cuda())
+    assert all(torch.equal(p, r) for p, r in zip(grads, again))
+
+
+def test_gelu_node_shapes_and_no_rows():
+    from airv2x_perception_amd.opencood_iface import act8_ops as A
+    z = torch.randn(3, 5, 132, generator=torch.Generator().manual_seed(4))
+    zd = z.cuda().requires_grad_()
+    h = A.gelu(zd)
+    near(h, torch.nn.functional.gelu(z.double()), z.double().abs() * 6 * U + 1e-9, "gelu")
+    q, s = held(z)
+    z8 = (q.double().view(15, 132) * s.double().repeat_interleave(128, 1)[:, :132]).view(z.shape)
+    dh = torch.randn(3, 5, 132)
+    (dz,) = torch.autograd.grad(h, zd, dh.cuda())
+    slope = 0.5 * (1 + torch.erf(z8 / math.sqrt(2))) + z8 * torch.exp(-z8 * z8 / 2) / math.sqrt(2 * math.pi)
+    near(dz, dh.double() * slope, dh.double().abs() * (1 + z8.abs()) * 8 * U, "dz")
+    w, b, gamma, beta = [t.cuda().requires_grad_() for t in (torch.randn(32, 64), torch.randn(32), torch.randn(64), torch.randn(64))]
+    e = torch.zeros(0, 64, device="cuda", requires_grad=True)
+    for y, leaves in ((A.linear(e, w, b), [e, w, b]), (A.norm_linear(e, gamma, beta, w, b), [e, gamma, beta, w, b]), (A.gelu_linear(e, w, b), [e, w, b])):
+        assert y.shape == (0, 32)
+        for t, gr in zip(leaves, torch.autograd.grad(y.sum(), leaves)):
+            assert gr.shape == t.shape and not gr.any()
+
+
+def test_frozen_parts_views_and_nan():
+    from airv2x_perception_amd.opencood_iface import act8_ops as A
+    x, w, b, res, dy, gamma, beta = [t.cuda() for t in data(9, 70, 64, 64)]
+    full = torch.autograd.grad(A.linear(x.requires_grad_(), w.requires_grad_(), b.requires_grad_()), [x, w, b], dy)
+    x, w, b = x.detach(), w.detach(), b.detach()
+    xr = x.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(A.linear(xr, w, b), xr, dy)[0], full[0])               # frozen weight: nothing kept
+    wr = w.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(A.linear(x, wr, b), wr, dy)[0], full[1])
+    br = b.clone().requires_grad_()
+    # the frozen weight's bias gradient comes from another summation order: both within 40 steps of the sum of sizes
+    near(torch.autograd.grad(A.linear(x, w, br), br, dy)[0], full[2].double().cpu(), dy.double().abs().sum(0).cpu() * 40 * U, "db")
+    # transposed storage and an address that is not a multiple of 16
+    xt = x.t().contiguous().t()
+    off = torch.empty(x.numel() + 1, device="cuda")[1:].view(x.shape)
+    off.copy_(x)
+    y = A.linear(x, w, b)
+    assert torch.equal(A.linear(xt, w, b), y) and torch.equal(A.linear(off, w, b), y)
+    assert torch.equal(A.linear(x, w.t().contiguous().t(), b), y)
+    with torch.no_grad():
+        assert torch.equal(A.norm_linear(x, gamma, beta, w, b), A.norm_linear(x, gamma, beta, w.clone().requires_grad_(), b))
+    # what the forward lost shows in the weight gradient
+    bad = x.clone()
+    bad[5, 7] = float("inf")
+    assert torch.autograd.grad(A.linear(bad, wr, b), wr, dy)[0].isnan().any()
+    with pytest.raises(RuntimeError):
+        g1 = torch.autograd.grad(A.linear(xr, wr, b).sum(), xr, create_graph=True)[0]
+        g1.sum().backward()
+
+
+@pytest.mark.parametrize("name", ["norm_linear", "gelu_linear"])
+def test_gradients_against_differences(name):
+    """The 8-bit copy is a constant of the backward, so the derivative taken at x8 must be that of the layer evaluated AT x8 (a point whose own 8-bit copy is
+    itself: whole numbers with a largest one of 127 times a power of two)."""
+    from airv2x_perception_amd.opencood_iface import act8_ops as A
+    g = torch.Generator().manual_seed(6)
+    x = torch.randint(-127, 128, (40, 128), generator=g).float()
+    x[:, 3] = 127
+    x = (x / 64).cuda()
+    assert torch.equal(A.unpack(A.pack(x)), x)
+    w, b, wy = (torch.randn(64, 128, generator=g) / 11).cuda(), torch.randn(64, generator=g).cuda(), torch.randn(40, 64, generator=g).cuda()
+    gamma, beta = (1 + 0.1 * torch.randn(128, generator=g)).cuda(), torch.randn(128, generator=g).cuda()
+    f = lambda x, w: ((A.norm_linear(x, gamma, beta, w, b) if name == "norm_linear" else A.gelu_linear(x, w, b)).double() * wy).sum()
+    xr, wr = x.clone().requires_grad_(), w.clone().requires_grad_()
+    gx, gw = torch.autograd.grad(f(xr, wr), [xr, wr])
+    sx, sw = torch.randn(40, 128, generator=g).cuda(), torch.randn(64, 128, generator=g).cuda() / 11
+    e = 2.0 ** -9
+    for grad, step, dx, dw in ((gx, sx, 1, 0), (gw, sw, 0, 1)):
+        diff = float(f(x + e * dx * sx, w + e * dw * sw) - f(x - e * dx * sx, w - e * dw * sw)) / (2 * e)
+        ana = float((grad.double() * step).sum())
+        size = float((grad.double().abs() * step.abs()).sum())
+        assert abs(diff - ana) <= size * 1e-4                         # e^2 times third derivatives of order one; fp32 noise 1e-7 / e
+
+
+def test_graph_replay_of_a_training_step():
+    from airv2x_perception_amd.opencood_iface import act8_ops as A
+    x, w, b, res, dy, gamma, beta = [t.cuda() for t in data(19, 300, 256, 256)]
+    buf = x.clone().requires_grad_()
+    w2 = (torch.randn(256, 256, device="cuda") / 16).requires_grad_()
+    w = w.requires_grad_()
+
+    def step():
+        z = A.norm_linear(buf, gamma, beta, w, b)
+        y = A.gelu_linear(z, w2, b, buf)
+        return torch.autograd.grad(y, [buf, w, w2], dy)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        with torch.no_grad():
+            buf.copy_(x * (1 + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        a = [t.clone() for t in got]
+        assert all(torch.equal(p, q) for p, q in zip(a, step()))
