@@ -257,8 +257,9 @@ SIGNATURES = {
                                   c_void_p, c_void_p]),
     "av2x_block_bounds": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p,
                                     c_void_p]),
+    "av2x_select_blocks_workspace_bytes": (c_uint64, [c_int32, c_int32, c_int32, c_int32, c_int32]),
     "av2x_select_blocks": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32,
-                                     c_void_p, c_void_p]),
+                                     c_void_p, c_void_p, c_void_p]),
     "av2x_block_lists_bytes": (c_uint64, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
     "av2x_block_lists": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p]),
     "av2x_block_sparse_workspace_bytes": (c_uint64, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),

@@ -112,10 +112,10 @@ __device__ __forceinline__ unsigned order_key(float s) {       // unsigned order
     return (unsigned)(b < 0 ? b ^ 0x7fffffff : b) ^ 0x80000000u;
 }
 
-// n largest of {key (lane) , c[0], c[1], ..} (candidates in this order, lane by lane), 0 = none, ties to the earliest.  Returns how many; the
-// chosen ones land in key / idx of lanes 0, 1, .. in order.
-template <int E>
-__device__ __forceinline__ int keep_largest(unsigned& key, int& idx, const unsigned (&c)[E], int base, int n, unsigned* lk, int* li, int lane) {
+// n largest of {key (lane), c[0], c[1], ..} (candidates in this order, lane by lane), 0 = none, ties to the earliest.  Returns how many; the
+// chosen ones land in key / idx of lanes 0, 1, .. in order.  Any number of ties: the n-th largest value is found bit by bit.
+template <int E, typename Idx>
+__device__ __forceinline__ int keep_largest(unsigned& key, int& idx, const unsigned (&c)[E], Idx&& index, int n, unsigned* lk, int* li, int lane) {
     unsigned t = 0;
     bool exact = false;
     for (int bit = 31; bit >= 0; --bit) {
@@ -145,7 +145,7 @@ __device__ __forceinline__ int keep_largest(unsigned& key, int& idx, const unsig
     };
     put(key, idx);
 #pragma unroll
-    for (int e = 0; e < E; ++e) put(c[e], base + e * 64 + lane);
+    for (int e = 0; e < E; ++e) put(c[e], index(e));
     __builtin_amdgcn_wave_barrier();
     key = lane < out ? lk[lane] : 0u;
     idx = lane < out ? li[lane] : -1;
@@ -153,18 +153,108 @@ __device__ __forceinline__ int keep_largest(unsigned& key, int& idx, const unsig
     return out;
 }
 
-// 16 queries x 1 kv head a workgroup: integers of the queries, scores of 512 blocks at a time on the fp16 matrix cores, the n best kept in
-// a wave's registers (four queries a wave)
-template <typename T, int D>
+// The same for a few newcomers: candidates above `least` join the kept ones in LDS (at most 64 together), every one counts how many are better, and the
+// n best stay, in order.  Returns false where they are too many (the caller goes bit by bit).
+template <int E, typename Idx>
+__device__ __forceinline__ bool merge_few(unsigned& key, int& idx, int& have, unsigned& least, const unsigned (&c)[E], Idx&& index, int n, unsigned* lk, int* li, int lane) {
+    unsigned long long m[E];
+    int total = have;
+#pragma unroll
+    for (int e = 0; e < E; ++e) { m[e] = __ballot(c[e] > least); total += __popcll(m[e]); }
+    if (total == have) return true;
+    if (total > 64) return false;
+    int at = have;
+    if (lane < have) { lk[lane] = key; li[lane] = idx; }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        if (m[e]) {
+            const int p = at + __builtin_amdgcn_mbcnt_hi((unsigned)(m[e] >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)m[e], 0));
+            if (c[e] > least) { lk[p] = c[e]; li[p] = index(e); }
+            at += __popcll(m[e]);
+        }
+    }
+    __builtin_amdgcn_wave_barrier();
+    unsigned k = lane < total ? lk[lane] : 0u;
+    int x = lane < total ? li[lane] : -1;
+    if (total > n) {
+        int rank = 0;           // how many are better: larger, or equal and earlier
+        for (int i = 0; i < total; ++i) {
+            const unsigned o = __builtin_amdgcn_readlane(k, i);
+            rank += o > k || (o == k && i < lane) ? 1 : 0;
+        }
+        const unsigned long long in = __ballot(lane < total && rank < n), last = __ballot(lane < total && rank == n - 1);
+        least = __builtin_amdgcn_readlane(k, __ffsll(last) - 1);
+        __builtin_amdgcn_wave_barrier();
+        if (lane < total && rank < n) {
+            const int p = __builtin_amdgcn_mbcnt_hi((unsigned)(in >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)in, 0));
+            lk[p] = k;
+            li[p] = x;
+        }
+        __builtin_amdgcn_wave_barrier();
+        total = n;
+        k = lane < n ? lk[lane] : 0u;
+        x = lane < n ? li[lane] : -1;
+    } else if (total == n) {
+        least = lane < n ? k : 0xffffffffu;
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) least = min(least, (unsigned)__shfl_xor((int)least, o));
+    }
+    __builtin_amdgcn_wave_barrier();
+    key = k;
+    idx = x;
+    have = total;
+    return true;
+}
+
+// the kept n and E x 64 newcomers; least: the smallest kept one once n are kept
+template <int E, typename Idx>
+__device__ __forceinline__ void take(unsigned& key, int& idx, int& have, unsigned& least, const unsigned (&c)[E], Idx&& index, int n, unsigned* lk, int* li, int lane) {
+    if (have < n) {
+        // nothing to compare with yet: the n-th largest of the group maxima is a bound that at least n candidates reach, and few more
+        unsigned g = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) g = max(g, c[e]);
+        const int step = n <= 16 ? 4 : 1;
+        if (n <= 16) {
+            g = max(g, (unsigned)__shfl_xor((int)g, 1));
+            g = max(g, (unsigned)__shfl_xor((int)g, 2));
+        }
+        int rank = 0;
+        for (int i = 0; i < 64; i += step) {
+            const unsigned o = __builtin_amdgcn_readlane(g, i);
+            rank += o > g || (o == g && i < lane) ? 1 : 0;
+        }
+        const unsigned long long at = __ballot(rank == n - 1 && lane % step == 0);
+        const unsigned t = at ? __builtin_amdgcn_readlane(g, __ffsll(at) - 1) : 0u;
+        least = have == 0 && t > 0 ? t - 1 : 0u;
+    }
+    if (!merge_few(key, idx, have, least, c, index, n, lk, li, lane)) {
+        have = keep_largest(key, idx, c, index, n, lk, li, lane);
+        least = 0u;
+        if (have == n) {
+            least = lane < n ? key : 0xffffffffu;
+#pragma unroll
+            for (int o = 32; o >= 1; o >>= 1) least = min(least, (unsigned)__shfl_xor((int)least, o));
+        }
+    } else if (have < n) {
+        least = 0u;
+    }
+}
+
+// 16 queries x 1 kv head x a range of blocks a workgroup: integers of the queries, scores of 512 blocks at a time on the fp16 matrix cores, the n best kept in
+// a wave's registers (four queries a wave).  PARTS: the range is one of several, its n best go to `part` as (key, block) pairs.
+template <typename T, int D, bool PARTS>
 __global__ __launch_bounds__(256) void bs_select_kernel(const T* __restrict__ q, long long qb, long long qt, long long qh, const _Float16* __restrict__ ints,
-                                                        const float* __restrict__ scale, int B, int T_, int G, int KV, int NB, int n, int32_t* __restrict__ out) {
+                                                        const float* __restrict__ scale, int T_, int G, int KV, int NB, int n, int parts, int per, int32_t* __restrict__ out,
+                                                        uint2* __restrict__ part) {
     __shared__ __align__(16) unsigned sc[16 * kScPitch];
     __shared__ __align__(16) _Float16 qi[16][2 * D + 8];
-    __shared__ unsigned lk[4][kMaxPick];
-    __shared__ int li[4][kMaxPick];
+    __shared__ unsigned lk[4][64];
+    __shared__ int li[4][64];
     constexpr int CH = D / 16, KS = 2 * D / 32;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int t0 = blockIdx.x * 16, h = blockIdx.y, b = blockIdx.z;
+    const int t0 = (PARTS ? blockIdx.x / parts : blockIdx.x) * 16, h = blockIdx.y, b = blockIdx.z;
+    const int first = PARTS ? (blockIdx.x % parts) * per : 0, last = PARTS ? min(NB, first + per) : NB;
     {
         const int row = tid >> 4, l = tid & 15, t = min(t0 + row, T_ - 1);
         const T* p = q + b * qb + t * qt + (long long)h * G * qh + l * CH;
@@ -197,10 +287,10 @@ __global__ __launch_bounds__(256) void bs_select_kernel(const T* __restrict__ q,
     for (int s = 0; s < KS; ++s) bf[s] = *reinterpret_cast<const f16x8*>(&qi[lane & 15][s * 32 + (lane >> 4) * 8]);
     const _Float16* kp = ints + ((size_t)b * KV + h) * NB * 2 * D;
     const float* sp = scale + ((size_t)b * KV + h) * NB;
-    unsigned key[4] = {0u, 0u, 0u, 0u};
+    unsigned key[4] = {0u, 0u, 0u, 0u}, least[4] = {0u, 0u, 0u, 0u};
     int idx[4] = {-1, -1, -1, -1}, have[4] = {0, 0, 0, 0};
-    for (int j0 = 0; j0 < NB; j0 += kChunk) {
-        const int tiles = (min(kChunk, NB - j0) + 15) / 16;
+    for (int j0 = first; j0 < last; j0 += kChunk) {
+        const int tiles = (min(kChunk, last - j0) + 15) / 16;
         for (int tl = wave; tl < kChunk / 16; tl += 4) {
             const int jr = j0 + tl * 16;
             f32x4 acc{0.f, 0.f, 0.f, 0.f};
@@ -216,7 +306,7 @@ __global__ __launch_bounds__(256) void bs_select_kernel(const T* __restrict__ q,
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int j = jr + (lane >> 4) * 4 + i;
-                const float s = j < NB ? sp[j] : -1.0f;
+                const float s = j < last ? sp[j] : -1.0f;
                 k4[i] = s < 0.f ? 0u : order_key(acc[i] * s);
             }
             *reinterpret_cast<uint4*>(&sc[(lane & 15) * kScPitch + tl * 16 + (lane >> 4) * 4]) = make_uint4(k4[0], k4[1], k4[2], k4[3]);
@@ -224,88 +314,144 @@ __global__ __launch_bounds__(256) void bs_select_kernel(const T* __restrict__ q,
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const int row = wave * 4 + u;
             unsigned c[kChunk / 64];
-            unsigned top = 0;
 #pragma unroll
-            for (int e = 0; e < kChunk / 64; ++e) { c[e] = sc[row * kScPitch + e * 64 + lane]; top = max(top, c[e]); }
-            // later blocks enter only above the smallest one kept (ties go to the earlier block)
-            unsigned least = have[u] == n ? key[u] : 0u;
-            if (have[u] == n) {
-                least = lane < n ? key[u] : 0xffffffffu;
-#pragma unroll
-                for (int o = 32; o >= 1; o >>= 1) least = min(least, (unsigned)__shfl_xor((int)least, o));
-            }
-            if (__ballot(top > least)) have[u] = keep_largest(key[u], idx[u], c, j0, n, lk[wave], li[wave], lane);
+            for (int e = 0; e < kChunk / 64; ++e) c[e] = sc[(wave * 4 + u) * kScPitch + e * 64 + lane];
+            take(key[u], idx[u], have[u], least[u], c, [&](int e) { return j0 + e * 64 + lane; }, n, lk[wave], li[wave], lane);
         }
         __syncthreads();
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
         const int t = t0 + wave * 4 + u;
-        if (t < T_ && lane < n) out[(((size_t)b * T_ + t) * KV + h) * n + lane] = lane < have[u] ? idx[u] : -1;
+        if (t >= T_ || lane >= n) continue;
+        const size_t at = ((size_t)b * T_ + t) * KV + h;
+        if constexpr (PARTS) part[(at * parts + blockIdx.x % parts) * n + lane] = lane < have[u] ? make_uint2(key[u], (unsigned)idx[u]) : make_uint2(0u, 0xffffffffu);
+        else out[at * n + lane] = lane < have[u] ? idx[u] : -1;
     }
+}
+
+// the n best of the parts' n best: one wave per (query, kv head); the parts are in the order of the blocks
+__global__ __launch_bounds__(64) void bs_select_join_kernel(const uint2* __restrict__ part, int parts, int n, int32_t* __restrict__ out) {
+    __shared__ unsigned lk[64];
+    __shared__ int li[64];
+    constexpr int E = 4;
+    const int lane = threadIdx.x, total = parts * n;
+    const uint2* p = part + (size_t)blockIdx.x * total;
+    unsigned key = 0u, least = 0u;
+    int idx = -1, have = 0;
+    for (int i0 = 0; i0 < total; i0 += E * 64) {
+        unsigned c[E];
+        int x[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const uint2 v = i0 + e * 64 + lane < total ? p[i0 + e * 64 + lane] : make_uint2(0u, 0xffffffffu);
+            c[e] = v.x;
+            x[e] = (int)v.y;
+        }
+        take(key, idx, have, least, c, [&](int e) { return x[e]; }, n, lk, li, lane);
+    }
+    if (lane < n) out[(size_t)blockIdx.x * n + lane] = lane < have ? idx : -1;
 }
 
 // ------------------------------------------------------------------------------------------------------------ lists
-// Counting sort of the mentions of a (sample, kv head) by block.  One wave takes a run of mentions in order; equal blocks among the 64 lanes
-// are found with one ballot per bit of the block number, counters live in LDS.  Same lists whatever the timing.
-template <bool FILL>
-__global__ __launch_bounds__(64) void bs_list_kernel(const int32_t* __restrict__ blocks, int T_, int KV, int NB, int n, int runs, int run_len, int bits,
-                                                     int32_t* __restrict__ hist, const int32_t* __restrict__ start, int32_t* __restrict__ list) {
+// Counting sort of the mentions of a (sample, kv head) by block, in three launches: counts of `runs` runs of mentions, places, fill.  In the fill one wave
+// takes a run in order; equal blocks among its 64 lanes are found with one ballot per bit of the block number, counters live in LDS.  Same lists
+// whatever the timing.
+__device__ __forceinline__ int mention(const int32_t* blocks, long long e, long long e1, size_t bt0, int KV, int h, int n, int& m) {
+    if (e >= e1) return -1;
+    const int t = (int)(e / n), s = (int)(e - (long long)t * n);
+    m = t * kMaxPick + s;
+    return blocks[((bt0 + t) * KV + h) * n + s];
+}
+
+__global__ __launch_bounds__(256) void bs_count_kernel(const int32_t* __restrict__ blocks, int T_, int KV, int NB, int n, int runs, int run_len, int32_t* __restrict__ hist) {
     extern __shared__ int cnt[];
-    const int lane = threadIdx.x, run = blockIdx.x, bh = blockIdx.y, b = bh / KV, h = bh % KV;
-    int32_t* hp = hist + ((size_t)bh * runs + run) * NB;
-    for (int j = lane; j < NB; j += 64) cnt[j] = FILL ? hp[j] + start[(size_t)bh * (NB + 1) + j] : 0;
+    const int run = blockIdx.x, bh = blockIdx.y, b = bh / KV, h = bh % KV;
+    for (int j = threadIdx.x; j < NB; j += 256) cnt[j] = 0;
     __syncthreads();
     const long long total = (long long)T_ * n, e0 = (long long)run * run_len, e1 = min(total, e0 + run_len);
-    for (long long e = e0; e < e1; e += 64) {
-        const bool in = e + lane < e1;
-        int j = -1, t = 0, s = 0;
-        if (in) {
-            t = (int)((e + lane) / n);
-            s = (int)((e + lane) - (long long)t * n);
-            j = blocks[(((size_t)b * T_ + t) * KV + h) * n + s];
-        }
-        const bool ok = in && j >= 0 && j < NB;
-        unsigned long long same = __ballot(ok);
-        for (int bit = 0; bit < bits; ++bit) {
-            const unsigned long long m = __ballot(ok && (j >> bit & 1));
-            same &= (j >> bit & 1) ? m : ~m;
-        }
-        const int rank = __popcll(same & ((1ull << lane) - 1));
-        const int at = ok ? cnt[j] + rank : 0;
-        __syncthreads();
-        if (ok && rank == 0) cnt[j] += __popcll(same);
-        __syncthreads();
-        if constexpr (FILL) {
-            if (ok) list[(size_t)bh * total + at] = t * kMaxPick + s;
-        }
+    for (long long e = e0 + threadIdx.x; e < e1; e += 1024) {
+        int j[4], m;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) j[u] = mention(blocks, e + u * 256, e1, (size_t)b * T_, KV, h, n, m);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (j[u] >= 0 && j[u] < NB) atomicAdd(&cnt[j[u]], 1);          // a count: any order
     }
-    if constexpr (!FILL) {
-        __syncthreads();
-        for (int j = lane; j < NB; j += 64) hp[j] = cnt[j];
+    __syncthreads();
+    int32_t* hp = hist + ((size_t)bh * runs + run) * NB;
+    for (int j = threadIdx.x; j < NB; j += 256) hp[j] = cnt[j];
+}
+
+__global__ __launch_bounds__(64) void bs_fill_kernel(const int32_t* __restrict__ blocks, int T_, int KV, int NB, int n, int runs, int run_len, int bits,
+                                                     const int32_t* __restrict__ hist, const int32_t* __restrict__ start, int32_t* __restrict__ list) {
+    extern __shared__ int cnt[];
+    const int lane = threadIdx.x, run = blockIdx.x, bh = blockIdx.y, b = bh / KV, h = bh % KV;
+    const int32_t* hp = hist + ((size_t)bh * runs + run) * NB;
+    for (int j = lane; j < NB; j += 64) cnt[j] = hp[j] + start[(size_t)bh * (NB + 1) + j];
+    __syncthreads();
+    const long long total = (long long)T_ * n, e0 = (long long)run * run_len, e1 = min(total, e0 + run_len);
+    constexpr int U = 4;
+    int j[U], m[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) j[u] = mention(blocks, e0 + u * 64 + lane, e1, (size_t)b * T_, KV, h, n, m[u]);
+    for (long long e = e0; e < e1; e += U * 64) {
+        int jn[U], mn[U];                                                  // the next mentions are on their way
+#pragma unroll
+        for (int u = 0; u < U; ++u) jn[u] = mention(blocks, e + (U + u) * 64 + lane, e1, (size_t)b * T_, KV, h, n, mn[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool ok = j[u] >= 0 && j[u] < NB;
+            unsigned long long same = __ballot(ok);
+            for (int bit = 0; bit < bits; ++bit) {
+                const unsigned long long x = __ballot(ok && (j[u] >> bit & 1));
+                same &= (j[u] >> bit & 1) ? x : ~x;
+            }
+            const int rank = __popcll(same & ((1ull << lane) - 1));
+            const int at = ok ? cnt[j[u]] + rank : 0;
+            __builtin_amdgcn_wave_barrier();
+            if (ok && rank == 0) cnt[j[u]] += __popcll(same);
+            __builtin_amdgcn_wave_barrier();
+            if (ok) list[(size_t)bh * total + at] = m[u];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) { j[u] = jn[u]; m[u] = mn[u]; }
     }
 }
 
-// one workgroup per (sample, kv head): counts of the runs -> places, starts of the lists, work items of at most `rows` rows
-__global__ __launch_bounds__(1024) void bs_scan_kernel(int32_t* __restrict__ hist, int runs, int NB, int G, int rows, int max_items, int32_t* __restrict__ start,
-                                                       int32_t* __restrict__ items, int32_t* __restrict__ n_items) {
+// counts of the runs -> places within a block's list, and its length
+__global__ __launch_bounds__(64) void bs_places_kernel(int32_t* __restrict__ hist, int runs, int NB, int32_t* __restrict__ len) {
+    const int j = blockIdx.x * 64 + threadIdx.x, bh = blockIdx.y;
+    if (j >= NB) return;
+    int32_t* hp = hist + (size_t)bh * runs * NB + j;
+    int sum = 0, r = 0;
+    for (; r + 8 <= runs; r += 8) {
+        int c[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = hp[(size_t)(r + i) * NB];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { hp[(size_t)(r + i) * NB] = sum; sum += c[i]; }
+    }
+    for (; r < runs; ++r) {
+        const int c = hp[(size_t)r * NB];
+        hp[(size_t)r * NB] = sum;
+        sum += c;
+    }
+    len[(size_t)bh * (NB + 1) + j] = sum;
+}
+
+// one workgroup per (sample, kv head): lengths -> starts of the lists (in place), work items of at most `rows` rows
+__global__ __launch_bounds__(1024) void bs_scan_kernel(int NB, int G, int rows, int max_items, int32_t* __restrict__ start, int32_t* __restrict__ items,
+                                                       int32_t* __restrict__ n_items) {
     __shared__ int ws[2][16];
     __shared__ int carry[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bh = blockIdx.x;
-    int32_t* hp = hist + (size_t)bh * runs * NB;
     if (tid < 2) carry[tid] = 0;
     __syncthreads();
     for (int j0 = 0; j0 < NB; j0 += 1024) {
         const int j = j0 + tid;
-        int len = 0;
-        if (j < NB)
-            for (int r = 0; r < runs; ++r) {
-                const int c = hp[(size_t)r * NB + j];
-                hp[(size_t)r * NB + j] = len;
-                len += c;
-            }
+        const int len = j < NB ? start[(size_t)bh * (NB + 1) + j] : 0;
         const int its = (int)(((long long)len * G + rows - 1) / rows);
         int a = len, c = its;          // inclusive scans over the workgroup
 #pragma unroll
@@ -917,7 +1063,7 @@ int bs_rows(const char* what, const void* p, const int64_t* s, int dtype) {
 }
 
 int bs_runs(int64_t bh, int64_t entries) {
-    int64_t r = 2048 / bh;
+    int64_t r = 512 / bh;
     const int64_t most = (entries + 255) / 256;
     if (r > most) r = most;
     return (int)(r < 1 ? 1 : r);
@@ -977,18 +1123,49 @@ extern "C" int av2x_block_bounds(const void* k, const uint8_t* mask, const int64
     });
 }
 
+namespace {
+
+// Few queries leave the chip idle while a workgroup walks the scores of all blocks: the blocks are cut into ranges of whole chunks until there are
+// about two workgroups a CU, and the ranges' choices joined (one query against 4400 blocks: 9 ranges of one chunk)
+int select_parts(int64_t B, int64_t T, int64_t KV, int64_t NB) {
+    const int64_t groups = (T + 15) / 16 * KV * B, chunks = (NB + kChunk - 1) / kChunk;
+    if (chunks < 2 || groups >= 256) return 1;
+    const int64_t want = (512 + groups - 1) / groups;
+    return (int)(want < chunks ? want : chunks);
+}
+
+}  // namespace
+
+extern "C" uint64_t av2x_select_blocks_workspace_bytes(int32_t batch, int32_t queries, int32_t keys, int32_t kv_heads, int32_t n) {
+    if (batch < 1 || queries < 1 || keys < 0 || kv_heads < 1 || n < 1) return 0;
+    const int p = select_parts(batch, queries, kv_heads, (keys + kKeys - 1) / kKeys);
+    return p == 1 ? 0 : (uint64_t)batch * queries * kv_heads * p * n * sizeof(uint2);
+}
+
 extern "C" int av2x_select_blocks(const void* q, const int64_t* strides, const uint16_t* ints, const float* scale, int32_t batch, int32_t queries, int32_t keys,
-                                  int32_t heads, int32_t kv_heads, int32_t dim, int32_t n, int32_t dtype, int32_t* blocks, av2x_stream_t stream) {
+                                  int32_t heads, int32_t kv_heads, int32_t dim, int32_t n, int32_t dtype, int32_t* blocks, void* workspace, av2x_stream_t stream) {
     const char* what = "av2x_select_blocks";
     if (int rc = bs_check(what, batch, queries, keys, heads, kv_heads, dim, n, dtype)) return rc;
     if (queries == 0) return 0;
-    const int NB = (keys + kKeys - 1) / kKeys;
-    if (!q || !blocks || (NB && (!ints || !scale))) return av2x::fail("%s: null tensor", what);
-    if (!tok_aligned(ints, 16)) return av2x::fail("%s: the bounds must be aligned to 16 bytes", what);
+    const int NB = (keys + kKeys - 1) / kKeys, parts = select_parts(batch, queries, kv_heads, NB);
+    if (!q || !blocks || (NB && (!ints || !scale)) || (parts > 1 && !workspace)) return av2x::fail("%s: null tensor", what);
+    if (!tok_aligned(ints, 16) || !tok_aligned(workspace, 8)) return av2x::fail("%s: the bounds must be aligned to 16 bytes", what);
+    const int per = ((NB + parts - 1) / parts + kChunk - 1) / kChunk * kChunk, used = parts > 1 ? (NB + per - 1) / per : 1;
+    hipStream_t st = av2x::as_stream(stream);
     return bs_go(dtype, dim, [&](auto t, auto d) {
         using T = typename decltype(t)::type;
-        bs_select_kernel<T, decltype(d)::value><<<dim3((queries + 15) / 16, kv_heads, batch), 256, 0, av2x::as_stream(stream)>>>(
-            static_cast<const T*>(q), strides[0], strides[1], strides[2], reinterpret_cast<const _Float16*>(ints), scale, batch, queries, heads / kv_heads, kv_heads, NB, n, blocks);
+        constexpr int D = decltype(d)::value;
+        const _Float16* ip = reinterpret_cast<const _Float16*>(ints);
+        const unsigned tiles = (unsigned)(queries + 15) / 16;
+        if (used == 1) {
+            bs_select_kernel<T, D, false><<<dim3(tiles, kv_heads, batch), 256, 0, st>>>(static_cast<const T*>(q), strides[0], strides[1], strides[2], ip, scale, queries,
+                                                                                      heads / kv_heads, kv_heads, NB, n, 1, NB, blocks, nullptr);
+            return av2x::check_launch(what);
+        }
+        bs_select_kernel<T, D, true><<<dim3(tiles * used, kv_heads, batch), 256, 0, st>>>(static_cast<const T*>(q), strides[0], strides[1], strides[2], ip, scale, queries,
+                                                                                        heads / kv_heads, kv_heads, NB, n, used, per, nullptr, static_cast<uint2*>(workspace));
+        if (int rc = av2x::check_launch(what)) return rc;
+        bs_select_join_kernel<<<(unsigned)(batch * queries * kv_heads), 64, 0, st>>>(static_cast<const uint2*>(workspace), used, n, blocks);
         return av2x::check_launch(what);
     });
 }
@@ -1013,13 +1190,15 @@ extern "C" int av2x_block_lists(const int32_t* blocks, int32_t batch, int32_t qu
     const size_t lds = (size_t)NB * 4;
     hipStream_t st = av2x::as_stream(stream);
     static av2x::LdsLimit lim0, lim1;
-    lim0.ensure((const void*)bs_list_kernel<false>, lds);
-    lim1.ensure((const void*)bs_list_kernel<true>, lds);
-    bs_list_kernel<false><<<dim3(l.runs, bh), 64, lds, st>>>(blocks, queries, kv_heads, NB, n, l.runs, run_len, bits, l.hist, nullptr, nullptr);
+    lim0.ensure((const void*)bs_count_kernel, lds);
+    lim1.ensure((const void*)bs_fill_kernel, lds);
+    bs_count_kernel<<<dim3(l.runs, bh), 256, lds, st>>>(blocks, queries, kv_heads, NB, n, l.runs, run_len, l.hist);
     if (int rc = av2x::check_launch(what)) return rc;
-    bs_scan_kernel<<<bh, 1024, 0, st>>>(l.hist, l.runs, NB, G, kItemRows, l.max_items, l.start, l.items, l.n_items);
+    bs_places_kernel<<<dim3((NB + 63) / 64, bh), 64, 0, st>>>(l.hist, l.runs, NB, l.start);
     if (int rc = av2x::check_launch(what)) return rc;
-    bs_list_kernel<true><<<dim3(l.runs, bh), 64, lds, st>>>(blocks, queries, kv_heads, NB, n, l.runs, run_len, bits, l.hist, l.start, l.list);
+    bs_scan_kernel<<<bh, 1024, 0, st>>>(NB, G, kItemRows, l.max_items, l.start, l.items, l.n_items);
+    if (int rc = av2x::check_launch(what)) return rc;
+    bs_fill_kernel<<<dim3(l.runs, bh), 64, lds, st>>>(blocks, queries, kv_heads, NB, n, l.runs, run_len, bits, l.hist, l.start, l.list);
     return av2x::check_launch(what);
 }
 

@@ -302,8 +302,10 @@ def select_blocks(q, bounds, blocks):
         r = _runner(q.device)
         if q.stride(-1) != 1:
             q = q.contiguous()
+        size = int(r.lib.av2x_select_blocks_workspace_bytes(b, t, nb * BLOCK, kv, blocks))
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
         _lib.check(r.lib.av2x_select_blocks(_P(q), _host64(*q.stride()[:3]), _P(bounds.ints), _P(bounds.scale), b, t, nb * BLOCK, h, kv, d, blocks, _DTYPES[q.dtype],
-                                            _P(out), r.stream()), "av2x_select_blocks")
+                                            _P(out), _P(ws), r.stream()), "av2x_select_blocks")
     return out
 
 

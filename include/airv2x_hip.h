@@ -1007,7 +1007,8 @@ int av2x_act8_wgrad(const float* dy, const int8_t* q, const float* scale, const 
  *                     strides: HOST {batch, token, head} of k.
  * av2x_select_blocks  score of a block = sum over the group's channels of max(q U, q L), q as whole numbers up to 127 (one scale a group), times the
  *                     block's scale: exact whatever the order of summation.  blocks (batch, queries, kv_heads, n) i32: the n best, ties to the lowest
- *                     block, ascending, -1 behind the last.  strides: HOST {batch, token, head} of q.
+ *                     block, ascending, -1 behind the last.  strides: HOST {batch, token, head} of q.  workspace:
+ *                     av2x_select_blocks_workspace_bytes (0: NULL).
  * av2x_block_lists    the mentions of every block, for the two calls below: av2x_block_lists_bytes bytes of device memory, kept by the caller
  * av2x_block_sparse_attention   out (batch, queries, heads, dim) = softmax(scale q k^T) v over the visible keys of a query's blocks (indices outside
  *                     0 .. NB - 1 are none; one that is named twice counts twice; no key at all: zeros), lse (batch, queries, heads) or NULL: log-sum-exp to
@@ -1017,8 +1018,9 @@ int av2x_act8_wgrad(const float* dy, const int8_t* q, const float* scale, const 
  * ------------------------------------------------------------------------------------ */
 int av2x_block_bounds(const void* k, const uint8_t* mask, const int64_t* strides, int32_t batch, int32_t keys, int32_t kv_heads, int32_t dim, int32_t dtype,
                       int32_t first_block, int32_t n_blocks, uint16_t* ints, float* scale, av2x_stream_t stream);
+uint64_t av2x_select_blocks_workspace_bytes(int32_t batch, int32_t queries, int32_t keys, int32_t kv_heads, int32_t n);
 int av2x_select_blocks(const void* q, const int64_t* strides, const uint16_t* ints, const float* scale, int32_t batch, int32_t queries, int32_t keys,
-                       int32_t heads, int32_t kv_heads, int32_t dim, int32_t n, int32_t dtype, int32_t* blocks, av2x_stream_t stream);
+                       int32_t heads, int32_t kv_heads, int32_t dim, int32_t n, int32_t dtype, int32_t* blocks, void* workspace, av2x_stream_t stream);
 uint64_t av2x_block_lists_bytes(int32_t batch, int32_t queries, int32_t keys, int32_t heads, int32_t kv_heads, int32_t n);
 int av2x_block_lists(const int32_t* blocks, int32_t batch, int32_t queries, int32_t keys, int32_t heads, int32_t kv_heads, int32_t n, void* lists,
                      av2x_stream_t stream);

@@ -74,7 +74,7 @@ def test_c_abi_refusals_of_the_blocks():
                      (dict(k=72), "aligned"), (dict(st=(ctypes.c_int64 * 3)(1024, 66, 32)), "aligned"), (dict(n=2 ** 21 + 1), "keys"), (dict(b=0), "batch")):
         assert bounds(**kw) != 0 and word in _err(), (kw, _err())
     assert bounds(count=0, k=None) == 0
-    sel = lambda q=64, t=4, h=2, kv=2, d=32, n=2, ints=64: lib.av2x_select_blocks(q, s3, ints, 64, 1, t, 100, h, kv, d, n, 0, 64, None)
+    sel = lambda q=64, t=4, h=2, kv=2, d=32, n=2, ints=64: lib.av2x_select_blocks(q, s3, ints, 64, 1, t, 100, h, kv, d, n, 0, 64, None, None)
     for kw, word in ((dict(n=0), "blocks"), (dict(n=65), "blocks"), (dict(h=3), "heads"), (dict(h=34, kv=1), "share"), (dict(h=16, kv=1, d=128), "share"), (dict(q=None), "null"),
                      (dict(ints=72), "16 bytes"), (dict(t=2 ** 26), "queries")):
         assert sel(**kw) != 0 and word in _err(), (kw, _err())
