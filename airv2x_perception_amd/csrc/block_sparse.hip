@@ -331,6 +331,262 @@ __global__ __launch_bounds__(256) void bs_select_kernel(const T* __restrict__ q,
     }
 }
 
+// The same for n <= 16, the common case: 32 queries a workgroup.  The scores themselves are not kept: the matrix cores' tile leaves the largest of every four
+// blocks in LDS (1536 blocks at a time, 50 KB), sixteen lanes a query look for the fours above the n-th best so far -- at first above the n-th largest of
+// the lanes' own maxima, which at least n scores reach -- and only their scores are computed again, exactly, one a lane.  What is above goes to a list of
+// pending entries; sixteen at a time count how many of the kept and of each other are better, which is their place.  Loops, not unrolled
+// code: an unrolled form of this filled the instruction cache (10 000 instructions) and ran at 1490 us where this one takes the time below.
+template <int R> __device__ __forceinline__ unsigned row_ror(unsigned x) {
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + R, 0xf, 0xf, false);
+}
+template <int R, int N, typename F> __device__ __forceinline__ void each_ror(F&& f) {
+    if constexpr (R < N) {
+        f(std::integral_constant<int, R>{});
+        each_ror<R + 1, N>(f);
+    }
+}
+template <int CTRL> __device__ __forceinline__ float dpp_f(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ int row_sum(int x) {
+    x += (int)row_ror<8>((unsigned)x);
+    x += (int)row_ror<4>((unsigned)x);
+    x += (int)row_ror<2>((unsigned)x);
+    return x + (int)row_ror<1>((unsigned)x);
+}
+__device__ __forceinline__ int rows_max(int x) {       // the largest of four rows' values, in a scalar
+    return max(max(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16)), max(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48)));
+}
+
+constexpr int kFours = 384;                  // fours of blocks in LDS
+constexpr int kGroupList = 64;               // fours of a query that are looked at in one go
+
+typedef unsigned long long u64;
+typedef u64 u64x2 __attribute__((ext_vector_type(2)));
+
+template <typename T, int D, bool PARTS>
+__global__ __launch_bounds__(512, 4) void bs_select16_kernel(const T* __restrict__ q, long long qb, long long qt, long long qh, const _Float16* __restrict__ ints,
+                                                             const float* __restrict__ scale, int T_, int G, int KV, int NB, int n, int parts, int per,
+                                                             int32_t* __restrict__ out, uint2* __restrict__ part) {
+    constexpr int NQ = 32, CH = D / 16, KS = 2 * D / 32, GT = KS <= 2 ? 4 : KS <= 4 ? 2 : 1, GP = kFours + 4, QP = 2 * D + 8;
+    constexpr int LB = D <= 64 ? D / 4 : 16, CPL = D <= 64 ? 1 : 2;      // lanes that add up one score, 16-byte pieces of each
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    __shared__ __align__(16) unsigned gm[NQ * GP];
+    __shared__ __align__(16) _Float16 qi[NQ * QP];
+    // entries: key of the score in the upper half, ~block in the lower one: larger is better, ties to the lower block; 0: none
+    __shared__ __align__(16) u64 kept[NQ][16], pend[NQ][32];
+    __shared__ unsigned short fours[NQ][kGroupList];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = lane & 15, row = lane >> 4;
+    const int t0 = (PARTS ? blockIdx.x / parts : blockIdx.x) * NQ, h = blockIdx.y, b = blockIdx.z;
+    const int first = PARTS ? (blockIdx.x % parts) * per : 0, last = PARTS ? min(NB, first + per) : NB;
+    for (int i = tid; i < NQ * 32; i += 512) { (&pend[0][0])[i] = 0ull; if (i < NQ * 16) (&kept[0][0])[i] = 0ull; }
+    {
+        const int r8 = tid >> 4, l8 = tid & 15, t = min(t0 + r8, T_ - 1);
+        const T* p = q + b * qb + t * qt + (long long)h * G * qh + l8 * CH;
+        float m = 0.f;
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int c = 0; c < CH; ++c) m = fmaxf(m, fabsf((float)p[g * qh + c]));
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+        const float r = 127.0f / fmaxf(m, kTinyBs);
+        float up[CH], lo[CH];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) up[c] = lo[c] = 0.f;
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const float x = fminf(fmaxf(rintf((float)p[g * qh + c] * r), -127.f), 127.f);
+                up[c] += fmaxf(x, 0.f);
+                lo[c] += fminf(x, 0.f);
+            }
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {       // at most 127 G <= 2048: exact in fp16
+            qi[r8 * QP + l8 * CH + c] = (_Float16)up[c];
+            qi[r8 * QP + D + l8 * CH + c] = (_Float16)lo[c];
+        }
+    }
+    __syncthreads();
+    const _Float16* kp = ints + ((size_t)b * KV + h) * NB * 2 * D;
+    const float* sp = scale + ((size_t)b * KV + h) * NB;
+    const int qr = wave * 4 + row;           // this row's query
+    u64* pe = pend[qr];
+    unsigned short* fo = fours[qr];
+    f16x8 y[CPL];
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) y[c] = *reinterpret_cast<const f16x8*>(&qi[qr * QP + (l % LB + c * LB) * 8]);
+    for (int j0 = first; j0 < last; j0 += kFours * 4) {
+        const int tiles = (min(kFours * 4, last - j0) + 15) / 16, steps = (tiles + 15) / 16;       // 16 tiles: 64 fours, four a lane
+        {
+            f16x8 bf[2][KS];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int s = 0; s < KS; ++s) bf[u][s] = *reinterpret_cast<const f16x8*>(&qi[(u * 16 + l) * QP + s * 32 + row * 8]);
+            for (int g0 = wave * GT; g0 < steps * 16; g0 += 8 * GT) {
+                f16x8 a[GT][KS];
+                float w[GT][4];
+#pragma unroll
+                for (int g = 0; g < GT; ++g) {
+                    const int jr = j0 + (g0 + g) * 16, ja = min(jr + l, NB - 1);
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) a[g][s] = *reinterpret_cast<const f16x8*>(kp + (size_t)ja * 2 * D + s * 32 + row * 8);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int j = jr + row * 4 + i;
+                        const float x = sp[min(j, NB - 1)];
+                        w[g][i] = j < last ? x : -1.0f;
+                    }
+                }
+#pragma unroll
+                for (int g = 0; g < GT; ++g)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        f32x4 acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int s = 0; s < KS; ++s) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[g][s], bf[u][s], acc, 0, 0, 0);
+                        unsigned m = 0u;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) m = max(m, w[g][i] < 0.f ? 0u : order_key(acc[i] * w[g][i]));
+                        gm[(u * 16 + l) * GP + (g0 + g) * 4 + row] = m;
+                    }
+            }
+        }
+        __syncthreads();
+        if (t0 + wave * 4 < T_) {
+            const unsigned* gp = gm + qr * GP + l * 4;
+            u64 k = kept[qr][l];
+            // what an entry has to beat: the n-th best (a block of this range may tie with it and come first), or every entry of a key
+            u64 bar = kept[qr][n - 1];
+            const bool none = kept[qr][0] == 0ull;
+            if (__ballot(none)) {
+                unsigned m = 0;
+                for (int i = 0; i < steps; ++i) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(gp + i * 64);
+                    m = max(max(m, max(x.x, x.y)), max(x.z, x.w));
+                }
+                int rank = 0;
+                each_ror<1, 16>([&](auto r) { rank += row_ror<decltype(r)::value>(m) > m ? 1 : 0; });
+                unsigned t = rank < n ? m : 0xffffffffu;
+                t = min(t, row_ror<8>(t));
+                t = min(t, row_ror<4>(t));
+                t = min(t, row_ror<2>(t));
+                t = min(t, row_ror<1>(t));
+                if (none && t > 0) bar = (u64)(t - 1) << 32 | 0xffffffffu;
+            }
+            int pc = 0;
+            // sixteen pending entries of every row enter; a loop over what is kept and what is new, two at a time
+            auto flush = [&]() {
+                const u64 x = pe[l];
+                const int have = __popc((unsigned)(__ballot(k != 0ull) >> (row * 16)) & 0xffffu);
+                int rk = l, rx = 0;
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const u64x2 y = *reinterpret_cast<const u64x2*>(&kept[qr][i]), z = *reinterpret_cast<const u64x2*>(pe + i);
+                    rx += (y[0] > x ? 1 : 0) + (y[1] > x ? 1 : 0) + (z[0] > x ? 1 : 0) + (z[1] > x ? 1 : 0);
+                    rk += (z[0] > k ? 1 : 0) + (z[1] > k ? 1 : 0);
+                }
+                const u64 later = pe[16 + l];
+                __builtin_amdgcn_wave_barrier();
+                if (k && rk < n) kept[qr][rk] = k;
+                if (x && rx < n) kept[qr][rx] = x;
+                pe[l] = later;
+                pe[16 + l] = 0ull;
+                __builtin_amdgcn_wave_barrier();
+                k = l < min(n, have + min(pc, 16)) ? kept[qr][l] : 0ull;
+                if (have + min(pc, 16) >= n) bar = max(bar, kept[qr][n - 1]);
+                pc = max(0, pc - 16);
+                __builtin_amdgcn_wave_barrier();
+            };
+            for (int s0 = 0, span = steps; s0 < steps;) {
+                const int s1 = min(steps, s0 + span);
+                const unsigned thr = (unsigned)(bar >> 32);                       // later fours lose ties
+                int cnt = 0;
+                for (int i = s0; i < s1; ++i) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(gp + i * 64);
+                    cnt += (x.x > thr ? 1 : 0) + (x.y > thr ? 1 : 0) + (x.z > thr ? 1 : 0) + (x.w > thr ? 1 : 0);
+                }
+                const int total = row_sum(cnt), most = rows_max(total);
+                if (most > kGroupList && span > 1) { span = 1; continue; }       // many ties: 64 fours of a query at a time
+                if (most > 0) {
+                    int pos = cnt;                                                // sum over the lanes before
+                    pos += __builtin_amdgcn_update_dpp(0, pos, 0x111, 0xf, 0xf, true);
+                    pos += __builtin_amdgcn_update_dpp(0, pos, 0x112, 0xf, 0xf, true);
+                    pos += __builtin_amdgcn_update_dpp(0, pos, 0x114, 0xf, 0xf, true);
+                    pos += __builtin_amdgcn_update_dpp(0, pos, 0x118, 0xf, 0xf, true);
+                    pos -= cnt;
+                    for (int i = s0; i < s1; ++i) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(gp + i * 64);
+                        const int g = (i * 16 + l) * 4;
+                        if (x.x > thr) fo[pos++] = (unsigned short)g;
+                        if (x.y > thr) fo[pos++] = (unsigned short)(g + 1);
+                        if (x.z > thr) fo[pos++] = (unsigned short)(g + 2);
+                        if (x.w > thr) fo[pos++] = (unsigned short)(g + 3);
+                    }
+                    __builtin_amdgcn_wave_barrier();
+                    // sixteen scores of every query: LB lanes read one block's bounds together (16 bytes each, whole lines) and add up, lane e keeps score e
+                    for (int r0 = 0; r0 < most; r0 += 4) {
+                        const bool there = r0 + (l >> 2) < total;
+                        const int j = there ? j0 + fo[r0 + (l >> 2)] * 4 + (l & 3) : NB;
+                        float w = sp[min(j, NB - 1)], dot = 0.f;
+                        w = j < last ? w : -1.0f;
+                        f16x8 x[LB][CPL];
+#pragma unroll
+                        for (int e = 0; e < LB; ++e) {
+                            const int f = r0 + (l / LB * LB + e) / 4;
+                            const int je = min(j0 + fo[min(f, kGroupList - 1)] * 4 + (e & 3), NB - 1);
+#pragma unroll
+                            for (int c = 0; c < CPL; ++c) x[e][c] = *reinterpret_cast<const f16x8*>(kp + (size_t)je * 2 * D + (l % LB + c * LB) * 8);
+                        }
+#pragma unroll
+                        for (int e = 0; e < LB; ++e) {
+                            float d = 0.f;
+#pragma unroll
+                            for (int c = 0; c < CPL; ++c)
+#pragma unroll
+                                for (int i = 0; i < 8; i += 2) d = __builtin_amdgcn_fdot2(h2{x[e][c][i], x[e][c][i + 1]}, h2{y[c][i], y[c][i + 1]}, d, false);      // whole numbers: exact
+                            d += dpp_f<0xB1>(d);
+                            d += dpp_f<0x4E>(d);
+                            if constexpr (LB >= 8) d += dpp_f<0x141>(d);
+                            if constexpr (LB >= 16) d += dpp_f<0x140>(d);
+                            dot = l % LB == e ? d : dot;
+                        }
+                        const unsigned key = w < 0.f ? 0u : order_key(dot * w);
+                        const u64 entry = key ? (u64)key << 32 | (unsigned)~j : 0ull;
+                        const bool in = entry > bar;
+                        const unsigned mine = (unsigned)(__ballot(in) >> (row * 16)) & 0xffffu;
+                        if (in) pe[pc + __popc(mine & ((1u << l) - 1))] = entry;
+                        pc += __popc(mine);
+                        __builtin_amdgcn_wave_barrier();
+                        while (rows_max(pc) > 16) flush();
+                    }
+                    while (rows_max(pc) > 0) flush();
+                }
+                s0 = s1;
+            }
+        }
+        __syncthreads();
+    }
+    {
+        const int t = t0 + qr;
+        const u64 k = kept[qr][l];
+        // in the order of the blocks: ~block is larger for the earlier ones
+        const unsigned x = (unsigned)k;
+        int rank = 0;
+        each_ror<1, 16>([&](auto r) { rank += row_ror<decltype(r)::value>(x) > x ? 1 : 0; });
+        __builtin_amdgcn_wave_barrier();
+        pe[l] = 0ull;
+        __builtin_amdgcn_wave_barrier();
+        if (k) pe[rank] = k;
+        __builtin_amdgcn_wave_barrier();
+        const u64 e = pe[l];
+        if (t >= T_ || l >= n) return;
+        const size_t at = ((size_t)b * T_ + t) * KV + h;
+        if constexpr (PARTS) part[(at * parts + blockIdx.x % parts) * n + l] = make_uint2((unsigned)(e >> 32), ~(unsigned)e);
+        else out[at * n + l] = e ? (int)~(unsigned)e : -1;
+    }
+}
+
 // the n best of the parts' n best: one wave per (query, kv head); the parts are in the order of the blocks
 __global__ __launch_bounds__(64) void bs_select_join_kernel(const uint2* __restrict__ part, int parts, int n, int32_t* __restrict__ out) {
     __shared__ unsigned lk[64];
@@ -1156,15 +1412,14 @@ extern "C" int av2x_select_blocks(const void* q, const int64_t* strides, const u
         using T = typename decltype(t)::type;
         constexpr int D = decltype(d)::value;
         const _Float16* ip = reinterpret_cast<const _Float16*>(ints);
-        const unsigned tiles = (unsigned)(queries + 15) / 16;
-        if (used == 1) {
-            bs_select_kernel<T, D, false><<<dim3(tiles, kv_heads, batch), 256, 0, st>>>(static_cast<const T*>(q), strides[0], strides[1], strides[2], ip, scale, queries,
-                                                                                      heads / kv_heads, kv_heads, NB, n, 1, NB, blocks, nullptr);
+        auto go = [&](auto kernel, int nq, int parts_, int per_, int32_t* out, uint2* part) {
+            kernel<<<dim3((unsigned)((queries + nq - 1) / nq) * parts_, kv_heads, batch), nq * 16, 0, st>>>(static_cast<const T*>(q), strides[0], strides[1], strides[2], ip, scale, queries,
+                                                                                                      heads / kv_heads, kv_heads, NB, n, parts_, per_, out, part);
             return av2x::check_launch(what);
-        }
-        bs_select_kernel<T, D, true><<<dim3(tiles * used, kv_heads, batch), 256, 0, st>>>(static_cast<const T*>(q), strides[0], strides[1], strides[2], ip, scale, queries,
-                                                                                        heads / kv_heads, kv_heads, NB, n, used, per, nullptr, static_cast<uint2*>(workspace));
-        if (int rc = av2x::check_launch(what)) return rc;
+        };
+        if (used == 1) return n <= 16 ? go(bs_select16_kernel<T, D, false>, 32, 1, NB, blocks, nullptr) : go(bs_select_kernel<T, D, false>, 16, 1, NB, blocks, nullptr);
+        uint2* ws = static_cast<uint2*>(workspace);
+        if (int rc = n <= 16 ? go(bs_select16_kernel<T, D, true>, 32, used, per, nullptr, ws) : go(bs_select_kernel<T, D, true>, 16, used, per, nullptr, ws)) return rc;
         bs_select_join_kernel<<<(unsigned)(batch * queries * kv_heads), 64, 0, st>>>(static_cast<const uint2*>(workspace), used, n, blocks);
         return av2x::check_launch(what);
     });

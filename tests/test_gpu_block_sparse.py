@@ -157,7 +157,7 @@ def test_bounds(dt, n, kv, d, masked):
 
 
 @pytest.mark.parametrize("dt,t,n,h,kv,d,blocks,masked", [(F32, 1, 1, 1, 1, 16, 1, None), (BF, 17, 700, 8, 8, 32, 4, "some"), (HF, 33, 2500, 8, 2, 64, 64, "empty"),
-                                                        (F32, 5, 35000, 2, 1, 16, 9, None), (BF, 16, 130, 4, 4, 128, 3, "some"), (F32, 3, 4000, 16, 1, 64, 63, "some")])
+                                                        (F32, 5, 35000, 2, 1, 16, 9, None), (HF, 70, 35000, 2, 2, 32, 16, None), (BF, 33, 900, 4, 2, 128, 12, "empty"), (BF, 16, 130, 4, 4, 128, 3, "some"), (F32, 3, 4000, 16, 1, 64, 63, "some")])
 def test_selection(dt, t, n, h, kv, d, blocks, masked):
     from airv2x_perception_amd.opencood_iface import token_attention as A
     q, k, _, _, mask = make(t + n, 2, t, n, h, kv, d, dt, masked)
@@ -186,6 +186,20 @@ def test_selection_of_equal_scores_and_of_odd_values():
     k[0, 5], k[0, 64 * 9 + 1] = float("nan"), float("inf")
     got = A.select_blocks(q.cuda(), A.block_bounds(k.cuda()), 5).cpu()
     assert ((got >= 0) & (got < 1300)).all() and (got.diff(dim=-1) > 0).all()
+
+
+@pytest.mark.parametrize("blocks", [1, 5, 16, 17])
+def test_selection_where_every_block_beats_the_ones_before(blocks):
+    """Scores that rise with the block for half of the queries and fall for the others, over three chunks and in ranges: every score is a newcomer."""
+    from airv2x_perception_amd.opencood_iface import token_attention as A
+    nb = 1300
+    k = (1 + torch.arange(nb).repeat_interleave(64) / nb)[None, :, None, None] * torch.ones(1, 1, 1, 16)
+    for t in (40, 5000):                               # ranges joined; one workgroup for all blocks
+        q = torch.rand(1, t, 1, 16, generator=torch.Generator().manual_seed(t)) + 0.1
+        q[:, 1::2] *= -1
+        got = A.select_blocks(q.cuda(), A.block_bounds(k.cuda()), blocks).cpu()[0, :, 0]
+        low = torch.arange(blocks, dtype=torch.int32)
+        assert torch.equal(got[::2], (low + nb - blocks).expand(t // 2, blocks)) and torch.equal(got[1::2], low.expand(t // 2, blocks))
 
 
 @pytest.mark.parametrize("dt", [F32, BF, HF])
