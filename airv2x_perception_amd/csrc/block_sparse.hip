@@ -42,7 +42,7 @@ struct BsArgs {
     const int32_t* n_items;                  // (B KV)
     int max_items;
     // forward
-    float* part;                             // (B, T, H, n, D)
+    void* part;                              // (B, T, H, n, D): of T in the forward, fp32 (dQ) in the backward
     f32x2* ml;                               // (B, T, H, n) maximum (scaled, base 2) and sum
     void* out;                               // (B, T, H, D)
     float* lse;                              // (B, T, H) base 2, +inf: no key; may be null
@@ -614,10 +614,10 @@ __global__ __launch_bounds__(64) void bs_select_join_kernel(const uint2* __restr
 // Counting sort of the mentions of a (sample, kv head) by block, in three launches: counts of `runs` runs of mentions, places, fill.  In the fill one wave
 // takes a run in order; equal blocks among its 64 lanes are found with one ballot per bit of the block number, counters live in LDS.  Same lists
 // whatever the timing.
-__device__ __forceinline__ int mention(const int32_t* blocks, long long e, long long e1, size_t bt0, int KV, int h, int n, int& m) {
+__device__ __forceinline__ int mention(const int32_t* blocks, unsigned e, unsigned e1, size_t bt0, int KV, int h, unsigned n, int& m) {
     if (e >= e1) return -1;
-    const int t = (int)(e / n), s = (int)(e - (long long)t * n);
-    m = t * kMaxPick + s;
+    const unsigned t = e / n, s = e - t * n;
+    m = (int)(t * kMaxPick + s);
     return blocks[((bt0 + t) * KV + h) * n + s];
 }
 
@@ -626,8 +626,8 @@ __global__ __launch_bounds__(256) void bs_count_kernel(const int32_t* __restrict
     const int run = blockIdx.x, bh = blockIdx.y, b = bh / KV, h = bh % KV;
     for (int j = threadIdx.x; j < NB; j += 256) cnt[j] = 0;
     __syncthreads();
-    const long long total = (long long)T_ * n, e0 = (long long)run * run_len, e1 = min(total, e0 + run_len);
-    for (long long e = e0 + threadIdx.x; e < e1; e += 1024) {
+    const unsigned total = (unsigned)T_ * n, e0 = min(total, (unsigned)run * run_len), e1 = min(total, e0 + run_len);
+    for (unsigned e = e0 + threadIdx.x; e < e1; e += 1024) {
         int j[4], m;
 #pragma unroll
         for (int u = 0; u < 4; ++u) j[u] = mention(blocks, e + u * 256, e1, (size_t)b * T_, KV, h, n, m);
@@ -647,12 +647,12 @@ __global__ __launch_bounds__(64) void bs_fill_kernel(const int32_t* __restrict__
     const int32_t* hp = hist + ((size_t)bh * runs + run) * NB;
     for (int j = lane; j < NB; j += 64) cnt[j] = hp[j] + start[(size_t)bh * (NB + 1) + j];
     __syncthreads();
-    const long long total = (long long)T_ * n, e0 = (long long)run * run_len, e1 = min(total, e0 + run_len);
+    const unsigned total = (unsigned)T_ * n, e0 = min(total, (unsigned)run * run_len), e1 = min(total, e0 + run_len);
     constexpr int U = 4;
     int j[U], m[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) j[u] = mention(blocks, e0 + u * 64 + lane, e1, (size_t)b * T_, KV, h, n, m[u]);
-    for (long long e = e0; e < e1; e += U * 64) {
+    for (unsigned e = e0; e < e1; e += U * 64) {
         int jn[U], mn[U];                                                  // the next mentions are on their way
 #pragma unroll
         for (int u = 0; u < U; ++u) jn[u] = mention(blocks, e + (U + u) * 64 + lane, e1, (size_t)b * T_, KV, h, n, mn[u]);
@@ -735,10 +735,13 @@ __global__ __launch_bounds__(1024) void bs_scan_kernel(int NB, int G, int rows, 
 }
 
 // ------------------------------------------------------------------------------------------------------------ tiles
-// Operands of the 32 x 32 matrix instructions.  16-bit types: k-step of 16, a lane holds eight consecutive k of its row; fp32: k-step of 2, a lane
-// holds one.  A contraction over d walks it in the order the lanes hold it: d = 16 s + 8 half + i (16 bit), d = half D / 2 + s (fp32).
-// Accumulators (both): column lane & 31, rows 8 (i / 4) + 4 half + i % 4.  A contraction over keys or queries takes that accumulator as the B operand as
-// it lies: step s of 16 covers rows 16 s + 4 half + {0..3, 8..11}, step s of 2 (fp32) row 8 (s / 4) + 4 half + s % 4.
+// Operands of the 32 x 32 x 16 matrix instructions: a lane holds eight consecutive k of its row; a contraction over d walks d = 16 s + 8 half + i.
+// Accumulators: column lane & 31, rows 8 (i / 4) + 4 half + i % 4; a contraction over keys or queries takes such a tile as the B operand as it lies: step s
+// of 16 covers rows 16 s + 4 half + {0..3, 8..11}.
+//
+// fp32 tensors run on the same instructions as two fp16 terms each: a row (queries, dO) or a block (K, V) is brought to the top of fp16's range by a power of two,
+// hi + lo hold it to 22 bits, three products of terms make one product.  Three 16-bit MFMAs take 3 / 16 of the time of the fp32 instruction
+// (backward of 281600 queries x 8 blocks: 1204 us with v_mfma_f32_32x32x2_f32).
 template <typename T> struct Op;
 template <> struct Op<__bf16> {
     typedef __bf16 frag __attribute__((ext_vector_type(8)));
@@ -748,19 +751,20 @@ template <> struct Op<_Float16> {
     typedef _Float16 frag __attribute__((ext_vector_type(8)));
     static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
-template <> struct Op<float> {
-    typedef float frag;
-    static __device__ __forceinline__ f32x16 mma(float a, float b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
+template <typename T> struct Held {              // how a tensor of T is held in LDS and registers
+    static constexpr bool two = is_f32<T>::value;
+    static constexpr int terms = two ? 2 : 1;
+    typedef typename std::conditional<two, _Float16, T>::type E;
+    typedef typename Op<E>::frag frag;
+    static constexpr bool narrow = std::is_same<E, _Float16>::value;      // P and dS need a common power of two
 };
 
 template <typename T, int D> struct Shape {
-    static constexpr bool F = is_f32<T>::value;
-    static constexpr int KS = F ? D / 2 : D / 16;               // k-steps over d
+    static constexpr int KS = D / 16;                           // k-steps over d
     static constexpr int DT = (D + 31) / 32;                    // 32-wide tiles of d
-    static constexpr int P = F ? D + 1 : D + 8;                 // row pitch of a [row][d] tile: banks
-    static constexpr int PT = F ? 0 : kKeys + 4;                // row pitch of a [d][key] tile (16-bit types only)
-    static constexpr int kOver = F && D < 32 ? 32 : 0;          // a 32-wide read of the last row stays inside
-    static constexpr int kRowTile = kKeys * P + kOver;
+    static constexpr int P = D + 8;                             // row pitch of a [row][d] tile: banks
+    static constexpr int PT = kKeys + 4;                        // row pitch of a [d][key] tile
+    static constexpr int kRowTile = kKeys * P;                  // of one term
     static constexpr int kTransTile = DT * 32 * PT;             // d padded to 32 with zeros
 };
 
@@ -771,133 +775,196 @@ __device__ __forceinline__ f32x16 zero16() {
     return z;
 }
 
-// rows [0, 64) of a block to LDS: [key][d], and (16-bit types) [d][key].  Keys behind the end or masked are zeros.
+// the power of two that brings m to 2^14 .. 2^15, the top of fp16: values down to 2^-18 of the largest keep 22 bits in two terms, and what is below that is off by
+// 2^-40 of it at most
+__device__ __forceinline__ float pow2_over(float m) {
+    return m > 1e-30f && m < INFINITY ? ldexpf(1.0f, __builtin_amdgcn_frexp_expf(m) - 15) : 1.0f;
+}
+
+// rows [0, 64) of a block to LDS: [key][d], and [d][key].  Keys behind the end or masked are zeros.  Returns the power of two that was taken out (fp32).
+// All 256 threads; ends with the writes, not with a barrier.
 template <typename T, int D, bool ROW, bool TRANS>
-__device__ __forceinline__ void load_block(const T* src, long long st, int t0, int nk, unsigned long long seen, T* row, T* tr) {
+__device__ __forceinline__ float load_block(const T* src, long long st, int t0, unsigned long long seen, typename Held<T>::E* row, typename Held<T>::E* tr, float* red) {
     using S = Shape<T, D>;
-    constexpr int V = 16 / sizeof(T), CPR = D / V;
-    for (int i = threadIdx.x; i < kKeys * CPR; i += blockDim.x) {
-        const int key = i & 63, c = i >> 6;
-        typedef T vec __attribute__((ext_vector_type(V)));
-        vec x;
+    using E = typename Held<T>::E;
+    constexpr int CPR = D / 8, N = kKeys * CPR / 256 > 0 ? kKeys * CPR / 256 : 1;
+    typedef T vec __attribute__((ext_vector_type(8)));
+    typedef E evec __attribute__((ext_vector_type(8)));
+    vec x[N];
+    float m = 0.f, back = 1.0f;
 #pragma unroll
-        for (int e = 0; e < V; ++e) x[e] = (T)0.f;
-        if (seen >> key & 1) x = *reinterpret_cast<const vec*>(src + (long long)(t0 + key) * st + c * V);
-        if constexpr (ROW) {
-            if constexpr (S::F) {
+    for (int u = 0; u < N; ++u) {
+        const int i = threadIdx.x + u * 256, key = i & 63, c = i >> 6;
 #pragma unroll
-                for (int e = 0; e < V; ++e) row[key * S::P + c * V + e] = x[e];
+        for (int e = 0; e < 8; ++e) x[u][e] = (T)0.f;
+        if (c < CPR && (seen >> key & 1)) {
+            const T* p = src + (long long)(t0 + key) * st + c * 8;
+            if constexpr (Held<T>::two) {
+                const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { x[u][e] = a[e]; x[u][4 + e] = b[e]; m = fmaxf(m, fmaxf(fabsf(a[e]), fabsf(b[e]))); }
             } else {
-                *reinterpret_cast<vec*>(row + key * S::P + c * V) = x;
+                x[u] = *reinterpret_cast<const vec*>(p);
             }
         }
-        if constexpr (TRANS && !S::F) {
+    }
+    if constexpr (Held<T>::two) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) tr[(c * V + e) * S::PT + key] = x[e];
+        for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+        __syncthreads();
+        back = pow2_over(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+    }
+    const float to = 1.0f / back;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+        const int i = threadIdx.x + u * 256, key = i & 63, c = i >> 6;
+        if (c >= CPR) continue;
+#pragma unroll
+        for (int k = 0; k < Held<T>::terms; ++k) {
+            evec y;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if constexpr (Held<T>::two) {
+                    const float v = x[u][e] * to;
+                    const _Float16 h = (_Float16)v;
+                    y[e] = k == 0 ? h : (_Float16)(v - (float)h);
+                } else {
+                    y[e] = x[u][e];
+                }
+            }
+            if constexpr (ROW) *reinterpret_cast<evec*>(row + k * S::kRowTile + key * S::P + c * 8) = y;
+            if constexpr (TRANS) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) tr[k * S::kTransTile + (c * 8 + e) * S::PT + key] = y[e];
+            }
         }
     }
-    if constexpr (TRANS && !S::F && D < 32) {
-        for (int i = threadIdx.x; i < (32 - D) * S::PT; i += blockDim.x) tr[D * S::PT + i] = (T)0.f;
+    if constexpr (TRANS && D < 32) {
+        for (int i = threadIdx.x; i < (32 - D) * S::PT; i += 256)
+#pragma unroll
+            for (int k = 0; k < Held<T>::terms; ++k) tr[k * S::kTransTile + D * S::PT + i] = (E)0.f;
     }
+    return back;
 }
 
-template <typename T, int D> __device__ __forceinline__ typename Op<T>::frag row_frag(const T* tile, int r, int s, int half) {
-    using S = Shape<T, D>;
-    if constexpr (S::F) return tile[r * S::P + half * (D / 2) + s];
-    else return *reinterpret_cast<const typename Op<T>::frag*>(tile + r * S::P + s * 16 + half * 8);
-}
-
-// a head vector as fragments, straight from global memory
-template <typename T, int D> __device__ __forceinline__ void global_frags(const T* p, bool in, int half, typename Op<T>::frag (&f)[Shape<T, D>::KS]) {
-    if constexpr (is_f32<T>::value) {
+// a head vector in pieces of one k-step and its power of two, straight from global memory; the two half waves hold halves of it
+template <typename T, int D> struct RowFrags {
+    typename Held<T>::frag f[Held<T>::terms][Shape<T, D>::KS];
+    float back = 1.0f;
+};
+template <typename T, int D> __device__ __forceinline__ void global_frags(const T* p, bool in, int half, RowFrags<T, D>& r) {
+    if constexpr (Held<T>::two) {
+        float x[D / 16][8], m = 0.f;
 #pragma unroll
-        for (int s = 0; s < D / 8; ++s) {
-            f32x4 x{0.f, 0.f, 0.f, 0.f};
-            if (in) x = *reinterpret_cast<const f32x4*>(p + half * (D / 2) + s * 4);
+        for (int s = 0; s < D / 16; ++s) {
+            f32x4 a{0.f, 0.f, 0.f, 0.f}, b = a;
+            if (in) { a = *reinterpret_cast<const f32x4*>(p + s * 16 + half * 8); b = *reinterpret_cast<const f32x4*>(p + s * 16 + half * 8 + 4); }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) f[s * 4 + e] = x[e];
+            for (int e = 0; e < 4; ++e) { x[s][e] = a[e]; x[s][4 + e] = b[e]; m = fmaxf(m, fmaxf(fabsf(a[e]), fabsf(b[e]))); }
         }
+        m = fmaxf(m, __shfl_xor(m, 32));
+        r.back = pow2_over(m);
+        const float to = 1.0f / r.back;
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float v = x[s][e] * to;
+                const _Float16 h = (_Float16)v;
+                r.f[0][s][e] = h;
+                r.f[1][s][e] = (_Float16)(v - (float)h);
+            }
     } else {
 #pragma unroll
         for (int s = 0; s < D / 16; ++s) {
-            typename Op<T>::frag x;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = (T)0.f;
-            if (in) x = *reinterpret_cast<const typename Op<T>::frag*>(p + s * 16 + half * 8);
-            f[s] = x;
+            for (int e = 0; e < 8; ++e) r.f[0][s][e] = (T)0.f;
+            if (in) r.f[0][s] = *reinterpret_cast<const typename Held<T>::frag*>(p + s * 16 + half * 8);
         }
     }
 }
 
-// 32 x 32 accumulator rows (keys or queries) as B operands, in two terms for the 16-bit types: the product then has the precision of
-// fp32 probabilities and the result's own rounding is the only one that counts
-template <typename T> struct Split {
-    typename Op<T>::frag hi[2], lo[2];
-    __device__ __forceinline__ explicit Split(const f32x16& p) {
+// acc += (32 rows of an LDS tile) x (32 row vectors in registers), over d; SWAP: the LDS rows are the columns of the result
+template <typename T, int D, bool SWAP>
+__device__ __forceinline__ f32x16 mma_d(const typename Held<T>::E* tile, int r, int half, const RowFrags<T, D>& q, f32x16 acc) {
+    using S = Shape<T, D>;
+    using O = Op<typename Held<T>::E>;
+    using frag = typename Held<T>::frag;
+    auto mul = [&](frag a, frag b) { acc = SWAP ? O::mma(b, a, acc) : O::mma(a, b, acc); };
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float x = p[s * 8 + e];
-                const T h = (T)x;
-                hi[s][e] = h;
-                lo[s][e] = (T)(x - (float)h);
-            }
-    }
-};
-
-// acc (d x columns) += A^T (d x 32 rows) p (32 rows x columns): A in LDS, [row][d] for fp32 (pitch P) or [d][row] for 16-bit types (pitch PT)
-template <typename T>
-__device__ __forceinline__ f32x16 mma_rows(const T* a, int pitch, int lane, const f32x16& p, f32x16 acc) {
-    const int half = lane >> 5, m = lane & 31;
-    if constexpr (is_f32<T>::value) {
-#pragma unroll
-        for (int s = 0; s < 16; ++s) acc = Op<T>::mma(a[(8 * (s / 4) + 4 * half + (s & 3)) * pitch + m], p[s], acc);
-    } else {
-        typedef T v4 __attribute__((ext_vector_type(4)));
-        const Split<T> x(p);
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const v4 u = *reinterpret_cast<const v4*>(a + m * pitch + s * 16 + half * 4), w = *reinterpret_cast<const v4*>(a + m * pitch + s * 16 + half * 4 + 8);
-            typename Op<T>::frag f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) { f[e] = u[e]; f[4 + e] = w[e]; }
-            acc = Op<T>::mma(f, x.lo[s], acc);
-            acc = Op<T>::mma(f, x.hi[s], acc);
+    for (int s = 0; s < S::KS; ++s) {
+        const frag hi = *reinterpret_cast<const frag*>(tile + r * S::P + s * 16 + half * 8);
+        if constexpr (Held<T>::two) {
+            const frag lo = *reinterpret_cast<const frag*>(tile + S::kRowTile + r * S::P + s * 16 + half * 8);
+            mul(lo, q.f[0][s]);
+            mul(hi, q.f[1][s]);
         }
+        mul(hi, q.f[0][s]);
     }
     return acc;
 }
 
-// The backward's P and dS have no largest value to be relative to, and fp16 ends at 2^-24: a tile is brought to at most 1 by a power of two before it is
-// split, and its product brought back (gradients of a scaled or a small loss keep their precision).  bf16 and fp32 have the range.
-template <typename T> struct Ranged {
-    f32x16 p;
+// A 32 x 32 tile of P or dS as B operand in two terms: the product then has the precision of fp32 probabilities and the result's own rounding is the only one
+// that counts.  RANGE: the backward's tiles have no largest value to be relative to, and fp16 ends at 2^-24: they are brought to the top of its range by a power of two, and
+// the product brought back (gradients of a scaled or a small loss keep their precision); bf16 has the range.
+template <typename T, bool RANGE> struct Split {
+    using E = typename Held<T>::E;
+    typename Held<T>::frag hi[2], lo[2];
     float back = 1.0f;
-    __device__ __forceinline__ explicit Ranged(const f32x16& x) : p(x) {
-        if constexpr (std::is_same<T, _Float16>::value) {
+    __device__ __forceinline__ explicit Split(const f32x16& p) {
+        float to = 1.0f;
+        if constexpr (RANGE && Held<T>::narrow) {
             float m = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(x[i]));
+            for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(p[i]));
 #pragma unroll
             for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-            const int e = m > 1e-30f && m < INFINITY ? __builtin_amdgcn_frexp_expf(m) : 0;
-            back = ldexpf(1.0f, e);
-            const float to = ldexpf(1.0f, -e);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) p[i] *= to;
+            back = pow2_over(m);
+            to = 1.0f / back;
         }
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float x = RANGE && Held<T>::narrow ? p[s * 8 + e] * to : p[s * 8 + e];
+                const E h = (E)x;
+                hi[s][e] = h;
+                lo[s][e] = (E)(x - (float)h);
+            }
     }
 };
-template <typename T> __device__ __forceinline__ f32x16 mma_rows(const T* a, int pitch, int lane, const Ranged<T>& x, f32x16 acc) {
-    if constexpr (std::is_same<T, _Float16>::value) {
-        const f32x16 t = mma_rows<T>(a, pitch, lane, x.p, zero16());
+
+// acc (d x columns) += A^T (d x 32 rows) p (32 rows x columns): A in LDS as [d][row], its second term `term` elements behind
+template <typename T, bool RANGE>
+__device__ __forceinline__ f32x16 mma_rows(const typename Held<T>::E* a, int pitch, int term, int lane, const Split<T, RANGE>& x, f32x16 acc) {
+    using E = typename Held<T>::E;
+    using O = Op<E>;
+    using frag = typename Held<T>::frag;
+    typedef E v4 __attribute__((ext_vector_type(4)));
+    const int half = lane >> 5, m = lane & 31;
+    constexpr bool far = RANGE && Held<T>::narrow;
+    f32x16 t = far ? zero16() : acc;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        auto get = [&](const E* p) {
+            const v4 u = *reinterpret_cast<const v4*>(p + m * pitch + s * 16 + half * 4), w = *reinterpret_cast<const v4*>(p + m * pitch + s * 16 + half * 4 + 8);
+            frag f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { f[e] = u[e]; f[4 + e] = w[e]; }
+            return f;
+        };
+        const frag hi = get(a);
+        if constexpr (Held<T>::two) t = O::mma(get(a + term), x.hi[s], t);
+        t = O::mma(hi, x.lo[s], t);
+        t = O::mma(hi, x.hi[s], t);
+    }
+    if constexpr (far) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[i] += t[i] * x.back;
         return acc;
-    } else {
-        return mma_rows<T>(a, pitch, lane, x.p, acc);
     }
+    return t;
 }
 
 __device__ __forceinline__ unsigned long long seen_keys(const BsArgs& a, int b, int j) {       // visible keys of a block, same in every lane
@@ -909,7 +976,7 @@ __device__ __forceinline__ unsigned long long seen_keys(const BsArgs& a, int b, 
 struct Row { bool in; int t, slot, head; };
 __device__ __forceinline__ Row row_of(const BsArgs& a, const int32_t* list, int len, int h, int r) {
     Row x;
-    const int e = a.G == 1 ? r : r / a.G;
+    const int e = a.G == 1 ? r : (int)((unsigned)r / (unsigned)a.G);
     x.in = e < len;
     const int m = x.in ? list[e] : 0;
     x.t = m / kMaxPick;
@@ -918,14 +985,19 @@ __device__ __forceinline__ Row row_of(const BsArgs& a, const int32_t* list, int 
     return x;
 }
 
-constexpr int kItemRows = 512;               // rows (mentions x heads of the group) of a work item
+constexpr int kItemRows = 1024;              // rows (mentions x heads of the group) of a work item
 
 // ------------------------------------------------------------------------------------------------------------ attention, many queries
+// A mention's result is the attention over its block alone, in the tensor's type -- a convex combination of values like the output, so its rounding is half a step
+// at most and enters the output with the block's weight -- and (maximum, sum): half the bytes of fp32 partial sums, which bound this kernel and the join.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void bs_forward_kernel(BsArgs a) {
     using S = Shape<T, D>;
-    __shared__ __align__(16) T lk[S::kRowTile];
-    __shared__ __align__(16) T lv[S::F ? S::kRowTile : S::kTransTile];
+    using E = typename Held<T>::E;
+    constexpr int TERMS = Held<T>::terms;
+    __shared__ __align__(16) E lk[TERMS * S::kRowTile];
+    __shared__ __align__(16) E lv[TERMS * S::kTransTile];
+    __shared__ float red[2][4];
     const int bh = blockIdx.y, b = bh / a.KV, h = bh % a.KV;
     if ((int)blockIdx.x >= a.n_items[bh]) return;
     const int32_t* it = a.items + ((size_t)bh * a.max_items + blockIdx.x) * 2;
@@ -934,56 +1006,54 @@ __global__ __launch_bounds__(256) void bs_forward_kernel(BsArgs a) {
     const int len = st[1] - st[0];
     const int32_t* list = a.list + (size_t)bh * a.T * a.n + st[0];
     const unsigned long long seen = seen_keys(a, b, j);
-    load_block<T, D, true, false>(static_cast<const T*>(a.k) + b * a.kb + h * a.kh, a.kt, j * kKeys, a.Nk, seen, lk, nullptr);
-    if constexpr (S::F) load_block<T, D, true, false>(static_cast<const T*>(a.v) + b * a.vb + h * a.vh, a.vt, j * kKeys, a.Nk, seen, lv, nullptr);
-    else load_block<T, D, false, true>(static_cast<const T*>(a.v) + b * a.vb + h * a.vh, a.vt, j * kKeys, a.Nk, seen, nullptr, lv);
+    const float kf = load_block<T, D, true, false>(static_cast<const T*>(a.k) + b * a.kb + h * a.kh, a.kt, j * kKeys, seen, lk, nullptr, red[0]);
+    const float vf = load_block<T, D, false, true>(static_cast<const T*>(a.v) + b * a.vb + h * a.vh, a.vt, j * kKeys, seen, nullptr, lv, red[1]);
     __syncthreads();
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int last = min(first + kItemRows, len * a.G);
-    const float c2 = a.scale * kLog2e;
+    const float c2 = a.scale * kLog2e * kf;
     for (int r0 = first + wave * 32; r0 < last; r0 += 128) {
         const Row r = row_of(a, list, len, h, r0 + (lane & 31));
-        typename Op<T>::frag qf[S::KS];
+        RowFrags<T, D> qf;
         global_frags<T, D>(static_cast<const T*>(a.q) + b * a.qb + r.t * a.qt + r.head * a.qh, r.in, half, qf);
+        const float c = c2 * qf.back;
         f32x16 s[2];
         float m = -INFINITY;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
-            s[kt] = zero16();
-#pragma unroll
-            for (int ks = 0; ks < S::KS; ++ks) s[kt] = Op<T>::mma(row_frag<T, D>(lk, kt * 32 + (lane & 31), ks, half), qf[ks], s[kt]);
+            s[kt] = mma_d<T, D, false>(lk, kt * 32 + (lane & 31), half, qf, zero16());
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int key = kt * 32 + 8 * (i / 4) + 4 * half + (i & 3);
-                s[kt][i] = seen >> key & 1 ? s[kt][i] * c2 : -INFINITY;
+                s[kt][i] = seen >> key & 1 ? s[kt][i] * c : -INFINITY;
                 m = fmaxf(m, s[kt][i]);
             }
         }
         m = fmaxf(m, __shfl_xor(m, 32));
-        const float base = m == -INFINITY ? 0.f : m;
+        constexpr float kTop = Held<T>::narrow ? 15.f : 0.f;               // fp16 terms: from the top of their range as well
+        const float base = m == -INFINITY ? 0.f : m - kTop;
         float l = 0.f;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[kt][i] = exp2f(s[kt][i] - base);
+                s[kt][i] = __builtin_amdgcn_exp2f(s[kt][i] - base);
                 l += s[kt][i];
             }
         l += __shfl_xor(l, 32);
+        const float inv = l == 0.f ? 0.f : vf / l;
+        if constexpr (Held<T>::narrow) l *= 1.0f / 32768.f;
         const size_t at = (((size_t)b * a.T + r.t) * a.H + r.head) * a.n + r.slot;
+        const Split<T, false> p0(s[0]), p1(s[1]);
 #pragma unroll
         for (int dt = 0; dt < S::DT; ++dt) {
-            f32x16 o = zero16();
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-                if constexpr (S::F) o = mma_rows<T>(lv + kt * 32 * S::P + dt * 32, S::P, lane, s[kt], o);
-                else o = mma_rows<T>(lv + dt * 32 * S::PT + kt * 32, S::PT, lane, s[kt], o);
-            }
+            f32x16 o = mma_rows<T>(lv + dt * 32 * S::PT, S::PT, S::kTransTile, lane, p0, zero16());
+            o = mma_rows<T>(lv + dt * 32 * S::PT + 32, S::PT, S::kTransTile, lane, p1, o);
             if (r.in) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int d = dt * 32 + 8 * i + 4 * half;
-                    if (d < D) *reinterpret_cast<f32x4*>(a.part + at * D + d) = f32x4{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]};
+                    if (d < D) tok_store4(static_cast<T*>(a.part) + at * D + d, f32x4{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]} * inv);
                 }
             }
         }
@@ -995,7 +1065,7 @@ __global__ __launch_bounds__(256) void bs_forward_kernel(BsArgs a) {
 // one wave per mention, all heads of its group: a lane per key for the scores, D / 8 lanes per key for the values
 template <typename T, int D>
 __global__ __launch_bounds__(64) void bs_few_kernel(BsArgs a) {
-    __shared__ float lq[D];
+    __shared__ __align__(16) float lq[D];
     __shared__ float lp[kKeys];
     const int lane = threadIdx.x;
     const long long w = blockIdx.x;                      // (b, t, kv head, slot)
@@ -1025,7 +1095,7 @@ __global__ __launch_bounds__(64) void bs_few_kernel(BsArgs a) {
         float m = s;
 #pragma unroll
         for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-        const float p = exp2f(s - (m == -INFINITY ? 0.f : m));
+        const float p = __builtin_amdgcn_exp2f(s - (m == -INFINITY ? 0.f : m));
         float l = p;
 #pragma unroll
         for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o);
@@ -1045,10 +1115,11 @@ __global__ __launch_bounds__(64) void bs_few_kernel(BsArgs a) {
         for (int o = LPK; o < 64; o <<= 1)
 #pragma unroll
             for (int e = 0; e < 4; ++e) { o0[e] += __shfl_xor(o0[e], o); o1[e] += __shfl_xor(o1[e], o); }
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
         const size_t at = (((size_t)b * a.T + t) * a.H + h * a.G + g) * a.n + slot;
         if (lane < LPK) {
-            *reinterpret_cast<f32x4*>(a.part + at * D + sub * 8) = o0;
-            *reinterpret_cast<f32x4*>(a.part + at * D + sub * 8 + 4) = o1;
+            tok_store4(static_cast<T*>(a.part) + at * D + sub * 8, o0 * inv);
+            tok_store4(static_cast<T*>(a.part) + at * D + sub * 8 + 4, o1 * inv);
         }
         if (lane == 0) a.ml[at] = f32x2{m, l};
     }
@@ -1061,23 +1132,37 @@ __global__ __launch_bounds__(256) void bs_join_kernel(BsArgs a, long long rows) 
     const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / L;
     const int sub = threadIdx.x % L;
     if (r >= rows) return;
-    const int hq = (int)(r % a.H);
+    const unsigned hq = (unsigned)(r % a.H);
     const long long bt = r / a.H;
-    const int32_t* bl = a.blocks + (bt * a.KV + hq / a.G) * a.n;
+    const int32_t* bl = a.blocks + (bt * a.KV + hq / (unsigned)a.G) * a.n;
     const f32x2* ml = a.ml + r * a.n;
-    float m = -INFINITY;
-    for (int s = 0; s < a.n; ++s)
-        if (bl[s] >= 0 && bl[s] < a.NB) m = fmaxf(m, ml[s].x);
-    const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
+    const T* part = static_cast<const T*>(a.part) + r * a.n * D + sub * 4;
+    float m = -INFINITY, l = 0.f;
     f32x4 o{0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.n; ++s)
-        if (bl[s] >= 0 && bl[s] < a.NB) {
-            const float w = exp2f(ml[s].x - base);
-            l += ml[s].y * w;
-            o += *reinterpret_cast<const f32x4*>(a.part + (r * a.n + s) * D + sub * 4) * w;
+    for (int s0 = 0; s0 < a.n; s0 += 8) {                // eight places at a time, all their loads in flight
+        f32x2 x[8];
+        f32x4 y[8];
+        float mm = m;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int s = s0 + u, j = s < a.n ? bl[s] : -1;
+            const bool ok = j >= 0 && j < a.NB;          // other places were never written
+            x[u] = ok ? ml[s] : f32x2{-INFINITY, 0.f};
+            y[u] = ok ? tok_load4(part + (long long)s * D) : f32x4{0.f, 0.f, 0.f, 0.f};
+            mm = fmaxf(mm, x[u].x);
         }
-    const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : __builtin_nanf(""));
+        const float base = mm == -INFINITY ? 0.f : mm, f = __builtin_amdgcn_exp2f(m - base);
+        l *= f;
+        o *= f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float w = __builtin_amdgcn_exp2f(x[u].x - base) * x[u].y;
+            l += w;
+            o += y[u] * w;
+        }
+        m = mm;
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
     tok_store4(static_cast<T*>(a.out) + r * D + sub * 4, o * inv);
     if (a.lse && sub == 0) a.lse[r] = l == 0.f ? INFINITY : m + log2f(l);
 }
@@ -1100,18 +1185,23 @@ __global__ __launch_bounds__(256) void bs_delta_kernel(const T* __restrict__ out
 
 // One workgroup per work item, four waves of 32 rows.  P and dP are computed twice, as keys x queries for dQ (a lane keeps a query) and as queries x
 // keys for dK, dV (a lane keeps a key): two more products instead of a transpose through LDS.  DA: the part of d whose dK, dV, dQ this workgroup
-// keeps (blockIdx.z-th).
+// keeps (blockIdx.z-th).  The powers of two of fp32 operands: those of K and V are common to the block, those of a query's Q and dO go into its P and dS.
 template <typename T, int D, int DA>
-__global__ __launch_bounds__(256, 1) void bs_backward_kernel(BsArgs a) {
+__global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsArgs a) {
     using S = Shape<T, D>;
-    constexpr bool F = S::F;
+    using E = typename Held<T>::E;
+    constexpr bool two = Held<T>::two;
+    constexpr int TERMS = Held<T>::terms;
     constexpr int AT = (DA + 31) / 32;                                     // d tiles of this workgroup
-    constexpr int QP = F ? DA + 1 : 32 + 4;                                // per-wave tile of 32 rows: [row][d] fp32, [d][row] 16 bit
-    constexpr int kWaveTile = F ? 32 * QP + S::kOver : AT * 32 * QP;
-    __shared__ __align__(16) T lk[S::kRowTile], lv[S::kRowTile];
-    __shared__ __align__(16) T lkt[F ? 1 : S::kTransTile];
-    __shared__ __align__(16) T lq[4][kWaveTile], lo[4][kWaveTile];
-    __shared__ __align__(16) f32x2 lld[4][32];
+    constexpr int QP = 32 + 4, kWaveTile = AT * 32 * QP;                   // per-wave tile of 32 rows: [d][row], of one term
+    constexpr size_t kTiles = sizeof(E) * TERMS * (2 * S::kRowTile + S::kTransTile + 8 * kWaveTile);
+    __shared__ __align__(16) char smem[kTiles > 32768 ? kTiles : 32768];   // the last sums take 32 KB
+    E* lk = reinterpret_cast<E*>(smem);
+    E* lv = lk + TERMS * S::kRowTile;
+    E* lkt = lv + TERMS * S::kRowTile;
+    E* lqs = lkt + TERMS * S::kTransTile;
+    __shared__ __align__(16) f32x4 lld[4][32];
+    __shared__ float red4[2][4];
     const int bh = blockIdx.y, b = bh / a.KV, h = bh % a.KV, d0 = blockIdx.z * DA;
     if ((int)blockIdx.x >= a.n_items[bh]) return;
     const int32_t* it = a.items + ((size_t)bh * a.max_items + blockIdx.x) * 2;
@@ -1120,146 +1210,147 @@ __global__ __launch_bounds__(256, 1) void bs_backward_kernel(BsArgs a) {
     const int len = st[1] - st[0];
     const int32_t* list = a.list + (size_t)bh * a.T * a.n + st[0];
     const unsigned long long seen = seen_keys(a, b, j);
-    load_block<T, D, true, true>(static_cast<const T*>(a.k) + b * a.kb + h * a.kh, a.kt, j * kKeys, a.Nk, seen, lk, lkt);
-    load_block<T, D, true, false>(static_cast<const T*>(a.v) + b * a.vb + h * a.vh, a.vt, j * kKeys, a.Nk, seen, lv, nullptr);
+    const float kf = load_block<T, D, true, true>(static_cast<const T*>(a.k) + b * a.kb + h * a.kh, a.kt, j * kKeys, seen, lk, lkt, red4[0]);
+    const float vf = load_block<T, D, true, false>(static_cast<const T*>(a.v) + b * a.vb + h * a.vh, a.vt, j * kKeys, seen, lv, nullptr, red4[1]);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    if constexpr (!F && DA < 32) {                                         // channels behind D: zeros, once
-        for (int i = lane; i < (32 - DA) * QP; i += 64) lq[wave][DA * QP + i] = lo[wave][DA * QP + i] = (T)0.f;
+    E* lq = lqs + wave * 2 * TERMS * kWaveTile;
+    E* lo = lq + TERMS * kWaveTile;
+    if constexpr (DA < 32) {                                               // channels behind D: zeros, once
+        for (int i = lane; i < (32 - DA) * QP; i += 64)
+#pragma unroll
+            for (int k = 0; k < TERMS; ++k) lq[k * kWaveTile + DA * QP + i] = lo[k * kWaveTile + DA * QP + i] = (E)0.f;
     }
     __syncthreads();
     const int last = min(first + kItemRows, len * a.G);
-    const float c2 = a.scale * kLog2e;
+    const float c2 = a.scale * kLog2e * kf;
     f32x16 dk[AT][2], dv[AT][2];
 #pragma unroll
     for (int t = 0; t < AT; ++t) { dk[t][0] = zero16(); dk[t][1] = zero16(); dv[t][0] = zero16(); dv[t][1] = zero16(); }
     for (int r0 = first + wave * 32; r0 < last; r0 += 128) {
         const Row r = row_of(a, list, len, h, r0 + (lane & 31));
         const size_t qrow = ((size_t)b * a.T + r.t) * a.H + r.head;
-        typename Op<T>::frag qf[S::KS], of[S::KS];
+        RowFrags<T, D> qf, of;
         global_frags<T, D>(static_cast<const T*>(a.q) + b * a.qb + r.t * a.qt + r.head * a.qh, r.in, half, qf);
         global_frags<T, D>(static_cast<const T*>(a.dout) + qrow * D, r.in, half, of);
         const f32x2 ld = r.in ? a.ld[qrow] : f32x2{INFINITY, 0.f};         // rows that are not there: P = 0
-        if (half == 0) lld[wave][lane & 31] = ld;
-        if constexpr (F) {
+        if (half == 0) lld[wave][lane & 31] = f32x4{ld.x, ld.y, qf.back, of.back};
 #pragma unroll
-            for (int s = 0; s < S::KS; ++s) {
-                const int d = half * (D / 2) + s - d0;
+        for (int s = 0; s < S::KS; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int d = s * 16 + half * 8 + e - d0;
                 if (DA == D || (d >= 0 && d < DA)) {
-                    lq[wave][(lane & 31) * QP + d] = qf[s];
-                    lo[wave][(lane & 31) * QP + d] = of[s];
-                }
-            }
-        } else {
 #pragma unroll
-            for (int s = 0; s < S::KS; ++s)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int d = s * 16 + half * 8 + e - d0;
-                    if (DA == D || (d >= 0 && d < DA)) {
-                        lq[wave][d * QP + (lane & 31)] = qf[s][e];
-                        lo[wave][d * QP + (lane & 31)] = of[s][e];
+                    for (int k = 0; k < TERMS; ++k) {
+                        lq[k * kWaveTile + d * QP + (lane & 31)] = qf.f[k][s][e];
+                        lo[k * kWaveTile + d * QP + (lane & 31)] = of.f[k][s][e];
                     }
                 }
-        }
+            }
         __builtin_amdgcn_wave_barrier();
         f32x16 dq[AT];
 #pragma unroll
         for (int t = 0; t < AT; ++t) dq[t] = zero16();
+        const float ca = c2 * qf.back, va = vf * of.back;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
-            f32x16 s = zero16(), p = zero16();
             // keys x queries
-#pragma unroll
-            for (int ks = 0; ks < S::KS; ++ks) {
-                s = Op<T>::mma(row_frag<T, D>(lk, kt * 32 + (lane & 31), ks, half), qf[ks], s);
-                p = Op<T>::mma(row_frag<T, D>(lv, kt * 32 + (lane & 31), ks, half), of[ks], p);
-            }
+            f32x16 s = mma_d<T, D, false>(lk, kt * 32 + (lane & 31), half, qf, zero16()), p = mma_d<T, D, false>(lv, kt * 32 + (lane & 31), half, of, zero16());
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int key = kt * 32 + 8 * (i / 4) + 4 * half + (i & 3);
-                const float w = seen >> key & 1 ? exp2f(s[i] * c2 - ld.x) : 0.f;
-                p[i] = w * (p[i] - ld.y) * a.scale;
+                const float w = seen >> key & 1 ? __builtin_amdgcn_exp2f(s[i] * ca - ld.x) : 0.f;
+                p[i] = w * (p[i] * va - ld.y) * a.scale;
             }
-            const Ranged<T> ds(p);
+            {
+                const Split<T, true> ds(p);
 #pragma unroll
-            for (int t = 0; t < AT; ++t) {
-                if constexpr (F) dq[t] = mma_rows<T>(lk + kt * 32 * S::P + d0 + t * 32, S::P, lane, ds, dq[t]);
-                else dq[t] = mma_rows<T>(lkt + (d0 + t * 32) * S::PT + kt * 32, S::PT, lane, ds, dq[t]);
+                for (int t = 0; t < AT; ++t) dq[t] = mma_rows<T>(lkt + (d0 + t * 32) * S::PT + kt * 32, S::PT, S::kTransTile, lane, ds, dq[t]);
             }
+            __builtin_amdgcn_sched_barrier(0);                             // one part's registers at a time
             // queries x keys
-            s = zero16();
-            p = zero16();
-#pragma unroll
-            for (int ks = 0; ks < S::KS; ++ks) {
-                s = Op<T>::mma(qf[ks], row_frag<T, D>(lk, kt * 32 + (lane & 31), ks, half), s);
-                p = Op<T>::mma(of[ks], row_frag<T, D>(lv, kt * 32 + (lane & 31), ks, half), p);
-            }
+            s = mma_d<T, D, true>(lk, kt * 32 + (lane & 31), half, qf, zero16());
+            p = mma_d<T, D, true>(lv, kt * 32 + (lane & 31), half, of, zero16());
             const bool vis = seen >> (kt * 32 + (lane & 31)) & 1;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const f32x2 x = lld[wave][8 * (i / 4) + 4 * half + (i & 3)];
-                s[i] = vis ? exp2f(s[i] * c2 - x.x) : 0.f;
-                p[i] = s[i] * (p[i] - x.y) * a.scale;
+                const f32x4 x = lld[wave][8 * (i / 4) + 4 * half + (i & 3)];
+                if constexpr (two) {
+                    const float w = vis ? __builtin_amdgcn_exp2f(s[i] * (c2 * x.z) - x.x) : 0.f;
+                    p[i] = w * (p[i] * (vf * x.w) - x.y) * (a.scale * x.z);
+                    s[i] = w * x.w;
+                } else {
+                    s[i] = vis ? __builtin_amdgcn_exp2f(s[i] * c2 - x.x) : 0.f;
+                    p[i] = s[i] * (p[i] - x.y) * a.scale;
+                }
             }
-            const Ranged<T> rp(s), rs(p);
+            {
+                const Split<T, true> rp(s);
 #pragma unroll
-            for (int t = 0; t < AT; ++t) {
-                constexpr int step = F ? 32 : 32 * QP;
-                dv[t][kt] = mma_rows<T>(lo[wave] + t * step, QP, lane, rp, dv[t][kt]);
-                dk[t][kt] = mma_rows<T>(lq[wave] + t * step, QP, lane, rs, dk[t][kt]);
+                for (int t = 0; t < AT; ++t) dv[t][kt] = mma_rows<T>(lo + t * 32 * QP, QP, kWaveTile, lane, rp, dv[t][kt]);
             }
+            __builtin_amdgcn_sched_barrier(0);
+            {
+                const Split<T, true> rs(p);
+#pragma unroll
+                for (int t = 0; t < AT; ++t) dk[t][kt] = mma_rows<T>(lq + t * 32 * QP, QP, kWaveTile, lane, rs, dk[t][kt]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
         __builtin_amdgcn_wave_barrier();
         if (r.in) {
-            float* dst = a.part + (qrow * a.n + r.slot) * D + d0;
+            float* dst = static_cast<float*>(a.part) + (qrow * a.n + r.slot) * D + d0;
 #pragma unroll
             for (int t = 0; t < AT; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int d = t * 32 + 8 * i + 4 * half;
-                    if (d < DA) *reinterpret_cast<f32x4*>(dst + d) = f32x4{dq[t][4 * i], dq[t][4 * i + 1], dq[t][4 * i + 2], dq[t][4 * i + 3]};
+                    if (d < DA) *reinterpret_cast<f32x4*>(dst + d) = f32x4{dq[t][4 * i], dq[t][4 * i + 1], dq[t][4 * i + 2], dq[t][4 * i + 3]} * kf;
                 }
         }
     }
-    // the four waves' sums, in order, through LDS: 32 keys x 32 channels at a time
-    float* red = reinterpret_cast<float*>(&lq[0][0]);
-    static_assert(sizeof(T) * 4 * kWaveTile >= 4096, "one tile of 32 x 32 sums");
+    // the four waves' sums, in order, through LDS; a block with one work item is done here, others leave a slab
+    float* red = reinterpret_cast<float*>(smem);
+    const bool whole = len * a.G <= kItemRows;
     float* slab = a.slab + ((size_t)bh * a.max_items + blockIdx.x) * 2 * kKeys * D;
 #pragma unroll
     for (int w2 = 0; w2 < 2; ++w2)
 #pragma unroll
-        for (int t = 0; t < AT; ++t)
+        for (int t = 0; t < AT; ++t) {
+            __syncthreads();
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-                const f32x16 x = w2 ? dv[t][kt] : dk[t][kt];
-                f32x16 y = x;
-                for (int w = 1; w < 4; ++w) {
-                    __syncthreads();
-                    if (wave == w) {
+            for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) red[i * 64 + lane] = x[i];
-                    }
-                    __syncthreads();
-                    if (wave == 0) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) y[i] += red[i * 64 + lane];
-                    }
+                for (int i = 0; i < 16; i += 4) {
+                    const f32x16& x = w2 ? dv[t][kt] : dk[t][kt];
+                    *reinterpret_cast<f32x4*>(red + (((wave * 2 + kt) * 4 + i / 4) * 64 + lane) * 4) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
                 }
-                if (wave == 0) {
-                    const int key = kt * 32 + (lane & 31);
+            __syncthreads();
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int d = t * 32 + 8 * i + 4 * half;
-                        if (d < DA) *reinterpret_cast<f32x4*>(slab + ((size_t)w2 * kKeys + key) * D + d0 + d) = f32x4{y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]};
-                    }
+            for (int u = 0; u < 2; ++u) {
+                const int i = threadIdx.x + u * 256, ln = i & 63, i4 = i >> 6 & 3, kt = i >> 8;
+                f32x4 y = *reinterpret_cast<const f32x4*>(red + i * 4);
+#pragma unroll
+                for (int w = 1; w < 4; ++w) y += *reinterpret_cast<const f32x4*>(red + (w * 512 + i) * 4);
+                const int key = kt * 32 + (ln & 31), d = t * 32 + 8 * i4 + 4 * (ln >> 5), tok = j * kKeys + key;
+                if (d >= DA) continue;
+                if (whole) {
+                    T* dst = static_cast<T*>(w2 ? a.dv : a.dk);
+                    if (dst && tok < a.Nk) tok_store4(dst + (((size_t)b * a.Nk + tok) * a.KV + h) * D + d0 + d, y);
+                } else {
+                    *reinterpret_cast<f32x4*>(slab + ((size_t)w2 * kKeys + key) * D + d0 + d) = y;
                 }
             }
+        }
 }
 
-// dK, dV of a block: the slabs of its items, in order (none: zeros).  One workgroup per (block, sample, kv head).
+// dK, dV of the blocks that nobody named (zeros) or that took several work items: their slabs, in order.  One workgroup per (block, sample, kv head).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void bs_dkv_kernel(BsArgs a) {
     const int j = blockIdx.x, bh = blockIdx.y, b = bh / a.KV, h = bh % a.KV;
+    const int32_t* st = a.start + (size_t)bh * (a.NB + 1) + j;
+    const int rows = (st[1] - st[0]) * a.G;
+    if (rows > 0 && rows <= kItemRows) return;
     // items are in the order of the blocks: the first one of block j
     const int32_t* it = a.items + (size_t)bh * a.max_items * 2;
     const int total = a.n_items[bh];
@@ -1288,11 +1379,13 @@ __global__ __launch_bounds__(256) void bs_dq_kernel(BsArgs a, long long rows) {
     const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / L;
     const int sub = threadIdx.x % L;
     if (r >= rows) return;
-    const int hq = (int)(r % a.H);
-    const int32_t* bl = a.blocks + (r / a.H * a.KV + hq / a.G) * a.n;
+    const unsigned hq = (unsigned)(r % a.H);
+    const int32_t* bl = a.blocks + (r / a.H * a.KV + hq / (unsigned)a.G) * a.n;
+    const float* part = static_cast<const float*>(a.part) + r * a.n * D + sub * 4;
     f32x4 o{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
     for (int s = 0; s < a.n; ++s)
-        if (bl[s] >= 0 && bl[s] < a.NB) o += *reinterpret_cast<const f32x4*>(a.part + (r * a.n + s) * D + sub * 4);
+        if (bl[s] >= 0 && bl[s] < a.NB) o += *reinterpret_cast<const f32x4*>(part + (long long)s * D);
     tok_store4(static_cast<T*>(a.dq) + r * D + sub * 4, o);
 }
 
@@ -1319,7 +1412,7 @@ int bs_rows(const char* what, const void* p, const int64_t* s, int dtype) {
 }
 
 int bs_runs(int64_t bh, int64_t entries) {
-    int64_t r = 512 / bh;
+    int64_t r = 1024 / bh;
     const int64_t most = (entries + 255) / 256;
     if (r > most) r = most;
     return (int)(r < 1 ? 1 : r);
@@ -1466,7 +1559,7 @@ Work bs_work(int64_t B, int64_t T, int64_t Nk, int64_t H, int64_t KV, int64_t D,
     Work w{};
     const size_t rows = (size_t)(B * T * H);
     w.part = 0;
-    size_t at = up16(rows * n * D * 4);
+    size_t at = up16(rows * n * D * 4);      // (a 16-bit forward uses half of it)
     if (!backward) {
         w.ml = at;
         at += up16(rows * n * 8);
@@ -1518,7 +1611,7 @@ extern "C" int av2x_block_sparse_attention(const void* q, const void* k, const v
     BsArgs a = bs_args(q, k, v, mask, blocks, lists, strides, scale, batch, queries, keys, heads, kv_heads, n);
     const Work w = bs_work(batch, queries, keys, heads, kv_heads, dim, n, false);
     char* ws = static_cast<char*>(workspace);
-    a.part = reinterpret_cast<float*>(ws + w.part);
+    a.part = ws + w.part;
     a.ml = reinterpret_cast<f32x2*>(ws + w.ml);
     a.out = out;
     a.lse = lse;
@@ -1555,7 +1648,7 @@ extern "C" int av2x_block_sparse_attention_backward(const void* q, const void* k
     const Work w = bs_work(batch, queries, keys, heads, kv_heads, dim, n, true);
     char* ws = static_cast<char*>(workspace);
     f32x2* ld = reinterpret_cast<f32x2*>(ws + w.ld);
-    a.part = reinterpret_cast<float*>(ws + w.part);
+    a.part = ws + w.part;
     a.slab = reinterpret_cast<float*>(ws + w.slab);
     a.ld = ld;
     a.dout = dout;
@@ -1563,7 +1656,7 @@ extern "C" int av2x_block_sparse_attention_backward(const void* q, const void* k
     hipStream_t st = av2x::as_stream(stream);
     return bs_go(dtype, dim, [&](auto t, auto d) {
         using T = typename decltype(t)::type;
-        constexpr int D = decltype(d)::value, DA = D > 64 ? 64 : D;
+        constexpr int D = decltype(d)::value, DA = D <= 64 ? D : Held<T>::two ? 32 : 64;      // fp32 heads of 128: what fits LDS
         const long long rows = (long long)batch * queries * heads;
         const unsigned by_row = (unsigned)((rows * (D / 4) + 255) / 256);
         bs_delta_kernel<T, D><<<by_row, 256, 0, st>>>(static_cast<const T*>(out), static_cast<const T*>(dout), lse, ld, rows);

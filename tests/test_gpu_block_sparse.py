@@ -2,7 +2,8 @@
 
 Bounds and selections are exact (whole numbers).  Attention: a score is off by at most e = D 2^-24 sum |q k| scale (products added in fp32), a probability by
 2 e + 2^-21 of itself (numerator, denominator, exp2; 16-bit types hold it in two terms: 2^-16), a sum over keys by 40 x 2^-24 of the sum of sizes.  A 16-bit
-result adds half its step, and the backward reads that rounded output in sum dO O.  fp16 has no steps below 2^-24: a result is off by 2^-25 there, and a
+result adds half its step, the parts it is joined from (one a block, a convex combination: at most sum of p |v|) half a step each, and the backward reads that
+rounded output in sum dO O.  fp32 runs on two fp16 terms of values relative to the largest of a row or block: 2^-22 of those.  fp16 has no steps below 2^-24: a result is off by 2^-25 there, and a
 probability or dS, held relative to the largest of its tile (at most a factor of 2 above it), by 2^-24 of that largest one.
 """
 import math
@@ -107,7 +108,7 @@ def check(q, k, v, do, blocks, mask, dt, scale=None, grads=True):
         es = es.masked_fill(p == 0, 0.0).amax(-1, keepdim=True) * 2
         ep = es + 2.0 ** -21 + (2.0 ** -16 if dt != F32 else 0.0)
         po = torch.einsum("bthn,bnhd->bthd", p, vv.abs())
-        ob = po * (ep * 2 + 40 * U) + half * o.abs() + least + flat * p.amax(-1, keepdim=True) * (p > 0).double().matmul(torch.ones(n, d, dtype=torch.double)) * vv.abs().max()
+        ob = po * (ep * 2 + 40 * U + half) + half * o.abs() + least + flat * p.amax(-1, keepdim=True) * (p > 0).double().matmul(torch.ones(n, d, dtype=torch.double)) * vv.abs().max()
     far = ((got.detach().double().cpu() - o.detach()).abs() / ob).max()
     assert float(far) <= 1, f"out: {float(far):.2f} x the bound"
     if not grads:
