@@ -264,10 +264,11 @@ SIGNATURES = {
     "av2x_block_lists": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p]),
     "av2x_block_sparse_workspace_bytes": (c_uint64, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
     "av2x_block_sparse_attention": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32,
-                                              c_int32, c_int32, c_int32, c_int32, c_int32, c_float, c_void_p, c_void_p, c_void_p, c_void_p]),
+                                              c_int32, c_int32, c_int32, c_int32, c_int32, c_float, c_void_p, c_void_p, c_void_p, c_void_p,
+                                              c_void_p]),
     "av2x_block_sparse_attention_backward": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                                                       c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_float,
-                                                       c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+                                                       c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32,
+                                                       c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "av2x_postprocess_workspace_bytes": (c_uint64, [c_int32, c_int32, c_int32, c_int32]),
     "av2x_postprocess_devt": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p,
                                         c_void_p, c_float, c_float, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p,

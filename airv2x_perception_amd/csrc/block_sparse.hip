@@ -46,6 +46,7 @@ struct BsArgs {
     f32x2* ml;                               // (B, T, H, n) maximum (scaled, base 2) and sum
     void* out;                               // (B, T, H, D)
     float* lse;                              // (B, T, H) base 2, +inf: no key; may be null
+    void* rest;                              // (B, T, H, D) out's rounding errors, or null
     // backward
     const void* dout;
     const f32x2* ld;                         // (B, T, H) log-sum-exp (base 2), sum dO O
@@ -988,9 +989,11 @@ __device__ __forceinline__ Row row_of(const BsArgs& a, const int32_t* list, int 
 constexpr int kItemRows = 1024;              // rows (mentions x heads of the group) of a work item
 
 // ------------------------------------------------------------------------------------------------------------ attention, many queries
-// A mention's result is the attention over its block alone, in the tensor's type -- a convex combination of values like the output, so its rounding is half a step
-// at most and enters the output with the block's weight -- and (maximum, sum): half the bytes of fp32 partial sums, which bound this kernel and the join.
-template <typename T, int D>
+// A mention's result is the attention over its block alone and (maximum, sum).  PT: without gradients it is held in the tensor's type -- a convex combination of
+// values like the output, so its rounding is half a step at most and enters the output with the block's weight (measured: 1.4 times the error of the output's
+// own rounding) -- which halves the bytes that bound this kernel and the join (281600 queries x 8 blocks, bf16: join 94 -> 51 us).  With gradients it stays fp32:
+// the backward's sum dO O would carry that rounding into every dS of the query.
+template <typename T, int D, typename PT>
 __global__ __launch_bounds__(256) void bs_forward_kernel(BsArgs a) {
     using S = Shape<T, D>;
     using E = typename Held<T>::E;
@@ -1053,7 +1056,7 @@ __global__ __launch_bounds__(256) void bs_forward_kernel(BsArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int d = dt * 32 + 8 * i + 4 * half;
-                    if (d < D) tok_store4(static_cast<T*>(a.part) + at * D + d, f32x4{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]} * inv);
+                    if (d < D) tok_store4(static_cast<PT*>(a.part) + at * D + d, f32x4{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]} * inv);
                 }
             }
         }
@@ -1063,7 +1066,7 @@ __global__ __launch_bounds__(256) void bs_forward_kernel(BsArgs a) {
 
 // ------------------------------------------------------------------------------------------------------------ attention, few queries
 // one wave per mention, all heads of its group: a lane per key for the scores, D / 8 lanes per key for the values
-template <typename T, int D>
+template <typename T, int D, typename PT>
 __global__ __launch_bounds__(64) void bs_few_kernel(BsArgs a) {
     __shared__ __align__(16) float lq[D];
     __shared__ float lp[kKeys];
@@ -1118,15 +1121,15 @@ __global__ __launch_bounds__(64) void bs_few_kernel(BsArgs a) {
         const float inv = l == 0.f ? 0.f : 1.0f / l;
         const size_t at = (((size_t)b * a.T + t) * a.H + h * a.G + g) * a.n + slot;
         if (lane < LPK) {
-            tok_store4(static_cast<T*>(a.part) + at * D + sub * 8, o0 * inv);
-            tok_store4(static_cast<T*>(a.part) + at * D + sub * 8 + 4, o1 * inv);
+            tok_store4(static_cast<PT*>(a.part) + at * D + sub * 8, o0 * inv);
+            tok_store4(static_cast<PT*>(a.part) + at * D + sub * 8 + 4, o1 * inv);
         }
         if (lane == 0) a.ml[at] = f32x2{m, l};
     }
 }
 
-// the n places of a query joined: D / 4 lanes a (query, head)
-template <typename T, int D>
+// the n places of a query joined: D / 4 lanes a (query, head).  rest: what the output's rounding took away, for the backward's sum dO O
+template <typename T, int D, typename PT>
 __global__ __launch_bounds__(256) void bs_join_kernel(BsArgs a, long long rows) {
     constexpr int L = D / 4;
     const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / L;
@@ -1136,7 +1139,7 @@ __global__ __launch_bounds__(256) void bs_join_kernel(BsArgs a, long long rows) 
     const long long bt = r / a.H;
     const int32_t* bl = a.blocks + (bt * a.KV + hq / (unsigned)a.G) * a.n;
     const f32x2* ml = a.ml + r * a.n;
-    const T* part = static_cast<const T*>(a.part) + r * a.n * D + sub * 4;
+    const PT* part = static_cast<const PT*>(a.part) + r * a.n * D + sub * 4;
     float m = -INFINITY, l = 0.f;
     f32x4 o{0.f, 0.f, 0.f, 0.f};
     for (int s0 = 0; s0 < a.n; s0 += 8) {                // eight places at a time, all their loads in flight
@@ -1163,20 +1166,27 @@ __global__ __launch_bounds__(256) void bs_join_kernel(BsArgs a, long long rows) 
         m = mm;
     }
     const float inv = l == 0.f ? 0.f : 1.0f / l;
-    tok_store4(static_cast<T*>(a.out) + r * D + sub * 4, o * inv);
+    o *= inv;
+    tok_store4(static_cast<T*>(a.out) + r * D + sub * 4, o);
+    if (a.rest) {
+        typedef typename tok_vec<T>::v4 v4;
+        tok_store4(static_cast<T*>(a.rest) + r * D + sub * 4, o - __builtin_convertvector(__builtin_convertvector(o, v4), f32x4));
+    }
     if (a.lse && sub == 0) a.lse[r] = l == 0.f ? INFINITY : m + log2f(l);
 }
 
 // ------------------------------------------------------------------------------------------------------------ backward
 // (log-sum-exp, sum dO O) of every (query, head), next to each other: a mention reads both at once
 template <typename T, int D>
-__global__ __launch_bounds__(256) void bs_delta_kernel(const T* __restrict__ out, const T* __restrict__ dout, const float* __restrict__ lse, f32x2* __restrict__ ld,
+__global__ __launch_bounds__(256) void bs_delta_kernel(const T* __restrict__ out, const T* __restrict__ rest, const T* __restrict__ dout, const float* __restrict__ lse, f32x2* __restrict__ ld,
                                                        long long rows) {
     constexpr int L = D / 4;
     const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / L;
     const int sub = threadIdx.x % L;
     if (r >= rows) return;
-    const f32x4 p = tok_load4(out + r * D + sub * 4) * tok_load4(dout + r * D + sub * 4);
+    f32x4 o = tok_load4(out + r * D + sub * 4);
+    if (rest) o += tok_load4(rest + r * D + sub * 4);
+    const f32x4 p = o * tok_load4(dout + r * D + sub * 4);
     float s = (p.x + p.y) + (p.z + p.w);
 #pragma unroll
     for (int o = 1; o < L; o <<= 1) s += __shfl_xor(s, o);
@@ -1596,11 +1606,11 @@ extern "C" uint64_t av2x_block_sparse_workspace_bytes(int32_t batch, int32_t que
 
 extern "C" int av2x_block_sparse_attention(const void* q, const void* k, const void* v, const int64_t* strides, const uint8_t* mask, const int32_t* blocks,
                                            const void* lists, int32_t batch, int32_t queries, int32_t keys, int32_t heads, int32_t kv_heads, int32_t dim, int32_t n,
-                                           int32_t dtype, float scale, void* out, float* lse, void* workspace, av2x_stream_t stream) {
+                                           int32_t dtype, float scale, void* out, float* lse, void* rest, void* workspace, av2x_stream_t stream) {
     const char* what = "av2x_block_sparse_attention";
     if (int rc = bs_check(what, batch, queries, keys, heads, kv_heads, dim, n, dtype)) return rc;
     if (queries == 0) return 0;
-    if (!out || !blocks || !workspace || !tok_aligned(out, 16) || !tok_aligned(workspace, 16) || !tok_aligned(lists, 16)) return av2x::fail("%s: null or unaligned tensor", what);
+    if (!out || !blocks || !workspace || !tok_aligned(out, 16) || !tok_aligned(workspace, 16) || !tok_aligned(lists, 16) || !tok_aligned(rest, 16)) return av2x::fail("%s: null or unaligned tensor", what);
     if (keys > 0) {
         if (int rc = bs_rows(what, q, strides, dtype)) return rc;
         if (int rc = bs_rows(what, k, strides + 3, dtype)) return rc;
@@ -1615,23 +1625,30 @@ extern "C" int av2x_block_sparse_attention(const void* q, const void* k, const v
     a.ml = reinterpret_cast<f32x2*>(ws + w.ml);
     a.out = out;
     a.lse = lse;
+    a.rest = rest;
+    const bool wide = lse || dtype == kTokF32;
     hipStream_t st = av2x::as_stream(stream);
     return bs_go(dtype, dim, [&](auto t, auto d) {
         using T = typename decltype(t)::type;
         constexpr int D = decltype(d)::value;
         if (a.NB > 0) {
-            if (lists) bs_forward_kernel<T, D><<<dim3(a.max_items, batch * kv_heads), 256, 0, st>>>(a);
-            else bs_few_kernel<T, D><<<(unsigned)mentions, 64, 0, st>>>(a);
+            const dim3 items(a.max_items, batch * kv_heads);
+            if (lists && wide) bs_forward_kernel<T, D, float><<<items, 256, 0, st>>>(a);
+            else if (lists) bs_forward_kernel<T, D, T><<<items, 256, 0, st>>>(a);
+            else if (wide) bs_few_kernel<T, D, float><<<(unsigned)mentions, 64, 0, st>>>(a);
+            else bs_few_kernel<T, D, T><<<(unsigned)mentions, 64, 0, st>>>(a);
             if (int rc = av2x::check_launch(what)) return rc;
         }
         const long long rows = (long long)batch * queries * heads;
-        bs_join_kernel<T, D><<<(unsigned)((rows * (D / 4) + 255) / 256), 256, 0, st>>>(a, rows);
+        const unsigned by_row = (unsigned)((rows * (D / 4) + 255) / 256);
+        if (wide) bs_join_kernel<T, D, float><<<by_row, 256, 0, st>>>(a, rows);
+        else bs_join_kernel<T, D, T><<<by_row, 256, 0, st>>>(a, rows);
         return av2x::check_launch(what);
     });
 }
 
 extern "C" int av2x_block_sparse_attention_backward(const void* q, const void* k, const void* v, const int64_t* strides, const uint8_t* mask, const int32_t* blocks,
-                                                    const void* lists, const void* out, const float* lse, const void* dout, int32_t batch, int32_t queries, int32_t keys,
+                                                    const void* lists, const void* out, const void* rest, const float* lse, const void* dout, int32_t batch, int32_t queries, int32_t keys,
                                                     int32_t heads, int32_t kv_heads, int32_t dim, int32_t n, int32_t dtype, float scale, void* dq, void* dk, void* dv,
                                                     void* workspace, av2x_stream_t stream) {
     const char* what = "av2x_block_sparse_attention_backward";
@@ -1640,7 +1657,7 @@ extern "C" int av2x_block_sparse_attention_backward(const void* q, const void* k
     const void* ptrs[] = {blocks, lists, out, lse, dout, workspace, dq};
     for (const void* p : ptrs)
         if (!p || !tok_aligned(p, 16)) return av2x::fail("%s: null or unaligned tensor", what);
-    if (!tok_aligned(dk, 16) || !tok_aligned(dv, 16)) return av2x::fail("%s: unaligned tensor", what);
+    if (!tok_aligned(dk, 16) || !tok_aligned(dv, 16) || !tok_aligned(rest, 16)) return av2x::fail("%s: unaligned tensor", what);
     if (int rc = bs_rows(what, q, strides, dtype)) return rc;
     if (int rc = bs_rows(what, k, strides + 3, dtype)) return rc;
     if (int rc = bs_rows(what, v, strides + 6, dtype)) return rc;
@@ -1659,7 +1676,7 @@ extern "C" int av2x_block_sparse_attention_backward(const void* q, const void* k
         constexpr int D = decltype(d)::value, DA = D <= 64 ? D : Held<T>::two ? 32 : 64;      // fp32 heads of 128: what fits LDS
         const long long rows = (long long)batch * queries * heads;
         const unsigned by_row = (unsigned)((rows * (D / 4) + 255) / 256);
-        bs_delta_kernel<T, D><<<by_row, 256, 0, st>>>(static_cast<const T*>(out), static_cast<const T*>(dout), lse, ld, rows);
+        bs_delta_kernel<T, D><<<by_row, 256, 0, st>>>(static_cast<const T*>(out), static_cast<const T*>(rest), static_cast<const T*>(dout), lse, ld, rows);
         if (int rc = av2x::check_launch(what)) return rc;
         bs_backward_kernel<T, D, DA><<<dim3(a.max_items, batch * kv_heads, D / DA), 256, 0, st>>>(a);
         if (int rc = av2x::check_launch(what)) return rc;

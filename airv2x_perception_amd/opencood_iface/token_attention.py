@@ -337,25 +337,26 @@ def _attend(q, k, v, blocks, mask, scale, grads):
     n, kv, s = k.shape[1], k.shape[2], blocks.shape[3]
     out = torch.empty((b, t, h, d), dtype=q.dtype, device=q.device)
     lse = torch.empty((b, t, h), dtype=torch.float32, device=q.device) if grads else None
+    rest = torch.empty_like(out) if grads and q.dtype != torch.float32 else None
     lists = _launch_lists(r, blocks, n, h) if b * t * kv * s > FEW_MENTIONS else None
     ws = torch.empty(int(r.lib.av2x_block_sparse_workspace_bytes(b, t, n, h, kv, d, s, 0)), dtype=torch.uint8, device=q.device)
     _lib.check(r.lib.av2x_block_sparse_attention(_P(q), _P(k), _P(v), _strides9(q, k, v), _P(mask), _P(blocks), _P(lists), b, t, n, h, kv, d, s, _DTYPES[q.dtype],
-                                                 scale, _P(out), _P(lse), _P(ws), r.stream()), "av2x_block_sparse_attention")
-    return out, lse, lists
+                                                 scale, _P(out), _P(lse), _P(rest), _P(ws), r.stream()), "av2x_block_sparse_attention")
+    return out, lse, rest, lists
 
 
 class _BlockSparseAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, blocks, mask, scale):
-        out, lse, lists = _attend(q, k, v, blocks, mask, scale, True)
-        ctx.save_for_backward(q, k, v, blocks, mask, out, lse, lists)
+        out, lse, rest, lists = _attend(q, k, v, blocks, mask, scale, True)
+        ctx.save_for_backward(q, k, v, blocks, mask, out, rest, lse, lists)
         ctx.scale = scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, blocks, mask, out, lse, lists = ctx.saved_tensors
+        q, k, v, blocks, mask, out, rest, lse, lists = ctx.saved_tensors
         r = _runner(q.device)
         b, t, h, d = q.shape
         n, kv, s = k.shape[1], k.shape[2], blocks.shape[3]
@@ -365,7 +366,7 @@ class _BlockSparseAttention(torch.autograd.Function):
         new = lambda x: torch.empty(x.shape, dtype=x.dtype, device=x.device)
         dq, dk, dv = new(q), new(k) if need[1] else None, new(v) if need[2] else None
         ws = torch.empty(int(r.lib.av2x_block_sparse_workspace_bytes(b, t, n, h, kv, d, s, 1)), dtype=torch.uint8, device=q.device)
-        _lib.check(r.lib.av2x_block_sparse_attention_backward(_P(q), _P(k), _P(v), _strides9(q, k, v), _P(mask), _P(blocks), _P(lists), _P(out), _P(lse),
+        _lib.check(r.lib.av2x_block_sparse_attention_backward(_P(q), _P(k), _P(v), _strides9(q, k, v), _P(mask), _P(blocks), _P(lists), _P(out), _P(rest), _P(lse),
                                                               _P(A8._aligned(dout)), b, t, n, h, kv, d, s, _DTYPES[q.dtype], ctx.scale, _P(dq), _P(dk), _P(dv), _P(ws),
                                                               r.stream()), "av2x_block_sparse_attention_backward")
         return dq, dk, dv, None, None, None

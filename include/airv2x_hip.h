@@ -1011,8 +1011,8 @@ int av2x_act8_wgrad(const float* dy, const int8_t* q, const float* scale, const 
  *                     av2x_select_blocks_workspace_bytes (0: NULL).
  * av2x_block_lists    the mentions of every block, for the two calls below: av2x_block_lists_bytes bytes of device memory, kept by the caller
  * av2x_block_sparse_attention   out (batch, queries, heads, dim) = softmax(scale q k^T) v over the visible keys of a query's blocks (indices outside
- *                     0 .. NB - 1 are none; one that is named twice counts twice; no key at all: zeros), lse (batch, queries, heads) or NULL: log-sum-exp to
- *                     base 2.  lists NULL: one wave per mention (few queries).  strides: HOST {q, k, v} x {batch, token, head}; 16-byte rows.
+ *                     0 .. NB - 1 are none; one that is named twice counts twice; no key at all: zeros), lse (batch, queries, heads): log-sum-exp to base 2, rest (as out, or
+ *                     NULL): out's rounding errors; both for the backward, lse NULL: no backward, 16-bit results of the blocks.  lists NULL: one wave per mention (few queries).  strides: HOST {q, k, v} x {batch, token, head}; 16-byte rows.
  * av2x_block_sparse_attention_backward   dq (as out), dk, dv (as k, v but contiguous; NULL: not wanted).  Bit-reproducible.
  * workspace: av2x_block_sparse_workspace_bytes.
  * ------------------------------------------------------------------------------------ */
@@ -1027,9 +1027,9 @@ int av2x_block_lists(const int32_t* blocks, int32_t batch, int32_t queries, int3
 uint64_t av2x_block_sparse_workspace_bytes(int32_t batch, int32_t queries, int32_t keys, int32_t heads, int32_t kv_heads, int32_t dim, int32_t n, int32_t backward);
 int av2x_block_sparse_attention(const void* q, const void* k, const void* v, const int64_t* strides, const uint8_t* mask, const int32_t* blocks, const void* lists,
                                 int32_t batch, int32_t queries, int32_t keys, int32_t heads, int32_t kv_heads, int32_t dim, int32_t n, int32_t dtype, float scale,
-                                void* out, float* lse, void* workspace, av2x_stream_t stream);
+                                void* out, float* lse, void* rest, void* workspace, av2x_stream_t stream);
 int av2x_block_sparse_attention_backward(const void* q, const void* k, const void* v, const int64_t* strides, const uint8_t* mask, const int32_t* blocks,
-                                         const void* lists, const void* out, const float* lse, const void* dout, int32_t batch, int32_t queries, int32_t keys,
+                                         const void* lists, const void* out, const void* rest, const float* lse, const void* dout, int32_t batch, int32_t queries, int32_t keys,
                                          int32_t heads, int32_t kv_heads, int32_t dim, int32_t n, int32_t dtype, float scale, void* dq, void* dk, void* dv,
                                          void* workspace, av2x_stream_t stream);
 

@@ -2,8 +2,7 @@
 
 Bounds and selections are exact (whole numbers).  Attention: a score is off by at most e = D 2^-24 sum |q k| scale (products added in fp32), a probability by
 2 e + 2^-21 of itself (numerator, denominator, exp2; 16-bit types hold it in two terms: 2^-16), a sum over keys by 40 x 2^-24 of the sum of sizes.  A 16-bit
-result adds half its step, the parts it is joined from (one a block, a convex combination: at most sum of p |v|) half a step each, and the backward reads that
-rounded output in sum dO O.  fp32 runs on two fp16 terms of values relative to the largest of a row or block: 2^-22 of those.  fp16 has no steps below 2^-24: a result is off by 2^-25 there, and a
+result adds half its step, and without gradients the parts it is joined from (one a block, a convex combination: at most sum of p |v|) half a step each.  fp32 runs on two fp16 terms of values relative to the largest of a row or block: 2^-22 of those.  fp16 has no steps below 2^-24: a result is off by 2^-25 there, and a
 probability or dS, held relative to the largest of its tile (at most a factor of 2 above it), by 2^-24 of that largest one.
 """
 import math
@@ -108,7 +107,8 @@ def check(q, k, v, do, blocks, mask, dt, scale=None, grads=True):
         es = es.masked_fill(p == 0, 0.0).amax(-1, keepdim=True) * 2
         ep = es + 2.0 ** -21 + (2.0 ** -16 if dt != F32 else 0.0)
         po = torch.einsum("bthn,bnhd->bthd", p, vv.abs())
-        ob = po * (ep * 2 + 40 * U + half) + half * o.abs() + least + flat * p.amax(-1, keepdim=True) * (p > 0).double().matmul(torch.ones(n, d, dtype=torch.double)) * vv.abs().max()
+        exact = po * (ep * 2 + 40 * U)                # before any rounding to 16 bits
+        ob = exact + (0 if grads else half) * po + half * o.abs() + least + flat * p.amax(-1, keepdim=True) * (p > 0).double().matmul(torch.ones(n, d, dtype=torch.double)) * vv.abs().max()
     far = ((got.detach().double().cpu() - o.detach()).abs() / ob).max()
     assert float(far) <= 1, f"out: {float(far):.2f} x the bound"
     if not grads:
@@ -121,7 +121,8 @@ def check(q, k, v, do, blocks, mask, dt, scale=None, grads=True):
         dp = torch.einsum("bthd,bnhd->bthn", dO, vv)
         dpb = torch.einsum("bthd,bnhd->bthn", dO.abs(), vv.abs())
         delta = (dO * o).sum(-1, keepdim=True)
-        deltab = (dO.abs() * ob).sum(-1, keepdim=True) + (dO.abs() * o.abs()).sum(-1, keepdim=True) * 8 * U
+        # the output with its rounding error beside it: half a step of half a step is left
+        deltab = (dO.abs() * (exact + least + half * half * o.abs())).sum(-1, keepdim=True) + (dO.abs() * o.abs()).sum(-1, keepdim=True) * 8 * U
         ds = p * (dp - delta) * abs(sc)
         dsb = ds.abs() * 2 * ep + p * (dpb * d * U * 2 + deltab + (dp.abs() + delta.abs()) * 2 * U) * abs(sc) + ds.abs() * (2.0 ** -16 if dt != F32 else 0) + flat * ds.abs().max() * (p > 0)
         fold = lambda x: x.view(b, n, kv, g, d).sum(3)
@@ -212,6 +213,7 @@ def test_attention_few_queries(dt, b, t, n, h, kv, d, blocks, masked):
     chosen = A.select_blocks(q.cuda(), A.block_bounds(k.cuda(), None if mask is None else mask.cuda()), blocks).cpu()
     assert b * t * kv * blocks <= A.FEW_MENTIONS
     check(q, k, v, do, chosen, mask, dt)
+    check(q, k, v, do, chosen, mask, dt, grads=False)
 
 
 @pytest.mark.parametrize("dt", [F32, BF, HF])
@@ -223,6 +225,7 @@ def test_attention_many_queries(monkeypatch, dt, b, t, n, h, kv, d, blocks, mask
     q, k, v, do, mask = make(t + n, b, t, n, h, kv, d, dt, masked)
     chosen = A.select_blocks(q.cuda(), A.block_bounds(k.cuda(), None if mask is None else mask.cuda()), blocks).cpu()
     check(q, k, v, do, chosen, mask, dt)
+    check(q, k, v, do, chosen, mask, dt, grads=False)
 
 
 @pytest.mark.parametrize("few", [0, 1 << 30])
@@ -244,6 +247,7 @@ def test_any_choice_of_blocks(monkeypatch, few, dt):
         for j in blocks[i].unique():
             if 0 <= j < 7:
                 named[i, j] = True
+    check(q, k, v, do, blocks, mask, dt, scale=-0.3, grads=False)
     out = check(q, k, v, do, blocks, mask, dt, scale=-0.3)
     assert not out[0, 3:7].any()
     kk, vv = k.clone(), v.clone()

@@ -78,12 +78,12 @@ def test_c_abi_refusals_of_the_blocks():
     for kw, word in ((dict(n=0), "blocks"), (dict(n=65), "blocks"), (dict(h=3), "heads"), (dict(h=34, kv=1), "share"), (dict(h=16, kv=1, d=128), "share"), (dict(q=None), "null"),
                      (dict(ints=72), "16 bytes"), (dict(t=2 ** 26), "queries")):
         assert sel(**kw) != 0 and word in _err(), (kw, _err())
-    att = lambda q=64, k=64, t=4, blocks=64, lists=None, out=64, st=s9, ws=64: lib.av2x_block_sparse_attention(q, k, 64, st, None, blocks, lists, 1, t, 100, 2, 2, 32, 2, 0, 1.0, out, None, ws, None)
+    att = lambda q=64, k=64, t=4, blocks=64, lists=None, out=64, st=s9, ws=64: lib.av2x_block_sparse_attention(q, k, 64, st, None, blocks, lists, 1, t, 100, 2, 2, 32, 2, 0, 1.0, out, None, None, ws, None)
     for kw, word in ((dict(q=None), "null"), (dict(k=72), "aligned"), (dict(blocks=None), "null"), (dict(out=72), "unaligned"), (dict(ws=None), "null"), (dict(lists=72), "unaligned"),
                      (dict(st=(ctypes.c_int64 * 9)(*[1024, 66, 32] * 3)), "aligned")):
         assert att(**kw) != 0 and word in _err(), (kw, _err())
     assert att(t=0, q=None) == 0
-    back = lambda lists=64, t=4, n=100, dk=64: lib.av2x_block_sparse_attention_backward(64, 64, 64, s9, None, 64, lists, 64, 64, 64, 1, t, n, 2, 2, 32, 2, 0, 1.0, 64, dk, 64, 64, None)
+    back = lambda lists=64, t=4, n=100, dk=64: lib.av2x_block_sparse_attention_backward(64, 64, 64, s9, None, 64, lists, 64, None, 64, 64, 1, t, n, 2, 2, 32, 2, 0, 1.0, 64, dk, 64, 64, None)
     for kw, word in ((dict(lists=None), "null"), (dict(t=0), "no queries"), (dict(n=0), "no keys"), (dict(dk=72), "unaligned")):
         assert back(**kw) != 0 and word in _err(), (kw, _err())
     assert lib.av2x_block_lists(64, 1, 4, 100, 2, 2, 2, None, None) != 0 and "null" in _err()
@@ -98,3 +98,17 @@ def test_module_declares_its_parameters():
         "q_gamma": (32,), "k_gamma": (32,), "norm.weight": (256,), "norm.bias": (256,), "to_qkv.weight": (384, 256), "to_out.weight": (256, 256), "to_out.bias": (256,)}
     with pytest.raises(ValueError):
         A.BlockSparseAttention(256, 8, 32, kv_heads=3)
+
+
+def test_the_bindings_have_the_headers_types():
+    import os
+    import re
+    txt = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "airv2x_hip.h")).read()
+    txt = re.sub(r"/\*.*?\*/", "", txt, flags=re.S)
+    types = {"int32_t": ctypes.c_int32, "int64_t": ctypes.c_int64, "uint64_t": ctypes.c_uint64, "float": ctypes.c_float, "int": ctypes.c_int32, "av2x_stream_t": ctypes.c_void_p}
+    seen = 0
+    for res, name, args in re.findall(r"(\w+)\s+(av2x_(?:qk_|act8_|block_|select_)\w+)\s*\((.*?)\);", txt, re.S):
+        want = [ctypes.c_void_p if "*" in a else types[a.split()[0]] for a in args.split(",")]
+        assert _lib.SIGNATURES[name] == (types[res], want), name
+        seen += 1
+    assert seen >= 18
