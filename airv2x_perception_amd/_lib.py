@@ -249,12 +249,11 @@ SIGNATURES = {
     "av2x_act8_gelu": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p]),
     "av2x_act8_gelu_backward": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p]),
     "av2x_act8_layernorm": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_float, c_void_p]),
-    "av2x_act8_layernorm_backward_workspace_bytes": (c_uint64, [c_int32]),
-    "av2x_act8_layernorm_backward": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32,
-                                               c_void_p, c_void_p]),
+    "av2x_act8_layernorm_backward": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p]),
     "av2x_act8_wgrad_workspace_bytes": (c_uint64, [c_int64, c_int32, c_int32]),
-    "av2x_act8_wgrad": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int32, c_int32, c_void_p, c_void_p,
-                                  c_void_p, c_void_p]),
+    "av2x_act8_wgrad": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int32, c_int32, c_void_p,
+                                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "av2x_act8_gemm": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32, c_void_p]),
     "av2x_block_bounds": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p,
                                     c_void_p]),
     "av2x_select_blocks_workspace_bytes": (c_uint64, [c_int32, c_int32, c_int32, c_int32, c_int32]),

@@ -6,7 +6,7 @@
 //
 //   act8_pack / act8_unpack          x -> (q, s), (q, s) -> x8                                                              HBM-bound
 //   act8_layernorm                   y = (x - mean) rstd gamma + beta, (q, s) of x, (mean, rstd)   one pass over x          HBM-bound
-//   act8_layernorm_backward          u = (x8 - mean) rstd, a = g gamma: dx = rstd (a - mean(a) - u mean(a u)), dgamma, dbeta  HBM-bound
+//   act8_layernorm_backward          u = (x8 - mean) rstd, a = g gamma: dx = rstd (a - mean(a) - u mean(a u))               HBM-bound
 //   act8_gelu / act8_gelu_backward   h = gelu(z) and (q, s) of z; dz = dh gelu'(z8)                                          HBM-bound
 //   act8_wgrad                       dW = dY^T X over the rows, db = sum dY, X = x8 | u gamma + beta | gelu(x8)             matrix cores / HBM
 //
@@ -126,21 +126,17 @@ __global__ __launch_bounds__(256) void act8_layernorm_kernel(const float* __rest
     }
 }
 
-constexpr int kLnGroups = 1024;       // workgroups of the backward pass = rows of its dgamma / dbeta partials
-
+// dx alone: the gradients of gamma and beta come out of the weight gradient (act8_affine_kernel)
 template <int CK>
 __global__ __launch_bounds__(256) void act8_layernorm_backward_kernel(const unsigned* __restrict__ q, const float* __restrict__ s,
                                                                       const f32x2* __restrict__ stats, const float* __restrict__ gamma,
-                                                                      const float* __restrict__ dy, float* __restrict__ dx, float* __restrict__ partial,
-                                                                      long long rows, int c) {
-    __shared__ f32x4 red[2][4][64 * CK];
+                                                                      const float* dy, float* dx, long long rows, int c) {      // dx may be dy
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, groups = (c + kGroup - 1) / kGroup;
-    f32x4 gm[CK], dg[CK], db[CK];
+    f32x4 gm[CK];
 #pragma unroll
     for (int k = 0; k < CK; ++k) {
         const int ch = k * 256 + lane * 4;
         gm[k] = ch < c ? *reinterpret_cast<const f32x4*>(gamma + ch) : f32x4{0.f, 0.f, 0.f, 0.f};
-        dg[k] = db[k] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     for (long long row = (long long)blockIdx.x * 4 + wave; row < rows; row += (long long)gridDim.x * 4) {
         const f32x2 st = stats[row];
@@ -153,11 +149,8 @@ __global__ __launch_bounds__(256) void act8_layernorm_backward_kernel(const unsi
             if (ch < c) {
                 const size_t at = (size_t)row * c + ch;
                 u[k] = (unpack4(q[at / 4], s[row * groups + ch / kGroup]) - st.x) * st.y;
-                d[k] = *reinterpret_cast<const f32x4*>(dy + at);
+                d[k] = *reinterpret_cast<const f32x4*>(dy + at) * gm[k];
             }
-            dg[k] += d[k] * u[k];
-            db[k] += d[k];
-            d[k] *= gm[k];
             sa += (d[k].x + d[k].y) + (d[k].z + d[k].w);
             sb += (d[k].x * u[k].x + d[k].y * u[k].y) + (d[k].z * u[k].z + d[k].w * u[k].w);
         }
@@ -170,34 +163,6 @@ __global__ __launch_bounds__(256) void act8_layernorm_backward_kernel(const unsi
             if (ch < c) *reinterpret_cast<f32x4*>(dx + (size_t)row * c + ch) = (d[k] - ma - u[k] * mb) * st.y;
         }
     }
-#pragma unroll
-    for (int k = 0; k < CK; ++k) { red[0][wave][k * 64 + lane] = dg[k]; red[1][wave][k * 64 + lane] = db[k]; }
-    __syncthreads();
-    if (wave < 2) {
-#pragma unroll
-        for (int k = 0; k < CK; ++k) {
-            const int ch = k * 256 + lane * 4;
-            const f32x4 t = (red[wave][0][k * 64 + lane] + red[wave][1][k * 64 + lane]) + (red[wave][2][k * 64 + lane] + red[wave][3][k * 64 + lane]);
-            if (ch < c) *reinterpret_cast<f32x4*>(partial + ((size_t)wave * gridDim.x + blockIdx.x) * c + ch) = t;
-        }
-    }
-}
-
-// out[c] = sum over n rows of partial[which][row][c]: 32 channels x 8 rows a workgroup, a fixed order
-__global__ __launch_bounds__(256) void act8_colsum_kernel(const float* __restrict__ partial, int n, int c, float* out0, float* out1) {
-    __shared__ float red[8][33];
-    const int ch = blockIdx.x * 32 + (threadIdx.x & 31), r = threadIdx.x >> 5;
-    float t = 0.f;
-    if (ch < c)
-        for (int i = r; i < n; i += 8) t += partial[((size_t)blockIdx.y * n + i) * c + ch];
-    red[r][threadIdx.x & 31] = t;
-    __syncthreads();
-    if (r == 0 && ch < c) {
-        t = 0.f;
-        for (int i = 0; i < 8; ++i) t += red[i][threadIdx.x];
-        float* o = blockIdx.y ? out1 : out0;
-        if (o) o[ch] = t;
-    }
 }
 
 // ------------------------------------------------------------------------------------------------------------ weight gradient
@@ -205,6 +170,7 @@ __global__ __launch_bounds__(256) void act8_colsum_kernel(const float* __restric
 // slab; act8_wgrad_reduce_kernel adds the slabs in order.  The 64 x 128 pieces of dY and q are transposed on the way to LDS: a thread
 // loads eight rows of four columns and writes, per column, the eight rows as one 16-byte fragment of an MFMA operand.  A column's eight
 // 16-byte fragments are rotated by its index (swz) so that sixteen lanes reading neighbouring columns meet all 64 banks once.
+// The workgroups of one share of the rows have neighbouring numbers on one XCD: its L2 serves dY to all tiles of inputs and q to all tiles of outputs.
 enum { kPlain = 0, kNorm = 1, kGelu = 2 };
 constexpr int kRows = 64;
 
@@ -230,13 +196,16 @@ __device__ __forceinline__ void split3(const float (&v)[8], bf16x8& hi, bf16x8& 
 template <int KIND>
 __global__ __launch_bounds__(256, 2) void act8_wgrad_kernel(const float* __restrict__ dy, const unsigned* __restrict__ q, const float* __restrict__ s,
                                                          const f32x2* __restrict__ stats, float* __restrict__ slabs, float* __restrict__ extra,
-                                                         long long rows, int co, int ci, int tiles_o, int tiles_i, long long rows_per) {
+                                                         long long rows, int co, int ci, int tiles_o, int tiles_i, long long rows_per, int splits) {
     constexpr int XP = KIND == kGelu ? 3 : 1;                        // bf16 terms of X
     extern __shared__ __align__(16) char smem[];
     __bf16* la = reinterpret_cast<__bf16*>(smem);                    // [3][128][64]
     __bf16* lb = la + 3 * 128 * 64;                                  // [XP][128][64]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int tile = blockIdx.x % (tiles_o * tiles_i), split = blockIdx.x / (tiles_o * tiles_i);
+    // workgroups go round the eight XCDs: number x of XCD c takes tile x % tiles of share 8 (x / tiles) + c
+    const int tiles = tiles_o * tiles_i, xcd = blockIdx.x & 7, local = blockIdx.x >> 3;
+    const int tile = local % tiles, split = local / tiles * 8 + xcd;
+    if (split >= splits) return;
     const int o0 = tile / tiles_i * 128, g = tile % tiles_i, i0 = g * 128, groups = tiles_i;
     const long long r0 = split * rows_per, r1 = min(rows, r0 + rows_per);
     const int cg = tid & 31, rc = tid >> 5;                          // four columns, eight rows
@@ -366,17 +335,19 @@ __global__ __launch_bounds__(256, 2) void act8_wgrad_kernel(const float* __restr
     }
 }
 
-// dW of one output row and up to 256 inputs: four waves take every fourth slab each
+// dW of one output row and up to 256 inputs: four waves take every fourth slab each.  kNorm: the sum before LayerNorm's affine, sum dY u, is kept in `pre`
 template <int KIND>
 __global__ __launch_bounds__(256) void act8_wgrad_reduce_kernel(const float* __restrict__ slabs, const float* __restrict__ extra, int splits, int co, int ci,
                                                                 const float* __restrict__ gamma, const float* __restrict__ beta, float* __restrict__ dw,
-                                                                float* __restrict__ db) {
+                                                                float* __restrict__ db, float* __restrict__ pre) {
     __shared__ f32x4 red[4][64];
     __shared__ float rs[2][4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, o = blockIdx.y, i = blockIdx.x * 256 + lane * 4;
     f32x4 t{0.f, 0.f, 0.f, 0.f};
-    if (i < ci)
+    if (i < ci) {
+#pragma unroll 4
         for (int sp = wave; sp < splits; sp += 4) t += *reinterpret_cast<const f32x4*>(slabs + ((size_t)sp * co + o) * ci + i);
+    }
     red[wave][lane] = t;
     float e0 = 0.f, e1 = 0.f;
     for (int sp = threadIdx.x; sp < splits; sp += 256) {
@@ -389,12 +360,133 @@ __global__ __launch_bounds__(256) void act8_wgrad_reduce_kernel(const float* __r
     __syncthreads();
     if (wave == 0) {
         const float d = (rs[0][0] + rs[0][1]) + (rs[0][2] + rs[0][3]), u = (rs[1][0] + rs[1][1]) + (rs[1][2] + rs[1][3]);
-        if (i < ci && dw) {
+        if (i < ci) {
             t = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
-            if constexpr (KIND == kNorm) t = (t - u) * *reinterpret_cast<const f32x4*>(gamma + i) + *reinterpret_cast<const f32x4*>(beta + i) * d;
-            *reinterpret_cast<f32x4*>(dw + (size_t)o * ci + i) = t;
+            if constexpr (KIND == kNorm) {
+                t -= u;
+                if (pre) *reinterpret_cast<f32x4*>(pre + (size_t)o * ci + i) = t;
+                t = t * *reinterpret_cast<const f32x4*>(gamma + i) + *reinterpret_cast<const f32x4*>(beta + i) * d;
+            }
+            if (dw) *reinterpret_cast<f32x4*>(dw + (size_t)o * ci + i) = t;
         }
         if (blockIdx.x == 0 && lane == 0 && db) db[o] = d;
+    }
+}
+
+// The affine's gradients without another pass over the rows:  dgamma_i = sum_r (dY W)[r, i] u[r, i] = sum_o W[o, i] (sum_r dY[r, o] u[r, i]),
+// dbeta_i = sum_o W[o, i] db_o.  Also the more exact way: dY W itself is rounded row by row.  32 channels x 32 rows of outputs a workgroup.
+__global__ __launch_bounds__(1024) void act8_affine_kernel(const float* __restrict__ w, const float* __restrict__ pre, const float* __restrict__ db, int co, int ci,
+                                                           float* __restrict__ dgamma, float* __restrict__ dbeta) {
+    __shared__ float red[2][32][33];
+    const int c = threadIdx.x & 31, r = threadIdx.x >> 5, i = blockIdx.x * 32 + c;
+    float g = 0.f, b = 0.f;
+    if (i < ci) {
+#pragma unroll 4
+        for (int o = r; o < co; o += 32) {
+            const float x = w[(size_t)o * ci + i];
+            g += x * pre[(size_t)o * ci + i];
+            b += x * db[o];
+        }
+    }
+    red[0][r][c] = g;
+    red[1][r][c] = b;
+    __syncthreads();
+    if (r < 2 && i < ci) {
+        float t = 0.f;
+        for (int k = 0; k < 32; ++k) t += red[r][k][c];
+        float* out = r ? dbeta : dgamma;
+        if (out) out[i] = t;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------ products for few rows
+// Y (rows x n) = A (rows x k) B + bias + residual, all fp32, six products of three bf16 terms each (exact to 2^-24 as the framework's large GEMM), B read as the
+// parameter lies: B = W^T of W (n, k) (forward) or W of W (k, n) (data gradient).  For few rows: the framework's GEMM wants W packed and split first, four
+// launches and their host time where a step has new weights; tiles of 64 x 64 fill the chip sooner (2200 x 256 x 256: 20 us there).
+// TRANS: B is (k, n): a thread transposes eight rows of four columns on the way to LDS, as in act8_wgrad_kernel.
+constexpr int kSmallK = 32;
+template <bool TRANS>
+__global__ __launch_bounds__(256) void act8_gemm_kernel(const float* __restrict__ a, const float* __restrict__ w, const float* __restrict__ bias,
+                                                        const float* __restrict__ residual, float* __restrict__ y, int rows, int n, int k) {
+    constexpr int P = kSmallK + 8;                                   // row pitch: sixteen lanes meet all banks
+    __shared__ __align__(16) __bf16 la[2][3][64 * P], lb[2][3][64 * P];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+    const int r0 = blockIdx.x * 64, n0 = blockIdx.y * 64;
+    const int row = tid >> 2, kc = (tid & 3) * 8;                    // 64 rows x 4 pieces of eight k
+    const int tk = (tid >> 4) * 2, tn = (tid & 15) * 4;              // TRANS: two k x four n
+    const int ra = min(r0 + row, rows - 1), rb = min(n0 + row, n - 1);
+    f32x4 pa[2], pb[2];
+    auto fetch = [&](int k0) {
+        const float* p = a + (size_t)ra * k + k0 + kc;
+        pa[0] = *reinterpret_cast<const f32x4*>(p);
+        pa[1] = *reinterpret_cast<const f32x4*>(p + 4);
+        if constexpr (TRANS) {
+            const float* p2 = w + (size_t)(k0 + tk) * n + min(n0 + tn, n - 4);
+            pb[0] = *reinterpret_cast<const f32x4*>(p2);
+            pb[1] = *reinterpret_cast<const f32x4*>(p2 + n);
+        } else {
+            const float* p2 = w + (size_t)rb * k + k0 + kc;
+            pb[0] = *reinterpret_cast<const f32x4*>(p2);
+            pb[1] = *reinterpret_cast<const f32x4*>(p2 + 4);
+        }
+    };
+    auto stage = [&](int buf) {
+        float v[8];
+        bf16x8 t[3];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = pa[e >> 2][e & 3];
+        split3(v, t[0], t[1], t[2]);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(&la[buf][p][row * P + kc]) = t[p];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = TRANS ? pb[e & 1][e >> 1] : pb[e >> 2][e & 3];
+        split3(v, t[0], t[1], t[2]);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            if constexpr (TRANS) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) *reinterpret_cast<bf16x2*>(&lb[buf][p][(tn + e) * P + tk]) = bf16x2{t[p][2 * e], t[p][2 * e + 1]};
+            } else {
+                *reinterpret_cast<bf16x8*>(&lb[buf][p][row * P + kc]) = t[p];
+            }
+        }
+    };
+    f32x16 acc;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+    const int m = (wave >> 1) * 32 + (lane & 31), c = (wave & 1) * 32 + (lane & 31);
+    fetch(0);
+    int buf = 0;
+    for (int k0 = 0; k0 < k; k0 += kSmallK, buf ^= 1) {
+        stage(buf);
+        __syncthreads();                                             // the other buffer's readers are past it: one barrier a step
+        if (k0 + kSmallK < k) fetch(k0 + kSmallK);
+#pragma unroll
+        for (int s = 0; s < kSmallK / 16; ++s) {
+            bf16x8 A[3], B[3];
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+                A[p] = *reinterpret_cast<const bf16x8*>(&la[buf][p][m * P + s * 16 + half * 8]);
+                B[p] = *reinterpret_cast<const bf16x8*>(&lb[buf][p][c * P + s * 16 + half * 8]);
+            }
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[2], B[0], acc, 0, 0, 0);       // smallest first
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[2], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[1], B[1], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[1], B[0], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[1], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[0], acc, 0, 0, 0);
+        }
+    }
+    const int col = n0 + c;
+    if (col >= n) return;
+    const float bv = bias ? bias[col] : 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const int r = r0 + (wave >> 1) * 32 + 8 * (e / 4) + 4 * half + (e & 3);
+        if (r >= rows) continue;
+        float v = acc[e] + bv;
+        if (residual) v += residual[(size_t)r * n + col];
+        y[(size_t)r * n + col] = v;
     }
 }
 
@@ -418,8 +510,9 @@ constexpr int kMaxC = 1 << 20;
 struct WgradPlan { int tiles_o, tiles_i, splits; int64_t rows_per; };
 WgradPlan wgrad_plan(int64_t rows, int co, int ci) {
     WgradPlan p{(co + 127) / 128, (ci + 127) / 128, 1, kRows};
-    // two workgroups a CU; at least one step of rows each
+    // two workgroups a CU; at least one step of rows each; whole rounds of the XCDs
     int64_t want = 512 / ((int64_t)p.tiles_o * p.tiles_i);
+    if (want > 8) want = want / 8 * 8;
     const int64_t steps = (rows + kRows - 1) / kRows;
     if (want > steps) want = steps;
     if (want < 1) want = 1;
@@ -479,59 +572,75 @@ extern "C" int av2x_act8_layernorm(const float* x, const float* gamma, const flo
     return av2x::check_launch("av2x_act8_layernorm");
 }
 
-extern "C" uint64_t av2x_act8_layernorm_backward_workspace_bytes(int32_t c) { return (uint64_t)2 * kLnGroups * (c > 0 ? c : 0) * 4; }
-
-extern "C" int av2x_act8_layernorm_backward(const int8_t* q, const float* scale, const float* stats, const float* gamma, const float* dy, float* dx,
-                                            float* dgamma, float* dbeta, int64_t rows, int32_t c, void* workspace, av2x_stream_t stream) {
-    const void* p[] = {gamma, workspace, q, scale, stats, dy, dx};
-    if (int rc = act8_check("av2x_act8_layernorm_backward", p, rows ? 7 : 2, rows, c, 1024)) return rc;
-    const unsigned grid = (unsigned)((rows + 3) / 4 < 1 ? 1 : (rows + 3) / 4 < kLnGroups ? (rows + 3) / 4 : kLnGroups);
-    float* partial = static_cast<float*>(workspace);
+extern "C" int av2x_act8_layernorm_backward(const int8_t* q, const float* scale, const float* stats, const float* gamma, const float* dy, float* dx, int64_t rows,
+                                            int32_t c, av2x_stream_t stream) {
+    const void* p[] = {gamma, q, scale, stats, dy, dx};
+    if (rows == 0) return 0;
+    if (int rc = act8_check("av2x_act8_layernorm_backward", p, 6, rows, c, 1024)) return rc;
+    const unsigned grid = (unsigned)((rows + 3) / 4 < 8192 ? (rows + 3) / 4 : 8192);
     auto go = [&](auto ck) {
-        act8_layernorm_backward_kernel<decltype(ck)::value><<<grid, 256, 0, av2x::as_stream(stream)>>>((const unsigned*)q, scale, (const f32x2*)stats, gamma, dy, dx,
-                                                                                                  partial, rows, c);
+        act8_layernorm_backward_kernel<decltype(ck)::value><<<grid, 256, 0, av2x::as_stream(stream)>>>((const unsigned*)q, scale, (const f32x2*)stats, gamma, dy, dx, rows, c);
     };
     if (c <= 256) go(std::integral_constant<int, 1>{});
     else if (c <= 512) go(std::integral_constant<int, 2>{});
     else go(std::integral_constant<int, 4>{});
-    if (int rc = av2x::check_launch("av2x_act8_layernorm_backward")) return rc;
-    if (!dgamma && !dbeta) return 0;
-    act8_colsum_kernel<<<dim3((c + 31) / 32, 2), 256, 0, av2x::as_stream(stream)>>>(partial, (int)grid, c, dgamma, dbeta);
-    return av2x::check_launch("av2x_act8_layernorm_backward: sums");
+    return av2x::check_launch("av2x_act8_layernorm_backward");
 }
 
 extern "C" uint64_t av2x_act8_wgrad_workspace_bytes(int64_t rows, int32_t cout, int32_t cin) {
     if (rows < 0 || cout < 1 || cin < 1) return 0;
     const WgradPlan p = wgrad_plan(rows, cout, cin);
-    return (uint64_t)p.splits * ((uint64_t)cout * cin + 2ull * cout) * 4;
+    return ((uint64_t)(p.splits + 1) * cout * cin + (2ull * p.splits + 1) * cout) * 4;
 }
 
-extern "C" int av2x_act8_wgrad(const float* dy, const int8_t* q, const float* scale, const float* stats, const float* gamma, const float* beta, int32_t kind,
-                               int64_t rows, int32_t cout, int32_t cin, float* dw, float* db, void* workspace, av2x_stream_t stream) {
+extern "C" int av2x_act8_wgrad(const float* dy, const int8_t* q, const float* scale, const float* stats, const float* gamma, const float* beta, const float* weight,
+                               int32_t kind, int64_t rows, int32_t cout, int32_t cin, float* dw, float* db, float* dgamma, float* dbeta, void* workspace,
+                               av2x_stream_t stream) {
     const char* what = "av2x_act8_wgrad";
     const void* p[] = {workspace, dy, q, scale};
     if (kind < 0 || kind > 2) return av2x::fail("%s: kind %d", what, kind);
     if (int rc = act8_check(what, p, rows ? 4 : 1, rows, cin, 65536)) return rc;
-    if (cout < 4 || cout % 4 || cout > 65536) return av2x::fail("%s: %d outputs (a multiple of 4, at most 65536)", what, cout);
+    if (cout < 4 || cout % 4 || cout > 65532) return av2x::fail("%s: %d outputs (a multiple of 4, at most 65532)", what, cout);
     if (kind == kNorm && (!gamma || !beta || (rows && !stats))) return av2x::fail("%s: LayerNorm's statistics and parameters are needed", what);
+    if ((dgamma || dbeta) && (kind != kNorm || !weight)) return av2x::fail("%s: the affine's gradients need LayerNorm (kind 1) and the weight", what);
     if (!tok_aligned(gamma, 16) || !tok_aligned(beta, 16) || !tok_aligned(dw, 16) || !tok_aligned(stats, 8)) return av2x::fail("%s: tensors must be aligned to 16 bytes", what);
     const WgradPlan pl = wgrad_plan(rows, cout, cin);
     float* slabs = static_cast<float*>(workspace);
     float* extra = slabs + (size_t)pl.splits * cout * cin;
-    const int64_t grid = (int64_t)pl.tiles_o * pl.tiles_i * pl.splits;
+    float* pre = extra + (size_t)2 * pl.splits * cout;
+    float* dbw = db ? db : pre + (size_t)cout * cin;
+    const int64_t grid = (int64_t)pl.tiles_o * pl.tiles_i * ((pl.splits + 7) / 8 * 8);
     if (grid > 0x7fffffff) return av2x::fail("%s: too large", what);
+    const bool affine = dgamma || dbeta;
+    hipStream_t st = av2x::as_stream(stream);
     auto go = [&](auto kd) {
         constexpr int K = decltype(kd)::value;
         constexpr size_t lds = (size_t)(3 + (K == kGelu ? 3 : 1)) * 128 * 64 * 2;
         static av2x::LdsLimit lim;
         lim.ensure((const void*)act8_wgrad_kernel<K>, lds);
-        act8_wgrad_kernel<K><<<(unsigned)grid, 256, lds, av2x::as_stream(stream)>>>(dy, (const unsigned*)q, scale, (const f32x2*)stats, slabs, extra, rows, cout, cin,
-                                                                             pl.tiles_o, pl.tiles_i, pl.rows_per);
+        act8_wgrad_kernel<K><<<(unsigned)grid, 256, lds, st>>>(dy, (const unsigned*)q, scale, (const f32x2*)stats, slabs, extra, rows, cout, cin, pl.tiles_o, pl.tiles_i,
+                                                             pl.rows_per, pl.splits);
         if (int rc = av2x::check_launch(what)) return rc;
-        act8_wgrad_reduce_kernel<K><<<dim3((cin + 255) / 256, cout), 256, 0, av2x::as_stream(stream)>>>(slabs, extra, pl.splits, cout, cin, gamma, beta, dw, db);
-        return av2x::check_launch("av2x_act8_wgrad: sums");
+        act8_wgrad_reduce_kernel<K><<<dim3((cin + 255) / 256, cout), 256, 0, st>>>(slabs, extra, pl.splits, cout, cin, gamma, beta, dw, affine ? dbw : db, affine ? pre : nullptr);
+        if (int rc = av2x::check_launch("av2x_act8_wgrad: sums")) return rc;
+        if (!affine) return 0;
+        act8_affine_kernel<<<(cin + 31) / 32, 1024, 0, st>>>(weight, pre, dbw, cout, cin, dgamma, dbeta);
+        return av2x::check_launch("av2x_act8_wgrad: affine");
     };
     if (kind == kPlain) return go(std::integral_constant<int, kPlain>{});
     if (kind == kNorm) return go(std::integral_constant<int, kNorm>{});
     return go(std::integral_constant<int, kGelu>{});
+}
+
+extern "C" int av2x_act8_gemm(const float* a, const float* w, const float* bias, const float* residual, float* y, int64_t rows, int32_t n, int32_t k, int32_t w_is_kn,
+                              av2x_stream_t stream) {
+    const char* what = "av2x_act8_gemm";
+    const void* p[] = {a, w, y};
+    if (rows == 0) return 0;
+    if (int rc = act8_check(what, p, 3, rows, k, 65536)) return rc;
+    if (k % 32 || n < 4 || n % 4 || n > 65536 * 32 || rows > (1ll << 30)) return av2x::fail("%s: %lld x %d x %d (k a multiple of 32, n of 4)", what, (long long)rows, n, k);
+    const dim3 grid((unsigned)((rows + 63) / 64), (unsigned)((n + 63) / 64));
+    if (w_is_kn) act8_gemm_kernel<true><<<grid, 256, 0, av2x::as_stream(stream)>>>(a, w, bias, residual, y, (int)rows, n, k);
+    else act8_gemm_kernel<false><<<grid, 256, 0, av2x::as_stream(stream)>>>(a, w, bias, residual, y, (int)rows, n, k);
+    return av2x::check_launch(what);
 }

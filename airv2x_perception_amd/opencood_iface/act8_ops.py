@@ -11,7 +11,7 @@ derivative taken at x8 instead of x:
 
     linear        dW = dY^T x8                           dx = dY W
     norm_linear   u = (x8 - mean) rstd (the forward's statistics)   dW = dY^T (u gamma + beta)   a = (dY W) gamma
-                  dx = rstd (a - mean(a) - u mean(a u))  dgamma = sum (dY W) u    dbeta = sum dY W
+                  dx = rstd (a - mean(a) - u mean(a u))  dgamma = sum (dY W) u = sum_o W (dY^T u)    dbeta = sum dY W = sum_o W db
     gelu(_linear) dW = dY^T gelu(z8)                     dz = (dY W) gelu'(z8)
 
 A group with an infinity or a NaN has a NaN scale: the gradients show it, as they would without the 8 bits (GradScaler's check works).
@@ -30,6 +30,9 @@ from .autograd import _P, _runner
 
 GROUP = 128           # channels of one scale
 LN_EPS = 1e-5
+# Up to this many rows the products run on av2x_act8_gemm, which reads the weight as it lies; from there on on the framework's GEMM, whose weights are packed and
+# split into terms first
+SMALL_ROWS = 16384
 
 
 class Packed8(NamedTuple):
@@ -106,12 +109,15 @@ def unpack(p):
 
 # ------------------------------------------------------------------------------------------------ raw launches
 def _gemm(r, x, weight, bias, residual):
-    """x W^T (+ b) (+ residual) through the engine's launcher, rows as one image line."""
+    """x W^T (+ b) (+ residual): the engine's launcher with the rows as one image line, or for few rows a GEMM on the parameter as it lies."""
     from .engine import ConvLayer
     cout, cin = weight.shape
     rows = x.numel() // cin
     y = torch.empty(tuple(x.shape[:-1]) + (cout,), dtype=torch.float32, device=x.device)
     if rows == 0:
+        return y
+    if rows <= SMALL_ROWS and not T.AMP_STEP[0]:
+        _lib.check(r.lib.av2x_act8_gemm(_P(x), _P(weight), _P(bias), _P(residual), _P(y), rows, cout, cin, 0, r.stream()), "av2x_act8_gemm")
         return y
     wp, coutp, _, ent = T._packed(r, weight.detach().view(cout, cin, 1, 1), owner=weight)
     L = ConvLayer(wp, None, bias.detach() if bias is not None else T._zeros(cout, x.device), cin, cout, coutp, 1, 1, 0, 0)
@@ -129,17 +135,24 @@ def _dgrad(dy, weight):
     rows = dy.numel() // cout
     if rows == 0:
         return torch.empty(tuple(dy.shape[:-1]) + (cin,), dtype=torch.float32, device=dy.device)
+    if rows <= SMALL_ROWS and not T.AMP_STEP[0]:
+        r = _runner(dy.device)
+        dx = torch.empty(tuple(dy.shape[:-1]) + (cin,), dtype=torch.float32, device=dy.device)
+        _lib.check(r.lib.av2x_act8_gemm(_P(dy), _P(weight), None, None, _P(dx), rows, cin, cout, 1, r.stream()), "av2x_act8_gemm")
+        return dx
     w4 = weight.detach().view(cout, cin, 1, 1)
     return T.conv_dgrad(dy.view(1, 1, rows, cout), w4, 1, 0, (1, rows), owner=weight).view(tuple(dy.shape[:-1]) + (cin,))
 
 
-def _wgrad(r, kind, dy, q, s, cin, stats=None, gamma=None, beta=None, want_w=True, want_b=True):
+def _wgrad(r, kind, dy, q, s, cin, stats=None, gamma=None, beta=None, want_w=True, want_b=True, weight=None, dgamma=None, dbeta=None):
+    """(dW, db) and, for LayerNorm -> Linear, its affine's gradients into dgamma, dbeta."""
     cout = dy.shape[-1]
     rows = dy.numel() // cout
     dw = torch.empty((cout, cin), dtype=torch.float32, device=dy.device) if want_w else None
     db = torch.empty(cout, dtype=torch.float32, device=dy.device) if want_b else None
     ws = torch.empty(int(r.lib.av2x_act8_wgrad_workspace_bytes(rows, cout, cin)), dtype=torch.uint8, device=dy.device)
-    _lib.check(r.lib.av2x_act8_wgrad(_P(dy), _P(q), _P(s), _P(stats), _P(gamma), _P(beta), kind, rows, cout, cin, _P(dw), _P(db), _P(ws), r.stream()),
+    _lib.check(r.lib.av2x_act8_wgrad(_P(dy), _P(q), _P(s), _P(stats), _P(gamma), _P(beta), _P(weight), kind, rows, cout, cin, _P(dw), _P(db), _P(dgamma), _P(dbeta), _P(ws),
+                                     r.stream()),
                "av2x_act8_wgrad")
     return dw, db
 
@@ -212,20 +225,18 @@ class _NormLinear8(torch.autograd.Function):
         need = ctx.needs_input_grad
         rows, c = stats.shape[0], weight.shape[1]
         dx = dgamma = dbeta = dw = db = None
-        if need[0] or need[1] or need[2]:
-            with T.amp_scope(ctx.amp):
-                dn = _dgrad(dy, weight)
+        if need[1] or need[2] or need[3]:
+            # dgamma, dbeta need no pass over the rows: they are sums over the weight gradient's sum dY^T u and over db
             dgamma = torch.empty_like(gamma) if need[1] else None
             dbeta = torch.empty_like(beta) if need[2] else None
-            ws = torch.empty(int(r.lib.av2x_act8_layernorm_backward_workspace_bytes(c)), dtype=torch.uint8, device=dy.device)
-            # dx takes dn's place: a wave has read its row before it writes it
-            _lib.check(r.lib.av2x_act8_layernorm_backward(_P(q), _P(s), _P(stats), _P(gamma), _P(dn), _P(dn), _P(dgamma), _P(dbeta), rows, c, _P(ws), r.stream()),
-                       "av2x_act8_layernorm_backward")
-            dx = dn if need[0] else None
-        if need[3]:
-            dw, db = _wgrad(r, 1, dy, q, s, c, stats, gamma, beta, want_b=need[4])
+            dw, db = _wgrad(r, 1, dy, q, s, c, stats, gamma, beta, need[3], need[4], weight, dgamma, dbeta)
         elif need[4]:
             db = _bias_grad(r, dy)
+        if need[0]:
+            with T.amp_scope(ctx.amp):
+                dx = _dgrad(dy, weight)
+            # in place: a wave has read its row before it writes it
+            _lib.check(r.lib.av2x_act8_layernorm_backward(_P(q), _P(s), _P(stats), _P(gamma), _P(dx), _P(dx), rows, c, r.stream()), "av2x_act8_layernorm_backward")
         return dx, dgamma, dbeta, dw, db
 
 

@@ -981,9 +981,12 @@ int av2x_qk_norm_rotate_backward(const void* q, const void* k, const int64_t* st
  * av2x_act8_pack / unpack      x -> (q, scale); (q, scale) -> x8
  * av2x_act8_gelu               h = gelu(z) and (q, scale) of z;  av2x_act8_gelu_backward: dz = dh gelu'(z8)
  * av2x_act8_layernorm          y = LayerNorm(x), (q, scale) of x, stats (rows, 2) = (mean, rstd); c <= 1024
- * av2x_act8_layernorm_backward dx, dgamma, dbeta (NULL: not wanted) of LayerNorm at x8 with the forward's statistics
+ * av2x_act8_layernorm_backward dx (may be dy) of LayerNorm at x8 with the forward's statistics
  * av2x_act8_wgrad              dw (cout, cin) = dy^T X, db (cout) = sum dy over the rows (NULL: not wanted);  X = x8 (kind 0), (x8 - mean) rstd gamma +
- *                              beta (kind 1: stats, gamma, beta), gelu(x8) (kind 2).  Products exact to 2^-24, fp32 sums, bit-reproducible.
+ *                              beta (kind 1: stats, gamma, beta), gelu(x8) (kind 2).  Kind 1 also gives dgamma, dbeta of the LayerNorm in front of the
+ *                              Linear with this weight (cout, cin) (NULL: not wanted).  Products exact to 2^-24, fp32 sums, bit-reproducible.
+ * av2x_act8_gemm               y (rows, n) = a (rows, k) B (+ bias) (+ residual) for few rows, products exact to 2^-24; w as it lies: (n, k), B = w^T, or
+ *                              (w_is_kn) (k, n), B = w.  k % 32 == 0, n % 4 == 0.
  * ------------------------------------------------------------------------------------ */
 int av2x_act8_pack(const float* x, int8_t* q, float* scale, int64_t rows, int32_t c, av2x_stream_t stream);
 int av2x_act8_unpack(const int8_t* q, const float* scale, float* out, int64_t rows, int32_t c, av2x_stream_t stream);
@@ -991,12 +994,13 @@ int av2x_act8_gelu(const float* z, float* h, int8_t* q, float* scale, int64_t ro
 int av2x_act8_gelu_backward(const int8_t* q, const float* scale, const float* dh, float* dz, int64_t rows, int32_t c, av2x_stream_t stream);
 int av2x_act8_layernorm(const float* x, const float* gamma, const float* beta, float* y, int8_t* q, float* scale, float* stats, int64_t rows, int32_t c,
                         float eps, av2x_stream_t stream);
-uint64_t av2x_act8_layernorm_backward_workspace_bytes(int32_t c);
-int av2x_act8_layernorm_backward(const int8_t* q, const float* scale, const float* stats, const float* gamma, const float* dy, float* dx, float* dgamma,
-                                 float* dbeta, int64_t rows, int32_t c, void* workspace, av2x_stream_t stream);
+int av2x_act8_layernorm_backward(const int8_t* q, const float* scale, const float* stats, const float* gamma, const float* dy, float* dx, int64_t rows, int32_t c,
+                                 av2x_stream_t stream);
 uint64_t av2x_act8_wgrad_workspace_bytes(int64_t rows, int32_t cout, int32_t cin);
-int av2x_act8_wgrad(const float* dy, const int8_t* q, const float* scale, const float* stats, const float* gamma, const float* beta, int32_t kind,
-                    int64_t rows, int32_t cout, int32_t cin, float* dw, float* db, void* workspace, av2x_stream_t stream);
+int av2x_act8_wgrad(const float* dy, const int8_t* q, const float* scale, const float* stats, const float* gamma, const float* beta, const float* weight, int32_t kind,
+                    int64_t rows, int32_t cout, int32_t cin, float* dw, float* db, float* dgamma, float* dbeta, void* workspace, av2x_stream_t stream);
+int av2x_act8_gemm(const float* a, const float* w, const float* bias, const float* residual, float* y, int64_t rows, int32_t n, int32_t k, int32_t w_is_kn,
+                   av2x_stream_t stream);
 
 /* ------------------------------------------------------------------------------------
  * Attention over blocks of 64 keys that an integer score selects for each query.

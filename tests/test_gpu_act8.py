@@ -63,8 +63,10 @@ def test_groups_with_infinities_and_nans_are_marked():
 
 @pytest.mark.parametrize("rows,ci,co", [(1, 64, 32), (63, 256, 256), (65, 96, 100), (2200, 256, 256), (777, 320, 68), (129, 512, 4), (1500, 36, 132)])
 @pytest.mark.parametrize("kind", ["linear", "norm_linear", "gelu_linear"])
-def test_forward_and_gradients(kind, rows, ci, co):
+@pytest.mark.parametrize("small", [1 << 30, 0])
+def test_forward_and_gradients(monkeypatch, small, kind, rows, ci, co):
     from airv2x_perception_amd.opencood_iface import act8_ops as A
+    monkeypatch.setattr(A, "SMALL_ROWS", small)                       # both GEMMs
     x, w, b, res, dy, gamma, beta = data(rows + ci, rows, ci, co)
     q, s = held(x)
     x8 = (q.double() * s.double().repeat_interleave(128, 1)[:, :ci])
@@ -125,8 +127,11 @@ def test_forward_and_gradients(kind, rows, ci, co):
         b1 = ab.mean(1, keepdim=True) + a.abs().mean(1, keepdim=True) * 16 * U
         b2 = (ab * u.abs() + a.abs() * ub).mean(1, keepdim=True) + (a * u).abs().mean(1, keepdim=True) * 16 * U
         near(grads[0], dx, (ab + b1 + u.abs() * b2 + ub * m2.abs()) / sd + (a.abs() + m1.abs() + (u * m2).abs()) / sd * 24 * U + 1e-12, "dx")
-        near(grads[3], (src * u).sum(0), (srcb * u.abs() + src.abs() * ub).sum(0) + (src * u).abs().sum(0) * 40 * U + 1e-12, "dgamma")
-        near(grads[4], src.sum(0), srcb.sum(0) + src.abs().sum(0) * 40 * U + 1e-12, "dbeta")
+        # sums over the outputs of W times dY^T u (bounds as dW's, before the affine) and times db
+        pre = D(dy).t() @ u
+        preb = D(dy).abs().t() @ ((u.abs() + 2 * (mean / sd).abs()) * 60 * U + ub)
+        near(grads[3], (src * u).sum(0), (D(w).abs() * (preb + pre.abs() * 40 * U)).sum(0) + 1e-12, "dgamma")
+        near(grads[4], src.sum(0), (D(w).abs() * ((D(dy).abs().sum(0) + D(dy).sum(0).abs()) * 40 * U)[:, None]).sum(0) + 1e-12, "dbeta")
     if kind != "norm_linear":
         assert torch.equal(grads[3].cpu(), dy)
     # the same call again: the same bits

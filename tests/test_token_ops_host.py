@@ -57,13 +57,17 @@ def test_c_abi_refusals_of_the_8_bit_layers():
     assert lib.av2x_act8_pack(64, 64, 64, -1, 64, None) != 0 and "rows" in _err()
     assert lib.av2x_act8_pack(None, None, None, 0, 64, None) == 0
     assert lib.av2x_act8_layernorm(64, 64, 64, 64, 64, 64, 64, 4, 1028, 1e-5, None) != 0 and "1024" in _err()
-    wg = lambda kind=0, rows=4, co=8, ci=64, stats=64, gamma=64, dw=64: lib.av2x_act8_wgrad(64, 64, 64, stats, gamma, 64, kind, rows, co, ci, dw, 64, 64, None)
+    wg = lambda kind=0, rows=4, co=8, ci=64, stats=64, gamma=64, dw=64, dg=None, w=None: lib.av2x_act8_wgrad(64, 64, 64, stats, gamma, 64, w, kind, rows, co, ci, dw, 64, dg, None, 64, None)
     for kw, word in ((dict(kind=3), "kind"), (dict(co=6), "outputs"), (dict(ci=2), "channels"), (dict(kind=1, stats=None), "statistics"), (dict(kind=1, gamma=None), "statistics"),
-                     (dict(dw=8), "aligned")):
+                     (dict(dw=8), "aligned"), (dict(dg=64, w=64), "LayerNorm"), (dict(kind=1, dg=64), "weight")):
         assert wg(**kw) != 0 and word in _err(), (kw, _err())
     # slabs for every split of the rows, and two sums an output
-    assert lib.av2x_act8_wgrad_workspace_bytes(1, 8, 64) == (8 * 64 + 16) * 4
-    assert lib.av2x_act8_wgrad_workspace_bytes(10 ** 6, 256, 256) <= 512 * (256 * 256 + 512) * 4
+    assert lib.av2x_act8_wgrad_workspace_bytes(1, 8, 64) == (2 * 8 * 64 + 3 * 8) * 4
+    assert lib.av2x_act8_wgrad_workspace_bytes(10 ** 6, 256, 256) <= 513 * (256 * 256 + 512) * 4
+    gemm = lambda a=64, rows=4, n=64, k=64: lib.av2x_act8_gemm(a, 64, None, None, 64, rows, n, k, 0, None)
+    for kw, word in ((dict(a=None), "null"), (dict(a=72), "aligned"), (dict(k=48), "multiple of 32"), (dict(n=6), "of 4"), (dict(rows=-1), "rows")):
+        assert gemm(**kw) != 0 and word in _err(), (kw, _err())
+    assert gemm(rows=0, a=None) == 0
 
 
 def test_c_abi_refusals_of_the_blocks():
