@@ -25,9 +25,31 @@ constexpr float kTiny = 1e-30f;
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
-__device__ __forceinline__ float gelu8_f(float v) { return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f)); }
-__device__ __forceinline__ float gelu8_df(float v) {
-    return 0.5f * (1.0f + erff(v * 0.70710678118654752f)) + v * 0.3989422804014327f * expf(-0.5f * v * v);
+// GELU from the normal tail:  Phi(-|z|) = exp(-z^2 / 2) t Q(t),  t = 1 / (1 + 0.3 |z|)  (the form of Abramowitz & Stegun 7.1.26; Q of degree 7 fitted here to
+// 5e-8 of the tail, 4e-7 with fp32 arithmetic), so gelu(z) = z - z Phi(-z) or z Phi(z) keeps its relative precision for negative z, and the derivative
+// shares the exponential.  16 instructions where erff and expf take about 90; the weight gradient evaluates it once per element and output tile.
+__device__ __forceinline__ float normal_tail(float a, float& e) {      // a = |z|; e = exp(-z^2 / 2)
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3f, a, 1.0f));
+    float q = 0.037535473704338074f;
+    q = fmaf(q, t, -0.16501864790916443f);
+    q = fmaf(q, t, 0.21996943652629852f);
+    q = fmaf(q, t, -0.06640082597732544f);
+    q = fmaf(q, t, 0.13541917502880096f);
+    q = fmaf(q, t, 0.09778428077697754f);
+    q = fmaf(q, t, 0.12110564112663269f);
+    q = fmaf(q, t, 0.11960549652576447f);
+    e = __builtin_amdgcn_exp2f(-0.7213475204444817f * a * a);
+    return q * t * e;
+}
+__device__ __forceinline__ float gelu8_f(float z) {
+    float e;
+    const float c = normal_tail(fabsf(z), e);
+    return z < 0.f ? z * c : c == 0.f ? z : fmaf(-z, c, z);           // c == 0: infinity stays infinity
+}
+__device__ __forceinline__ float gelu8_df(float z) {
+    float e;
+    const float c = normal_tail(fabsf(z), e);
+    return fmaf(z * 0.3989422804014327f, e, z < 0.f ? c : 1.0f - c);
 }
 
 // the 32 lanes of a group agree on its scale and quantise their four channels each
@@ -166,19 +188,19 @@ __global__ __launch_bounds__(256) void act8_layernorm_backward_kernel(const unsi
 }
 
 // ------------------------------------------------------------------------------------------------------------ weight gradient
-// Tile 128 outputs x 128 inputs (one scale group) x 64 rows, four waves of 64 x 64; a workgroup walks its share of the rows and writes a
-// slab; act8_wgrad_reduce_kernel adds the slabs in order.  The 64 x 128 pieces of dY and q are transposed on the way to LDS: a thread
-// loads eight rows of four columns and writes, per column, the eight rows as one 16-byte fragment of an MFMA operand.  A column's eight
-// 16-byte fragments are rotated by its index (swz) so that sixteen lanes reading neighbouring columns meet all 64 banks once.
+// Tile 128 outputs x 128 inputs (one scale group) x 32 rows, four waves of 64 x 64, two workgroups a CU; a workgroup walks its share of the rows and writes a slab;
+// act8_wgrad_reduce_kernel adds the slabs in order.  The pieces of dY and q are transposed on the way to LDS: a thread loads four rows of four columns and
+// writes, per column, its rows as half a fragment of an MFMA operand.  dY, q and the rows' scales of the next step are on their way during the products.
 // The workgroups of one share of the rows have neighbouring numbers on one XCD: its L2 serves dY to all tiles of inputs and q to all tiles of outputs.
 enum { kPlain = 0, kNorm = 1, kGelu = 2 };
-constexpr int kRows = 64;
+// Element offset of eight rows of a column, 32 rows a column.  Pitch 80 bytes: sixteen neighbouring columns (readers) start in sixteen different 16-byte slots of the
+// banks; every fourth column (writers) meets only four, so the fragment within a column turns with col / 16.
+constexpr int kPitch = 40;
+__device__ __forceinline__ int swz(int col, int chunk) { return col * kPitch + ((chunk ^ (col >> 4)) & 3) * 8; }
 
-__device__ __forceinline__ int swz(int col, int chunk) { return col * 64 + ((chunk ^ (col >> 1)) & 7) * 8; }      // element offset, 64 rows a column
-
-__device__ __forceinline__ void split3(const float (&v)[8], bf16x8& hi, bf16x8& mid, bf16x8& lo) {
+template <int N, typename V> __device__ __forceinline__ void split3(const float (&v)[N], V& hi, V& mid, V& lo) {
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
+    for (int i = 0; i < N; i += 2) {
         f32x2 a{v[i], v[i + 1]};
         const bf16x2 h = __builtin_convertvector(a, bf16x2);
         const f32x2 hf = __builtin_convertvector(h, f32x2);
@@ -198,9 +220,13 @@ __global__ __launch_bounds__(256, 2) void act8_wgrad_kernel(const float* __restr
                                                          const f32x2* __restrict__ stats, float* __restrict__ slabs, float* __restrict__ extra,
                                                          long long rows, int co, int ci, int tiles_o, int tiles_i, long long rows_per, int splits) {
     constexpr int XP = KIND == kGelu ? 3 : 1;                        // bf16 terms of X
+    constexpr int R = 32, RT = R / 8;                               // rows of a step, of a thread
+    constexpr int PLANE = 128 * kPitch;
+    typedef __bf16 bfv __attribute__((ext_vector_type(RT)));
     extern __shared__ __align__(16) char smem[];
-    __bf16* la = reinterpret_cast<__bf16*>(smem);                    // [3][128][64]
-    __bf16* lb = la + 3 * 128 * 64;                                  // [XP][128][64]
+    __bf16* la = reinterpret_cast<__bf16*>(smem);                    // [3][128][R]
+    __bf16* lb = la + 3 * PLANE;                                     // [XP][128][R]
+    f32x2* meta = reinterpret_cast<f32x2*>(lb + XP * PLANE);         // [2][R]: scale of a row on dY's (gelu: on X's) side, mean rstd
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // workgroups go round the eight XCDs: number x of XCD c takes tile x % tiles of share 8 (x / tiles) + c
     const int tiles = tiles_o * tiles_i, xcd = blockIdx.x & 7, local = blockIdx.x >> 3;
@@ -208,9 +234,9 @@ __global__ __launch_bounds__(256, 2) void act8_wgrad_kernel(const float* __restr
     if (split >= splits) return;
     const int o0 = tile / tiles_i * 128, g = tile % tiles_i, i0 = g * 128, groups = tiles_i;
     const long long r0 = split * rows_per, r1 = min(rows, r0 + rows_per);
-    const int cg = tid & 31, rc = tid >> 5;                          // four columns, eight rows
+    const int cg = tid & 31, rc = tid >> 5;                          // four columns, RT rows
     const int oc = o0 + cg * 4, ic = i0 + cg * 4;
-    const bool oin = oc < co, iin = ic < ci;
+    const bool oin = oc < co;
     const int wo = (wave >> 1) * 64, wi = (wave & 1) * 64;
     f32x16 acc[2][2];
 #pragma unroll
@@ -220,95 +246,119 @@ __global__ __launch_bounds__(256, 2) void act8_wgrad_kernel(const float* __restr
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
     f32x4 sum{0.f, 0.f, 0.f, 0.f}, sumu{0.f, 0.f, 0.f, 0.f};
-    f32x4 pd[8];
-    unsigned pq[8];
+    f32x4 pd[RT];
+    unsigned pq[RT];
+    float ps = 0.f;
+    f32x2 pst{0.f, 0.f};
+    // columns behind the last are read from the last ones: their results are not stored
+    const float* dyp = dy + (size_t)(r0 + rc * RT) * co + min(oc, co - 4);
+    const unsigned* qp = q + ((size_t)(r0 + rc * RT) * ci + min(ic, ci - 4)) / 4;
+    const int ciq = ci / 4;
     auto fetch = [&](long long r) {
+        if (r + R <= r1) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const long long row = r + rc * 8 + j;
-            const bool rin = row < r1;
-            pd[j] = rin && oin ? *reinterpret_cast<const f32x4*>(dy + (size_t)row * co + oc) : f32x4{0.f, 0.f, 0.f, 0.f};
-            pq[j] = rin && iin ? q[((size_t)row * ci + ic) / 4] : 0u;
+            for (int j = 0; j < RT; ++j) {
+                pd[j] = *reinterpret_cast<const f32x4*>(dyp + (size_t)j * co);
+                pq[j] = qp[(size_t)j * ciq];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < RT; ++j) {
+                const bool in = r + rc * RT + j < r1;
+                pd[j] = in ? *reinterpret_cast<const f32x4*>(dyp + (size_t)j * co) : f32x4{0.f, 0.f, 0.f, 0.f};
+                pq[j] = in ? qp[(size_t)j * ciq] : 0u;
+            }
+        }
+        dyp += (size_t)R * co;
+        qp += (size_t)R * ciq;
+        if (tid < R) {
+            const long long row = min(r + tid, r1 - 1);              // rows behind the last meet dY = 0
+            ps = s[row * groups + g];
+            if constexpr (KIND == kNorm) pst = stats[row];
         }
     };
-    fetch(r0);
-    for (long long r = r0; r < r1; r += kRows) {
-        float sc[8], mu[8];
+    auto put_meta = [&](int buf) {
+        if (tid < R) meta[buf * R + tid] = KIND == kNorm ? f32x2{ps * pst.y, pst.x * pst.y} : f32x2{ps, 0.f};
+    };
+    if (r0 < r1) {
+        fetch(r0);
+        put_meta(0);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (long long r = r0; r < r1; r += R, buf ^= 1) {
+        f32x2 mt[RT];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const long long row = min(r + rc * 8 + j, r1 - 1);
-            sc[j] = s[row * groups + g];
-            mu[j] = 0.f;
-            if constexpr (KIND == kNorm) {
-                const f32x2 st = stats[row];
-                sc[j] *= st.y;
-                mu[j] = st.x * st.y;
-            }
-        }
+        for (int j = 0; j < RT; ++j) mt[j] = meta[buf * R + rc * RT + j];
         if constexpr (KIND == kNorm) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sumu += pd[j] * mu[j];
+            for (int j = 0; j < RT; ++j) sumu += pd[j] * mt[j].y;
         }
         // pairwise: the rows of one step, then the running sum
-        sum += ((pd[0] + pd[1]) + (pd[2] + pd[3])) + ((pd[4] + pd[5]) + (pd[6] + pd[7]));
+        if constexpr (RT == 8) sum += ((pd[0] + pd[1]) + (pd[2] + pd[3])) + ((pd[4] + pd[5]) + (pd[6] + pd[7]));
+        else sum += (pd[0] + pd[1]) + (pd[2] + pd[3]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            float v[8], x[8];
-            bf16x8 t[3];
+            float v[RT], x[RT];
+            bfv t[3];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[j] = KIND == kGelu ? pd[j][e] : pd[j][e] * sc[j];
+            for (int j = 0; j < RT; ++j) {
+                v[j] = KIND == kGelu ? pd[j][e] : pd[j][e] * mt[j].x;
                 x[j] = (float)(signed char)(pq[j] >> (8 * e) & 0xff);
             }
-            split3(v, t[0], t[1], t[2]);
-            const int at = swz(cg * 4 + e, rc);
+            split3<RT>(v, t[0], t[1], t[2]);
+            const int at = swz(cg * 4 + e, rc * RT / 8) + rc * RT % 8;
 #pragma unroll
-            for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(la + p * 128 * 64 + at) = t[p];
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<bfv*>(la + p * PLANE + at) = t[p];
             if constexpr (KIND == kGelu) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = gelu8_f(x[j] * sc[j]);
-                split3(x, t[0], t[1], t[2]);
+                for (int j = 0; j < RT; ++j) x[j] = gelu8_f(x[j] * mt[j].x);
+                split3<RT>(x, t[0], t[1], t[2]);
 #pragma unroll
-                for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(lb + p * 128 * 64 + at) = t[p];
+                for (int p = 0; p < 3; ++p) *reinterpret_cast<bfv*>(lb + p * PLANE + at) = t[p];
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; j += 2) {
+                for (int j = 0; j < RT; j += 2) {
                     const bf16x2 h = __builtin_convertvector((f32x2{x[j], x[j + 1]}), bf16x2);     // |x| <= 127: exact
                     t[0][j] = h[0]; t[0][j + 1] = h[1];
                 }
-                *reinterpret_cast<bf16x8*>(lb + at) = t[0];
+                *reinterpret_cast<bfv*>(lb + at) = t[0];
             }
         }
         __syncthreads();
-        if (r + kRows < r1) fetch(r + kRows);                        // in flight under the products
+        const bool more = r + R < r1;
+        if (more) fetch(r + R);                                      // in flight under the products
 #pragma unroll
-        for (int ks = 0; ks < kRows / 16; ++ks) {
+        for (int ks = 0; ks < R / 16; ++ks) {
             const int chunk = ks * 2 + (lane >> 5);
             bf16x8 A[2][3], B[2][XP];
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
 #pragma unroll
-                for (int p = 0; p < 3; ++p) A[m][p] = *reinterpret_cast<const bf16x8*>(la + p * 128 * 64 + swz(wo + m * 32 + (lane & 31), chunk));
+                for (int p = 0; p < 3; ++p) A[m][p] = *reinterpret_cast<const bf16x8*>(la + p * PLANE + swz(wo + m * 32 + (lane & 31), chunk));
 #pragma unroll
-                for (int p = 0; p < XP; ++p) B[m][p] = *reinterpret_cast<const bf16x8*>(lb + p * 128 * 64 + swz(wi + m * 32 + (lane & 31), chunk));
+                for (int p = 0; p < XP; ++p) B[m][p] = *reinterpret_cast<const bf16x8*>(lb + p * PLANE + swz(wi + m * 32 + (lane & 31), chunk));
             }
+            // terms from the smallest products to the largest; the four tiles of a term follow each other, so that no product waits for the one before
+            auto term = [&](int pa, int pb) {
 #pragma unroll
-            for (int a = 0; a < 2; ++a)
+                for (int a = 0; a < 2; ++a)
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    if constexpr (KIND == kGelu) {                   // smallest first
-                        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[a][2], B[b][0], acc[a][b], 0, 0, 0);
-                        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[a][0], B[b][2], acc[a][b], 0, 0, 0);
-                        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[a][1], B[b][1], acc[a][b], 0, 0, 0);
-                        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[a][1], B[b][0], acc[a][b], 0, 0, 0);
-                        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[a][0], B[b][1], acc[a][b], 0, 0, 0);
-                    } else {
-                        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[a][2], B[b][0], acc[a][b], 0, 0, 0);
-                        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[a][1], B[b][0], acc[a][b], 0, 0, 0);
-                    }
-                    acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[a][0], B[b][0], acc[a][b], 0, 0, 0);
-                }
+                    for (int b = 0; b < 2; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[a][pa], B[b][pb], acc[a][b], 0, 0, 0);
+            };
+            if constexpr (KIND == kGelu) {
+                term(2, 0);
+                term(0, 2);
+                term(1, 1);
+                term(1, 0);
+                term(0, 1);
+            } else {
+                term(2, 0);
+                term(1, 0);
+            }
+            term(0, 0);
         }
+        if (more) put_meta(buf ^ 1);
         __syncthreads();
     }
     float* slab = slabs + (size_t)split * co * ci;
@@ -403,7 +453,7 @@ __global__ __launch_bounds__(1024) void act8_affine_kernel(const float* __restri
 // Y (rows x n) = A (rows x k) B + bias + residual, all fp32, six products of three bf16 terms each (exact to 2^-24 as the framework's large GEMM), B read as the
 // parameter lies: B = W^T of W (n, k) (forward) or W of W (k, n) (data gradient).  For few rows: the framework's GEMM wants W packed and split first, four
 // launches and their host time where a step has new weights; tiles of 64 x 64 fill the chip sooner (2200 x 256 x 256: 20 us there).
-// TRANS: B is (k, n): a thread transposes eight rows of four columns on the way to LDS, as in act8_wgrad_kernel.
+// TRANS: B is (k, n): a thread transposes two rows of four columns on the way to LDS.
 constexpr int kSmallK = 32;
 template <bool TRANS>
 __global__ __launch_bounds__(256) void act8_gemm_kernel(const float* __restrict__ a, const float* __restrict__ w, const float* __restrict__ bias,
@@ -435,12 +485,12 @@ __global__ __launch_bounds__(256) void act8_gemm_kernel(const float* __restrict_
         bf16x8 t[3];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = pa[e >> 2][e & 3];
-        split3(v, t[0], t[1], t[2]);
+        split3<8>(v, t[0], t[1], t[2]);
 #pragma unroll
         for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(&la[buf][p][row * P + kc]) = t[p];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = TRANS ? pb[e & 1][e >> 1] : pb[e >> 2][e & 3];
-        split3(v, t[0], t[1], t[2]);
+        split3<8>(v, t[0], t[1], t[2]);
 #pragma unroll
         for (int p = 0; p < 3; ++p) {
             if constexpr (TRANS) {
@@ -509,6 +559,7 @@ constexpr int kMaxC = 1 << 20;
 
 struct WgradPlan { int tiles_o, tiles_i, splits; int64_t rows_per; };
 WgradPlan wgrad_plan(int64_t rows, int co, int ci) {
+    constexpr int kRows = 64;
     WgradPlan p{(co + 127) / 128, (ci + 127) / 128, 1, kRows};
     // two workgroups a CU; at least one step of rows each; whole rounds of the XCDs
     int64_t want = 512 / ((int64_t)p.tiles_o * p.tiles_i);
@@ -615,7 +666,7 @@ extern "C" int av2x_act8_wgrad(const float* dy, const int8_t* q, const float* sc
     hipStream_t st = av2x::as_stream(stream);
     auto go = [&](auto kd) {
         constexpr int K = decltype(kd)::value;
-        constexpr size_t lds = (size_t)(3 + (K == kGelu ? 3 : 1)) * 128 * 64 * 2;
+        constexpr size_t lds = (size_t)(K == kGelu ? 6 : 4) * 128 * kPitch * 2 + 2 * 32 * 8;
         static av2x::LdsLimit lim;
         lim.ensure((const void*)act8_wgrad_kernel<K>, lds);
         act8_wgrad_kernel<K><<<(unsigned)grid, 256, lds, st>>>(dy, (const unsigned*)q, scale, (const f32x2*)stats, slabs, extra, rows, cout, cin, pl.tiles_o, pl.tiles_i,
