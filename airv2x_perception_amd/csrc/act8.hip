@@ -220,13 +220,12 @@ __global__ __launch_bounds__(256, 2) void act8_wgrad_kernel(const float* __restr
                                                          const f32x2* __restrict__ stats, float* __restrict__ slabs, float* __restrict__ extra,
                                                          long long rows, int co, int ci, int tiles_o, int tiles_i, long long rows_per, int splits) {
     constexpr int XP = KIND == kGelu ? 3 : 1;                        // bf16 terms of X
-    constexpr int R = 32, RT = R / 8;                               // rows of a step, of a thread
+    constexpr int R = 32, RT = R / 8;                                // rows of a step, of a thread
     constexpr int PLANE = 128 * kPitch;
     typedef __bf16 bfv __attribute__((ext_vector_type(RT)));
     extern __shared__ __align__(16) char smem[];
     __bf16* la = reinterpret_cast<__bf16*>(smem);                    // [3][128][R]
     __bf16* lb = la + 3 * PLANE;                                     // [XP][128][R]
-    f32x2* meta = reinterpret_cast<f32x2*>(lb + XP * PLANE);         // [2][R]: scale of a row on dY's (gelu: on X's) side, mean rstd
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // workgroups go round the eight XCDs: number x of XCD c takes tile x % tiles of share 8 (x / tiles) + c
     const int tiles = tiles_o * tiles_i, xcd = blockIdx.x & 7, local = blockIdx.x >> 3;
@@ -246,88 +245,74 @@ __global__ __launch_bounds__(256, 2) void act8_wgrad_kernel(const float* __restr
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
     f32x4 sum{0.f, 0.f, 0.f, 0.f}, sumu{0.f, 0.f, 0.f, 0.f};
-    f32x4 pd[RT];
-    unsigned pq[RT];
-    float ps = 0.f;
-    f32x2 pst{0.f, 0.f};
+    struct Raw { f32x4 d[RT]; unsigned q[RT]; float s[RT]; f32x2 st[RT]; };
     // columns behind the last are read from the last ones: their results are not stored
     const float* dyp = dy + (size_t)(r0 + rc * RT) * co + min(oc, co - 4);
     const unsigned* qp = q + ((size_t)(r0 + rc * RT) * ci + min(ic, ci - 4)) / 4;
+    const float* sp = s + (size_t)(r0 + rc * RT) * groups + g;
+    const f32x2* tp = stats + (r0 + rc * RT);
     const int ciq = ci / 4;
-    auto fetch = [&](long long r) {
-        if (r + R <= r1) {
+    long long rf = r0;                                               // the step that is fetched next
+    auto fetch = [&](Raw& w) {
+        if (rf + R <= r1) {
 #pragma unroll
             for (int j = 0; j < RT; ++j) {
-                pd[j] = *reinterpret_cast<const f32x4*>(dyp + (size_t)j * co);
-                pq[j] = qp[(size_t)j * ciq];
+                w.d[j] = *reinterpret_cast<const f32x4*>(dyp + (size_t)j * co);
+                w.q[j] = qp[(size_t)j * ciq];
+                w.s[j] = sp[(size_t)j * groups];
+                if constexpr (KIND == kNorm) w.st[j] = tp[j];
             }
         } else {
 #pragma unroll
             for (int j = 0; j < RT; ++j) {
-                const bool in = r + rc * RT + j < r1;
-                pd[j] = in ? *reinterpret_cast<const f32x4*>(dyp + (size_t)j * co) : f32x4{0.f, 0.f, 0.f, 0.f};
-                pq[j] = in ? qp[(size_t)j * ciq] : 0u;
+                const bool in = rf + rc * RT + j < r1;
+                w.d[j] = in ? *reinterpret_cast<const f32x4*>(dyp + (size_t)j * co) : f32x4{0.f, 0.f, 0.f, 0.f};
+                w.q[j] = in ? qp[(size_t)j * ciq] : 0u;
+                w.s[j] = in ? sp[(size_t)j * groups] : 0.f;
+                if constexpr (KIND == kNorm) w.st[j] = in ? tp[j] : f32x2{0.f, 0.f};
             }
         }
+        rf += R;
         dyp += (size_t)R * co;
         qp += (size_t)R * ciq;
-        if (tid < R) {
-            const long long row = min(r + tid, r1 - 1);              // rows behind the last meet dY = 0
-            ps = s[row * groups + g];
-            if constexpr (KIND == kNorm) pst = stats[row];
+        sp += (size_t)R * groups;
+        tp += R;
+    };
+    bfv ta[4][3], tb[4][XP];                                         // one step's terms, per column
+    auto convert = [&](const Raw& w, int e) {                        // column e of the four
+        float v[RT], x[RT];
+#pragma unroll
+        for (int j = 0; j < RT; ++j) {
+            v[j] = KIND == kGelu ? w.d[j][e] : KIND == kNorm ? w.d[j][e] * (w.s[j] * w.st[j].y) : w.d[j][e] * w.s[j];
+            x[j] = (float)(signed char)(w.q[j] >> (8 * e) & 0xff);
+            if constexpr (KIND == kNorm) sumu[e] += w.d[j][e] * (w.st[j].x * w.st[j].y);
+        }
+        sum[e] += (w.d[0][e] + w.d[1][e]) + (w.d[2][e] + w.d[3][e]);
+        split3<RT>(v, ta[e][0], ta[e][1], ta[e][2]);
+        if constexpr (KIND == kGelu) {
+#pragma unroll
+            for (int j = 0; j < RT; ++j) x[j] = gelu8_f(x[j] * w.s[j]);
+            split3<RT>(x, tb[e][0], tb[e][1], tb[e][2]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < RT; j += 2) {
+                const bf16x2 h = __builtin_convertvector((f32x2{x[j], x[j + 1]}), bf16x2);     // |x| <= 127: exact
+                tb[e][0][j] = h[0]; tb[e][0][j + 1] = h[1];
+            }
         }
     };
-    auto put_meta = [&](int buf) {
-        if (tid < R) meta[buf * R + tid] = KIND == kNorm ? f32x2{ps * pst.y, pst.x * pst.y} : f32x2{ps, 0.f};
-    };
-    if (r0 < r1) {
-        fetch(r0);
-        put_meta(0);
-    }
-    __syncthreads();
-    int buf = 0;
-    for (long long r = r0; r < r1; r += R, buf ^= 1) {
-        f32x2 mt[RT];
-#pragma unroll
-        for (int j = 0; j < RT; ++j) mt[j] = meta[buf * R + rc * RT + j];
-        if constexpr (KIND == kNorm) {
-#pragma unroll
-            for (int j = 0; j < RT; ++j) sumu += pd[j] * mt[j].y;
-        }
-        // pairwise: the rows of one step, then the running sum
-        if constexpr (RT == 8) sum += ((pd[0] + pd[1]) + (pd[2] + pd[3])) + ((pd[4] + pd[5]) + (pd[6] + pd[7]));
-        else sum += (pd[0] + pd[1]) + (pd[2] + pd[3]);
+    // one step: its terms go to LDS, the one after next is fetched, the next one is converted between the products
+    auto step = [&](Raw& next, Raw& later) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            float v[RT], x[RT];
-            bfv t[3];
-#pragma unroll
-            for (int j = 0; j < RT; ++j) {
-                v[j] = KIND == kGelu ? pd[j][e] : pd[j][e] * mt[j].x;
-                x[j] = (float)(signed char)(pq[j] >> (8 * e) & 0xff);
-            }
-            split3<RT>(v, t[0], t[1], t[2]);
             const int at = swz(cg * 4 + e, rc * RT / 8) + rc * RT % 8;
 #pragma unroll
-            for (int p = 0; p < 3; ++p) *reinterpret_cast<bfv*>(la + p * PLANE + at) = t[p];
-            if constexpr (KIND == kGelu) {
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<bfv*>(la + p * PLANE + at) = ta[e][p];
 #pragma unroll
-                for (int j = 0; j < RT; ++j) x[j] = gelu8_f(x[j] * mt[j].x);
-                split3<RT>(x, t[0], t[1], t[2]);
-#pragma unroll
-                for (int p = 0; p < 3; ++p) *reinterpret_cast<bfv*>(lb + p * PLANE + at) = t[p];
-            } else {
-#pragma unroll
-                for (int j = 0; j < RT; j += 2) {
-                    const bf16x2 h = __builtin_convertvector((f32x2{x[j], x[j + 1]}), bf16x2);     // |x| <= 127: exact
-                    t[0][j] = h[0]; t[0][j + 1] = h[1];
-                }
-                *reinterpret_cast<bfv*>(lb + at) = t[0];
-            }
+            for (int p = 0; p < XP; ++p) *reinterpret_cast<bfv*>(lb + p * PLANE + at) = tb[e][p];
         }
         __syncthreads();
-        const bool more = r + R < r1;
-        if (more) fetch(r + R);                                      // in flight under the products
+        fetch(later);
 #pragma unroll
         for (int ks = 0; ks < R / 16; ++ks) {
             const int chunk = ks * 2 + (lane >> 5);
@@ -350,16 +335,30 @@ __global__ __launch_bounds__(256, 2) void act8_wgrad_kernel(const float* __restr
                 term(2, 0);
                 term(0, 2);
                 term(1, 1);
+                convert(next, ks * 2);
                 term(1, 0);
                 term(0, 1);
             } else {
                 term(2, 0);
+                convert(next, ks * 2);
                 term(1, 0);
             }
+            convert(next, ks * 2 + 1);
             term(0, 0);
         }
-        if (more) put_meta(buf ^ 1);
         __syncthreads();
+    };
+    if (r0 < r1) {
+        Raw u, v;
+        fetch(u);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) convert(u, e);
+        fetch(u);
+        const long long n = (r1 - r0 + R - 1) / R;                   // (two more are fetched and converted: zeros)
+        for (long long i = 0; i < n; i += 2) {
+            step(u, v);
+            if (i + 1 < n) step(v, u);
+        }
     }
     float* slab = slabs + (size_t)split * co * ci;
 #pragma unroll
@@ -666,7 +665,7 @@ extern "C" int av2x_act8_wgrad(const float* dy, const int8_t* q, const float* sc
     hipStream_t st = av2x::as_stream(stream);
     auto go = [&](auto kd) {
         constexpr int K = decltype(kd)::value;
-        constexpr size_t lds = (size_t)(K == kGelu ? 6 : 4) * 128 * kPitch * 2 + 2 * 32 * 8;
+        constexpr size_t lds = (size_t)(K == kGelu ? 6 : 4) * 128 * kPitch * 2;
         static av2x::LdsLimit lim;
         lim.ensure((const void*)act8_wgrad_kernel<K>, lds);
         act8_wgrad_kernel<K><<<(unsigned)grid, 256, lds, st>>>(dy, (const unsigned*)q, scale, (const f32x2*)stats, slabs, extra, rows, cout, cin, pl.tiles_o, pl.tiles_i,
