@@ -113,6 +113,11 @@ __device__ __forceinline__ unsigned order_key(float s) {       // unsigned order
     return (unsigned)(b < 0 ? b ^ 0x7fffffff : b) ^ 0x80000000u;
 }
 
+__device__ __forceinline__ float key_score(unsigned k) {       // the score of a key; the key below zero's (-0, which no score has) is that of the number below zero
+    if (k == 0x7fffffffu) k = 0x7ffffffeu;
+    return __builtin_bit_cast(float, k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+
 // n largest of {key (lane), c[0], c[1], ..} (candidates in this order, lane by lane), 0 = none, ties to the earliest.  Returns how many; the
 // chosen ones land in key / idx of lanes 0, 1, .. in order.  Any number of ties: the n-th largest value is found bit by bit.
 template <int E, typename Idx>
@@ -372,7 +377,7 @@ __global__ __launch_bounds__(512, 4) void bs_select16_kernel(const T* __restrict
     constexpr int NQ = 32, CH = D / 16, KS = 2 * D / 32, GT = KS <= 2 ? 4 : KS <= 4 ? 2 : 1, GP = kFours + 4, QP = 2 * D + 8;
     constexpr int LB = D <= 64 ? D / 4 : 16, CPL = D <= 64 ? 1 : 2;      // lanes that add up one score, 16-byte pieces of each
     typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-    __shared__ __align__(16) unsigned gm[NQ * GP];
+    __shared__ __align__(16) float gm[NQ * GP];                                // the largest score of every four, -inf: no block
     __shared__ __align__(16) _Float16 qi[NQ * QP];
     // entries: key of the score in the upper half, ~block in the lower one: larger is better, ties to the lower block; 0: none
     __shared__ __align__(16) u64 kept[NQ][16], pend[NQ][32];
@@ -426,19 +431,37 @@ __global__ __launch_bounds__(512, 4) void bs_select16_kernel(const T* __restrict
                 for (int s = 0; s < KS; ++s) bf[u][s] = *reinterpret_cast<const f16x8*>(&qi[(u * 16 + l) * QP + s * 32 + row * 8]);
             for (int g0 = wave * GT; g0 < steps * 16; g0 += 8 * GT) {
                 f16x8 a[GT][KS];
-                float w[GT][4];
+                f32x4 w[GT], none[GT];                                            // score = dot * w + none: -inf where there is no block
+                const int jr = j0 + g0 * 16;
+                if (jr + GT * 16 <= last) {
+                    const _Float16* p = kp + (unsigned)((jr + l) * 2 * D + row * 8);
 #pragma unroll
-                for (int g = 0; g < GT; ++g) {
-                    const int jr = j0 + (g0 + g) * 16, ja = min(jr + l, NB - 1);
+                    for (int g = 0; g < GT; ++g) {
 #pragma unroll
-                    for (int s = 0; s < KS; ++s) a[g][s] = *reinterpret_cast<const f16x8*>(kp + (size_t)ja * 2 * D + s * 32 + row * 8);
+                        for (int s = 0; s < KS; ++s) a[g][s] = *reinterpret_cast<const f16x8*>(p + g * 16 * 2 * D + s * 32);
+                        __builtin_memcpy(&w[g], sp + jr + g * 16 + row * 4, 16);
+                    }
+                } else {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int j = jr + row * 4 + i;
-                        const float x = sp[min(j, NB - 1)];
-                        w[g][i] = j < last ? x : -1.0f;
+                    for (int g = 0; g < GT; ++g) {
+                        const int ja = min(jr + g * 16 + l, NB - 1);
+#pragma unroll
+                        for (int s = 0; s < KS; ++s) a[g][s] = *reinterpret_cast<const f16x8*>(kp + (unsigned)(ja * 2 * D + s * 32 + row * 8));
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int j = jr + g * 16 + row * 4 + i;
+                            const float x = sp[min(j, NB - 1)];
+                            w[g][i] = j < last ? x : -1.0f;
+                        }
                     }
                 }
+#pragma unroll
+                for (int g = 0; g < GT; ++g)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        none[g][i] = w[g][i] < 0.f ? -INFINITY : 0.f;
+                        w[g][i] = fmaxf(w[g][i], 0.f);
+                    }
 #pragma unroll
                 for (int g = 0; g < GT; ++g)
 #pragma unroll
@@ -446,29 +469,30 @@ __global__ __launch_bounds__(512, 4) void bs_select16_kernel(const T* __restrict
                         f32x4 acc{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                         for (int s = 0; s < KS; ++s) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[g][s], bf[u][s], acc, 0, 0, 0);
-                        unsigned m = 0u;
+                        float m = fmaf(acc[0], w[g][0], none[g][0]);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) m = max(m, w[g][i] < 0.f ? 0u : order_key(acc[i] * w[g][i]));
+                        for (int i = 1; i < 4; ++i) m = fmaxf(m, fmaf(acc[i], w[g][i], none[g][i]));
                         gm[(u * 16 + l) * GP + (g0 + g) * 4 + row] = m;
                     }
             }
         }
         __syncthreads();
         if (t0 + wave * 4 < T_) {
-            const unsigned* gp = gm + qr * GP + l * 4;
+            const float* gp = gm + qr * GP + l * 4;
             u64 k = kept[qr][l];
             // what an entry has to beat: the n-th best (a block of this range may tie with it and come first), or every entry of a key
             u64 bar = kept[qr][n - 1];
             const bool none = kept[qr][0] == 0ull;
             if (__ballot(none)) {
-                unsigned m = 0;
+                float m = -INFINITY;
                 for (int i = 0; i < steps; ++i) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(gp + i * 64);
-                    m = max(max(m, max(x.x, x.y)), max(x.z, x.w));
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(gp + i * 64);
+                    m = fmaxf(fmaxf(m, fmaxf(x.x, x.y)), fmaxf(x.z, x.w));
                 }
+                const unsigned mk = m == -INFINITY ? 0u : order_key(m);
                 int rank = 0;
-                each_ror<1, 16>([&](auto r) { rank += row_ror<decltype(r)::value>(m) > m ? 1 : 0; });
-                unsigned t = rank < n ? m : 0xffffffffu;
+                each_ror<1, 16>([&](auto r) { rank += row_ror<decltype(r)::value>(mk) > mk ? 1 : 0; });
+                unsigned t = rank < n ? mk : 0xffffffffu;
                 t = min(t, row_ror<8>(t));
                 t = min(t, row_ror<4>(t));
                 t = min(t, row_ror<2>(t));
@@ -501,10 +525,10 @@ __global__ __launch_bounds__(512, 4) void bs_select16_kernel(const T* __restrict
             };
             for (int s0 = 0, span = steps; s0 < steps;) {
                 const int s1 = min(steps, s0 + span);
-                const unsigned thr = (unsigned)(bar >> 32);                       // later fours lose ties
+                const float thr = bar ? key_score((unsigned)(bar >> 32)) : -INFINITY;      // later fours lose ties
                 int cnt = 0;
                 for (int i = s0; i < s1; ++i) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(gp + i * 64);
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(gp + i * 64);
                     cnt += (x.x > thr ? 1 : 0) + (x.y > thr ? 1 : 0) + (x.z > thr ? 1 : 0) + (x.w > thr ? 1 : 0);
                 }
                 const int total = row_sum(cnt), most = rows_max(total);
@@ -517,7 +541,7 @@ __global__ __launch_bounds__(512, 4) void bs_select16_kernel(const T* __restrict
                     pos += __builtin_amdgcn_update_dpp(0, pos, 0x118, 0xf, 0xf, true);
                     pos -= cnt;
                     for (int i = s0; i < s1; ++i) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(gp + i * 64);
+                        const f32x4 x = *reinterpret_cast<const f32x4*>(gp + i * 64);
                         const int g = (i * 16 + l) * 4;
                         if (x.x > thr) fo[pos++] = (unsigned short)g;
                         if (x.y > thr) fo[pos++] = (unsigned short)(g + 1);
@@ -532,12 +556,14 @@ __global__ __launch_bounds__(512, 4) void bs_select16_kernel(const T* __restrict
                         float w = sp[min(j, NB - 1)], dot = 0.f;
                         w = j < last ? w : -1.0f;
                         f16x8 x[LB][CPL];
+                        const unsigned end = (unsigned)(NB - 1) * (2 * D) + l % LB * 8;          // the last block's bounds
 #pragma unroll
-                        for (int e = 0; e < LB; ++e) {
-                            const int f = r0 + (l / LB * LB + e) / 4;
-                            const int je = min(j0 + fo[min(f, kGroupList - 1)] * 4 + (e & 3), NB - 1);
+                        for (int f = 0; f < LB / 4; ++f) {
+                            const unsigned at = (unsigned)(j0 + fo[min(r0 + l / LB * (LB / 4) + f, kGroupList - 1)] * 4) * (2 * D) + l % LB * 8;
 #pragma unroll
-                            for (int c = 0; c < CPL; ++c) x[e][c] = *reinterpret_cast<const f16x8*>(kp + (size_t)je * 2 * D + (l % LB + c * LB) * 8);
+                            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                                for (int c = 0; c < CPL; ++c) x[f * 4 + e][c] = *reinterpret_cast<const f16x8*>(kp + min(at + e * 2 * D, end) + c * LB * 8);
                         }
 #pragma unroll
                         for (int e = 0; e < LB; ++e) {

@@ -198,6 +198,8 @@ def qk_norm_rotate(q, k, gamma_q, gamma_k, positions, freqs, eps=1e-6, interleav
         oq, ok = _QkNormRotate.apply(q3, k3, gq, gk, pos, freqs, float(eps), bool(interleaved))
     else:
         oq, ok = _rotate_forward(q3, k3, gq, gk, pos, freqs, float(eps), bool(interleaved))
+    if q.dim() == 3:
+        return oq, ok
     return oq.view(shape), ok.view(kshape) if ok is not None else None
 
 
@@ -219,8 +221,10 @@ def qkv_norm_rotate(qkv, heads, kv_heads, gamma_q, gamma_k, positions, freqs, ep
     else:
         q, k = _rotate_forward(x[:, :heads], x[:, heads:heads + kv_heads], gq, gk, pos, freqs, float(eps), bool(interleaved))
         v = x[:, heads + kv_heads:]
+    if len(lead) == 1:
+        return q, k, v
     d = x.shape[-1]
-    return q.view(lead + (heads, d)), k.view(lead + (kv_heads, d)), v.unflatten(0, lead) if len(lead) > 1 else v
+    return q.view(lead + (heads, d)), k.view(lead + (kv_heads, d)), v.unflatten(0, lead)
 
 
 # ------------------------------------------------------------------------------------------------ blocks
