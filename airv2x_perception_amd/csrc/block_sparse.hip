@@ -42,8 +42,7 @@ struct BsArgs {
     const int32_t* n_items;                  // (B KV)
     int max_items;
     // forward
-    void* part;                              // (B, T, H, n, D): of T in the forward, fp32 (dQ) in the backward
-    f32x2* ml;                               // (B, T, H, n) maximum (scaled, base 2) and sum
+    void* part;                              // forward: (B, T, H, n) records; backward: (B, T, H, n, D) fp32, dQ
     void* out;                               // (B, T, H, D)
     float* lse;                              // (B, T, H) base 2, +inf: no key; may be null
     void* rest;                              // (B, T, H, D) out's rounding errors, or null
@@ -880,16 +879,24 @@ template <typename T, int D> struct RowFrags {
     typename Held<T>::frag f[Held<T>::terms][Shape<T, D>::KS];
     float back = 1.0f;
 };
-template <typename T, int D> __device__ __forceinline__ void global_frags(const T* p, bool in, int half, RowFrags<T, D>& r) {
+template <typename T, int D> struct RawRow { typename tok_vec<T>::v8 x[D / 16]; };
+template <typename T, int D> __device__ __forceinline__ RawRow<T, D> load_row(const T* p, bool in, int half) {
+    RawRow<T, D> r;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r.x[s][e] = (T)0.f;
+        if (in) r.x[s] = *reinterpret_cast<const typename tok_vec<T>::v8*>(p + s * 16 + half * 8);
+    }
+    return r;
+}
+template <typename T, int D> __device__ __forceinline__ void to_frags(const RawRow<T, D>& w, RowFrags<T, D>& r) {
     if constexpr (Held<T>::two) {
-        float x[D / 16][8], m = 0.f;
+        float m = 0.f;
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-            f32x4 a{0.f, 0.f, 0.f, 0.f}, b = a;
-            if (in) { a = *reinterpret_cast<const f32x4*>(p + s * 16 + half * 8); b = *reinterpret_cast<const f32x4*>(p + s * 16 + half * 8 + 4); }
+        for (int s = 0; s < D / 16; ++s)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { x[s][e] = a[e]; x[s][4 + e] = b[e]; m = fmaxf(m, fmaxf(fabsf(a[e]), fabsf(b[e]))); }
-        }
+            for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(w.x[s][e]));
         m = fmaxf(m, __shfl_xor(m, 32));
         r.back = pow2_over(m);
         const float to = 1.0f / r.back;
@@ -897,18 +904,14 @@ template <typename T, int D> __device__ __forceinline__ void global_frags(const 
         for (int s = 0; s < D / 16; ++s)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float v = x[s][e] * to;
+                const float v = w.x[s][e] * to;
                 const _Float16 h = (_Float16)v;
                 r.f[0][s][e] = h;
                 r.f[1][s][e] = (_Float16)(v - (float)h);
             }
     } else {
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) r.f[0][s][e] = (T)0.f;
-            if (in) r.f[0][s] = *reinterpret_cast<const typename Held<T>::frag*>(p + s * 16 + half * 8);
-        }
+        for (int s = 0; s < D / 16; ++s) r.f[0][s] = w.x[s];
     }
 }
 
@@ -1015,10 +1018,23 @@ __device__ __forceinline__ Row row_of(const BsArgs& a, const int32_t* list, int 
 constexpr int kItemRows = 1024;              // rows (mentions x heads of the group) of a work item
 
 // ------------------------------------------------------------------------------------------------------------ attention, many queries
-// A mention's result is the attention over its block alone and (maximum, sum).  PT: without gradients it is held in the tensor's type -- a convex combination of
+// A mention's record: (maximum (scaled, base 2), sum) and the attention over its block alone, next to each other -- they are written to places all over the
+// workspace, and 8 bytes of their own would cost a memory request as large as the rest.  PT: without gradients it is held in the tensor's type -- a convex combination of
 // values like the output, so its rounding is half a step at most and enters the output with the block's weight (measured: 1.4 times the error of the output's
 // own rounding) -- which halves the bytes that bound this kernel and the join (281600 queries x 8 blocks, bf16: join 94 -> 51 us).  With gradients it stays fp32:
 // the backward's sum dO O would carry that rounding into every dS of the query.
+template <int D, typename PT> struct Record {
+    static constexpr size_t bytes = 8 + D * sizeof(PT);
+    static __device__ __forceinline__ char* at(void* part, size_t i) { return static_cast<char*>(part) + i * bytes; }
+    static __device__ __forceinline__ const char* at(const void* part, size_t i) { return static_cast<const char*>(part) + i * bytes; }
+    typedef typename tok_vec<PT>::v4 v4 __attribute__((aligned(8)));
+    static __device__ __forceinline__ void put(char* r, int d, f32x4 v) { *reinterpret_cast<v4*>(r + 8 + d * sizeof(PT)) = __builtin_convertvector(v, typename tok_vec<PT>::v4); }
+    static __device__ __forceinline__ f32x4 get(const char* r, int d) {
+        const typename tok_vec<PT>::v4 x = *reinterpret_cast<const v4*>(r + 8 + d * sizeof(PT));
+        return __builtin_convertvector(x, f32x4);
+    }
+};
+
 template <typename T, int D, typename PT>
 __global__ __launch_bounds__(256) void bs_forward_kernel(BsArgs a) {
     using S = Shape<T, D>;
@@ -1034,17 +1050,26 @@ __global__ __launch_bounds__(256) void bs_forward_kernel(BsArgs a) {
     const int32_t* st = a.start + (size_t)bh * (a.NB + 1) + j;
     const int len = st[1] - st[0];
     const int32_t* list = a.list + (size_t)bh * a.T * a.n + st[0];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int last = min(first + kItemRows, len * a.G);
+    const T* qbase = static_cast<const T*>(a.q) + b * a.qb;
+    // the first queries are on their way before K and V, the next ones during the work on these
+    Row r = row_of(a, list, len, h, first + wave * 32 + (lane & 31));
+    RawRow<T, D> raw = load_row<T, D>(qbase + r.t * a.qt + r.head * a.qh, r.in, half);
     const unsigned long long seen = seen_keys(a, b, j);
     const float kf = load_block<T, D, true, false>(static_cast<const T*>(a.k) + b * a.kb + h * a.kh, a.kt, j * kKeys, seen, lk, nullptr, red[0]);
     const float vf = load_block<T, D, false, true>(static_cast<const T*>(a.v) + b * a.vb + h * a.vh, a.vt, j * kKeys, seen, nullptr, lv, red[1]);
     __syncthreads();
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    const int last = min(first + kItemRows, len * a.G);
     const float c2 = a.scale * kLog2e * kf;
+    Row ahead = row_of(a, list, len, h, first + wave * 32 + 128 + (lane & 31));
     for (int r0 = first + wave * 32; r0 < last; r0 += 128) {
-        const Row r = row_of(a, list, len, h, r0 + (lane & 31));
         RowFrags<T, D> qf;
-        global_frags<T, D>(static_cast<const T*>(a.q) + b * a.qb + r.t * a.qt + r.head * a.qh, r.in, half, qf);
+        to_frags<T, D>(raw, qf);
+        const Row next = ahead;
+        if (r0 + 128 < last) {
+            raw = load_row<T, D>(qbase + next.t * a.qt + next.head * a.qh, next.in, half);
+            ahead = row_of(a, list, len, h, r0 + 256 + (lane & 31));
+        }
         const float c = c2 * qf.back;
         f32x16 s[2];
         float m = -INFINITY;
@@ -1072,7 +1097,7 @@ __global__ __launch_bounds__(256) void bs_forward_kernel(BsArgs a) {
         l += __shfl_xor(l, 32);
         const float inv = l == 0.f ? 0.f : vf / l;
         if constexpr (Held<T>::narrow) l *= 1.0f / 32768.f;
-        const size_t at = (((size_t)b * a.T + r.t) * a.H + r.head) * a.n + r.slot;
+        char* rec = Record<D, PT>::at(a.part, (((size_t)b * a.T + r.t) * a.H + r.head) * a.n + r.slot);
         const Split<T, false> p0(s[0]), p1(s[1]);
 #pragma unroll
         for (int dt = 0; dt < S::DT; ++dt) {
@@ -1082,11 +1107,12 @@ __global__ __launch_bounds__(256) void bs_forward_kernel(BsArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int d = dt * 32 + 8 * i + 4 * half;
-                    if (d < D) tok_store4(static_cast<PT*>(a.part) + at * D + d, f32x4{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]} * inv);
+                    if (d < D) Record<D, PT>::put(rec, d, f32x4{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]} * inv);
                 }
             }
         }
-        if (r.in && half == 0) a.ml[at] = f32x2{m, l};
+        if (r.in && half == 0) *reinterpret_cast<f32x2*>(rec) = f32x2{m, l};
+        r = next;
     }
 }
 
@@ -1145,12 +1171,12 @@ __global__ __launch_bounds__(64) void bs_few_kernel(BsArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) { o0[e] += __shfl_xor(o0[e], o); o1[e] += __shfl_xor(o1[e], o); }
         const float inv = l == 0.f ? 0.f : 1.0f / l;
-        const size_t at = (((size_t)b * a.T + t) * a.H + h * a.G + g) * a.n + slot;
+        char* rec = Record<D, PT>::at(a.part, (((size_t)b * a.T + t) * a.H + h * a.G + g) * a.n + slot);
         if (lane < LPK) {
-            tok_store4(static_cast<PT*>(a.part) + at * D + sub * 8, o0 * inv);
-            tok_store4(static_cast<PT*>(a.part) + at * D + sub * 8 + 4, o1 * inv);
+            Record<D, PT>::put(rec, sub * 8, o0 * inv);
+            Record<D, PT>::put(rec, sub * 8 + 4, o1 * inv);
         }
-        if (lane == 0) a.ml[at] = f32x2{m, l};
+        if (lane == 0) *reinterpret_cast<f32x2*>(rec) = f32x2{m, l};
     }
 }
 
@@ -1164,8 +1190,7 @@ __global__ __launch_bounds__(256) void bs_join_kernel(BsArgs a, long long rows) 
     const unsigned hq = (unsigned)(r % a.H);
     const long long bt = r / a.H;
     const int32_t* bl = a.blocks + (bt * a.KV + hq / (unsigned)a.G) * a.n;
-    const f32x2* ml = a.ml + r * a.n;
-    const PT* part = static_cast<const PT*>(a.part) + r * a.n * D + sub * 4;
+    const char* part = Record<D, PT>::at(a.part, (size_t)(r * a.n));
     float m = -INFINITY, l = 0.f;
     f32x4 o{0.f, 0.f, 0.f, 0.f};
     for (int s0 = 0; s0 < a.n; s0 += 8) {                // eight places at a time, all their loads in flight
@@ -1176,8 +1201,13 @@ __global__ __launch_bounds__(256) void bs_join_kernel(BsArgs a, long long rows) 
         for (int u = 0; u < 8; ++u) {
             const int s = s0 + u, j = s < a.n ? bl[s] : -1;
             const bool ok = j >= 0 && j < a.NB;          // other places were never written
-            x[u] = ok ? ml[s] : f32x2{-INFINITY, 0.f};
-            y[u] = ok ? tok_load4(part + (long long)s * D) : f32x4{0.f, 0.f, 0.f, 0.f};
+            x[u] = f32x2{-INFINITY, 0.f};
+            y[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (ok) {
+                const char* rec = part + (size_t)s * Record<D, PT>::bytes;
+                x[u] = *reinterpret_cast<const f32x2*>(rec);
+                y[u] = Record<D, PT>::get(rec, sub * 4);
+            }
             mm = fmaxf(mm, x[u].x);
         }
         const float base = mm == -INFINITY ? 0.f : mm, f = __builtin_amdgcn_exp2f(m - base);
@@ -1262,13 +1292,15 @@ __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsA
     f32x16 dk[AT][2], dv[AT][2];
 #pragma unroll
     for (int t = 0; t < AT; ++t) { dk[t][0] = zero16(); dk[t][1] = zero16(); dv[t][0] = zero16(); dv[t][1] = zero16(); }
+    Row ahead = row_of(a, list, len, h, first + wave * 32 + (lane & 31));
     for (int r0 = first + wave * 32; r0 < last; r0 += 128) {
-        const Row r = row_of(a, list, len, h, r0 + (lane & 31));
+        const Row r = ahead;
         const size_t qrow = ((size_t)b * a.T + r.t) * a.H + r.head;
         RowFrags<T, D> qf, of;
-        global_frags<T, D>(static_cast<const T*>(a.q) + b * a.qb + r.t * a.qt + r.head * a.qh, r.in, half, qf);
-        global_frags<T, D>(static_cast<const T*>(a.dout) + qrow * D, r.in, half, of);
+        to_frags<T, D>(load_row<T, D>(static_cast<const T*>(a.q) + b * a.qb + r.t * a.qt + r.head * a.qh, r.in, half), qf);
+        to_frags<T, D>(load_row<T, D>(static_cast<const T*>(a.dout) + qrow * D, r.in, half), of);
         const f32x2 ld = r.in ? a.ld[qrow] : f32x2{INFINITY, 0.f};         // rows that are not there: P = 0
+        ahead = row_of(a, list, len, h, r0 + 128 + (lane & 31));
         if (half == 0) lld[wave][lane & 31] = f32x4{ld.x, ld.y, qf.back, of.back};
 #pragma unroll
         for (int s = 0; s < S::KS; ++s)
@@ -1590,16 +1622,13 @@ namespace {
 
 size_t up16(size_t x) { return (x + 15) & ~(size_t)15; }
 
-struct Work { size_t part, ml, ld, slab, bytes; };       // byte offsets
+struct Work { size_t part, ld, slab, bytes; };       // byte offsets
 Work bs_work(int64_t B, int64_t T, int64_t Nk, int64_t H, int64_t KV, int64_t D, int64_t n, bool backward) {
     Work w{};
     const size_t rows = (size_t)(B * T * H);
     w.part = 0;
-    size_t at = up16(rows * n * D * 4);      // (a 16-bit forward uses half of it)
-    if (!backward) {
-        w.ml = at;
-        at += up16(rows * n * 8);
-    } else {
+    size_t at = up16(rows * n * (backward ? D * 4 : D * 4 + 8));      // (a 16-bit forward uses about half of it)
+    if (backward) {
         w.ld = at;
         at += up16(rows * 8);
         w.slab = at;
@@ -1648,7 +1677,6 @@ extern "C" int av2x_block_sparse_attention(const void* q, const void* k, const v
     const Work w = bs_work(batch, queries, keys, heads, kv_heads, dim, n, false);
     char* ws = static_cast<char*>(workspace);
     a.part = ws + w.part;
-    a.ml = reinterpret_cast<f32x2*>(ws + w.ml);
     a.out = out;
     a.lse = lse;
     a.rest = rest;
