@@ -427,6 +427,7 @@ class BlockSparseAttention(nn.Module):
             raise RuntimeError("BlockSparseAttention (MI355X build) has no CPU path: move the module to the GPU")
         b, t, c = x.shape
         amp = _amp_requested(self)
+        x = x.contiguous()
         with T.amp_scope(amp):
             w = self.to_qkv.weight
             if self.act8:

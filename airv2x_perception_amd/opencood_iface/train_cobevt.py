@@ -47,22 +47,19 @@ def swap_fusion_encoder(P, x, n_valid, fax, training=True, prefix="fusion_net.")
     for i in range(fax["depth"]):
         for gi, part in enumerate(("window", "grid")):
             a, f = f"{prefix}layers.{i}.{part}_attention", f"{prefix}layers.{i}.{part}_ffd"
-            xn = F.layer_norm(x, P[a + ".norm.weight"], P[a + ".norm.bias"])
-            qkv = F.linear(xn, P[a + ".fn.to_qkv.weight"])
+            qkv = F.norm_linear(x, P[a + ".norm.weight"], P[a + ".norm.bias"], P[a + ".fn.to_qkv.weight"])
             att = F.fax_attention(qkv, P[a + ".fn.relative_position_bias_table.weight"], n_valid, ws, heads, dh, gi)
             if p_drop > 0 and training:     # to_out = Sequential(Linear, Dropout) (:42-44): the residual is added after the dropout
-                x = F.dropout(F.linear(att, P[a + ".fn.to_out.0.weight"]), p_drop, True, x)
+                x = F.dropout(F.token_linear(att, P[a + ".fn.to_out.0.weight"]), p_drop, True, x)
             else:
-                x = F.linear(att, P[a + ".fn.to_out.0.weight"], None, x)
-            xn = F.layer_norm(x, P[f + ".norm.weight"], P[f + ".norm.bias"])
-            hdn = F.gelu(F.linear(xn, P[f + ".fn.net.0.weight"], P[f + ".fn.net.0.bias"]))
+                x = F.token_linear(att, P[a + ".fn.to_out.0.weight"], None, x)
+            z = F.norm_linear(x, P[f + ".norm.weight"], P[f + ".norm.bias"], P[f + ".fn.net.0.weight"], P[f + ".fn.net.0.bias"])
             if p_drop > 0 and training:     # FeedForward = Linear, GELU, Dropout, Linear, Dropout (base_transformer.py:28-35)
-                x = F.dropout(F.linear(F.dropout(hdn, p_drop), P[f + ".fn.net.3.weight"], P[f + ".fn.net.3.bias"]), p_drop, True, x)
+                x = F.dropout(F.token_linear(F.dropout(F.token_gelu(z), p_drop), P[f + ".fn.net.3.weight"], P[f + ".fn.net.3.bias"]), p_drop, True, x)
             else:
-                x = F.linear(hdn, P[f + ".fn.net.3.weight"], P[f + ".fn.net.3.bias"], x)
+                x = F.gelu_linear(z, P[f + ".fn.net.3.weight"], P[f + ".fn.net.3.bias"], x)
     m = F.agent_mean(x)
-    m = F.layer_norm(m, P[prefix + "mlp_head.2.weight"], P[prefix + "mlp_head.2.bias"])
-    return F.linear(m, P[prefix + "mlp_head.3.weight"], P[prefix + "mlp_head.3.bias"])
+    return F.norm_linear(m, P[prefix + "mlp_head.2.weight"], P[prefix + "mlp_head.2.bias"], P[prefix + "mlp_head.3.weight"], P[prefix + "mlp_head.3.bias"])
 
 
 def _forward_train(model, data_dict):
@@ -118,7 +115,8 @@ def _forward_train(model, data_dict):
 
 def forward_train(model, data_dict):
     """One train-mode forward.  torch.autocast around the call (tools/train.py:118) or ``model.amp = True`` selects AMP for THIS
-    step only: the flag lives for the duration of the forward (train_ops.amp_scope) and every node carries it into its backward."""
+    step only: the flag lives for the duration of the forward (train_ops.amp_scope) and every node carries it into its backward.
+    ``model.act8 = True``: the fusion's token layers keep their saved activations in 8 bits (act8_ops)."""
     from .airv2x_where2com import _amp_requested
-    with T.amp_scope(_amp_requested(model)):
+    with T.amp_scope(_amp_requested(model)), T.act8_scope(getattr(model, "act8", False)):
         return _forward_train(model, data_dict)

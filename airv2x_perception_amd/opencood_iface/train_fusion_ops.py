@@ -134,6 +134,39 @@ def gelu(z):
     return GeluFn.apply(z)
 
 
+# ------------------------------------------------------------------------------------------------ with either kind of saved activation
+def norm_linear(x, gamma, beta, weight, bias=None):
+    """Linear(LayerNorm(x)); under train_ops.act8_scope as one node that keeps x in 8 bits."""
+    if T.ACT8_STEP[0]:
+        from . import act8_ops
+        return act8_ops.norm_linear(x, gamma, beta, weight, bias)
+    return linear(layer_norm(x, gamma, beta), weight, bias)
+
+
+def token_linear(x, weight, bias=None, residual=None):
+    """linear; under train_ops.act8_scope with x kept in 8 bits."""
+    if T.ACT8_STEP[0]:
+        from . import act8_ops
+        return act8_ops.linear(x, weight, bias, residual)
+    return linear(x, weight, bias, residual)
+
+
+def token_gelu(z):
+    """gelu; under train_ops.act8_scope with z kept in 8 bits."""
+    if T.ACT8_STEP[0]:
+        from . import act8_ops
+        return act8_ops.gelu(z)
+    return gelu(z)
+
+
+def gelu_linear(z, weight, bias=None, residual=None):
+    """Linear(GELU(z)) (+ residual); under train_ops.act8_scope as one node that keeps z in 8 bits."""
+    if T.ACT8_STEP[0]:
+        from . import act8_ops
+        return act8_ops.gelu_linear(z, weight, bias, residual)
+    return linear(gelu(z), weight, bias, residual)
+
+
 class DropoutFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p, residual):

@@ -173,6 +173,27 @@ class amp_scope:
         return False
 
 
+# Token layers of the transformer fusions with 8-bit saved activations (act8_ops): while set, train_fusion_ops' norm_linear / token_linear / token_gelu / gelu_linear
+# build those nodes.  A node is what its forward made it, so the flag matters to the forward alone.
+ACT8_STEP = [False]
+
+
+class act8_scope:
+    """``with act8_scope(flag):`` -- ACT8_STEP inside the block, the previous value afterwards."""
+
+    def __init__(self, on):
+        self.on = bool(on)
+
+    def __enter__(self):
+        self.prev = ACT8_STEP[0]
+        ACT8_STEP[0] = self.on
+        return self
+
+    def __exit__(self, *exc):
+        ACT8_STEP[0] = self.prev
+        return False
+
+
 def conv_raw(x, weight, stride, pad, scale=None, shift=None, act=0, flipped=False, owner=None):
     """act(scale * conv2d(x, w) + shift) through the engine's launcher (direct or Winograd kernels, autotuned).  ``flipped``:
     convolve with the 180-degree-rotated, channel-transposed weights (the data gradient)."""

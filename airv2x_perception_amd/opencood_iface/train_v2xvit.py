@@ -89,36 +89,38 @@ def encoder(P, x, prior, scm, enc, training=True, p="fusion_net.encoder"):
             q = f"{p}.layers.{di}.0.layers.{nb}"
             h = q + ".0.fn"
             # ---- x = HGT(LN(x)) + x
-            xn = F.layer_norm(x, P[q + ".0.norm.weight"], P[q + ".0.norm.bias"])
             fold = {t: folded_projection(P, h, t, heads, dh) for t in set(types)}
-            proj = torch.cat([F.linear(xn[a:b], fold[t][0], fold[t][1]) for (a, b, t) in groups], 0)
+            g0, b0 = P[q + ".0.norm.weight"], P[q + ".0.norm.bias"]
+            if T.ACT8_STEP[0]:      # the norm is per token: every group's slice with its own Linear, one 8-bit copy of x for both
+                proj = torch.cat([F.norm_linear(x[a:b], g0, b0, fold[t][0], fold[t][1]) for (a, b, t) in groups], 0)
+            else:
+                xn = F.layer_norm(x, g0, b0)
+                proj = torch.cat([F.linear(xn[a:b], fold[t][0], fold[t][1]) for (a, b, t) in groups], 0)
             att = F.hgt_attention(proj, mask, types, heads, dh)
             outs = []
             for (a, b, t) in groups:
                 if cav["dropout"] > 0 and training:     # out = drop_out(to_out(out)) (hmsa.py:153-154), residual added by PreNorm's caller
-                    outs.append(F.dropout(F.linear(att[a:b], P[f"{h}.a_linears.{t}.weight"], P[f"{h}.a_linears.{t}.bias"]), cav["dropout"], True, x[a:b]))
+                    outs.append(F.dropout(F.token_linear(att[a:b], P[f"{h}.a_linears.{t}.weight"], P[f"{h}.a_linears.{t}.bias"]), cav["dropout"], True, x[a:b]))
                 else:
-                    outs.append(F.linear(att[a:b], P[f"{h}.a_linears.{t}.weight"], P[f"{h}.a_linears.{t}.bias"], x[a:b]))
+                    outs.append(F.token_linear(att[a:b], P[f"{h}.a_linears.{t}.weight"], P[f"{h}.a_linears.{t}.bias"], x[a:b]))
             x = torch.cat(outs, 0) if len(outs) > 1 else outs[0]
             # ---- x = SplitAttn(window attentions(LN(x))) + x
             w = q + ".1.fn"
-            xn = F.layer_norm(x, P[q + ".1.norm.weight"], P[q + ".1.norm.bias"])
-            qkv3 = F.linear(xn, torch.cat([P[f"{w}.pwmsa.{i}.to_qkv.weight"] for i in range(3)], 0))
+            qkv3 = F.norm_linear(x, P[q + ".1.norm.weight"], P[q + ".1.norm.bias"], torch.cat([P[f"{w}.pwmsa.{i}.to_qkv.weight"] for i in range(3)], 0))
             wat = F.pyramid_window_attention(qkv3, [P[f"{w}.pwmsa.{i}.pos_embedding"] for i in range(3)], wcfg)
             br = []
             for i in range(3):
-                o = F.linear(wat[i], P[f"{w}.pwmsa.{i}.to_out.0.weight"], P[f"{w}.pwmsa.{i}.to_out.0.bias"])
+                o = F.token_linear(wat[i], P[f"{w}.pwmsa.{i}.to_out.0.weight"], P[f"{w}.pwmsa.{i}.to_out.0.bias"])
                 br.append(F.dropout(o, pw["dropout"], training))      # to_out = Sequential(Linear, Dropout) (mswin.py:47)
             sa = w + ".split_attn"
             x = F.split_attn(br[0], br[1], br[2], x, P[sa + ".fc1.weight"], P[sa + ".bn1.weight"], P[sa + ".bn1.bias"], P[sa + ".fc2.weight"])
         f = f"{p}.layers.{di}.1"
         pdrop = enc["feed_forward"]["dropout"]
-        xn = F.layer_norm(x, P[f + ".norm.weight"], P[f + ".norm.bias"])
-        hdn = F.gelu(F.linear(xn, P[f + ".fn.net.0.weight"], P[f + ".fn.net.0.bias"]))
+        z = F.norm_linear(x, P[f + ".norm.weight"], P[f + ".norm.bias"], P[f + ".fn.net.0.weight"], P[f + ".fn.net.0.bias"])
         if pdrop > 0 and training:
-            x = F.dropout(F.linear(F.dropout(hdn, pdrop), P[f + ".fn.net.3.weight"], P[f + ".fn.net.3.bias"]), pdrop, True, x)
+            x = F.dropout(F.token_linear(F.dropout(F.token_gelu(z), pdrop), P[f + ".fn.net.3.weight"], P[f + ".fn.net.3.bias"]), pdrop, True, x)
         else:
-            x = F.linear(hdn, P[f + ".fn.net.3.weight"], P[f + ".fn.net.3.bias"], x)
+            x = F.gelu_linear(z, P[f + ".fn.net.3.weight"], P[f + ".fn.net.3.bias"], x)
     return x[0:1]
 
 
@@ -168,7 +170,8 @@ def _forward_train(model, data_dict):
 
 def forward_train(model, data_dict):
     """One train-mode forward.  torch.autocast around the call (tools/train.py:118) or ``model.amp = True`` selects AMP for THIS
-    step only: the flag lives for the duration of the forward (train_ops.amp_scope) and every node carries it into its backward."""
+    step only: the flag lives for the duration of the forward (train_ops.amp_scope) and every node carries it into its backward.
+    ``model.act8 = True``: the fusion's token layers keep their saved activations in 8 bits (act8_ops)."""
     from .airv2x_where2com import _amp_requested
-    with T.amp_scope(_amp_requested(model)):
+    with T.amp_scope(_amp_requested(model)), T.act8_scope(getattr(model, "act8", False)):
         return _forward_train(model, data_dict)
