@@ -222,10 +222,13 @@ __global__ __launch_bounds__(256, 2) void act8_wgrad_kernel(const float* __restr
     constexpr int XP = KIND == kGelu ? 3 : 1;                        // bf16 terms of X
     constexpr int R = 32, RT = R / 8;                                // rows of a step, of a thread
     constexpr int PLANE = 128 * kPitch;
+    // two buffers where two workgroups of them just fill the 160 KB of a CU: one barrier a step, and a wave writes its part of the next step without waiting
+    constexpr bool TWO = KIND != kGelu;
+    constexpr int BUF = (3 + XP) * PLANE;
     typedef __bf16 bfv __attribute__((ext_vector_type(RT)));
     extern __shared__ __align__(16) char smem[];
-    __bf16* la = reinterpret_cast<__bf16*>(smem);                    // [3][128][R]
-    __bf16* lb = la + 3 * PLANE;                                     // [XP][128][R]
+    __bf16* la = reinterpret_cast<__bf16*>(smem);                    // [buffer][3][128][kPitch]
+    __bf16* lb = la + 3 * PLANE;                                     // [buffer][XP][128][kPitch]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // workgroups go round the eight XCDs: number x of XCD c takes tile x % tiles of share 8 (x / tiles) + c
     const int tiles = tiles_o * tiles_i, xcd = blockIdx.x & 7, local = blockIdx.x >> 3;
@@ -301,17 +304,18 @@ __global__ __launch_bounds__(256, 2) void act8_wgrad_kernel(const float* __restr
             }
         }
     };
-    // one step: its terms go to LDS, the one after next is fetched, the next one is converted between the products
-    auto step = [&](Raw& next, Raw& later) {
+    auto put = [&](int buf) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int at = swz(cg * 4 + e, rc * RT / 8) + rc * RT % 8;
+            const int at = buf * BUF + swz(cg * 4 + e, rc * RT / 8) + rc * RT % 8;
 #pragma unroll
             for (int p = 0; p < 3; ++p) *reinterpret_cast<bfv*>(la + p * PLANE + at) = ta[e][p];
 #pragma unroll
             for (int p = 0; p < XP; ++p) *reinterpret_cast<bfv*>(lb + p * PLANE + at) = tb[e][p];
         }
-        __syncthreads();
+    };
+    // one step: the one after next is fetched, the next one is converted between the products and goes to LDS
+    auto step = [&](Raw& next, Raw& later, int buf) {
         fetch(later);
 #pragma unroll
         for (int ks = 0; ks < R / 16; ++ks) {
@@ -320,9 +324,9 @@ __global__ __launch_bounds__(256, 2) void act8_wgrad_kernel(const float* __restr
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
 #pragma unroll
-                for (int p = 0; p < 3; ++p) A[m][p] = *reinterpret_cast<const bf16x8*>(la + p * PLANE + swz(wo + m * 32 + (lane & 31), chunk));
+                for (int p = 0; p < 3; ++p) A[m][p] = *reinterpret_cast<const bf16x8*>(la + buf * BUF + p * PLANE + swz(wo + m * 32 + (lane & 31), chunk));
 #pragma unroll
-                for (int p = 0; p < XP; ++p) B[m][p] = *reinterpret_cast<const bf16x8*>(lb + p * PLANE + swz(wi + m * 32 + (lane & 31), chunk));
+                for (int p = 0; p < XP; ++p) B[m][p] = *reinterpret_cast<const bf16x8*>(lb + buf * BUF + p * PLANE + swz(wi + m * 32 + (lane & 31), chunk));
             }
             // terms from the smallest products to the largest; the four tiles of a term follow each other, so that no product waits for the one before
             auto term = [&](int pa, int pb) {
@@ -346,6 +350,8 @@ __global__ __launch_bounds__(256, 2) void act8_wgrad_kernel(const float* __restr
             convert(next, ks * 2 + 1);
             term(0, 0);
         }
+        if constexpr (!TWO) __syncthreads();
+        put(TWO ? buf ^ 1 : 0);
         __syncthreads();
     };
     if (r0 < r1) {
@@ -354,12 +360,15 @@ __global__ __launch_bounds__(256, 2) void act8_wgrad_kernel(const float* __restr
 #pragma unroll
         for (int e = 0; e < 4; ++e) convert(u, e);
         fetch(u);
+        put(0);
+        __syncthreads();
         const long long n = (r1 - r0 + R - 1) / R;                   // (two more are fetched and converted: zeros)
         for (long long i = 0; i < n; i += 2) {
-            step(u, v);
-            if (i + 1 < n) step(v, u);
+            step(u, v, 0);
+            if (i + 1 < n) step(v, u, TWO ? 1 : 0);
         }
     }
+    __syncthreads();
     float* slab = slabs + (size_t)split * co * ci;
 #pragma unroll
     for (int a = 0; a < 2; ++a)
@@ -665,7 +674,7 @@ extern "C" int av2x_act8_wgrad(const float* dy, const int8_t* q, const float* sc
     hipStream_t st = av2x::as_stream(stream);
     auto go = [&](auto kd) {
         constexpr int K = decltype(kd)::value;
-        constexpr size_t lds = (size_t)(K == kGelu ? 6 : 4) * 128 * kPitch * 2;
+        constexpr size_t lds = (size_t)(K == kGelu ? 6 : 2 * 4) * 128 * kPitch * 2;
         static av2x::LdsLimit lim;
         lim.ensure((const void*)act8_wgrad_kernel<K>, lds);
         act8_wgrad_kernel<K><<<(unsigned)grid, 256, lds, st>>>(dy, (const unsigned*)q, scale, (const f32x2*)stats, slabs, extra, rows, cout, cin, pl.tiles_o, pl.tiles_i,

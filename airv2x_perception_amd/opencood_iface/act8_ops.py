@@ -130,7 +130,11 @@ def _gemm(r, x, weight, bias, residual):
     return y
 
 
-def _dgrad(dy, weight):
+def _dgrad(dy, weight, amp):
+    """dY W in the forward's precision."""
+    if amp != T.AMP_STEP[0]:
+        with T.amp_scope(amp):
+            return _dgrad(dy, weight, amp)
     cout, cin = weight.shape
     rows = dy.numel() // cout
     if rows == 0:
@@ -193,8 +197,7 @@ class _Linear8(torch.autograd.Function):
         dy = _aligned(dy)
         r = _runner(dy.device)
         need = ctx.needs_input_grad
-        with T.amp_scope(ctx.amp):
-            dx = _dgrad(dy, weight) if need[0] else None
+        dx = _dgrad(dy, weight, ctx.amp) if need[0] else None
         dw = db = None
         if need[1]:
             dw, db = _wgrad(r, 0, dy, q, s, weight.shape[1], want_b=need[2])
@@ -233,8 +236,7 @@ class _NormLinear8(torch.autograd.Function):
         elif need[4]:
             db = _bias_grad(r, dy)
         if need[0]:
-            with T.amp_scope(ctx.amp):
-                dx = _dgrad(dy, weight)
+            dx = _dgrad(dy, weight, ctx.amp)
             # in place: a wave has read its row before it writes it
             _lib.check(r.lib.av2x_act8_layernorm_backward(_P(q), _P(s), _P(stats), _P(gamma), _P(dx), _P(dx), rows, c, r.stream()), "av2x_act8_layernorm_backward")
         return dx, dgamma, dbeta, dw, db
@@ -282,8 +284,7 @@ class _GeluLinear8(torch.autograd.Function):
         need = ctx.needs_input_grad
         dz = dw = db = None
         if need[0]:
-            with T.amp_scope(ctx.amp):
-                dh = _dgrad(dy, weight)
+            dh = _dgrad(dy, weight, ctx.amp)
             dz = _gelu_backward(r, q, s, dh, dh)          # element by element, in place
         if need[1]:
             dw, db = _wgrad(r, 2, dy, q, s, weight.shape[1], want_b=need[2])
