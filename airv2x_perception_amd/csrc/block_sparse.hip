@@ -936,8 +936,9 @@ __device__ __forceinline__ f32x16 mma_d(const typename Held<T>::E* tile, int r, 
 }
 
 // A 32 x 32 tile of P or dS as B operand in two terms: the product then has the precision of fp32 probabilities and the result's own rounding is the only one
-// that counts.  RANGE: the backward's tiles have no largest value to be relative to, and fp16 ends at 2^-24: they are brought to the top of its range by a power of two, and
-// the product brought back (gradients of a scaled or a small loss keep their precision); bf16 has the range.
+// that counts.  RANGE: the backward's tiles have no largest value to be relative to, and fp16 ends at 2^-24: a column (a lane and the one 32 further, in the
+// operand and in the result) is brought to the top of its range by a power of two, and the product brought back (gradients of a scaled or a small loss keep their
+// precision); bf16 has the range.  The first fp16 term is cut, not rounded (one instruction for two): the second, rounded, holds what it leaves.
 template <typename T, bool RANGE> struct Split {
     using E = typename Held<T>::E;
     typename Held<T>::frag hi[2], lo[2];
@@ -948,19 +949,28 @@ template <typename T, bool RANGE> struct Split {
             float m = 0.f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(p[i]));
-#pragma unroll
-            for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+            m = fmaxf(m, __shfl_xor(m, 32));
             back = pow2_over(m);
             to = 1.0f / back;
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float x = RANGE && Held<T>::narrow ? p[s * 8 + e] * to : p[s * 8 + e];
-                const E h = (E)x;
+            for (int e = 0; e < 8; e += 2) {
+                const float x = RANGE && Held<T>::narrow ? p[s * 8 + e] * to : p[s * 8 + e], y = RANGE && Held<T>::narrow ? p[s * 8 + e + 1] * to : p[s * 8 + e + 1];
+                E h, g;
+                if constexpr (Held<T>::narrow) {
+                    const auto c = __builtin_amdgcn_cvt_pkrtz(x, y);
+                    h = (E)c[0];
+                    g = (E)c[1];
+                } else {
+                    h = (E)x;
+                    g = (E)y;
+                }
                 hi[s][e] = h;
+                hi[s][e + 1] = g;
                 lo[s][e] = (E)(x - (float)h);
+                lo[s][e + 1] = (E)(y - (float)g);
             }
     }
 };
@@ -1000,6 +1010,13 @@ __device__ __forceinline__ f32x16 mma_rows(const typename Held<T>::E* a, int pit
 __device__ __forceinline__ unsigned long long seen_keys(const BsArgs& a, int b, int j) {       // visible keys of a block, same in every lane
     const int t = j * kKeys + (threadIdx.x & 63);
     return __ballot(t < a.Nk && (!a.mask || a.mask[(size_t)b * a.Nk + t]));
+}
+
+// scores of keys that are not visible: -inf (rows of a tile of keys x queries)
+__device__ __forceinline__ void hide(f32x16& s, unsigned long long seen, int kt, int half) {
+    const unsigned bits = (unsigned)(seen >> (kt * 32)) >> (4 * half);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = bits >> (8 * (i / 4) + (i & 3)) & 1 ? s[i] : -INFINITY;
 }
 
 // the mention a row stands for: row = mention * G + head of the group
@@ -1077,11 +1094,10 @@ __global__ __launch_bounds__(256) void bs_forward_kernel(BsArgs a) {
         for (int kt = 0; kt < 2; ++kt) {
             s[kt] = mma_d<T, D, false>(lk, kt * 32 + (lane & 31), half, qf, zero16());
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int key = kt * 32 + 8 * (i / 4) + 4 * half + (i & 3);
-                s[kt][i] = seen >> key & 1 ? s[kt][i] * c : -INFINITY;
-                m = fmaxf(m, s[kt][i]);
-            }
+            for (int i = 0; i < 16; ++i) s[kt][i] *= c;
+            if (seen != ~0ull) hide(s[kt], seen, kt, half);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) m = fmaxf(m, s[kt][i]);
         }
         m = fmaxf(m, __shfl_xor(m, 32));
         constexpr float kTop = Held<T>::narrow ? 15.f : 0.f;               // fp16 terms: from the top of their range as well
@@ -1301,7 +1317,9 @@ __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsA
         to_frags<T, D>(load_row<T, D>(static_cast<const T*>(a.dout) + qrow * D, r.in, half), of);
         const f32x2 ld = r.in ? a.ld[qrow] : f32x2{INFINITY, 0.f};         // rows that are not there: P = 0
         ahead = row_of(a, list, len, h, r0 + 128 + (lane & 31));
-        if (half == 0) lld[wave][lane & 31] = f32x4{ld.x, ld.y, qf.back, of.back};
+        // a query's factors: of its scores (powers of two of Q and K, scale), of its dP (dO and V); they go into dS and P of dK and dV too, and leave at the end
+        const float ca = c2 * qf.back, va = vf * of.back;
+        if (half == 0) lld[wave][lane & 31] = f32x4{ca, ld.x, va, ld.y};
 #pragma unroll
         for (int s = 0; s < S::KS; ++s)
 #pragma unroll
@@ -1319,17 +1337,15 @@ __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsA
         f32x16 dq[AT];
 #pragma unroll
         for (int t = 0; t < AT; ++t) dq[t] = zero16();
-        const float ca = c2 * qf.back, va = vf * of.back;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
             // keys x queries
             f32x16 s = mma_d<T, D, false>(lk, kt * 32 + (lane & 31), half, qf, zero16()), p = mma_d<T, D, false>(lv, kt * 32 + (lane & 31), half, of, zero16());
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int key = kt * 32 + 8 * (i / 4) + 4 * half + (i & 3);
-                const float w = seen >> key & 1 ? __builtin_amdgcn_exp2f(s[i] * ca - ld.x) : 0.f;
-                p[i] = w * (p[i] * va - ld.y) * a.scale;
-            }
+            for (int i = 0; i < 16; ++i) s[i] = fmaf(s[i], ca, -ld.x);
+            if (seen != ~0ull) hide(s, seen, kt, half);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(s[i]) * fmaf(p[i], va, -ld.y);
             {
                 const Split<T, true> ds(p);
 #pragma unroll
@@ -1339,18 +1355,13 @@ __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsA
             // queries x keys
             s = mma_d<T, D, true>(lk, kt * 32 + (lane & 31), half, qf, zero16());
             p = mma_d<T, D, true>(lv, kt * 32 + (lane & 31), half, of, zero16());
-            const bool vis = seen >> (kt * 32 + (lane & 31)) & 1;
+            // (keys that are not visible: their columns are left out at the end)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const f32x4 x = lld[wave][8 * (i / 4) + 4 * half + (i & 3)];
-                if constexpr (two) {
-                    const float w = vis ? __builtin_amdgcn_exp2f(s[i] * (c2 * x.z) - x.x) : 0.f;
-                    p[i] = w * (p[i] * (vf * x.w) - x.y) * (a.scale * x.z);
-                    s[i] = w * x.w;
-                } else {
-                    s[i] = vis ? __builtin_amdgcn_exp2f(s[i] * c2 - x.x) : 0.f;
-                    p[i] = s[i] * (p[i] - x.y) * a.scale;
-                }
+                const float w = __builtin_amdgcn_exp2f(fmaf(s[i], x[0], -x[1]));
+                p[i] = w * fmaf(p[i], x[2], -x[3]) * x[0];
+                s[i] = w * x[2];
             }
             {
                 const Split<T, true> rp(s);
@@ -1373,13 +1384,14 @@ __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsA
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int d = t * 32 + 8 * i + 4 * half;
-                    if (d < DA) *reinterpret_cast<f32x4*>(dst + d) = f32x4{dq[t][4 * i], dq[t][4 * i + 1], dq[t][4 * i + 2], dq[t][4 * i + 3]} * kf;
+                    if (d < DA) *reinterpret_cast<f32x4*>(dst + d) = f32x4{dq[t][4 * i], dq[t][4 * i + 1], dq[t][4 * i + 2], dq[t][4 * i + 3]} * (kf * a.scale);
                 }
         }
     }
     // the four waves' sums, in order, through LDS; a block with one work item is done here, others leave a slab
     float* red = reinterpret_cast<float*>(smem);
     const bool whole = len * a.G <= kItemRows;
+    const float dkf = 1.0f / (kLog2e * kf), dvf = 1.0f / vf;               // of the factors above: scale stays in dK
     float* slab = a.slab + ((size_t)bh * a.max_items + blockIdx.x) * 2 * kKeys * D;
 #pragma unroll
     for (int w2 = 0; w2 < 2; ++w2)
@@ -1402,6 +1414,7 @@ __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsA
                 for (int w = 1; w < 4; ++w) y += *reinterpret_cast<const f32x4*>(red + (w * 512 + i) * 4);
                 const int key = kt * 32 + (ln & 31), d = t * 32 + 8 * i4 + 4 * (ln >> 5), tok = j * kKeys + key;
                 if (d >= DA) continue;
+                y = seen >> key & 1 ? y * (w2 ? dvf : dkf) : f32x4{0.f, 0.f, 0.f, 0.f};
                 if (whole) {
                     T* dst = static_cast<T*>(w2 ? a.dv : a.dk);
                     if (dst && tok < a.Nk) tok_store4(dst + (((size_t)b * a.Nk + tok) * a.KV + h) * D + d0 + d, y);
