@@ -179,20 +179,24 @@ __global__ __launch_bounds__(256) void qk_rotate_backward_kernel(RotArgs a) {
         a.partial[((size_t)(i / D) * gridDim.x + blockIdx.x) * D + i % D] = (red[0][i / D][i % D] + red[1][i / D][i % D]) + (red[2][i / D][i % D] + red[3][i / D][i % D]);
 }
 
-// one workgroup per (q | k, 16 channels): 16 x 16 threads, each a strided sum, then the 16 of a channel
-__global__ __launch_bounds__(256) void qk_rotate_dgamma_kernel(const float* __restrict__ partial, int groups, int d, float* dq, float* dk) {
-    __shared__ float red[16][17];
-    const int which = blockIdx.y, c = blockIdx.x * 16 + (threadIdx.x & 15), r = threadIdx.x >> 4;
-    float s = 0.f;
-    for (int i = r; i < groups; i += 16) s += partial[((size_t)which * groups + i) * d + c];
-    red[r][threadIdx.x & 15] = s;
-    __syncthreads();
-    if (r == 0) {
-        s = 0.f;
-        for (int i = 0; i < 16; ++i) s += red[i][threadIdx.x];
-        float* out = which ? dk : dq;
-        if (out) out[c] = s;
+// One workgroup per (q | k, 16 channels): 64 threads a channel take every 64th row, four sums each (a single chain of loads and adds is
+// bound by their latency: 42 us for 2048 groups with 16 threads a channel), then a tree over the 64.  A fixed order for a given number of groups.
+__global__ __launch_bounds__(1024) void qk_rotate_dgamma_kernel(const float* __restrict__ partial, int groups, int d, float* dq, float* dk) {
+    __shared__ float red[64][16];
+    float* out = blockIdx.y ? dk : dq;
+    if (!out) return;
+    const int ch = threadIdx.x & 15, r = threadIdx.x >> 4, c = blockIdx.x * 16 + ch;
+    const float* src = partial + (size_t)blockIdx.y * groups * d + c;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = r; i < groups; i += 256)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] += i + 64 * j < groups ? src[(size_t)(i + 64 * j) * d] : 0.f;
+    red[r][ch] = (s[0] + s[1]) + (s[2] + s[3]);
+    for (int o = 32; o; o >>= 1) {
+        __syncthreads();
+        if (r < o) red[r][ch] += red[r + o][ch];
     }
+    if (r == 0) out[c] = red[0][ch];
 }
 
 template <typename F> int rot_dim(int dim, bool inter, F&& f) {
@@ -283,7 +287,7 @@ extern "C" int av2x_qk_norm_rotate_backward(const void* q, const void* k, const 
         AV2X_TOK_DISPATCH(dtype, T, (qk_rotate_backward_kernel<T, decltype(d)::value, decltype(inter)::value><<<(unsigned)grid, 256, 0, av2x::as_stream(stream)>>>(a)));
         if (int rc = av2x::check_launch("av2x_qk_norm_rotate_backward")) return rc;
         if (!dgamma_q && !dgamma_k) return 0;
-        qk_rotate_dgamma_kernel<<<dim3(dim / 16, 2), 256, 0, av2x::as_stream(stream)>>>(a.partial, (int)grid, dim, dgamma_q, dgamma_k);
+        qk_rotate_dgamma_kernel<<<dim3(dim / 16, 2), 1024, 0, av2x::as_stream(stream)>>>(a.partial, (int)grid, dim, dgamma_q, dgamma_k);
         return av2x::check_launch("av2x_qk_norm_rotate_backward: dgamma");
     });
 }
