@@ -22,6 +22,7 @@ constexpr int kKeys = 64;                    // keys of a block
 constexpr int kMaxPick = 64;                 // blocks a query may have
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kTinyBs = 1e-30f;
+constexpr float kHugeBs = 1e32f;             // keys and queries beyond it, infinities too, count as it: every score is a number (2^24 kHugeBs / 127 < FLT_MAX)
 
 template <typename T> struct is_f32 : std::false_type {};
 template <> struct is_f32<float> : std::true_type {};
@@ -88,6 +89,7 @@ __global__ __launch_bounds__(256) void bs_bounds_kernel(const T* __restrict__ k,
     for (int i = 0; i < 4; ++i) m = fmaxf(m, fmaxf(fabsf(hi[i]), fabsf(lo[i])));
 #pragma unroll
     for (int o = 1; o < LPK; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    m = fminf(m, kHugeBs);
     const float r = 127.0f / fmaxf(m, kTinyBs);
     if (lane < LPK) {
         const size_t at = ((size_t)b * kv + h) * nb + j;
@@ -269,7 +271,7 @@ __global__ __launch_bounds__(256) void bs_select_kernel(const T* __restrict__ q,
             for (int c = 0; c < CH; ++c) m = fmaxf(m, fabsf((float)p[g * qh + c]));
 #pragma unroll
         for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-        const float r = 127.0f / fmaxf(m, kTinyBs);
+        const float r = 127.0f / fminf(fmaxf(m, kTinyBs), kHugeBs);
         float up[CH], lo[CH];
 #pragma unroll
         for (int c = 0; c < CH; ++c) up[c] = lo[c] = 0.f;
@@ -394,7 +396,7 @@ __global__ __launch_bounds__(512, 4) void bs_select16_kernel(const T* __restrict
             for (int c = 0; c < CH; ++c) m = fmaxf(m, fabsf((float)p[g * qh + c]));
 #pragma unroll
         for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-        const float r = 127.0f / fmaxf(m, kTinyBs);
+        const float r = 127.0f / fminf(fmaxf(m, kTinyBs), kHugeBs);
         float up[CH], lo[CH];
 #pragma unroll
         for (int c = 0; c < CH; ++c) up[c] = lo[c] = 0.f;
@@ -804,7 +806,7 @@ __device__ __forceinline__ f32x16 zero16() {
 // the power of two that brings m to 2^14 .. 2^15, the top of fp16: values down to 2^-18 of the largest keep 22 bits in two terms, and what is below that is off by
 // 2^-40 of it at most
 __device__ __forceinline__ float pow2_over(float m) {
-    return m > 1e-30f && m < INFINITY ? ldexpf(1.0f, __builtin_amdgcn_frexp_expf(m) - 15) : 1.0f;
+    return m < INFINITY ? ldexpf(1.0f, max(__builtin_amdgcn_frexp_expf(m) - 15, -126)) : 1.0f;      // (its reciprocal stays finite)
 }
 
 // rows [0, 64) of a block to LDS: [key][d], and [d][key].  Keys behind the end or masked are zeros.  Returns the power of two that was taken out (fp32).
@@ -1267,7 +1269,8 @@ __global__ __launch_bounds__(256) void bs_delta_kernel(const T* __restrict__ out
 
 // One workgroup per work item, four waves of 32 rows.  P and dP are computed twice, as keys x queries for dQ (a lane keeps a query) and as queries x
 // keys for dK, dV (a lane keeps a key): two more products instead of a transpose through LDS.  DA: the part of d whose dK, dV, dQ this workgroup
-// keeps (blockIdx.z-th).  The powers of two of fp32 operands: those of K and V are common to the block, those of a query's Q and dO go into its P and dS.
+// keeps (blockIdx.z-th).  The powers of two of fp32 operands: those of K and V are common to the block and are applied on their own -- in one factor with a
+// query's they would leave fp32's range where both are small --, those of a query's Q and dO go into its dS and P.
 template <typename T, int D, int DA>
 __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsArgs a) {
     using S = Shape<T, D>;
@@ -1317,9 +1320,7 @@ __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsA
         to_frags<T, D>(load_row<T, D>(static_cast<const T*>(a.dout) + qrow * D, r.in, half), of);
         const f32x2 ld = r.in ? a.ld[qrow] : f32x2{INFINITY, 0.f};         // rows that are not there: P = 0
         ahead = row_of(a, list, len, h, r0 + 128 + (lane & 31));
-        // a query's factors: of its scores (powers of two of Q and K, scale), of its dP (dO and V); they go into dS and P of dK and dV too, and leave at the end
-        const float ca = c2 * qf.back, va = vf * of.back;
-        if (half == 0) lld[wave][lane & 31] = f32x4{ca, ld.x, va, ld.y};
+        if (half == 0) lld[wave][lane & 31] = f32x4{qf.back, ld.x, of.back, ld.y};
 #pragma unroll
         for (int s = 0; s < S::KS; ++s)
 #pragma unroll
@@ -1342,10 +1343,10 @@ __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsA
             // keys x queries
             f32x16 s = mma_d<T, D, false>(lk, kt * 32 + (lane & 31), half, qf, zero16()), p = mma_d<T, D, false>(lv, kt * 32 + (lane & 31), half, of, zero16());
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = fmaf(s[i], ca, -ld.x);
+            for (int i = 0; i < 16; ++i) s[i] = fmaf(s[i] * c2, qf.back, -ld.x);
             if (seen != ~0ull) hide(s, seen, kt, half);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(s[i]) * fmaf(p[i], va, -ld.y);
+            for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(s[i]) * fmaf(p[i] * vf, of.back, -ld.y);
             {
                 const Split<T, true> ds(p);
 #pragma unroll
@@ -1359,8 +1360,8 @@ __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsA
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const f32x4 x = lld[wave][8 * (i / 4) + 4 * half + (i & 3)];
-                const float w = __builtin_amdgcn_exp2f(fmaf(s[i], x[0], -x[1]));
-                p[i] = w * fmaf(p[i], x[2], -x[3]) * x[0];
+                const float w = __builtin_amdgcn_exp2f(fmaf(s[i] * c2, x[0], -x[1]));
+                p[i] = w * fmaf(p[i] * vf, x[2], -x[3]) * x[0];
                 s[i] = w * x[2];
             }
             {
@@ -1391,7 +1392,6 @@ __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsA
     // the four waves' sums, in order, through LDS; a block with one work item is done here, others leave a slab
     float* red = reinterpret_cast<float*>(smem);
     const bool whole = len * a.G <= kItemRows;
-    const float dkf = 1.0f / (kLog2e * kf), dvf = 1.0f / vf;               // of the factors above: scale stays in dK
     float* slab = a.slab + ((size_t)bh * a.max_items + blockIdx.x) * 2 * kKeys * D;
 #pragma unroll
     for (int w2 = 0; w2 < 2; ++w2)
@@ -1414,7 +1414,7 @@ __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsA
                 for (int w = 1; w < 4; ++w) y += *reinterpret_cast<const f32x4*>(red + (w * 512 + i) * 4);
                 const int key = kt * 32 + (ln & 31), d = t * 32 + 8 * i4 + 4 * (ln >> 5), tok = j * kKeys + key;
                 if (d >= DA) continue;
-                y = seen >> key & 1 ? y * (w2 ? dvf : dkf) : f32x4{0.f, 0.f, 0.f, 0.f};
+                y = seen >> key & 1 ? y * (w2 ? 1.0f : a.scale) : f32x4{0.f, 0.f, 0.f, 0.f};
                 if (whole) {
                     T* dst = static_cast<T*>(w2 ? a.dv : a.dk);
                     if (dst && tok < a.Nk) tok_store4(dst + (((size_t)b * a.Nk + tok) * a.KV + h) * D + d0 + d, y);
@@ -1472,6 +1472,7 @@ __global__ __launch_bounds__(256) void bs_dq_kernel(BsArgs a, long long rows) {
 
 // ------------------------------------------------------------------------------------------------------------ host
 constexpr int kMaxBlocks = 32768;            // LDS counters of the list kernels: 128 KB
+constexpr int64_t kMaxRows = 0x7fffffff - 4 * kItemRows;      // rows of a block's list: loops step past the last one
 
 int bs_check(const char* what, int32_t B, int32_t T, int32_t Nk, int32_t H, int32_t KV, int32_t D, int32_t n, int32_t dtype) {
     if (D != 16 && D != 32 && D != 64 && D != 128) return av2x::fail("%s: dim %d is not 16, 32, 64 or 128", what, D);
@@ -1480,7 +1481,7 @@ int bs_check(const char* what, int32_t B, int32_t T, int32_t Nk, int32_t H, int3
     if (H / KV > 16 || H / KV * D > 1024) return av2x::fail("%s: %d heads of %d channels share keys (at most 16, 1024 channels)", what, H / KV, D);
     if (n < 1 || n > kMaxPick) return av2x::fail("%s: %d blocks a query (1 .. %d)", what, n, kMaxPick);
     if ((Nk + kKeys - 1) / kKeys > kMaxBlocks) return av2x::fail("%s: %d keys (at most %d)", what, Nk, kMaxBlocks * kKeys);
-    if (T > (1 << 25) || (int64_t)T * n > 0x7fffffff || (int64_t)T * n * (H / KV) > 0x7fffffff || B > 65535 / KV) return av2x::fail("%s: too many queries", what);
+    if (T > (1 << 25) || (int64_t)T * n * (H / KV) > kMaxRows || B > 65535 / KV) return av2x::fail("%s: too many queries", what);
     return 0;
 }
 
@@ -1685,7 +1686,7 @@ extern "C" int av2x_block_sparse_attention(const void* q, const void* k, const v
         if (int rc = bs_rows(what, v, strides + 6, dtype)) return rc;
     }
     const long long mentions = (long long)batch * queries * kv_heads * n;
-    if (!lists && mentions > 0x7fffffff) return av2x::fail("%s: so many queries need lists", what);
+    if (!lists && mentions > 1 << 25) return av2x::fail("%s: so many queries need lists", what);
     BsArgs a = bs_args(q, k, v, mask, blocks, lists, strides, scale, batch, queries, keys, heads, kv_heads, n);
     const Work w = bs_work(batch, queries, keys, heads, kv_heads, dim, n, false);
     char* ws = static_cast<char*>(workspace);

@@ -320,7 +320,7 @@ def _check_sizes(what, b, t, n, h, kv, d, blocks):
         raise ValueError(f"{what}: {h // kv} heads of {d} channels share their keys (at most 16 heads and 1024 channels)")
     if (n + BLOCK - 1) // BLOCK > 32768:
         raise ValueError(f"{what}: {n} keys (at most {32768 * BLOCK})")
-    if t > 1 << 25 or t * blocks * (h // kv) >= 1 << 31 or b * kv > 65535:
+    if t > 1 << 25 or t * blocks * (h // kv) > (1 << 31) - 1 - 4096 or b * kv > 65535:
         raise ValueError(f"{what}: too many queries ({b} x {t})")
 
 

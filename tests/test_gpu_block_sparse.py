@@ -373,3 +373,94 @@ def test_both_forms_on_another_stream_and_in_two_graphs(monkeypatch):
             kept = [[t.clone() for t in got] for _, got in graphs]
             want = step()
             assert all(torch.equal(a, b) for got in kept for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("few", [0, 1 << 30])
+def test_the_most_keys(monkeypatch, few):
+    """32768 blocks: the choice is the formula's, and attention over them is bit for bit that over the chosen ones alone."""
+    from airv2x_perception_amd.opencood_iface import token_attention as A
+    monkeypatch.setattr(A, "FEW_MENTIONS", few)
+    n = 64 * 32768
+    q, k, v, do, _ = make(55, 1, 5, 64 * 50, 2, 1, 16, BF)
+    g = torch.Generator().manual_seed(5)
+    at = torch.randperm(32768, generator=g)[:50].sort()[0]
+    big_k, big_v = (torch.full((1, 32768, 64, 1, 16), 0.01, dtype=BF) for _ in range(2))
+    big_k[0, at], big_v[0, at] = k.view(50, 64, 1, 16), v.view(50, 64, 1, 16)
+    big_k, big_v = big_k.view(1, n, 1, 16).cuda(), big_v.view(1, n, 1, 16).cuda()
+    bounds = A.block_bounds(big_k)
+    for m in (6, 20):
+        blocks = A.select_blocks(q.cuda(), bounds, m)
+        assert torch.equal(blocks.cpu(), chosen_of(q, bounds.ints.cpu(), bounds.scale.cpu(), m))
+    blocks = at[torch.randint(0, 50, (1, 5, 1, 9), generator=g)].int()
+    blocks[0, 0, 0, 0] = 32768                             # one behind the last
+    back = torch.full((32769,), -1, dtype=torch.int32)
+    back[at] = torch.arange(50, dtype=torch.int32)
+    res = []
+    for kk, vv, bl in ((big_k, big_v, blocks), (k.cuda(), v.cuda(), back[blocks.long()])):
+        leaves = [x.detach().clone().requires_grad_() for x in (q.cuda(), kk, vv)]
+        out = A.block_sparse_attention(*leaves, bl.cuda())
+        res.append([out.detach()] + list(torch.autograd.grad(out, leaves, do.cuda())))
+    assert torch.equal(res[0][0], res[1][0]) and torch.equal(res[0][1], res[1][1])
+    for x, y in zip(res[0][2:], res[1][2:]):
+        x = x.view(32768, 64, 1, 16)
+        assert torch.equal(x[at.cuda()].view_as(y), y)
+        x[at.cuda()] = 0
+        assert not x.any()
+    one_more = big_k.new_zeros(1, n + 1, 1, 16)
+    with pytest.raises(ValueError, match="at most"):
+        A.block_sparse_attention(q.cuda(), one_more, one_more, blocks.cuda())
+
+
+@pytest.mark.parametrize("few", [0, 1 << 30])
+def test_offsets_beyond_32_bits(monkeypatch, few):
+    """Tokens 2^20 + 64 elements apart: the last ones lie 2^31 elements (2^32 bytes) behind the first."""
+    from airv2x_perception_amd.opencood_iface import token_attention as A
+    monkeypatch.setattr(A, "FEW_MENTIONS", few)
+    t, step = 2060, (1 << 20) + 64
+    q, k, v, do, mask = [x.cuda() for x in make(65, 1, t, t, 1, 1, 16, BF, "some")]
+    buf = torch.empty((t - 1) * step + 64, dtype=BF, device="cuda")
+    far = [buf.as_strided((1, t, 1, 16), (0, step, 16, 1), 16 * i) for i in range(3)]
+    with torch.no_grad():
+        for x, y in zip(far, (q, k, v)):
+            x.copy_(y)
+    assert far[1][0, -1].data_ptr() - far[1].data_ptr() > 1 << 32
+    res = []
+    for x in (far, (q, k, v)):
+        leaves = [y.detach().requires_grad_() for y in x]
+        bounds = A.block_bounds(leaves[1], mask)
+        blocks = A.select_blocks(leaves[0], bounds, 3)
+        out = A.block_sparse_attention(*leaves, blocks, mask)
+        res.append([bounds.ints, bounds.scale, blocks, out.detach()] + list(torch.autograd.grad(out, leaves, do)))
+    assert all(torch.equal(x, y) for x, y in zip(*res))
+
+
+@pytest.mark.parametrize("few", [0, 1 << 30])
+def test_tiny_and_huge_sizes_in_fp32(monkeypatch, few):
+    """Powers of two on q, k, v and dO (taken out again through the scale) leave the results the same up to powers of two: nothing leaves fp32's range on the way."""
+    from airv2x_perception_amd.opencood_iface import token_attention as A
+    monkeypatch.setattr(A, "FEW_MENTIONS", few)
+    q, k, v, do, _ = [x.cuda() if x is not None else None for x in make(75, 1, 40, 300, 2, 1, 32, F32)]
+    blocks = A.select_blocks(q, A.block_bounds(k), 3)
+
+    def run(eq, ek, ev, eo):
+        leaves = [(x * 2.0 ** e).requires_grad_() for x, e in ((q, eq), (k, ek), (v, ev))]
+        out = A.block_sparse_attention(*leaves, blocks, None, 0.25 * 2.0 ** -(eq + ek))
+        g = torch.autograd.grad(out, leaves, do * 2.0 ** eo)
+        return [x.double() * 2.0 ** -e for x, e in zip((out.detach(), *g), (ev, ev + eo - eq, ev + eo - ek, eo))]
+
+    want = run(0, 0, 0, 0)
+    for e in ((-50, -45, 0, 0), (40, -60, 0, 0), (0, 0, -20, -50), (0, 0, 50, -80), (30, 40, 0, -60)):
+        assert all(torch.equal(x, y) for x, y in zip(run(*e), want)), e
+
+
+def test_selection_with_infinite_and_huge_keys():
+    """A key or query beyond 1e32, an infinity too, counts as 1e32: both selection kernels make the choice of that formula."""
+    from airv2x_perception_amd.opencood_iface import token_attention as A
+    q, k, _, _, _ = make(85, 1, 40, 64 * 40, 1, 1, 16, F32)
+    k[0, 64 * 3 + 1, 0, 2], k[0, 64 * 7, 0, 5], k[0, 64 * 9, 0, 1] = math.inf, -math.inf, 3e38
+    q[0, 4, 0, 3], q[0, 5, 0, 3] = math.inf, -2e35
+    bounds = A.block_bounds(k.cuda())
+    ints, scale = bounds_of(k.clamp(-1e32, 1e32), None)
+    assert torch.equal(bounds.ints.cpu(), ints) and torch.equal(bounds.scale.cpu(), scale)
+    for n in (5, 17):
+        assert torch.equal(A.select_blocks(q.cuda(), bounds, n).cpu(), chosen_of(q.clamp(-1e32, 1e32), ints, scale, n))
