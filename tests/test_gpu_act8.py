@@ -241,3 +241,58 @@ def test_graph_replay_of_a_training_step():
         torch.cuda.synchronize()
         a = [t.clone() for t in got]
         assert all(torch.equal(p, q) for p, q in zip(a, step()))
+
+
+@pytest.mark.parametrize("small", [1 << 30, 0])
+def test_a_recorded_step_sees_the_weights_of_its_replay(monkeypatch, small):
+    """Steps of gradient descent inside a graph against the same steps eagerly: no product of a replay uses an earlier step's weights."""
+    from airv2x_perception_amd.opencood_iface import act8_ops as A
+    monkeypatch.setattr(A, "SMALL_ROWS", small)
+    x, w, b, res, dy, gamma, beta = [t.cuda() for t in data(23, 300, 256, 256)]
+    start = [w, w.flip(0) * 0.5]
+
+    def make():
+        return [torch.nn.Parameter(t.clone()) for t in start]
+
+    def step(ws):
+        y = A.gelu_linear(A.norm_linear(x, gamma, beta, ws[0], b), ws[1], b, x)
+        for p, g in zip(ws, torch.autograd.grad(y, ws, dy)):
+            with torch.no_grad():
+                p.sub_(g, alpha=1e-4)
+        return y.detach()
+
+    eager, ws = make(), make()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(ws)                                                      # warms up, and leaves packings behind
+    torch.cuda.current_stream().wait_stream(s)
+    step(eager)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(ws)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        have = [got.clone()] + [p.detach().clone() for p in ws]
+        want = [step(eager)] + [p.detach() for p in eager]
+        assert all(torch.equal(p, q) for p, q in zip(have, want))
+
+
+def test_more_than_2_31_elements():
+    """The element-wise nodes take them (2^31 + 1280 here); the last rows are as those rows alone."""
+    from airv2x_perception_amd.opencood_iface import act8_ops as A
+    rows, c = (1 << 21) // 2 + 10, 2048
+    x = torch.empty(rows, c, device="cuda").normal_()
+    p = A.pack(x)
+    tail = A.pack(x[-70:])
+    assert torch.equal(p.q[-70:], tail.q) and torch.equal(p.scale[-70 * 16:].view(-1, 16)[-70:], tail.scale)
+    del p
+    z = x.requires_grad_()
+    h = A.gelu(z)
+    last = x[-70:].detach().clone().requires_grad_()
+    assert torch.equal(h[-70:], A.gelu(last))
+    d, = torch.autograd.grad(h, z, x.detach())
+    assert torch.equal(d[-70:], torch.autograd.grad(A.gelu(last), last, last.detach())[0])
+    with pytest.raises(ValueError, match="2\\^31"):
+        A.linear(x, torch.zeros(32, c, device="cuda"))
