@@ -365,14 +365,14 @@ __device__ __forceinline__ int rows_max(int x) {       // the largest of four ro
     return max(max(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16)), max(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48)));
 }
 
-constexpr int kFours = 384;                  // fours of blocks in LDS
+constexpr int kFours = 384;                  // fours of blocks in LDS: six steps of 64, four bits of a word each
 constexpr int kGroupList = 64;               // fours of a query that are looked at in one go
 
 typedef unsigned long long u64;
 typedef u64 u64x2 __attribute__((ext_vector_type(2)));
 
 template <typename T, int D, bool PARTS>
-__global__ __launch_bounds__(512, 4) void bs_select16_kernel(const T* __restrict__ q, long long qb, long long qt, long long qh, const _Float16* __restrict__ ints,
+__global__ __launch_bounds__(512, (D <= 64 ? 4 : 2)) void bs_select16_kernel(const T* __restrict__ q, long long qb, long long qt, long long qh, const _Float16* __restrict__ ints,
                                                              const float* __restrict__ scale, int T_, int G, int KV, int NB, int n, int parts, int per,
                                                              int32_t* __restrict__ out, uint2* __restrict__ part) {
     constexpr int NQ = 32, CH = D / 16, KS = 2 * D / 32, GT = KS <= 2 ? 4 : KS <= 4 ? 2 : 1, GP = kFours + 4, QP = 2 * D + 8;
@@ -382,7 +382,8 @@ __global__ __launch_bounds__(512, 4) void bs_select16_kernel(const T* __restrict
     __shared__ __align__(16) _Float16 qi[NQ * QP];
     // entries: key of the score in the upper half, ~block in the lower one: larger is better, ties to the lower block; 0: none
     __shared__ __align__(16) u64 kept[NQ][16], pend[NQ][32];
-    __shared__ unsigned short fours[NQ][kGroupList];
+    __shared__ __align__(16) unsigned short fours[NQ][kGroupList];               // before them, in the same bytes: 32 maxima of a query's scores
+    static_assert(sizeof(fours[0]) == 32 * sizeof(float), "one row of maxima");
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = lane & 15, row = lane >> 4;
     const int t0 = (PARTS ? blockIdx.x / parts : blockIdx.x) * NQ, h = blockIdx.y, b = blockIdx.z;
     const int first = PARTS ? (blockIdx.x % parts) * per : 0, last = PARTS ? min(NB, first + per) : NB;
@@ -430,6 +431,7 @@ __global__ __launch_bounds__(512, 4) void bs_select16_kernel(const T* __restrict
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int s = 0; s < KS; ++s) bf[u][s] = *reinterpret_cast<const f16x8*>(&qi[(u * 16 + l) * QP + s * 32 + row * 8]);
+            float mx[2] = {-INFINITY, -INFINITY};                                 // over this wave's blocks, one row's share of each tile
             for (int g0 = wave * GT; g0 < steps * 16; g0 += 8 * GT) {
                 f16x8 a[GT][KS];
                 f32x4 w[GT], none[GT];                                            // score = dot * w + none: -inf where there is no block
@@ -474,8 +476,11 @@ __global__ __launch_bounds__(512, 4) void bs_select16_kernel(const T* __restrict
 #pragma unroll
                         for (int i = 1; i < 4; ++i) m = fmaxf(m, fmaf(acc[i], w[g][i], none[g][i]));
                         gm[(u * 16 + l) * GP + (g0 + g) * 4 + row] = m;
+                        mx[u] = fmaxf(mx[u], m);
                     }
             }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) reinterpret_cast<float*>(fours[u * 16 + l])[wave * 4 + row] = mx[u];
         }
         __syncthreads();
         if (t0 + wave * 4 < T_) {
@@ -485,20 +490,21 @@ __global__ __launch_bounds__(512, 4) void bs_select16_kernel(const T* __restrict
             u64 bar = kept[qr][n - 1];
             const bool none = kept[qr][0] == 0ull;
             if (__ballot(none)) {
-                float m = -INFINITY;
-                for (int i = 0; i < steps; ++i) {
-                    const f32x4 x = *reinterpret_cast<const f32x4*>(gp + i * 64);
-                    m = fmaxf(fmaxf(m, fmaxf(x.x, x.y)), fmaxf(x.z, x.w));
-                }
-                const unsigned mk = m == -INFINITY ? 0u : order_key(m);
-                int rank = 0;
-                each_ror<1, 16>([&](auto r) { rank += row_ror<decltype(r)::value>(mk) > mk ? 1 : 0; });
-                unsigned t = rank < n ? mk : 0xffffffffu;
+                const f32x2 m = *reinterpret_cast<const f32x2*>(&fo[l * 4]);
+                const unsigned ma = m.x == -INFINITY ? 0u : order_key(m.x), mb = m.y == -INFINITY ? 0u : order_key(m.y);
+                int ra = mb > ma ? 1 : 0, rb = ma > mb ? 1 : 0;
+                each_ror<1, 16>([&](auto r) {
+                    const unsigned oa = row_ror<decltype(r)::value>(ma), ob = row_ror<decltype(r)::value>(mb);
+                    ra += (oa > ma ? 1 : 0) + (ob > ma ? 1 : 0);
+                    rb += (oa > mb ? 1 : 0) + (ob > mb ? 1 : 0);
+                });
+                unsigned t = min(ra < n ? ma : 0xffffffffu, rb < n ? mb : 0xffffffffu);
                 t = min(t, row_ror<8>(t));
                 t = min(t, row_ror<4>(t));
                 t = min(t, row_ror<2>(t));
                 t = min(t, row_ror<1>(t));
                 if (none && t > 0) bar = (u64)(t - 1) << 32 | 0xffffffffu;
+                __builtin_amdgcn_wave_barrier();
             }
             int pc = 0;
             // sixteen pending entries of every row enter; a loop over what is kept and what is new, two at a time
@@ -506,10 +512,14 @@ __global__ __launch_bounds__(512, 4) void bs_select16_kernel(const T* __restrict
                 const u64 x = pe[l];
                 const int have = __popc((unsigned)(__ballot(k != 0ull) >> (row * 16)) & 0xffffu);
                 int rk = l, rx = 0;
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const u64x2 y = *reinterpret_cast<const u64x2*>(&kept[qr][i]), z = *reinterpret_cast<const u64x2*>(pe + i);
-                    rx += (y[0] > x ? 1 : 0) + (y[1] > x ? 1 : 0) + (z[0] > x ? 1 : 0) + (z[1] > x ? 1 : 0);
+                for (int i = 0; i < n; i += 2) {
+                    const u64x2 y = *reinterpret_cast<const u64x2*>(&kept[qr][i]);
+                    rx += (y[0] > x ? 1 : 0) + (y[1] > x ? 1 : 0);
+                }
+                const int fresh = min(16, rows_max(pc));
+                for (int i = 0; i < fresh; i += 2) {
+                    const u64x2 z = *reinterpret_cast<const u64x2*>(pe + i);
+                    rx += (z[0] > x ? 1 : 0) + (z[1] > x ? 1 : 0);
                     rk += (z[0] > k ? 1 : 0) + (z[1] > k ? 1 : 0);
                 }
                 const u64 later = pe[16 + l];
@@ -527,11 +537,12 @@ __global__ __launch_bounds__(512, 4) void bs_select16_kernel(const T* __restrict
             for (int s0 = 0, span = steps; s0 < steps;) {
                 const int s1 = min(steps, s0 + span);
                 const float thr = bar ? key_score((unsigned)(bar >> 32)) : -INFINITY;      // later fours lose ties
-                int cnt = 0;
-                for (int i = s0; i < s1; ++i) {
+                unsigned hit = 0;                                                 // four bits a step
+                for (int i = s0, bit = 0; i < s1; ++i, bit += 4) {
                     const f32x4 x = *reinterpret_cast<const f32x4*>(gp + i * 64);
-                    cnt += (x.x > thr ? 1 : 0) + (x.y > thr ? 1 : 0) + (x.z > thr ? 1 : 0) + (x.w > thr ? 1 : 0);
+                    hit |= ((x.x > thr ? 1u : 0u) | (x.y > thr ? 2u : 0u) | (x.z > thr ? 4u : 0u) | (x.w > thr ? 8u : 0u)) << bit;
                 }
+                const int cnt = __popc(hit);
                 const int total = row_sum(cnt), most = rows_max(total);
                 if (most > kGroupList && span > 1) { span = 1; continue; }       // many ties: 64 fours of a query at a time
                 if (most > 0) {
@@ -541,13 +552,12 @@ __global__ __launch_bounds__(512, 4) void bs_select16_kernel(const T* __restrict
                     pos += __builtin_amdgcn_update_dpp(0, pos, 0x114, 0xf, 0xf, true);
                     pos += __builtin_amdgcn_update_dpp(0, pos, 0x118, 0xf, 0xf, true);
                     pos -= cnt;
-                    for (int i = s0; i < s1; ++i) {
-                        const f32x4 x = *reinterpret_cast<const f32x4*>(gp + i * 64);
-                        const int g = (i * 16 + l) * 4;
-                        if (x.x > thr) fo[pos++] = (unsigned short)g;
-                        if (x.y > thr) fo[pos++] = (unsigned short)(g + 1);
-                        if (x.z > thr) fo[pos++] = (unsigned short)(g + 2);
-                        if (x.w > thr) fo[pos++] = (unsigned short)(g + 3);
+                    while (__ballot(hit != 0)) {
+                        if (hit) {
+                            const int bit = __ffs((int)hit) - 1;
+                            hit &= hit - 1;
+                            fo[pos++] = (unsigned short)((s0 + (bit >> 2)) * 64 + l * 4 + (bit & 3));
+                        }
                     }
                     __builtin_amdgcn_wave_barrier();
                     // sixteen scores of every query: LB lanes read one block's bounds together (16 bytes each, whole lines) and add up, lane e keeps score e

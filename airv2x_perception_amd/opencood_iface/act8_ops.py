@@ -30,9 +30,12 @@ from .autograd import _P, _runner
 
 GROUP = 128           # channels of one scale
 LN_EPS = 1e-5
-# Up to this many rows the products run on av2x_act8_gemm, which reads the weight as it lies; from there on on the framework's GEMM, whose weights are packed and
-# split into terms first
-SMALL_ROWS = 16384
+# Up to this many multiply-adds the products run on av2x_act8_gemm, which reads the weight as it lies; from there on on the framework's GEMM, whose weights are
+# packed and split into terms first, once for every new value of a weight.  Measured (us, forward + data gradient, packing included, small / large):
+#   256 -> 256    4400 rows: 27 / 40,  16384: 51 / 53,   32768: 98 / 71
+#   256 -> 768    2200 rows: 40 / 60,  4400: 58 / 65,    8192: 69 / 74,   16384: 129 / 97
+#   512 -> 512    2200 rows: 43 / 65,  4400: 73 / 69,    8192: 85 / 78,   16384: 162 / 111
+SMALL_PRODUCT = 1 << 30
 
 
 class Packed8(NamedTuple):
@@ -121,7 +124,7 @@ def _gemm(r, x, weight, bias, residual):
     y = torch.empty(tuple(x.shape[:-1]) + (cout,), dtype=torch.float32, device=x.device)
     if rows == 0:
         return y
-    if rows <= SMALL_ROWS and not T.AMP_STEP[0]:
+    if rows * cin * cout <= SMALL_PRODUCT and not T.AMP_STEP[0]:
         _lib.check(r.lib.av2x_act8_gemm(_P(x), _P(weight), _P(bias), _P(residual), _P(y), rows, cout, cin, 0, r.stream()), "av2x_act8_gemm")
         return y
     wp, coutp, _, ent = T._packed(r, weight.detach().view(cout, cin, 1, 1), owner=_owner(weight))
@@ -144,7 +147,7 @@ def _dgrad(dy, weight, amp):
     rows = dy.numel() // cout
     if rows == 0:
         return torch.empty(tuple(dy.shape[:-1]) + (cin,), dtype=torch.float32, device=dy.device)
-    if rows <= SMALL_ROWS and not T.AMP_STEP[0]:
+    if rows * cin * cout <= SMALL_PRODUCT and not T.AMP_STEP[0]:
         r = _runner(dy.device)
         dx = torch.empty(tuple(dy.shape[:-1]) + (cin,), dtype=torch.float32, device=dy.device)
         _lib.check(r.lib.av2x_act8_gemm(_P(dy), _P(weight), None, None, _P(dx), rows, cin, cout, 1, r.stream()), "av2x_act8_gemm")

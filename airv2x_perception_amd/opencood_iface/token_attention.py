@@ -33,9 +33,13 @@ BLOCK = 64                      # keys of one block
 DIMS = (16, 32, 64, 128)        # channels of a head
 MAX_BLOCKS = 64                 # blocks of one query
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-# Up to this many (query, head group, block) mentions one wave takes each of them; from there on the mentions are sorted by block and a block is
-# read once for all its queries
-FEW_MENTIONS = 8192
+# Few queries: one wave takes each (query, head group, block) mention and reads its block directly.  Many: the mentions are sorted by block and a block is read once
+# for all its queries, which costs four launches and more work items the more blocks there are.  The waves' time goes with heads x channels, so up to this many
+# mentions x heads of a group x max(D, 64) / 64, more by one part in 1536 for every block, the waves are taken.  Measured (us, waves / sorted):
+#   8 heads of 32, bf16          8800 keys: 8192 mentions 19 / 24, 16384: 28 / 25     140800 keys: 16384: 38 / 54, 32768: 64 / 59
+#   8 heads of 64 over 2, bf16   8800 keys: 1024 mentions 23 / 27, 4096: 36 / 34      140800 keys: 4096: 39 / 48, 8192: 64 / 58
+#   4 heads of 128, fp32         8800 keys: 4096 mentions 42 / 43, 8192: 66 / 47      140800 keys: 8192: 77 / 146, 32768: 277 / 251
+FEW_MENTIONS = 12288
 
 
 class BlockBounds(NamedTuple):
@@ -342,7 +346,8 @@ def _attend(q, k, v, blocks, mask, scale, grads):
     out = torch.empty((b, t, h, d), dtype=q.dtype, device=q.device)
     lse = torch.empty((b, t, h), dtype=torch.float32, device=q.device) if grads else None
     rest = torch.empty_like(out) if grads and q.dtype != torch.float32 else None
-    lists = _launch_lists(r, blocks, n, h) if b * t * kv * s > FEW_MENTIONS else None
+    few = b * t * h * s * max(d, 64) <= 64 * FEW_MENTIONS * (1 + (n + BLOCK - 1) // BLOCK / 1536)
+    lists = None if few else _launch_lists(r, blocks, n, h)
     ws = torch.empty(int(r.lib.av2x_block_sparse_workspace_bytes(b, t, n, h, kv, d, s, 0)), dtype=torch.uint8, device=q.device)
     _lib.check(r.lib.av2x_block_sparse_attention(_P(q), _P(k), _P(v), _strides9(q, k, v), _P(mask), _P(blocks), _P(lists), b, t, n, h, kv, d, s, _DTYPES[q.dtype],
                                                  scale, _P(out), _P(lse), _P(rest), _P(ws), r.stream()), "av2x_block_sparse_attention")
