@@ -12,6 +12,7 @@
 // one workgroup holds the block's K and V in LDS and takes the queries that named it through matrix instructions, 32 per wave; every mention
 // writes its (o, max, sum) to a place of its own and a second pass joins the n places of a query.  No atomics: dK and dV of a block are summed
 // by the workgroups that hold it, in the order of its list.  With few queries one wave takes one mention and reads its block directly.
+#include <algorithm>
 #include <type_traits>
 
 #include "token_common.hpp"
@@ -41,7 +42,7 @@ struct BsArgs {
     const int32_t* start;                    // (B KV, NB + 1)
     const int32_t* items;                    // (B KV, max_items) 2 x int32: block, first row
     const int32_t* n_items;                  // (B KV)
-    int max_items;
+    int max_items, item_rows;
     // forward
     void* part;                              // forward: (B, T, H, n) records; backward: (B, T, H, n, D) fp32, dQ
     void* out;                               // (B, T, H, D)
@@ -342,7 +343,10 @@ __global__ __launch_bounds__(256) void bs_select_kernel(const T* __restrict__ q,
 // blocks in LDS (1536 blocks at a time, 50 KB), sixteen lanes a query look for the fours above the n-th best so far -- at first above the n-th largest of
 // the lanes' own maxima, which at least n scores reach -- and only their scores are computed again, exactly, one a lane.  What is above goes to a list of
 // pending entries; sixteen at a time count how many of the kept and of each other are better, which is their place.  Loops, not unrolled
-// code: an unrolled form of this filled the instruction cache (10 000 instructions) and ran at 1490 us where this one takes the time below.
+// code: an unrolled form of this filled the instruction cache (10 000 instructions) and ran at 1490 us.  281600 queries x 2200 blocks of 32 channels, bf16, n = 8:
+// 513 us, 1.2e12 scores a second.  Bound by the vector units: 2100 instructions a wave and four queries, of which the scores take a quarter (the matrix products: 33 us);
+// the rest picks.  n = 1 / 8 / 16: 408 / 478 / 584 us where the kernel above takes 1075 / 1650 / 1812; 35200 queries of 2 x 64 channels x 550 blocks: 78 / 96 / 125 and
+// 178 / 266 / 269; one query x 2200 blocks: 11 / 13 / 21 and 28 / 28 / 28.
 template <int R> __device__ __forceinline__ unsigned row_ror(unsigned x) {
     return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + R, 0xf, 0xf, false);
 }
@@ -512,15 +516,15 @@ __global__ __launch_bounds__(512, (D <= 64 ? 4 : 2)) void bs_select16_kernel(con
                 const u64 x = pe[l];
                 const int have = __popc((unsigned)(__ballot(k != 0ull) >> (row * 16)) & 0xffffu);
                 int rk = l, rx = 0;
-                for (int i = 0; i < n; i += 2) {
-                    const u64x2 y = *reinterpret_cast<const u64x2*>(&kept[qr][i]);
-                    rx += (y[0] > x ? 1 : 0) + (y[1] > x ? 1 : 0);
+                for (int i = 0; i < n; i += 4) {
+                    const u64x2 y = *reinterpret_cast<const u64x2*>(&kept[qr][i]), z = *reinterpret_cast<const u64x2*>(&kept[qr][i + 2]);
+                    rx += (y[0] > x ? 1 : 0) + (y[1] > x ? 1 : 0) + (z[0] > x ? 1 : 0) + (z[1] > x ? 1 : 0);
                 }
                 const int fresh = min(16, rows_max(pc));
-                for (int i = 0; i < fresh; i += 2) {
-                    const u64x2 z = *reinterpret_cast<const u64x2*>(pe + i);
-                    rx += (z[0] > x ? 1 : 0) + (z[1] > x ? 1 : 0);
-                    rk += (z[0] > k ? 1 : 0) + (z[1] > k ? 1 : 0);
+                for (int i = 0; i < fresh; i += 4) {
+                    const u64x2 y = *reinterpret_cast<const u64x2*>(pe + i), z = *reinterpret_cast<const u64x2*>(pe + i + 2);
+                    rx += (y[0] > x ? 1 : 0) + (y[1] > x ? 1 : 0) + (z[0] > x ? 1 : 0) + (z[1] > x ? 1 : 0);
+                    rk += (y[0] > k ? 1 : 0) + (y[1] > k ? 1 : 0) + (z[0] > k ? 1 : 0) + (z[1] > k ? 1 : 0);
                 }
                 const u64 later = pe[16 + l];
                 __builtin_amdgcn_wave_barrier();
@@ -1044,7 +1048,11 @@ __device__ __forceinline__ Row row_of(const BsArgs& a, const int32_t* list, int 
     return x;
 }
 
-constexpr int kItemRows = 1024;              // rows (mentions x heads of the group) of a work item
+// Rows (mentions x heads of the group) of a work item: 1024, which reads K and V once for all queries of a block of average fame, down to 512 where that leaves fewer
+// than 1024 items.  Measured (us, forward / with backward, items of 512 | 1024 | 2048): 35200 x 35200, 8 heads of 32, 8 blocks, fp32: 328 / 1020 | 333 / 1008 | 355 / 1067;
+// 4400 x 8789, 4 of 64, bf16: 54 / 158 | 62 / 180 | 69 / 201; 600 x 35189, 8 of 64 over 2, 16 blocks: 50 / 136 | 58 / 160 | 73 / 212; 256 or 128 there cost
+// the backward more slabs than they bring (4400: 164, 189).
+constexpr int kItemRows = 1024, kItemLeast = 512;
 
 // ------------------------------------------------------------------------------------------------------------ attention, many queries
 // A mention's record: (maximum (scaled, base 2), sum) and the attention over its block alone, next to each other -- they are written to places all over the
@@ -1080,7 +1088,7 @@ __global__ __launch_bounds__(256) void bs_forward_kernel(BsArgs a) {
     const int len = st[1] - st[0];
     const int32_t* list = a.list + (size_t)bh * a.T * a.n + st[0];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    const int last = min(first + kItemRows, len * a.G);
+    const int last = min(first + a.item_rows, len * a.G);
     const T* qbase = static_cast<const T*>(a.q) + b * a.qb;
     // the first queries are on their way before K and V, the next ones during the work on these
     Row r = row_of(a, list, len, h, first + wave * 32 + (lane & 31));
@@ -1316,7 +1324,7 @@ __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsA
             for (int k = 0; k < TERMS; ++k) lq[k * kWaveTile + DA * QP + i] = lo[k * kWaveTile + DA * QP + i] = (E)0.f;
     }
     __syncthreads();
-    const int last = min(first + kItemRows, len * a.G);
+    const int last = min(first + a.item_rows, len * a.G);
     const float c2 = a.scale * kLog2e * kf;
     f32x16 dk[AT][2], dv[AT][2];
 #pragma unroll
@@ -1401,7 +1409,7 @@ __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsA
     }
     // the four waves' sums, in order, through LDS; a block with one work item is done here, others leave a slab
     float* red = reinterpret_cast<float*>(smem);
-    const bool whole = len * a.G <= kItemRows;
+    const bool whole = len * a.G <= a.item_rows;
     float* slab = a.slab + ((size_t)bh * a.max_items + blockIdx.x) * 2 * kKeys * D;
 #pragma unroll
     for (int w2 = 0; w2 < 2; ++w2)
@@ -1441,7 +1449,7 @@ __global__ __launch_bounds__(256) void bs_dkv_kernel(BsArgs a) {
     const int j = blockIdx.x, bh = blockIdx.y, b = bh / a.KV, h = bh % a.KV;
     const int32_t* st = a.start + (size_t)bh * (a.NB + 1) + j;
     const int rows = (st[1] - st[0]) * a.G;
-    if (rows > 0 && rows <= kItemRows) return;
+    if (rows > 0 && rows <= a.item_rows) return;
     // items are in the order of the blocks: the first one of block j
     const int32_t* it = a.items + (size_t)bh * a.max_items * 2;
     const int total = a.n_items[bh];
@@ -1510,12 +1518,13 @@ int bs_runs(int64_t bh, int64_t entries) {
     return (int)(r < 1 ? 1 : r);
 }
 
-struct Lists { int32_t *hist, *start, *list, *items, *n_items; int runs, max_items; size_t bytes; };
+struct Lists { int32_t *hist, *start, *list, *items, *n_items; int runs, max_items, item_rows; size_t bytes; };
 Lists bs_lists(void* base, int32_t B, int32_t T, int32_t Nk, int32_t H, int32_t KV, int32_t n) {
     Lists l{};
     const int64_t bh = (int64_t)B * KV, NB = (Nk + kKeys - 1) / kKeys, entries = (int64_t)T * n, rows = entries * (H / KV);
     l.runs = bs_runs(bh, entries);
-    l.max_items = (int)(rows / kItemRows + NB + 1);
+    l.item_rows = (int)std::min<int64_t>(kItemRows, std::max<int64_t>(kItemLeast, bh * rows / 1024 / 128 * 128));
+    l.max_items = (int)(rows / l.item_rows + NB + 1);
     int32_t* p = static_cast<int32_t*>(base);
     size_t at = 0;
     auto take = [&](int64_t count) { int32_t* r = p ? p + at : nullptr; at += (size_t)((count + 3) & ~3ll); return r; };
@@ -1567,7 +1576,9 @@ extern "C" int av2x_block_bounds(const void* k, const uint8_t* mask, const int64
 namespace {
 
 // Few queries leave the chip idle while a workgroup walks the scores of all blocks: the blocks are cut into ranges of whole chunks until there are
-// about two workgroups a CU, and the ranges' choices joined (one query against 4400 blocks: 9 ranges of one chunk)
+// about two workgroups a CU, and the ranges' choices joined (one query against 4400 blocks: 9 ranges of one chunk).  Measured (us, ranges / one walk):
+// 8 heads of 32, 2200 blocks, n = 8: 1 query 13 / 20, 256: 18 / 23, 496 (the last before the rule): 25 / 24; n = 24: 35 / 84, 60 / 88, 62 / 88;
+// 4 heads of 128: n = 8: 20 / 44, 27 / 57, 45 / 56
 int select_parts(int64_t B, int64_t T, int64_t KV, int64_t NB) {
     const int64_t groups = (T + 15) / 16 * KV * B, chunks = (NB + kChunk - 1) / kChunk;
     if (chunks < 2 || groups >= 256) return 1;
@@ -1636,7 +1647,7 @@ extern "C" int av2x_block_lists(const int32_t* blocks, int32_t batch, int32_t qu
     if (int rc = av2x::check_launch(what)) return rc;
     bs_places_kernel<<<dim3((NB + 63) / 64, bh), 64, 0, st>>>(l.hist, l.runs, NB, l.start);
     if (int rc = av2x::check_launch(what)) return rc;
-    bs_scan_kernel<<<bh, 1024, 0, st>>>(NB, G, kItemRows, l.max_items, l.start, l.items, l.n_items);
+    bs_scan_kernel<<<bh, 1024, 0, st>>>(NB, G, l.item_rows, l.max_items, l.start, l.items, l.n_items);
     if (int rc = av2x::check_launch(what)) return rc;
     bs_fill_kernel<<<dim3(l.runs, bh), 64, lds, st>>>(blocks, queries, kv_heads, NB, n, l.runs, run_len, bits, l.hist, l.start, l.list);
     return av2x::check_launch(what);
@@ -1671,7 +1682,7 @@ BsArgs bs_args(const void* q, const void* k, const void* v, const uint8_t* mask,
     a.scale = scale;
     if (lists) {
         const Lists l = bs_lists(const_cast<void*>(lists), B, T, Nk, H, KV, n);
-        a.list = l.list; a.start = l.start; a.items = l.items; a.n_items = l.n_items; a.max_items = l.max_items;
+        a.list = l.list; a.start = l.start; a.items = l.items; a.n_items = l.n_items; a.max_items = l.max_items; a.item_rows = l.item_rows;
     }
     return a;
 }
