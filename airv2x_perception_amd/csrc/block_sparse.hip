@@ -682,18 +682,53 @@ __global__ __launch_bounds__(256) void bs_count_kernel(const int32_t* __restrict
     for (int j = threadIdx.x; j < NB; j += 256) hp[j] = cnt[j];
 }
 
-__global__ __launch_bounds__(64) void bs_fill_kernel(const int32_t* __restrict__ blocks, int T_, int KV, int NB, int n, int runs, int run_len, int bits,
-                                                     const int32_t* __restrict__ hist, const int32_t* __restrict__ start, int32_t* __restrict__ list) {
-    extern __shared__ int cnt[];
-    const int lane = threadIdx.x, run = blockIdx.x, bh = blockIdx.y, b = bh / KV, h = bh % KV;
-    const int32_t* hp = hist + ((size_t)bh * runs + run) * NB;
-    for (int j = lane; j < NB; j += 64) cnt[j] = hp[j] + start[(size_t)bh * (NB + 1) + j];
-    __syncthreads();
-    const unsigned total = (unsigned)T_ * n, e0 = min(total, (unsigned)run * run_len), e1 = min(total, e0 + run_len);
+// W waves share a run (a part each, in order): a step of 64 mentions is one chain of dependent instructions, about 3000 cycles, so the time is the steps of a
+// wave; more runs would do as well, but each costs counters in memory.  Four waves where their counters fit in 64 KB of LDS, else one.
+template <int W>
+__global__ __launch_bounds__(W * 64) void bs_fill_kernel(const int32_t* __restrict__ blocks, int T_, int KV, int NB, int n, int runs, int run_len, int bits,
+                                                         const int32_t* __restrict__ hist, const int32_t* __restrict__ start, int32_t* __restrict__ list) {
+    extern __shared__ int counters[];                    // [W][NB]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, run = blockIdx.x, bh = blockIdx.y, b = bh / KV, h = bh % KV;
+    const unsigned total = (unsigned)T_ * n, first = min(total, (unsigned)run * run_len), last = min(total, first + run_len);
+    const unsigned part = (run_len / 64 + W - 1) / W * 64, e0 = min(last, first + wave * part), e1 = min(last, e0 + part);
+    int* cnt = counters + wave * NB;
     constexpr int U = 4;
     int j[U], m[U];
+    if constexpr (W > 1) {
+        for (int i = threadIdx.x; i < W * NB; i += W * 64) counters[i] = 0;
+        __syncthreads();
+        for (unsigned e = e0; e < e1; e += U * 64) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) j[u] = mention(blocks, e + u * 64 + lane, e1, (size_t)b * T_, KV, h, n, m[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (j[u] >= 0 && j[u] < NB) atomicAdd(&cnt[j[u]], 1);      // a count: any order
+        }
+        __syncthreads();
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) j[u] = mention(blocks, e0 + u * 64 + lane, e1, (size_t)b * T_, KV, h, n, m[u]);
+    const int32_t *hp = hist + ((size_t)bh * runs + run) * NB, *sp = start + (size_t)bh * (NB + 1);
+    for (int j0 = threadIdx.x; j0 < NB; j0 += 4 * W * 64) {
+        int x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = j0 + i * W * 64;
+            x[i] = at < NB ? hp[at] + sp[at] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = j0 + i * W * 64;
+            if (at >= NB) break;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const int c = W > 1 ? counters[w * NB + at] : 0;
+                counters[w * NB + at] = x[i];
+                x[i] += c;
+            }
+        }
+    }
+    __syncthreads();
     for (unsigned e = e0; e < e1; e += U * 64) {
         int jn[U], mn[U];                                                  // the next mentions are on their way
 #pragma unroll
@@ -1642,14 +1677,15 @@ extern "C" int av2x_block_lists(const int32_t* blocks, int32_t batch, int32_t qu
     hipStream_t st = av2x::as_stream(stream);
     static av2x::LdsLimit lim0, lim1;
     lim0.ensure((const void*)bs_count_kernel, lds);
-    lim1.ensure((const void*)bs_fill_kernel, lds);
+    lim1.ensure((const void*)bs_fill_kernel<1>, lds);
     bs_count_kernel<<<dim3(l.runs, bh), 256, lds, st>>>(blocks, queries, kv_heads, NB, n, l.runs, run_len, l.hist);
     if (int rc = av2x::check_launch(what)) return rc;
     bs_places_kernel<<<dim3((NB + 63) / 64, bh), 64, 0, st>>>(l.hist, l.runs, NB, l.start);
     if (int rc = av2x::check_launch(what)) return rc;
     bs_scan_kernel<<<bh, 1024, 0, st>>>(NB, G, l.item_rows, l.max_items, l.start, l.items, l.n_items);
     if (int rc = av2x::check_launch(what)) return rc;
-    bs_fill_kernel<<<dim3(l.runs, bh), 64, lds, st>>>(blocks, queries, kv_heads, NB, n, l.runs, run_len, bits, l.hist, l.start, l.list);
+    if (4 * lds <= 65536) bs_fill_kernel<4><<<dim3(l.runs, bh), 256, 4 * lds, st>>>(blocks, queries, kv_heads, NB, n, l.runs, run_len, bits, l.hist, l.start, l.list);
+    else bs_fill_kernel<1><<<dim3(l.runs, bh), 64, lds, st>>>(blocks, queries, kv_heads, NB, n, l.runs, run_len, bits, l.hist, l.start, l.list);
     return av2x::check_launch(what);
 }
 
