@@ -1108,7 +1108,7 @@ template <int D, typename PT> struct Record {
 };
 
 template <typename T, int D, typename PT>
-__global__ __launch_bounds__(256) void bs_forward_kernel(BsArgs a) {
+__global__ __launch_bounds__(256, (Held<T>::two ? (D <= 32 ? 3 : D == 64 ? 2 : 1) : (D <= 32 ? 4 : D == 64 ? 3 : 2))) void bs_forward_kernel(BsArgs a) {
     using S = Shape<T, D>;
     using E = typename Held<T>::E;
     constexpr int TERMS = Held<T>::terms;
