@@ -8,12 +8,17 @@
 // over D / 8 lanes that hold both elements of their four pairs -- the rotation needs no exchange, the norm log2(D / 8) shuffles.  Angles:
 // the product pos * freq and its whole part in fp64 (a position of 1e6 keeps its phase), cos / sin of the rest in fp32, once per token
 // and pair in LDS for all its heads.
+// Measured: 140800 tokens x (8 + 8) heads of 32 in fp32: forward 114 us (577 MB, 5.1 TB/s), backward with the values' gradient 230 us (1.15 GB, 5.0 TB/s; a large copy
+// reaches 4.9); 35200 tokens in bf16: 18.6 us; one token 2.8 us.
 #include "token_common.hpp"
 
 namespace {
 
 constexpr int kTurnLds = 2048;     // (cos, sin) pairs a workgroup holds: 16 KB
-constexpr int kBwdGroups = 2048;   // workgroups of the backward pass: rows of the dgamma partials
+// Head vectors per group of lanes and step.  Forward (us at 1 / 2 / 4 / 8 / 16): 140800 x 16 heads of 32 fp32: 117 / 116 / 120 / 125 / 138; 35200 x 8 heads of 128: 57 / 54 / 56 / 62 / 70.
+// Backward, whose steps have two barriers (forward + backward at 4 / 8 / 16): 378 / 369 / 395; 181 / 183 / 191.
+constexpr int kFwdVectors = 2, kBwdVectors = 8;
+constexpr int kBwdGroups = 2048;   // workgroups of the backward pass: rows of the dgamma partials (1024: 35200 tokens in bf16 8 us slower; 4096: no faster)
 
 struct RotArgs {
     const void *x[2];              // q, k
@@ -224,12 +229,15 @@ int rot_check(const char* what, const void* const* ptrs, int n_ptrs, const int64
     return 0;
 }
 
-int rot_tokens(int dim, int nv) {
-    // about eight head vectors per group of lanes and step, the angles of all its tokens in LDS
+// Tokens of a workgroup's step: `vectors` head vectors per group of lanes, the angles of all its tokens in LDS; on short inputs fewer, until there are 512 workgroups
+// (300 tokens: forward 3.7 us, 8.5 without; 8800: 8.0 and 10.4).
+int rot_tokens(int64_t rows, int dim, int nv, int vectors) {
     const int per_step = 256 / (dim / 8);
-    int tok = (8 * per_step + nv - 1) / nv;
+    int tok = (vectors * per_step + nv - 1) / nv;
     if (tok > kTurnLds / (dim / 2)) tok = kTurnLds / (dim / 2);
-    return tok < 1 ? 1 : tok;
+    if (tok < 1) tok = 1;
+    while (tok > 1 && (rows + tok - 1) / tok < 512) tok = (tok + 1) / 2;
+    return tok;
 }
 
 }  // namespace
@@ -246,9 +254,7 @@ extern "C" int av2x_qk_norm_rotate(const void* q, const void* k, const int64_t* 
     a.x[0] = q; a.x[1] = k; a.sr[0] = strides[0]; a.sh[0] = strides[1]; a.sr[1] = strides[2]; a.sh[1] = strides[3];
     a.gamma[0] = gamma_q; a.gamma[1] = gamma_k; a.pos = positions; a.freqs = freqs; a.y[0] = out_q; a.y[1] = out_k;
     a.rows = rows; a.heads[0] = heads; a.heads[1] = kv_heads; a.axes = axes; a.eps = eps;
-    a.tok = rot_tokens(dim, heads + kv_heads);
-    // short inputs: fewer tokens per workgroup until the chip has work (256 CUs)
-    while (a.tok > 1 && (rows + a.tok - 1) / a.tok < 512) a.tok = (a.tok + 1) / 2;
+    a.tok = rot_tokens(rows, dim, heads + kv_heads, kFwdVectors);
     const int64_t grid = (rows + a.tok - 1) / a.tok;
     if (grid > 0x7fffffff) return av2x::fail("av2x_qk_norm_rotate: too many tokens");
     return rot_dim(dim, interleaved != 0, [&](auto d, auto inter) {
@@ -278,8 +284,7 @@ extern "C" int av2x_qk_norm_rotate_backward(const void* q, const void* k, const 
     a.dv = dv; a.vr = dstrides[4]; a.vh = dstrides[5];
     a.partial = static_cast<float*>(workspace);
     a.rows = rows; a.heads[0] = heads; a.heads[1] = kv_heads; a.axes = axes; a.eps = eps;
-    a.tok = rot_tokens(dim, heads + kv_heads);
-    while (a.tok > 1 && (rows + a.tok - 1) / a.tok < 512) a.tok = (a.tok + 1) / 2;
+    a.tok = rot_tokens(rows, dim, heads + kv_heads, kBwdVectors);
     int64_t grid = (rows + a.tok - 1) / a.tok;
     if (grid > kBwdGroups) grid = kBwdGroups;
     if (grid < 1) grid = 1;                       // no tokens: the partials are zeros, and so are the gammas' gradients
