@@ -460,7 +460,8 @@ __global__ __launch_bounds__(1024) void act8_affine_kernel(const float* __restri
 // ------------------------------------------------------------------------------------------------------------ products for few rows
 // Y (rows x n) = A (rows x k) B + bias + residual, all fp32, six products of three bf16 terms each (exact to 2^-24 as the framework's large GEMM), B read as the
 // parameter lies: B = W^T of W (n, k) (forward) or W of W (k, n) (data gradient).  For few rows: the framework's GEMM wants W packed and split first, four
-// launches and their host time where a step has new weights; tiles of 64 x 64 fill the chip sooner (2200 x 256 x 256: 20 us there).
+// launches and their host time where a step has new weights; tiles of 64 x 64 fill the chip sooner (2200 x 256 x 256: 9 us against 19
+// with packing).  A tile's products are few: bound by the loads' latency and the split of both operands.
 // TRANS: B is (k, n): a thread transposes two rows of four columns on the way to LDS.
 constexpr int kSmallK = 32;
 template <bool TRANS>
@@ -569,7 +570,8 @@ struct WgradPlan { int tiles_o, tiles_i, splits; int64_t rows_per; };
 WgradPlan wgrad_plan(int64_t rows, int co, int ci) {
     constexpr int kRows = 64;
     WgradPlan p{(co + 127) / 128, (ci + 127) / 128, 1, kRows};
-    // two workgroups a CU; at least one step of rows each; whole rounds of the XCDs
+    // two workgroups a CU; at least one step of rows each; whole rounds of the XCDs.  (us at 256 / 512 / 1024 shares x tiles: 140800 rows 256 -> 768: 404 / 219 / 229,
+    // 35200 rows: 95 / 64 / 72, 8800 rows 256 -> 256: 23 / 25 / 31)
     int64_t want = 512 / ((int64_t)p.tiles_o * p.tiles_i);
     if (want > 8) want = want / 8 * 8;
     const int64_t steps = (rows + kRows - 1) / kRows;
