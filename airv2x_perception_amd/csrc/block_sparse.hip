@@ -66,21 +66,23 @@ __global__ __launch_bounds__(256) void bs_bounds_kernel(const T* __restrict__ k,
     if (w >= total) return;
     const int lane = threadIdx.x & 63, sub = lane % LPK;
     const int h = (int)(w % kv), j = first + (int)(w / kv % count), b = (int)(w / kv / count);
+    const int key = j * kKeys + lane;
+    const unsigned long long seen = __ballot(key < nk && (!mask || mask[(size_t)b * nk + key]));
+    const int one = seen ? __ffsll(seen) - 1 : 0;        // stands in for keys that are not visible: all loads are in flight together
+    const bool some = seen != 0;
     f32x4 hi{-INFINITY, -INFINITY, -INFINITY, -INFINITY}, lo{INFINITY, INFINITY, INFINITY, INFINITY};
-    int some = 0;
+    if (some) {
+        const T* p = k + b * kb + (long long)j * kKeys * kt + h * kh + sub * 4;
 #pragma unroll
-    for (int s = 0; s < kKeys / KPS; ++s) {
-        const int t = j * kKeys + s * KPS + lane / LPK;
-        if (t < nk && (!mask || mask[(size_t)b * nk + t])) {
-            const f32x4 x = tok_load4(k + b * kb + t * kt + h * kh + sub * 4);
-            some = 1;
+        for (int s = 0; s < kKeys / KPS; ++s) {
+            const int t = s * KPS + lane / LPK;
+            const f32x4 x = tok_load4(p + (seen >> t & 1 ? t : one) * kt);
 #pragma unroll
             for (int i = 0; i < 4; ++i) { hi[i] = fmaxf(hi[i], x[i]); lo[i] = fminf(lo[i], x[i]); }
         }
     }
 #pragma unroll
     for (int o = LPK; o < 64; o <<= 1) {
-        some |= __shfl_xor(some, o);
 #pragma unroll
         for (int i = 0; i < 4; ++i) { hi[i] = fmaxf(hi[i], __shfl_xor(hi[i], o)); lo[i] = fminf(lo[i], __shfl_xor(lo[i], o)); }
     }
@@ -753,25 +755,34 @@ __global__ __launch_bounds__(W * 64) void bs_fill_kernel(const int32_t* __restri
     }
 }
 
-// counts of the runs -> places within a block's list, and its length
-__global__ __launch_bounds__(64) void bs_places_kernel(int32_t* __restrict__ hist, int runs, int NB, int32_t* __restrict__ len) {
-    const int j = blockIdx.x * 64 + threadIdx.x, bh = blockIdx.y;
-    if (j >= NB) return;
+// counts of the runs -> places within a block's list, and its length.  64 blocks a workgroup, 16 threads a block with a stretch of the runs each
+__global__ __launch_bounds__(1024) void bs_places_kernel(int32_t* __restrict__ hist, int runs, int NB, int32_t* __restrict__ len) {
+    __shared__ int sums[16][64];
+    const int c = threadIdx.x & 63, part = threadIdx.x >> 6, j = blockIdx.x * 64 + c, bh = blockIdx.y;
+    const int per = (runs + 15) / 16, r0 = min(runs, part * per), r1 = min(runs, r0 + per);
     int32_t* hp = hist + (size_t)bh * runs * NB + j;
-    int sum = 0, r = 0;
-    for (; r + 8 <= runs; r += 8) {
-        int c[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = hp[(size_t)(r + i) * NB];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) { hp[(size_t)(r + i) * NB] = sum; sum += c[i]; }
+    int sum = 0;
+    if (j < NB) {
+#pragma unroll 8
+        for (int r = r0; r < r1; ++r) sum += hp[(size_t)r * NB];
     }
-    for (; r < runs; ++r) {
-        const int c = hp[(size_t)r * NB];
-        hp[(size_t)r * NB] = sum;
-        sum += c;
+    sums[part][c] = sum;
+    __syncthreads();
+    if (j >= NB) return;
+    int at = 0;
+    for (int p = 0; p < part; ++p) at += sums[p][c];
+    if (part == 15) len[(size_t)bh * (NB + 1) + j] = at + sum;
+    for (int r = r0; r < r1; r += 8) {
+        int x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = r + i < r1 ? hp[(size_t)(r + i) * NB] : 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (r + i < r1) {
+                hp[(size_t)(r + i) * NB] = at;
+                at += x[i];
+            }
     }
-    len[(size_t)bh * (NB + 1) + j] = sum;
 }
 
 // one workgroup per (sample, kv head): lengths -> starts of the lists (in place), work items of at most `rows` rows
@@ -1680,7 +1691,7 @@ extern "C" int av2x_block_lists(const int32_t* blocks, int32_t batch, int32_t qu
     lim1.ensure((const void*)bs_fill_kernel<1>, lds);
     bs_count_kernel<<<dim3(l.runs, bh), 256, lds, st>>>(blocks, queries, kv_heads, NB, n, l.runs, run_len, l.hist);
     if (int rc = av2x::check_launch(what)) return rc;
-    bs_places_kernel<<<dim3((NB + 63) / 64, bh), 64, 0, st>>>(l.hist, l.runs, NB, l.start);
+    bs_places_kernel<<<dim3((NB + 63) / 64, bh), 1024, 0, st>>>(l.hist, l.runs, NB, l.start);
     if (int rc = av2x::check_launch(what)) return rc;
     bs_scan_kernel<<<bh, 1024, 0, st>>>(NB, G, l.item_rows, l.max_items, l.start, l.items, l.n_items);
     if (int rc = av2x::check_launch(what)) return rc;
