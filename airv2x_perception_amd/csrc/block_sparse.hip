@@ -56,7 +56,8 @@ struct BsArgs {
 };
 
 // ------------------------------------------------------------------------------------------------------------ bounds
-// one wave per (block, kv head): D / 4 lanes a key, 256 / D keys a step
+// One wave per (block, kv head): D / 4 lanes a key, 256 / D keys a step.  Bound by HBM: K is read once (140800 keys x 8 heads of 32, bf16: 15 us, 4.7 TB/s; 26 us where each
+// load waits for its key's mask).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void bs_bounds_kernel(const T* __restrict__ k, const uint8_t* __restrict__ mask, long long kb, long long kt, long long kh,
                                                         int nk, int kv, int nb, int first, int count, _Float16* __restrict__ ints, float* __restrict__ scale,
@@ -656,8 +657,8 @@ __global__ __launch_bounds__(64) void bs_select_join_kernel(const uint2* __restr
 
 // ------------------------------------------------------------------------------------------------------------ lists
 // Counting sort of the mentions of a (sample, kv head) by block, in three launches: counts of `runs` runs of mentions, places, fill.  In the fill one wave
-// takes a run in order; equal blocks among its 64 lanes are found with one ballot per bit of the block number, counters live in LDS.  Same lists
-// whatever the timing.
+// takes a run (or a part of one) in order; equal blocks among its 64 lanes are found with one ballot per bit of the block number, counters live in LDS.  Same
+// lists whatever the timing.  Bound by latency: 2.25 million mentions of 2200 blocks: count 7, places 8, scan 7, fill 37 us.
 __device__ __forceinline__ int mention(const int32_t* blocks, unsigned e, unsigned e1, size_t bt0, int KV, int h, unsigned n, int& m) {
     if (e >= e1) return -1;
     const unsigned t = e / n, s = e - t * n;
@@ -829,7 +830,7 @@ __global__ __launch_bounds__(1024) void bs_scan_kernel(int NB, int G, int rows, 
 //
 // fp32 tensors run on the same instructions as two fp16 terms each: a row (queries, dO) or a block (K, V) is brought to the top of fp16's range by a power of two,
 // hi + lo hold it to 22 bits, three products of terms make one product.  Three 16-bit MFMAs take 3 / 16 of the time of the fp32 instruction
-// (backward of 281600 queries x 8 blocks: 1204 us with v_mfma_f32_32x32x2_f32).
+// (backward of 281600 queries x 8 blocks: 597 us, 1204 with v_mfma_f32_32x32x2_f32).
 template <typename T> struct Op;
 template <> struct Op<__bf16> {
     typedef __bf16 frag __attribute__((ext_vector_type(8)));
@@ -1118,6 +1119,9 @@ template <int D, typename PT> struct Record {
     }
 };
 
+// 281600 queries x 8 blocks of 32 channels: bf16 170 us, fp32 206 us.  The products take 25 and 48 us at the matrix cores' measured rate, the records 33 and 73 us at HBM's; the
+// vector units bound it: about 20 instructions for each score a lane holds (scaling, maximum, exponential, sum, two terms).  The launch bounds keep one more wave
+// on a SIMD than the compiler would (heads of 64 fp32: 136 us against 166, of 128 bf16: 103 against 115).
 template <typename T, int D, typename PT>
 __global__ __launch_bounds__(256, (Held<T>::two ? (D <= 32 ? 3 : D == 64 ? 2 : 1) : (D <= 32 ? 4 : D == 64 ? 3 : 2))) void bs_forward_kernel(BsArgs a) {
     using S = Shape<T, D>;
@@ -1199,7 +1203,8 @@ __global__ __launch_bounds__(256, (Held<T>::two ? (D <= 32 ? 3 : D == 64 ? 2 : 1
 }
 
 // ------------------------------------------------------------------------------------------------------------ attention, few queries
-// one wave per mention, all heads of its group: a lane per key for the scores, D / 8 lanes per key for the values
+// One wave per mention, all heads of its group: a lane per key for the scores, D / 8 lanes per key for the values.  Bound by the latency of two rounds of loads
+// (one query x 8 heads x 16 blocks: 5.5 us).
 template <typename T, int D, typename PT>
 __global__ __launch_bounds__(64) void bs_few_kernel(BsArgs a) {
     __shared__ __align__(16) float lq[D];
@@ -1262,7 +1267,7 @@ __global__ __launch_bounds__(64) void bs_few_kernel(BsArgs a) {
     }
 }
 
-// the n places of a query joined: D / 4 lanes a (query, head).  rest: what the output's rounding took away, for the backward's sum dO O
+// The n places of a query joined: D / 4 lanes a (query, head).  Bound by HBM (281600 x 8 records of 72 bytes: 53 us; of 136 bytes: 75 us, 4.6 TB/s).  rest: what the output's rounding took away, for the backward's sum dO O
 template <typename T, int D, typename PT>
 __global__ __launch_bounds__(256) void bs_join_kernel(BsArgs a, long long rows) {
     constexpr int L = D / 4;
@@ -1335,6 +1340,8 @@ __global__ __launch_bounds__(256) void bs_delta_kernel(const T* __restrict__ out
 // keys for dK, dV (a lane keeps a key): two more products instead of a transpose through LDS.  DA: the part of d whose dK, dV, dQ this workgroup
 // keeps (blockIdx.z-th).  The powers of two of fp32 operands: those of K and V are common to the block and are applied on their own -- in one factor with a
 // query's they would leave fp32's range where both are small --, those of a query's Q and dO go into its dS and P.
+// 281600 queries x 8 blocks of 32 channels, fp32: 597 us; 17600 x 8 of 64, bf16: 81 us.  Seven products (three terms each in fp32: 194 GFLOP, 170 us at the matrix cores'
+// measured rate); the vector units bound it: two exponentials and four splits into terms for every score, at two waves a SIMD (256 registers).
 template <typename T, int D, int DA>
 __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsArgs a) {
     using S = Shape<T, D>;
