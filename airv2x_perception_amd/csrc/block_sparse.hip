@@ -870,11 +870,12 @@ __device__ __forceinline__ float pow2_over(float m) {
     return m < INFINITY ? ldexpf(1.0f, max(__builtin_amdgcn_frexp_expf(m) - 15, -126)) : 1.0f;      // (its reciprocal stays finite)
 }
 
-// rows [0, 64) of a block to LDS: [key][d], and [d][key].  Keys behind the end or masked are zeros.  Returns the power of two that was taken out (fp32).
+// rows [0, 64) of a block to LDS: [key][d], and [d][key] of DA channels from d0 on.  Keys behind the end or masked are zeros.  Returns the power of two that was taken out (fp32).
 // All 256 threads; ends with the writes, not with a barrier.
-template <typename T, int D, bool ROW, bool TRANS>
-__device__ __forceinline__ float load_block(const T* src, long long st, int t0, unsigned long long seen, typename Held<T>::E* row, typename Held<T>::E* tr, float* red) {
+template <typename T, int D, bool ROW, bool TRANS, int DA = D>
+__device__ __forceinline__ float load_block(const T* src, long long st, int t0, unsigned long long seen, typename Held<T>::E* row, typename Held<T>::E* tr, float* red, int d0 = 0) {
     using S = Shape<T, D>;
+    constexpr int kTrans = Shape<T, DA>::kTransTile;
     using E = typename Held<T>::E;
     constexpr int CPR = D / 8, N = kKeys * CPR / 256 > 0 ? kKeys * CPR / 256 : 1;
     typedef T vec __attribute__((ext_vector_type(8)));
@@ -924,15 +925,18 @@ __device__ __forceinline__ float load_block(const T* src, long long st, int t0, 
             }
             if constexpr (ROW) *reinterpret_cast<evec*>(row + k * S::kRowTile + key * S::P + c * 8) = y;
             if constexpr (TRANS) {
+                const int d = c * 8 - d0;
+                if (DA == D || (d >= 0 && d < DA)) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) tr[k * S::kTransTile + (c * 8 + e) * S::PT + key] = y[e];
+                    for (int e = 0; e < 8; ++e) tr[k * kTrans + (d + e) * S::PT + key] = y[e];
+                }
             }
         }
     }
     if constexpr (TRANS && D < 32) {
         for (int i = threadIdx.x; i < (32 - D) * S::PT; i += 256)
 #pragma unroll
-            for (int k = 0; k < Held<T>::terms; ++k) tr[k * S::kTransTile + D * S::PT + i] = (E)0.f;
+            for (int k = 0; k < Held<T>::terms; ++k) tr[k * kTrans + D * S::PT + i] = (E)0.f;
     }
     return back;
 }
@@ -1350,12 +1354,13 @@ __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsA
     constexpr int TERMS = Held<T>::terms;
     constexpr int AT = (DA + 31) / 32;                                     // d tiles of this workgroup
     constexpr int QP = 32 + 4, kWaveTile = AT * 32 * QP;                   // per-wave tile of 32 rows: [d][row], of one term
-    constexpr size_t kTiles = sizeof(E) * TERMS * (2 * S::kRowTile + S::kTransTile + 8 * kWaveTile);
+    constexpr int kTrans = Shape<T, DA>::kTransTile;
+    constexpr size_t kTiles = sizeof(E) * TERMS * (2 * S::kRowTile + kTrans + 8 * kWaveTile);
     __shared__ __align__(16) char smem[kTiles > 32768 ? kTiles : 32768];   // the last sums take 32 KB
     E* lk = reinterpret_cast<E*>(smem);
     E* lv = lk + TERMS * S::kRowTile;
     E* lkt = lv + TERMS * S::kRowTile;
-    E* lqs = lkt + TERMS * S::kTransTile;
+    E* lqs = lkt + TERMS * kTrans;
     __shared__ __align__(16) f32x4 lld[4][32];
     __shared__ float red4[2][4];
     const int bh = blockIdx.y, b = bh / a.KV, h = bh % a.KV, d0 = blockIdx.z * DA;
@@ -1366,7 +1371,7 @@ __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsA
     const int len = st[1] - st[0];
     const int32_t* list = a.list + (size_t)bh * a.T * a.n + st[0];
     const unsigned long long seen = seen_keys(a, b, j);
-    const float kf = load_block<T, D, true, true>(static_cast<const T*>(a.k) + b * a.kb + h * a.kh, a.kt, j * kKeys, seen, lk, lkt, red4[0]);
+    const float kf = load_block<T, D, true, true, DA>(static_cast<const T*>(a.k) + b * a.kb + h * a.kh, a.kt, j * kKeys, seen, lk, lkt, red4[0], d0);
     const float vf = load_block<T, D, true, false>(static_cast<const T*>(a.v) + b * a.vb + h * a.vh, a.vt, j * kKeys, seen, lv, nullptr, red4[1]);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     E* lq = lqs + wave * 2 * TERMS * kWaveTile;
@@ -1421,7 +1426,7 @@ __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsA
             {
                 const Split<T, true> ds(p);
 #pragma unroll
-                for (int t = 0; t < AT; ++t) dq[t] = mma_rows<T>(lkt + (d0 + t * 32) * S::PT + kt * 32, S::PT, S::kTransTile, lane, ds, dq[t]);
+                for (int t = 0; t < AT; ++t) dq[t] = mma_rows<T>(lkt + t * 32 * S::PT + kt * 32, S::PT, kTrans, lane, ds, dq[t]);
             }
             __builtin_amdgcn_sched_barrier(0);                             // one part's registers at a time
             // queries x keys
@@ -1694,8 +1699,10 @@ extern "C" int av2x_block_lists(const int32_t* blocks, int32_t batch, int32_t qu
     const size_t lds = (size_t)NB * 4;
     hipStream_t st = av2x::as_stream(stream);
     static av2x::LdsLimit lim0, lim1;
-    lim0.ensure((const void*)bs_count_kernel, lds);
-    lim1.ensure((const void*)bs_fill_kernel<1>, lds);
+    if (lds > 65536) {                                   // one limit for all sizes: calls of other threads never lower it
+        lim0.ensure((const void*)bs_count_kernel, kMaxBlocks * 4);
+        lim1.ensure((const void*)bs_fill_kernel<1>, kMaxBlocks * 4);
+    }
     bs_count_kernel<<<dim3(l.runs, bh), 256, lds, st>>>(blocks, queries, kv_heads, NB, n, l.runs, run_len, l.hist);
     if (int rc = av2x::check_launch(what)) return rc;
     bs_places_kernel<<<dim3((NB + 63) / 64, bh), 1024, 0, st>>>(l.hist, l.runs, NB, l.start);
@@ -1816,7 +1823,7 @@ extern "C" int av2x_block_sparse_attention_backward(const void* q, const void* k
     hipStream_t st = av2x::as_stream(stream);
     return bs_go(dtype, dim, [&](auto t, auto d) {
         using T = typename decltype(t)::type;
-        constexpr int D = decltype(d)::value, DA = D <= 64 ? D : Held<T>::two ? 32 : 64;      // fp32 heads of 128: what fits LDS
+        constexpr int D = decltype(d)::value, DA = D <= 64 ? D : 64;      // heads of 128: what fits LDS and registers
         const long long rows = (long long)batch * queries * heads;
         const unsigned by_row = (unsigned)((rows * (D / 4) + 255) / 256);
         bs_delta_kernel<T, D><<<by_row, 256, 0, st>>>(static_cast<const T*>(out), static_cast<const T*>(rest), static_cast<const T*>(dout), lse, ld, rows);

@@ -15,7 +15,8 @@ derivative taken at x8 instead of x:
     gelu(_linear) dW = dY^T gelu(z8)                     dz = (dY W) gelu'(z8)
 
 A group with an infinity or a NaN has a NaN scale: the gradients show it, as they would without the 8 bits (GradScaler's check works).
-``model.act8 = True`` trains Airv2xCoBEVT / Airv2xV2XVit's fusion with these nodes (train_ops.act8_scope).
+A step can be captured into a HIP graph, while no eager graph of the same leaves is alive (torch's engine would wait for the stream of a leaf's old node); its weights are
+packed on every replay.  ``model.act8 = True`` trains Airv2xCoBEVT / Airv2xV2XVit's fusion with these nodes (train_ops.act8_scope).
 """
 from __future__ import annotations
 

@@ -11,7 +11,8 @@ rotation instead of a table tied to a window:
     out = block_sparse_attention(q, k, v, blocks, mask)
 
 Tensors are fp32, bf16 or fp16 on the current HIP device; sums, softmax statistics and gradients of gammas are fp32.  There is no CPU path.
-Everything runs on the current stream and allocates through torch: a step can be captured into a HIP graph.
+Everything runs on the current stream and allocates through torch: a step can be captured into a HIP graph.  (A backward pass only while no eager graph of the same
+leaves is alive: torch's engine waits for the stream of a leaf's old node, which ends the capture and the process.)
 """
 from __future__ import annotations
 
