@@ -347,8 +347,9 @@ __global__ __launch_bounds__(256) void bs_select_kernel(const T* __restrict__ q,
 // the lanes' own maxima, which at least n scores reach -- and only their scores are computed again, exactly, one a lane.  What is above goes to a list of
 // pending entries; sixteen at a time count how many of the kept and of each other are better, which is their place.  Loops, not unrolled
 // code: an unrolled form of this filled the instruction cache (10 000 instructions) and ran at 1490 us.  281600 queries x 2200 blocks of 32 channels, bf16, n = 8:
-// 513 us, 1.2e12 scores a second.  Bound by the vector units: 2100 instructions a wave and four queries, of which the scores take a quarter (the matrix products: 33 us);
-// the rest picks.  n = 1 / 8 / 16: 408 / 478 / 584 us where the kernel above takes 1075 / 1650 / 1812; 35200 queries of 2 x 64 channels x 550 blocks: 78 / 96 / 125 and
+// 513 us, 1.2e12 scores a second.  Without the picking it takes two thirds of that, half of which is the bounds' way from L2 (2.5 GB, once for every 32 queries: 8 TB/s);
+// the matrix products are 33 us.  64 queries a workgroup halve those bytes but leave one workgroup a CU, whose scores and picks no longer overlap (568 us against 479
+// under the same clock); the next tiles fetched ahead gained nothing.  n = 1 / 8 / 16: 408 / 478 / 584 us where the kernel above takes 1075 / 1650 / 1812; 35200 queries of 2 x 64 channels x 550 blocks: 78 / 96 / 125 and
 // 178 / 266 / 269; one query x 2200 blocks: 11 / 13 / 21 and 28 / 28 / 28.
 template <int R> __device__ __forceinline__ unsigned row_ror(unsigned x) {
     return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + R, 0xf, 0xf, false);
@@ -439,11 +440,15 @@ __global__ __launch_bounds__(512, (D <= 64 ? 4 : 2)) void bs_select16_kernel(con
 #pragma unroll
                 for (int s = 0; s < KS; ++s) bf[u][s] = *reinterpret_cast<const f16x8*>(&qi[(u * 16 + l) * QP + s * 32 + row * 8]);
             float mx[2] = {-INFINITY, -INFINITY};                                 // over this wave's blocks, one row's share of each tile
-            for (int g0 = wave * GT; g0 < steps * 16; g0 += 8 * GT) {
+            // a wave takes GT neighbouring tiles at a time; tiles too few for all waves go round them one by one, so that every row has maxima for the first bound
+            // (4400 queries x 138 blocks, n = 8 / 16: 26 / 36 us, 33 / 55 with neighbouring tiles; 35200 x 550, n = 8: 218 and 211 the other way)
+            const bool spread = steps * 16 < 8 * GT;
+            const int gs = spread ? 8 : 1;
+            for (int g0 = spread ? wave : wave * GT; g0 < steps * 16; g0 += 8 * GT) {
                 f16x8 a[GT][KS];
                 f32x4 w[GT], none[GT];                                            // score = dot * w + none: -inf where there is no block
                 const int jr = j0 + g0 * 16;
-                if (jr + GT * 16 <= last) {
+                if (!spread && jr + GT * 16 <= last) {
                     const _Float16* p = kp + (unsigned)((jr + l) * 2 * D + row * 8);
 #pragma unroll
                     for (int g = 0; g < GT; ++g) {
@@ -454,12 +459,12 @@ __global__ __launch_bounds__(512, (D <= 64 ? 4 : 2)) void bs_select16_kernel(con
                 } else {
 #pragma unroll
                     for (int g = 0; g < GT; ++g) {
-                        const int ja = min(jr + g * 16 + l, NB - 1);
+                        const int jg = jr + g * gs * 16, ja = min(jg + l, NB - 1);
 #pragma unroll
                         for (int s = 0; s < KS; ++s) a[g][s] = *reinterpret_cast<const f16x8*>(kp + (unsigned)(ja * 2 * D + s * 32 + row * 8));
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const int j = jr + g * 16 + row * 4 + i;
+                            const int j = jg + row * 4 + i;
                             const float x = sp[min(j, NB - 1)];
                             w[g][i] = j < last ? x : -1.0f;
                         }
@@ -473,7 +478,9 @@ __global__ __launch_bounds__(512, (D <= 64 ? 4 : 2)) void bs_select16_kernel(con
                         w[g][i] = fmaxf(w[g][i], 0.f);
                     }
 #pragma unroll
-                for (int g = 0; g < GT; ++g)
+                for (int g = 0; g < GT; ++g) {
+                    const int tile = g0 + g * gs;
+                    if (tile >= steps * 16) break;
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         f32x4 acc{0.f, 0.f, 0.f, 0.f};
@@ -482,9 +489,10 @@ __global__ __launch_bounds__(512, (D <= 64 ? 4 : 2)) void bs_select16_kernel(con
                         float m = fmaf(acc[0], w[g][0], none[g][0]);
 #pragma unroll
                         for (int i = 1; i < 4; ++i) m = fmaxf(m, fmaf(acc[i], w[g][i], none[g][i]));
-                        gm[(u * 16 + l) * GP + (g0 + g) * 4 + row] = m;
+                        gm[(u * 16 + l) * GP + tile * 4 + row] = m;
                         mx[u] = fmaxf(mx[u], m);
                     }
+                }
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) reinterpret_cast<float*>(fours[u * 16 + l])[wave * 4 + row] = mx[u];
