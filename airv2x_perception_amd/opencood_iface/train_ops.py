@@ -97,10 +97,12 @@ _ZEROS = {}
 
 
 def _zeros(c, device):
-    """Cached all-zero shift vector (read-only)."""
+    """Cached all-zero shift vector (read-only).  One that is first needed while a graph is recorded belongs to that graph: it holds zeros from its replay on only."""
     z = _ZEROS.get((c, device))
     if z is None:
-        z = _ZEROS[(c, device)] = torch.zeros(c, device=device)
+        z = torch.zeros(c, device=device)
+        if not torch.cuda.is_current_stream_capturing():
+            _ZEROS[(c, device)] = z
     return z
 
 

@@ -279,6 +279,27 @@ def test_a_recorded_step_sees_the_weights_of_its_replay(monkeypatch, small):
         assert all(torch.equal(p, q) for p, q in zip(have, want))
 
 
+def test_a_recording_leaves_nothing_behind(monkeypatch):
+    """A Linear without a bias, first run while a graph is recorded: neither its zeros nor its packings are taken by later eager calls."""
+    from airv2x_perception_amd.opencood_iface import act8_ops as A, train_ops as T
+    monkeypatch.setattr(A, "SMALL_PRODUCT", 0)
+    x, w, b, res, dy, gamma, beta = [t.cuda() for t in data(29, 300, 256, 256)]
+    w = torch.nn.Parameter(w)
+    want = A.linear(x, w).detach()
+    monkeypatch.setattr(T, "_ZEROS", {})
+    monkeypatch.setattr(T, "_PACKED", {})
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = A.linear(x, w).detach()
+    assert not T._ZEROS and not T._PACKED
+    assert torch.equal(A.linear(x, w).detach(), want)                 # before any replay
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(A.linear(x, w).detach(), want)
+
+
 def test_more_than_2_31_elements():
     """The element-wise nodes take them (2^31 + 1280 here); the last rows are as those rows alone."""
     from airv2x_perception_amd.opencood_iface import act8_ops as A
