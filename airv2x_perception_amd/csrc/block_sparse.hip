@@ -1115,26 +1115,21 @@ constexpr int kItemRows = 1024, kItemLeast = 512;
 
 // ------------------------------------------------------------------------------------------------------------ attention, many queries
 // A mention's record: (maximum (scaled, base 2), sum) and the attention over its block alone, next to each other -- they are written to places all over the
-// workspace, and 8 bytes of their own would cost a memory request as large as the rest.  PT: without gradients it is held in the tensor's type -- a convex combination of
-// values like the output, so its rounding is half a step at most and enters the output with the block's weight (measured: 1.4 times the error of the output's
-// own rounding) -- which halves the bytes that bound this kernel and the join (281600 queries x 8 blocks, bf16: join 94 -> 51 us).  With gradients it stays fp32:
-// the backward's sum dO O would carry that rounding into every dS of the query.
-template <int D, typename PT> struct Record {
-    static constexpr size_t bytes = 8 + D * sizeof(PT);
+// workspace, and 8 bytes of their own would cost a memory request as large as the rest.  All in fp32 whatever the tensors' type: the output is rounded once, and is the
+// same with and without gradients (held in 16 bits the records halve the bytes of the join, at 1.4 times the error of the output's own rounding).
+template <int D> struct Record {
+    static constexpr size_t bytes = 8 + D * 4;
     static __device__ __forceinline__ char* at(void* part, size_t i) { return static_cast<char*>(part) + i * bytes; }
     static __device__ __forceinline__ const char* at(const void* part, size_t i) { return static_cast<const char*>(part) + i * bytes; }
-    typedef typename tok_vec<PT>::v4 v4 __attribute__((aligned(8)));
-    static __device__ __forceinline__ void put(char* r, int d, f32x4 v) { *reinterpret_cast<v4*>(r + 8 + d * sizeof(PT)) = __builtin_convertvector(v, typename tok_vec<PT>::v4); }
-    static __device__ __forceinline__ f32x4 get(const char* r, int d) {
-        const typename tok_vec<PT>::v4 x = *reinterpret_cast<const v4*>(r + 8 + d * sizeof(PT));
-        return __builtin_convertvector(x, f32x4);
-    }
+    typedef f32x4 v4 __attribute__((aligned(8)));
+    static __device__ __forceinline__ void put(char* r, int d, f32x4 v) { *reinterpret_cast<v4*>(r + 8 + d * 4) = v; }
+    static __device__ __forceinline__ f32x4 get(const char* r, int d) { return *reinterpret_cast<const v4*>(r + 8 + d * 4); }
 };
 
-// 281600 queries x 8 blocks of 32 channels: bf16 170 us, fp32 206 us.  The products take 25 and 48 us at the matrix cores' measured rate, the records 33 and 73 us at HBM's; the
+// 281600 queries x 8 blocks of 32 channels: bf16 197 us, fp32 206 us.  The products take 25 and 48 us at the matrix cores' measured rate, the records 62 us at HBM's; the
 // vector units bound it: about 20 instructions for each score a lane holds (scaling, maximum, exponential, sum, two terms).  The launch bounds keep one more wave
 // on a SIMD than the compiler would (heads of 64 fp32: 136 us against 166, of 128 bf16: 103 against 115).
-template <typename T, int D, typename PT>
+template <typename T, int D>
 __global__ __launch_bounds__(256, (Held<T>::two ? (D <= 32 ? 3 : D == 64 ? 2 : 1) : (D <= 32 ? 4 : D == 64 ? 3 : 2))) void bs_forward_kernel(BsArgs a) {
     using S = Shape<T, D>;
     using E = typename Held<T>::E;
@@ -1195,7 +1190,7 @@ __global__ __launch_bounds__(256, (Held<T>::two ? (D <= 32 ? 3 : D == 64 ? 2 : 1
         l += __shfl_xor(l, 32);
         const float inv = l == 0.f ? 0.f : vf / l;
         if constexpr (Held<T>::narrow) l *= 1.0f / 32768.f;
-        char* rec = Record<D, PT>::at(a.part, (((size_t)b * a.T + r.t) * a.H + r.head) * a.n + r.slot);
+        char* rec = Record<D>::at(a.part, (((size_t)b * a.T + r.t) * a.H + r.head) * a.n + r.slot);
         const Split<T, false> p0(s[0]), p1(s[1]);
 #pragma unroll
         for (int dt = 0; dt < S::DT; ++dt) {
@@ -1205,7 +1200,7 @@ __global__ __launch_bounds__(256, (Held<T>::two ? (D <= 32 ? 3 : D == 64 ? 2 : 1
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int d = dt * 32 + 8 * i + 4 * half;
-                    if (d < D) Record<D, PT>::put(rec, d, f32x4{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]} * inv);
+                    if (d < D) Record<D>::put(rec, d, f32x4{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]} * inv);
                 }
             }
         }
@@ -1217,7 +1212,7 @@ __global__ __launch_bounds__(256, (Held<T>::two ? (D <= 32 ? 3 : D == 64 ? 2 : 1
 // ------------------------------------------------------------------------------------------------------------ attention, few queries
 // One wave per mention, all heads of its group: a lane per key for the scores, D / 8 lanes per key for the values.  Bound by the latency of two rounds of loads
 // (one query x 8 heads x 16 blocks: 5.5 us).
-template <typename T, int D, typename PT>
+template <typename T, int D>
 __global__ __launch_bounds__(64) void bs_few_kernel(BsArgs a) {
     __shared__ __align__(16) float lq[D];
     __shared__ float lp[kKeys];
@@ -1270,17 +1265,17 @@ __global__ __launch_bounds__(64) void bs_few_kernel(BsArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) { o0[e] += __shfl_xor(o0[e], o); o1[e] += __shfl_xor(o1[e], o); }
         const float inv = l == 0.f ? 0.f : 1.0f / l;
-        char* rec = Record<D, PT>::at(a.part, (((size_t)b * a.T + t) * a.H + h * a.G + g) * a.n + slot);
+        char* rec = Record<D>::at(a.part, (((size_t)b * a.T + t) * a.H + h * a.G + g) * a.n + slot);
         if (lane < LPK) {
-            Record<D, PT>::put(rec, sub * 8, o0 * inv);
-            Record<D, PT>::put(rec, sub * 8 + 4, o1 * inv);
+            Record<D>::put(rec, sub * 8, o0 * inv);
+            Record<D>::put(rec, sub * 8 + 4, o1 * inv);
         }
         if (lane == 0) *reinterpret_cast<f32x2*>(rec) = f32x2{m, l};
     }
 }
 
-// The n places of a query joined: D / 4 lanes a (query, head).  Bound by HBM (281600 x 8 records of 72 bytes: 53 us; of 136 bytes: 75 us, 4.6 TB/s).  rest: what the output's rounding took away, for the backward's sum dO O
-template <typename T, int D, typename PT>
+// The n places of a query joined: D / 4 lanes a (query, head).  Bound by HBM (281600 x 8 records of 136 bytes: 73 us, 4.4 TB/s).  rest: what the output's rounding took away, for the backward's sum dO O
+template <typename T, int D>
 __global__ __launch_bounds__(256) void bs_join_kernel(BsArgs a, long long rows) {
     constexpr int L = D / 4;
     const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / L;
@@ -1289,7 +1284,7 @@ __global__ __launch_bounds__(256) void bs_join_kernel(BsArgs a, long long rows) 
     const unsigned hq = (unsigned)(r % a.H);
     const long long bt = r / a.H;
     const int32_t* bl = a.blocks + (bt * a.KV + hq / (unsigned)a.G) * a.n;
-    const char* part = Record<D, PT>::at(a.part, (size_t)(r * a.n));
+    const char* part = Record<D>::at(a.part, (size_t)(r * a.n));
     float m = -INFINITY, l = 0.f;
     f32x4 o{0.f, 0.f, 0.f, 0.f};
     for (int s0 = 0; s0 < a.n; s0 += 8) {                // eight places at a time, all their loads in flight
@@ -1303,9 +1298,9 @@ __global__ __launch_bounds__(256) void bs_join_kernel(BsArgs a, long long rows) 
             x[u] = f32x2{-INFINITY, 0.f};
             y[u] = f32x4{0.f, 0.f, 0.f, 0.f};
             if (ok) {
-                const char* rec = part + (size_t)s * Record<D, PT>::bytes;
+                const char* rec = part + (size_t)s * Record<D>::bytes;
                 x[u] = *reinterpret_cast<const f32x2*>(rec);
-                y[u] = Record<D, PT>::get(rec, sub * 4);
+                y[u] = Record<D>::get(rec, sub * 4);
             }
             mm = fmaxf(mm, x[u].x);
         }
@@ -1731,7 +1726,7 @@ Work bs_work(int64_t B, int64_t T, int64_t Nk, int64_t H, int64_t KV, int64_t D,
     Work w{};
     const size_t rows = (size_t)(B * T * H);
     w.part = 0;
-    size_t at = up16(rows * n * (backward ? D * 4 : D * 4 + 8));      // (a 16-bit forward uses about half of it)
+    size_t at = up16(rows * n * (backward ? D * 4 : D * 4 + 8));
     if (backward) {
         w.ld = at;
         at += up16(rows * 8);
@@ -1784,23 +1779,19 @@ extern "C" int av2x_block_sparse_attention(const void* q, const void* k, const v
     a.out = out;
     a.lse = lse;
     a.rest = rest;
-    const bool wide = lse || dtype == kTokF32;
     hipStream_t st = av2x::as_stream(stream);
     return bs_go(dtype, dim, [&](auto t, auto d) {
         using T = typename decltype(t)::type;
         constexpr int D = decltype(d)::value;
         if (a.NB > 0) {
             const dim3 items(a.max_items, batch * kv_heads);
-            if (lists && wide) bs_forward_kernel<T, D, float><<<items, 256, 0, st>>>(a);
-            else if (lists) bs_forward_kernel<T, D, T><<<items, 256, 0, st>>>(a);
-            else if (wide) bs_few_kernel<T, D, float><<<(unsigned)mentions, 64, 0, st>>>(a);
-            else bs_few_kernel<T, D, T><<<(unsigned)mentions, 64, 0, st>>>(a);
+            if (lists) bs_forward_kernel<T, D><<<items, 256, 0, st>>>(a);
+            else bs_few_kernel<T, D><<<(unsigned)mentions, 64, 0, st>>>(a);
             if (int rc = av2x::check_launch(what)) return rc;
         }
         const long long rows = (long long)batch * queries * heads;
         const unsigned by_row = (unsigned)((rows * (D / 4) + 255) / 256);
-        if (wide) bs_join_kernel<T, D, float><<<by_row, 256, 0, st>>>(a, rows);
-        else bs_join_kernel<T, D, T><<<by_row, 256, 0, st>>>(a, rows);
+        bs_join_kernel<T, D><<<by_row, 256, 0, st>>>(a, rows);
         return av2x::check_launch(what);
     });
 }
