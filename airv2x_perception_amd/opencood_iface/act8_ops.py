@@ -112,11 +112,6 @@ def unpack(p):
 
 
 # ------------------------------------------------------------------------------------------------ raw launches
-def _owner(weight):
-    """Whose packing the framework's GEMM may keep from step to step; nobody's in a graph that is being recorded, whose replays have to see the weight as it is then."""
-    return None if torch.cuda.is_current_stream_capturing() else weight
-
-
 def _gemm(r, x, weight, bias, residual):
     """x W^T (+ b) (+ residual): the engine's launcher with the rows as one image line, or for few rows a GEMM on the parameter as it lies."""
     from .engine import ConvLayer
@@ -128,7 +123,7 @@ def _gemm(r, x, weight, bias, residual):
     if rows * cin * cout <= SMALL_PRODUCT and not T.AMP_STEP[0]:
         _lib.check(r.lib.av2x_act8_gemm(_P(x), _P(weight), _P(bias), _P(residual), _P(y), rows, cout, cin, 0, r.stream()), "av2x_act8_gemm")
         return y
-    wp, coutp, _, ent = T._packed(r, weight.detach().view(cout, cin, 1, 1), owner=_owner(weight))
+    wp, coutp, _, ent = T._packed(r, weight.detach().view(cout, cin, 1, 1), owner=weight)
     L = ConvLayer(wp, None, bias.detach() if bias is not None else T._zeros(cout, x.device), cin, cout, coutp, 1, 1, 0, 0)
     T.seed_x3p(r, L, ent)
     r.amp = T.AMP_STEP[0] and cin % 8 == 0
@@ -154,7 +149,7 @@ def _dgrad(dy, weight, amp):
         _lib.check(r.lib.av2x_act8_gemm(_P(dy), _P(weight), None, None, _P(dx), rows, cin, cout, 1, r.stream()), "av2x_act8_gemm")
         return dx
     w4 = weight.detach().view(cout, cin, 1, 1)
-    return T.conv_dgrad(dy.view(1, 1, rows, cout), w4, 1, 0, (1, rows), owner=_owner(weight)).view(tuple(dy.shape[:-1]) + (cin,))
+    return T.conv_dgrad(dy.view(1, 1, rows, cout), w4, 1, 0, (1, rows), owner=weight).view(tuple(dy.shape[:-1]) + (cin,))
 
 
 def _wgrad(r, kind, dy, q, s, cin, stats=None, gamma=None, beta=None, want_w=True, want_b=True, weight=None, dgamma=None, dbeta=None):

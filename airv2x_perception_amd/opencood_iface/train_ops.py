@@ -118,7 +118,10 @@ def _packed(r, weight, flipped=False, owner=None):
     # is keyed on it -- the view is a new object on every call (it shares the parameter's storage and version counter)
     own = owner if owner is not None else weight
     key = (id(own), flipped, tuple(weight.shape))
-    ent = _PACKED.get(key)
+    # while a graph is recorded nothing is taken from the cache or left in it: a replay has to pack the weight as it is then, and what the recording
+    # allocates holds a packing from its first replay on only
+    recording = torch.cuda.is_current_stream_capturing()
+    ent = None if recording else _PACKED.get(key)
     # ``_version`` does not move for writes through ``.data`` nor for ``module.to(device)`` (which re-points ``.data``): the storage
     # address and the device are part of the validity check, like the eval engine's _version()
     stamp = (weight._version, weight.data_ptr(), weight.device)
@@ -129,7 +132,7 @@ def _packed(r, weight, flipped=False, owner=None):
     # engine.wino_rule's weight side: the class's transformed weights are made by conv_raw, for the kernel it picks, on first need
     u = bool(r.winograd and ks == 3 and cin >= 64 and cin % 8 == 0 and cout % 64 == 0 and cout == coutp)
     ent = [stamp, weakref.ref(own) if (own.is_leaf and isinstance(own, torch.nn.Parameter)) else None, wp, coutp, u, None, None, None, None, None]
-    if ent[1] is not None:
+    if ent[1] is not None and not recording:
         if len(_PACKED) > 4096:
             _PACKED.clear()
         _PACKED[key] = ent

@@ -1,0 +1,62 @@
+"""GPU: recorded steps of the token operators and of the layer made of them, replayed with weights that changed since the recording, against eager steps.
+
+A backward pass is recorded only while no eager graph of the same leaves is alive, so a step keeps none.
+"""
+import copy
+
+import pytest
+import torch
+
+from tests.test_gpu_token_layer import layer
+
+pytestmark = pytest.mark.gpu
+
+
+def on_a_side_stream(f):
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        f()
+    torch.cuda.current_stream().wait_stream(s)
+
+
+def make_step(m, t=260):
+    g = torch.Generator().manual_seed(t)
+    x = torch.randn(1, t, 256, generator=g).cuda().requires_grad_()
+    dy = torch.randn(1, t, 256, generator=g).cuda()
+    pos = torch.stack([torch.arange(t) // 20, torch.arange(t) % 20], 1).int().cuda()
+
+    def step(m=m):
+        y = m(x, pos)
+        return [y.detach()] + list(torch.autograd.grad(y, [x] + list(m.parameters()), dy))
+    return step
+
+
+@pytest.mark.parametrize("act8", [False, True])
+@pytest.mark.parametrize("warm", [False, True])
+def test_a_recorded_layer_follows_its_weights(monkeypatch, warm, act8):
+    """With packings of the weights left by an eager step before the recording, and with none; eager calls before the first replay and between replays."""
+    from airv2x_perception_amd.opencood_iface import act8_ops as A8, train_ops as T
+    monkeypatch.setattr(A8, "SMALL_PRODUCT", 0)                 # every Linear on the GEMM that packs its weights
+    m = layer(7, 256, 8, 2, 32, 3)
+    m.act8 = act8
+    step = make_step(m)
+    on_a_side_stream(step if warm else lambda: step(copy.deepcopy(m)))
+    if not warm:
+        monkeypatch.setattr(T, "_PACKED", {})
+        monkeypatch.setattr(T, "_ZEROS", {})
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    want = step(copy.deepcopy(m))
+    assert all(torch.equal(a, b) for a, b in zip(step(), want))  # before any replay
+    for i in range(3):
+        with torch.no_grad():
+            for p in m.parameters():
+                p.mul_(1 + 0.25 * (i + 1)).add_(0.01)
+        graph.replay()
+        torch.cuda.synchronize()
+        have = [t.clone() for t in got]
+        want = step(copy.deepcopy(m))                           # parameters that no cache knows
+        assert all(torch.equal(a, b) for a, b in zip(have, want))
+        assert all(torch.equal(a, b) for a, b in zip(step(), want))
