@@ -16,7 +16,8 @@ derivative taken at x8 instead of x:
 
 A group with an infinity or a NaN has a NaN scale: the gradients show it, as they would without the 8 bits (GradScaler's check works).
 A step can be captured into a HIP graph, while no eager graph of the same leaves is alive (torch's engine would wait for the stream of a leaf's old node); its weights are
-packed on every replay.  ``model.act8 = True`` trains Airv2xCoBEVT / Airv2xV2XVit's fusion with these nodes (train_ops.act8_scope).
+packed on every replay, and in every later eager call (train_ops.forget_packings: for weights that a replay changes without running their layers).
+``model.act8 = True`` trains Airv2xCoBEVT / Airv2xV2XVit's fusion with these nodes (train_ops.act8_scope).
 """
 from __future__ import annotations
 
@@ -121,6 +122,7 @@ def _gemm(r, x, weight, bias, residual):
     if rows == 0:
         return y
     if rows * cin * cout <= SMALL_PRODUCT and not T.AMP_STEP[0]:
+        T._may_keep(weight)                               # (a recorded step uses it, though it packs nothing)
         _lib.check(r.lib.av2x_act8_gemm(_P(x), _P(weight), _P(bias), _P(residual), _P(y), rows, cout, cin, 0, r.stream()), "av2x_act8_gemm")
         return y
     wp, coutp, _, ent = T._packed(r, weight.detach().view(cout, cin, 1, 1), owner=weight)
@@ -145,6 +147,7 @@ def _dgrad(dy, weight, amp):
         return torch.empty(tuple(dy.shape[:-1]) + (cin,), dtype=torch.float32, device=dy.device)
     if rows * cin * cout <= SMALL_PRODUCT and not T.AMP_STEP[0]:
         r = _runner(dy.device)
+        T._may_keep(weight)
         dx = torch.empty(tuple(dy.shape[:-1]) + (cin,), dtype=torch.float32, device=dy.device)
         _lib.check(r.lib.av2x_act8_gemm(_P(dy), _P(weight), None, None, _P(dx), rows, cin, cout, 1, r.stream()), "av2x_act8_gemm")
         return dx

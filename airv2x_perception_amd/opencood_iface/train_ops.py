@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import weakref
 from ctypes import byref, c_void_p
 
 import torch
@@ -110,18 +111,39 @@ def _zeros(c, device):
 _PACKED = {}       # id(parameter) -> (version, weakref, packed, coutp, winograd-transformed | None): one packing per optimiser step
 
 
+_RECORDED = {}     # id(parameter) -> weakref: weights of recorded steps
+
+
+def _may_keep(own):
+    """Whether a packing of the weight ``own`` may be taken from the cache or left in it.  Not while a graph is recorded: a replay has to pack the weight
+    as it is then, and what the recording allocates holds a packing from its first replay on only.  And not for a weight that a recorded step uses: replays
+    change it in place without moving its version counter, the cache's only sign of a change."""
+    if torch.cuda.is_current_stream_capturing():
+        if isinstance(own, torch.nn.Parameter):
+            if len(_RECORDED) > 4096:
+                for k in [k for k, ref in list(_RECORDED.items()) if ref() is None]:
+                    _RECORDED.pop(k, None)
+            _RECORDED[id(own)] = weakref.ref(own)
+        return False
+    ref = _RECORDED.get(id(own))
+    return ref is None or ref() is not own
+
+
+def forget_packings():
+    """Drops all kept packings.  To be called where weights changed in a way that moves neither their version counter nor their storage: after replays of a
+    graph that updates them but does not run their layers (a recorded optimizer step beside eager forward and backward passes)."""
+    _PACKED.clear()
+
+
 def _packed(r, weight, flipped=False, owner=None):
     """The kernel packing of a convolution weight (``flipped``: of its 180-degree-rotated, channel-transposed form -- the data
     gradient's weights), cached per parameter and version counter: a training step uses every weight in up to three passes."""
-    import weakref
     # ``owner``: the nn.Parameter a reshaped view was taken from (nn.Linear's (cout, cin) weight seen as a 1x1 convolution): the cache
     # is keyed on it -- the view is a new object on every call (it shares the parameter's storage and version counter)
     own = owner if owner is not None else weight
     key = (id(own), flipped, tuple(weight.shape))
-    # while a graph is recorded nothing is taken from the cache or left in it: a replay has to pack the weight as it is then, and what the recording
-    # allocates holds a packing from its first replay on only
-    recording = torch.cuda.is_current_stream_capturing()
-    ent = None if recording else _PACKED.get(key)
+    keep = _may_keep(own)
+    ent = _PACKED.get(key) if keep else None
     # ``_version`` does not move for writes through ``.data`` nor for ``module.to(device)`` (which re-points ``.data``): the storage
     # address and the device are part of the validity check, like the eval engine's _version()
     stamp = (weight._version, weight.data_ptr(), weight.device)
@@ -132,7 +154,7 @@ def _packed(r, weight, flipped=False, owner=None):
     # engine.wino_rule's weight side: the class's transformed weights are made by conv_raw, for the kernel it picks, on first need
     u = bool(r.winograd and ks == 3 and cin >= 64 and cin % 8 == 0 and cout % 64 == 0 and cout == coutp)
     ent = [stamp, weakref.ref(own) if (own.is_leaf and isinstance(own, torch.nn.Parameter)) else None, wp, coutp, u, None, None, None, None, None]
-    if ent[1] is not None and not recording:
+    if ent[1] is not None and keep:
         if len(_PACKED) > 4096:
             _PACKED.clear()
         _PACKED[key] = ent

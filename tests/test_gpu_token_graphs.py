@@ -60,3 +60,55 @@ def test_a_recorded_layer_follows_its_weights(monkeypatch, warm, act8):
         want = step(copy.deepcopy(m))                           # parameters that no cache knows
         assert all(torch.equal(a, b) for a, b in zip(have, want))
         assert all(torch.equal(a, b) for a, b in zip(step(), want))
+
+
+@pytest.mark.parametrize("recorded,eager", [(0, 0), (1 << 62, 0), (0, 1 << 62)])
+@pytest.mark.parametrize("act8", [False, True])
+def test_eager_calls_follow_weights_that_replays_change(monkeypatch, act8, recorded, eager):
+    """A recorded step of gradient descent changes the weights without moving their version counters: eager calls between its replays use them as they are.
+    ``recorded``, ``eager``: which of the 8-bit layers' products the recording and the eager calls run."""
+    from airv2x_perception_amd.opencood_iface import act8_ops as A8
+    m = layer(9, 256, 8, 2, 32, 3)
+    m.act8 = act8
+    step = make_step(m)
+
+    def descend():
+        for p, g in zip(m.parameters(), step()[2:]):
+            with torch.no_grad():
+                p.sub_(g, alpha=1e-3)
+
+    monkeypatch.setattr(A8, "SMALL_PRODUCT", recorded)
+    on_a_side_stream(descend)
+    monkeypatch.setattr(A8, "SMALL_PRODUCT", eager)
+    on_a_side_stream(step)                                      # packings of the last eager version
+    monkeypatch.setattr(A8, "SMALL_PRODUCT", recorded)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        descend()
+    monkeypatch.setattr(A8, "SMALL_PRODUCT", eager)
+    before = None
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        got, want = step(), step(copy.deepcopy(m))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert before is None or not torch.equal(before, got[0])
+        before = got[0]
+
+
+def test_packings_are_forgotten_on_demand():
+    """A graph that updates weights without running their layers."""
+    from airv2x_perception_amd.opencood_iface import train_ops as T
+    m = layer(10, 256, 8, 2, 32, 3)
+    step = make_step(m)
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with torch.no_grad():
+            for p in m.parameters():
+                p.mul_(1.5)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        T.forget_packings()
+        assert all(torch.equal(a, b) for a, b in zip(step(), step(copy.deepcopy(m))))
