@@ -80,6 +80,10 @@ def _aligned(x):
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
+def _maybe(x):
+    return _aligned(x) if x is not None else None
+
+
 def _empty_pack(x):
     c = x.shape[-1]
     rows = x.numel() // c
@@ -189,7 +193,7 @@ class _Linear8(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, keep):
         r = _runner(x.device)
         x, weight = _aligned(x), weight.contiguous()
-        y = _gemm(r, x, weight, bias, _aligned(residual) if residual is not None else None)
+        y = _gemm(r, x, weight, _maybe(bias), _maybe(residual))
         q = s = None
         if keep:                                          # only the weight gradient reads the input
             q, s = pack(x)
@@ -221,7 +225,7 @@ class _NormLinear8(torch.autograd.Function):
         rows, c, q, s = _empty_pack(x)
         xn, stats = torch.empty_like(x), torch.empty((rows, 2), dtype=torch.float32, device=x.device)
         _lib.check(r.lib.av2x_act8_layernorm(_P(x), _P(gamma), _P(beta), _P(xn), _P(q), _P(s), _P(stats), rows, c, LN_EPS, r.stream()), "av2x_act8_layernorm")
-        y = _gemm(r, xn, weight, bias, None)
+        y = _gemm(r, xn, weight, _maybe(bias), None)
         ctx.save_for_backward(weight, gamma, beta, q, s, stats)
         ctx.amp = T.AMP_STEP[0]
         return y
@@ -277,7 +281,7 @@ class _GeluLinear8(torch.autograd.Function):
         r = _runner(z.device)
         z, weight = _aligned(z), weight.contiguous()
         h, q, s = _gelu_forward(r, z)
-        y = _gemm(r, h, weight, bias, _aligned(residual) if residual is not None else None)
+        y = _gemm(r, h, weight, _maybe(bias), _maybe(residual))
         ctx.save_for_backward(weight, q, s)
         ctx.amp = T.AMP_STEP[0]
         return y

@@ -36,10 +36,10 @@ class LayerNormFn(torch.autograd.Function):
     def forward(ctx, x, gamma, beta):
         T._check_dev(x)
         r = _runner(x.device)
-        x = x.contiguous()
+        x, gamma = x.contiguous(), gamma.contiguous()
         c = x.shape[-1]
         y = torch.empty_like(x)
-        _lib.check(r.lib.av2x_layernorm(_P(x), _P(gamma.detach()), _P(beta.detach()), _P(y), x.numel() // c, c, LN_EPS, r.stream()), "av2x_layernorm")
+        _lib.check(r.lib.av2x_layernorm(_P(x), _P(gamma.detach()), _P(beta.detach().contiguous()), _P(y), x.numel() // c, c, LN_EPS, r.stream()), "av2x_layernorm")
         ctx.save_for_backward(x, gamma)
         return y
 
@@ -77,7 +77,7 @@ class LinearFn(torch.autograd.Function):
         cout = weight.shape[0]
         w4 = weight.detach().view(cout, cin, 1, 1)
         wp, coutp, _, ent = T._packed(r, w4, owner=weight)    # keyed on the nn.Linear parameter: one packing per optimiser step
-        L = ConvLayer(wp, None, bias.detach() if bias is not None else T._zeros(cout, x.device), cin, cout, coutp, 1, 1, 0, 0)
+        L = ConvLayer(wp, None, bias.detach().contiguous() if bias is not None else T._zeros(cout, x.device), cin, cout, coutp, 1, 1, 0, 0)
         T.seed_x3p(r, L, ent)
         y = torch.empty((n, h, w, cout), dtype=torch.float32, device=x.device)
         r.amp = T.AMP_STEP[0]

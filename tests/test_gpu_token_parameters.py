@@ -1,0 +1,54 @@
+"""GPU: parameters of the token layers as a program may hold them -- columns of a matrix, one stored element for all, views at odd places of one flat buffer --
+give the bits of the same values in a tensor of their own."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def column(v):
+    """v as a column of a matrix."""
+    m = torch.full((v.numel(), 3), float("nan"), device="cuda")
+    m[:, 1] = v
+    return m[:, 1]
+
+
+def odd(v):
+    """v behind one element of a flat buffer: contiguous, on an address that is no multiple of 16."""
+    b = torch.full((v.numel() + 1,), float("nan"), device="cuda")
+    b[1:] = v.flatten()
+    return b[1:].view(v.shape)
+
+
+def same(f, make, own):
+    """f(*tensors) and its gradients with views and with tensors of their own."""
+    res = []
+    for args in (make, own):
+        args = [a.detach().requires_grad_() for a in args]
+        y = f(*args)
+        res.append([y.detach()] + list(torch.autograd.grad(y, args, torch.ones_like(y).cumsum(0) / 7)))
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+@pytest.mark.parametrize("small", [1 << 62, 0])
+@pytest.mark.parametrize("kind", ["column", "one", "odd"])
+def test_bias_of_the_8_bit_layers(monkeypatch, small, kind):
+    from airv2x_perception_amd.opencood_iface import act8_ops as A
+    monkeypatch.setattr(A, "SMALL_PRODUCT", small)
+    g = torch.Generator().manual_seed(3)
+    x, w, gamma, beta = [torch.randn(*s, generator=g).cuda() for s in ((70, 64), (96, 64), (64,), (64,))]
+    b = torch.randn(1, generator=g).cuda().expand(96) if kind == "one" else torch.randn(96, generator=g).cuda()
+    view = b if kind == "one" else column(b) if kind == "column" else odd(b)
+    for f in (lambda x, w, b: A.linear(x, w, b), lambda x, w, b: A.norm_linear(x, gamma, beta, w, b), lambda x, w, b: A.gelu_linear(x, w, b)):
+        same(f, (x, w, view), (x, w, b.contiguous()))
+
+
+@pytest.mark.parametrize("kind", ["column", "one", "odd"])
+def test_vectors_of_the_fp32_layers(kind):
+    from airv2x_perception_amd.opencood_iface import train_fusion_ops as F
+    g = torch.Generator().manual_seed(4)
+    x, w, gamma, beta = [torch.randn(*s, generator=g).cuda() for s in ((2, 5, 7, 256), (96, 256), (256,), (256,))]
+    b = torch.randn(96, generator=g).cuda()
+    view = {"column": column, "odd": odd, "one": lambda v: v[:1].expand(v.numel())}[kind]
+    same(F.linear, (x, w, view(b)), (x, w, view(b).contiguous()))
+    same(F.layer_norm, (x, view(gamma), view(beta)), (x, view(gamma).contiguous(), view(beta).contiguous()))
