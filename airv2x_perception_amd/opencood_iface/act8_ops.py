@@ -127,7 +127,7 @@ def _gemm(r, x, weight, bias, residual):
         return y
     if rows * cin * cout <= SMALL_PRODUCT and not T.AMP_STEP[0]:
         T._may_keep(weight)                               # (a recorded step uses it, though it packs nothing)
-        _lib.check(r.lib.av2x_act8_gemm(_P(x), _P(weight), _P(bias), _P(residual), _P(y), rows, cout, cin, 0, r.stream()), "av2x_act8_gemm")
+        _lib.check(r.lib.av2x_act8_gemm(_P(x), _P(_aligned(weight)), _P(bias), _P(residual), _P(y), rows, cout, cin, 0, r.stream()), "av2x_act8_gemm")
         return y
     wp, coutp, _, ent = T._packed(r, weight.detach().view(cout, cin, 1, 1), owner=weight)
     L = ConvLayer(wp, None, bias.detach() if bias is not None else T._zeros(cout, x.device), cin, cout, coutp, 1, 1, 0, 0)
@@ -153,7 +153,7 @@ def _dgrad(dy, weight, amp):
         r = _runner(dy.device)
         T._may_keep(weight)
         dx = torch.empty(tuple(dy.shape[:-1]) + (cin,), dtype=torch.float32, device=dy.device)
-        _lib.check(r.lib.av2x_act8_gemm(_P(dy), _P(weight), None, None, _P(dx), rows, cin, cout, 1, r.stream()), "av2x_act8_gemm")
+        _lib.check(r.lib.av2x_act8_gemm(_P(dy), _P(_aligned(weight)), None, None, _P(dx), rows, cin, cout, 1, r.stream()), "av2x_act8_gemm")
         return dx
     w4 = weight.detach().view(cout, cin, 1, 1)
     return T.conv_dgrad(dy.view(1, 1, rows, cout), w4, 1, 0, (1, rows), owner=weight).view(tuple(dy.shape[:-1]) + (cin,))

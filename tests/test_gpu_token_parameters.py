@@ -52,3 +52,15 @@ def test_vectors_of_the_fp32_layers(kind):
     view = {"column": column, "odd": odd, "one": lambda v: v[:1].expand(v.numel())}[kind]
     same(F.linear, (x, w, view(b)), (x, w, view(b).contiguous()))
     same(F.layer_norm, (x, view(gamma), view(beta)), (x, view(gamma).contiguous(), view(beta).contiguous()))
+
+
+@pytest.mark.parametrize("small", [1 << 62, 0])
+def test_weights_at_odd_places_of_a_flat_buffer(monkeypatch, small):
+    from airv2x_perception_amd.opencood_iface import act8_ops as A, train_fusion_ops as F
+    monkeypatch.setattr(A, "SMALL_PRODUCT", small)
+    g = torch.Generator().manual_seed(5)
+    x, w, b, gamma, beta, res = [torch.randn(*s, generator=g).cuda() for s in ((70, 64), (96, 64), (96,), (64,), (64,), (70, 96))]
+    for f in (lambda x, w, b: A.linear(x, w, b, res), lambda x, w, b: A.norm_linear(x, gamma, beta, w, b), lambda x, w, b: A.gelu_linear(x, w, b, res),
+              lambda x, w, b: F.linear(x.view(1, 7, 10, 64), w, b)):
+        same(f, (x, odd(w), odd(b)), (x, w, b))
+    same(lambda x, w, gm, bt: A.norm_linear(x, gm, bt, w), (odd(x), odd(w), odd(gamma), odd(beta)), (x, w, gamma, beta))
