@@ -61,9 +61,14 @@ def _check_token(what, x, dim_axes, name):
         raise ValueError(f"{what}: heads of {x.shape[-1]} channels ({', '.join(map(str, DIMS))} are supported)")
 
 
+def _steps(x):
+    """Strides of the axes before the channels; an axis of one element takes no steps, whatever its stride says."""
+    return [s if n > 1 else 0 for s, n in zip(x.stride()[:-1], x.shape[:-1])]
+
+
 def _strided(x, elems):
     """x itself where the kernels can read it in pieces of ``elems`` elements, else a contiguous copy."""
-    ok = x.stride(-1) == 1 and x.data_ptr() % (elems * x.element_size()) == 0 and all(s % elems == 0 for s in x.stride()[:-1])
+    ok = x.stride(-1) == 1 and x.data_ptr() % (elems * x.element_size()) == 0 and all(s % elems == 0 for s in _steps(x))
     if ok:
         return x
     x = x.contiguous()
@@ -112,7 +117,7 @@ def _rotate_forward(q, k, gq, gk, pos, freqs, eps, inter):
     kv = k.shape[1] if k is not None else 0
     oq = torch.empty((rows, h, d), dtype=q.dtype, device=q.device)
     ok = torch.empty((rows, kv, d), dtype=q.dtype, device=q.device) if k is not None else None
-    st = _host64(q.stride(0), q.stride(1), k.stride(0) if kv else 0, k.stride(1) if kv else 0)
+    st = _host64(*_steps(q), *(_steps(k) if kv else (0, 0)))
     _lib.check(r.lib.av2x_qk_norm_rotate(_P(q), _P(k), st, _P(gq), _P(gk), _P(pos), _P(freqs), _P(oq), _P(ok), rows, h, kv, d, pos.shape[-1], 1 if inter else 0,
                                          _DTYPES[q.dtype], eps, r.stream()), "av2x_qk_norm_rotate")
     return oq, ok
@@ -125,9 +130,8 @@ def _rotate_backward(q, k, gq, gk, pos, freqs, eps, inter, doq, dok, dov, dq, dk
     dgq = torch.empty_like(gq) if want[0] else None
     dgk = torch.empty_like(gk) if kv and want[1] else None
     ws = torch.empty(int(r.lib.av2x_qk_norm_rotate_backward_workspace_bytes(d)), dtype=torch.uint8, device=q.device)
-    st = _host64(q.stride(0), q.stride(1), k.stride(0) if kv else 0, k.stride(1) if kv else 0)
-    dst = _host64(dq.stride(0), dq.stride(1), dk.stride(0) if kv else 0, dk.stride(1) if kv else 0, dv.stride(0) if dv is not None else 0,
-                  dv.stride(1) if dv is not None else 0)
+    st = _host64(*_steps(q), *(_steps(k) if kv else (0, 0)))
+    dst = _host64(*_steps(dq), *(_steps(dk) if kv else (0, 0)), *(_steps(dv) if dv is not None else (0, 0)))
     fit = lambda t: A8._aligned(t) if t is not None else None
     doq, dok, dov = fit(doq), fit(dok), fit(dov)
     _lib.check(r.lib.av2x_qk_norm_rotate_backward(_P(q), _P(k), st, _P(gq), _P(gk), _P(pos), _P(freqs), _P(doq), _P(dok), _P(dov), _P(dq), _P(dk), _P(dv), dst,
@@ -257,7 +261,7 @@ def _launch_bounds(k, mask, ints, scale, first, count):
     r = _runner(k.device)
     b, n, kv, d = k.shape
     k = _strided(k, 4)
-    _lib.check(r.lib.av2x_block_bounds(_P(k), _P(mask), _host64(*k.stride()[:3]), b, n, kv, d, _DTYPES[k.dtype], first, count, _P(ints), _P(scale), r.stream()),
+    _lib.check(r.lib.av2x_block_bounds(_P(k), _P(mask), _host64(*_steps(k)), b, n, kv, d, _DTYPES[k.dtype], first, count, _P(ints), _P(scale), r.stream()),
                "av2x_block_bounds")
 
 
@@ -313,7 +317,7 @@ def select_blocks(q, bounds, blocks):
             q = q.contiguous()
         size = int(r.lib.av2x_select_blocks_workspace_bytes(b, t, nb * BLOCK, kv, blocks))
         ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-        _lib.check(r.lib.av2x_select_blocks(_P(q), _host64(*q.stride()[:3]), _P(bounds.ints), _P(bounds.scale), b, t, nb * BLOCK, h, kv, d, blocks, _DTYPES[q.dtype],
+        _lib.check(r.lib.av2x_select_blocks(_P(q), _host64(*_steps(q)), _P(bounds.ints), _P(bounds.scale), b, t, nb * BLOCK, h, kv, d, blocks, _DTYPES[q.dtype],
                                             _P(out), _P(ws), r.stream()), "av2x_select_blocks")
     return out
 
@@ -337,7 +341,7 @@ def _launch_lists(r, blocks, n, h):
 
 
 def _strides9(q, k, v):
-    return _host64(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+    return _host64(*_steps(q), *_steps(k), *_steps(v))
 
 
 def _attend(q, k, v, blocks, mask, scale, grads):
