@@ -429,7 +429,16 @@ class BlockSparseAttention(nn.Module):
         self.to_qkv = nn.Linear(dim, (heads + 2 * kv_heads) * dim_head, bias=False)
         self.q_gamma, self.k_gamma = nn.Parameter(torch.ones(dim_head)), nn.Parameter(torch.ones(dim_head))
         self.to_out = nn.Linear(heads * dim_head, dim)
-        self.register_buffer("freqs", rotation_freqs(dim_head, axes, base), persistent=False)
+        self.rotation = (dim_head, axes, base)
+        self.register_buffer("freqs", rotation_freqs(*self.rotation), persistent=False)
+
+    def _apply(self, fn, recurse=True):
+        """Moves and casts (.to, .float, .half, ..): the frequencies move along and stay fp64."""
+        freqs = self.freqs
+        super()._apply(fn, recurse)
+        device = self.freqs.device
+        self.freqs = freqs.to(device) if not freqs.is_meta else rotation_freqs(*self.rotation, device=device)
+        return self
 
     def forward(self, x, positions, mask=None):
         from .airv2x_where2com import _amp_requested

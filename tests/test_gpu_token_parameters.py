@@ -64,3 +64,16 @@ def test_weights_at_odd_places_of_a_flat_buffer(monkeypatch, small):
               lambda x, w, b: F.linear(x.view(1, 7, 10, 64), w, b)):
         same(f, (x, odd(w), odd(b)), (x, w, b))
     same(lambda x, w, gm, bt: A.norm_linear(x, gm, bt, w), (odd(x), odd(w), odd(gamma), odd(beta)), (x, w, gamma, beta))
+
+
+@pytest.mark.parametrize("act8", [False, True])
+def test_a_layer_that_was_cast_and_back(act8):
+    import copy
+    from tests.test_gpu_token_layer import layer
+    m = layer(11, 256, 4, 2, 32, 2)
+    m.act8 = act8
+    x = torch.randn(1, 70, 256, generator=torch.Generator().manual_seed(11)).cuda()
+    pos = torch.stack([torch.arange(70) // 9, torch.arange(70) % 9], 1).int().cuda()
+    want = m(x, pos)
+    for cast in (lambda m: m.float(), lambda m: m.double().float(), lambda m: m.cpu().to(torch.float32).cuda()):
+        assert torch.equal(cast(copy.deepcopy(m))(x, pos), want)
