@@ -60,7 +60,17 @@ class LayerNormFn(torch.autograd.Function):
         return dx, dg, db
 
 
+def _check_vectors(what, n, *vectors):
+    """The kernels read n fp32 values of each."""
+    for v in vectors:
+        T._check_dev(v)
+        if tuple(v.shape) != (n,):
+            raise ValueError(f"{what}: a parameter of shape {tuple(v.shape)} where {n} values are needed")
+
+
 def layer_norm(x, gamma, beta):
+    T._check_dev(x)
+    _check_vectors("layer_norm", x.shape[-1], gamma, beta)
     return LayerNormFn.apply(x, gamma, beta)
 
 
@@ -107,6 +117,16 @@ class LinearFn(torch.autograd.Function):
 
 
 def linear(x, weight, bias=None, residual=None):
+    T._check_dev(x)
+    T._check_dev(weight)
+    if x.dim() != 4 or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
+        raise ValueError(f"linear: a weight of shape {tuple(weight.shape)} for tokens {tuple(x.shape)}")
+    if bias is not None:
+        _check_vectors("linear", weight.shape[0], bias)
+    if residual is not None:
+        T._check_dev(residual)
+        if tuple(residual.shape) != tuple(x.shape[:-1]) + (weight.shape[0],):
+            raise ValueError(f"linear: a residual of shape {tuple(residual.shape)} for tokens {tuple(x.shape)} and {weight.shape[0]} outputs")
     return LinearFn.apply(x, weight, bias, residual)
 
 

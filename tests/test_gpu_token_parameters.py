@@ -77,3 +77,51 @@ def test_a_layer_that_was_cast_and_back(act8):
     want = m(x, pos)
     for cast in (lambda m: m.float(), lambda m: m.double().float(), lambda m: m.cpu().to(torch.float32).cuda()):
         assert torch.equal(cast(copy.deepcopy(m))(x, pos), want)
+
+
+def test_the_fp32_layers_refuse_parameters_that_do_not_fit():
+    """Before anything is launched."""
+    from airv2x_perception_amd.opencood_iface import train_fusion_ops as F
+    from tests.test_gpu_token_layer import layer
+    x, w, v = torch.zeros(1, 2, 5, 256, device="cuda"), torch.zeros(64, 256, device="cuda"), torch.zeros(256, device="cuda")
+    for a, b, e in ((v.half(), v, RuntimeError), (v, v.double(), RuntimeError), (v.cpu(), v, RuntimeError), (v[:255], v, ValueError), (v, v[None], ValueError)):
+        with pytest.raises(e):
+            F.layer_norm(x, a, b)
+    bias, res = torch.zeros(64, device="cuda"), torch.zeros(1, 2, 5, 64, device="cuda")
+    for args, e in (((x.half(), w), RuntimeError), ((x, w.half()), RuntimeError), ((x, w[:, :128]), ValueError), ((x[0], w), ValueError), ((x, w, bias.half()), RuntimeError),
+                    ((x, w, bias[:63]), ValueError), ((x, w, bias.cpu()), RuntimeError), ((x, w, bias, res.half()), RuntimeError), ((x, w, bias, res[:, :1]), ValueError)):
+        with pytest.raises(e):
+            F.linear(*args)
+    assert F.linear(x, w, bias, res).shape == res.shape
+    pos = torch.zeros(70, 2, dtype=torch.int32, device="cuda")
+    for act8 in (False, True):
+        for cast in ("half", "double", "bfloat16"):
+            m = getattr(layer(12, 256, 4, 2, 32, 2), cast)()
+            m.act8 = act8
+            for t in (torch.float32, torch.half):
+                with pytest.raises((RuntimeError, ValueError), match="fp32"):
+                    m(torch.zeros(1, 70, 256, dtype=t, device="cuda"), pos)
+
+
+@pytest.mark.parametrize("act8", [False, True])
+@pytest.mark.parametrize("b,t,heads,dh", [(3, 1, 2, 16), (2, 13, 1, 32), (1, 70, 1, 128)])
+def test_small_layers(act8, b, t, heads, dh):
+    """One head, one token, samples of fewer tokens than a GEMM tile: the formulas of the layer in 64 bits (fp32: 2e-5, 8 bits: 2 %, as test_gpu_token_layer derives)."""
+    from tests.test_gpu_token_layer import choice, layer, reference, rel
+    m = layer(13, 256, heads, heads, dh, 2)
+    m.act8 = act8
+    g = torch.Generator().manual_seed(13)
+    x, dy = torch.randn(b, t, 256, generator=g).cuda().requires_grad_(), torch.randn(b, t, 256, generator=g).cuda()
+    pos = torch.stack([torch.arange(t) // 5, torch.arange(t) % 5], 1).int().cuda()
+    y = m(x, pos)
+    grads = torch.autograd.grad(y, [x] + list(m.parameters()), dy)
+    names = [n for n, _ in m.named_parameters()]
+    want, xr, P = reference(m, x, pos, None, choice(m, x.detach(), pos, None))
+    # a softmax over one key is 1 whatever q, k and their norms are: those gradients are zero, and rounding away from it
+    wg = torch.autograd.grad(want, [xr] + [P[n] for n in names], dy.double().cpu())
+    assert rel(y, want) <= 2e-5
+    for n, a, r in zip(["x"] + names, grads, wg):
+        if t > 1 or n not in ("q_gamma", "k_gamma"):
+            assert rel(a, r) <= (0.02 if act8 else 2e-5), (n, rel(a, r))
+        else:
+            assert float(a.abs().max()) <= 1e-4
