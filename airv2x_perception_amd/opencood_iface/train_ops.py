@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import threading
 import weakref
 from ctypes import byref, c_void_p
 
@@ -163,11 +164,25 @@ def _packed(r, weight, flipped=False, owner=None):
     return wp, coutp, u, ent
 
 
+class _StepFlag(threading.local):
+    """A flag of the step that the calling thread runs, read and written as flag[0]: steps on several threads (one a device) do not see each other's."""
+    on = False
+
+    def __getitem__(self, _):
+        return self.on
+
+    def __setitem__(self, _, on):
+        self.on = bool(on)
+
+    def __eq__(self, other):
+        return [self.on] == other
+
+
 # AMP training (tools/train.py:50,107-130: the forward runs under ``amp.autocast`` and the loss goes through a GradScaler): while
 # set, every Conv2d / ConvTranspose2d product of the step -- forward AND the data gradients, which autograd runs in the forward's
 # dtype -- uses bf16 matrix-core operands with fp32 accumulation (conv_igemm_bf16); BatchNorm statistics, the pillar encoder,
 # the attention, the loss and the weight gradients stay fp32, activations stay fp32 in HBM.  forward_train() sets it per step.
-AMP_STEP = [False]
+AMP_STEP = _StepFlag()
 
 
 def set_amp_step(on):
@@ -202,7 +217,7 @@ class amp_scope:
 
 # Token layers of the transformer fusions with 8-bit saved activations (act8_ops): while set, train_fusion_ops' norm_linear / token_linear / token_gelu / gelu_linear
 # build those nodes.  A node is what its forward made it, so the flag matters to the forward alone.
-ACT8_STEP = [False]
+ACT8_STEP = _StepFlag()
 
 
 class act8_scope:

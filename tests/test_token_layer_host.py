@@ -25,3 +25,31 @@ def test_a_layer_built_without_storage():
     assert m.freqs.is_meta
     m = m.to_empty(device="cpu")
     assert torch.equal(m.freqs, A.rotation_freqs(32, 2))
+
+
+@pytest.mark.parametrize("scope,flag", [("act8_scope", "ACT8_STEP"), ("amp_scope", "AMP_STEP")])
+def test_a_steps_flags_are_its_threads(scope, flag):
+    """Two models in forward on two threads: neither sees the other's setting, in either order of entering and leaving."""
+    import threading
+    from airv2x_perception_amd.opencood_iface import train_ops as T
+    scope, flag = getattr(T, scope), getattr(T, flag)
+    inside, leave, seen = threading.Event(), threading.Event(), []
+
+    def other():
+        with scope(True):
+            inside.set()
+            leave.wait(20)
+            seen.append(flag[0])
+        seen.append(flag[0])
+
+    t = threading.Thread(target=other)
+    t.start()
+    assert inside.wait(20)
+    assert flag == [False] and not flag[0]
+    with scope(True):
+        with scope(False):
+            leave.set()
+            t.join(20)
+            assert not flag[0]
+        assert flag[0]
+    assert not flag[0] and seen == [True, False]
