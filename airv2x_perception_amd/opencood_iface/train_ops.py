@@ -99,17 +99,19 @@ _ZEROS = {}
 
 
 def _zeros(c, device):
-    """Cached all-zero shift vector (read-only).  One that is first needed while a graph is recorded belongs to that graph: it holds zeros from its replay on only."""
-    z = _ZEROS.get((c, device))
+    """Cached all-zero shift vector (read-only), one a stream: on another one it may not be written yet.  One that is first needed while a graph is recorded belongs
+    to that graph: it holds zeros from its replay on only."""
+    key = (c, device, torch.cuda.current_stream(device).cuda_stream)
+    z = _ZEROS.get(key)
     if z is None:
         z = torch.zeros(c, device=device)
         if not torch.cuda.is_current_stream_capturing():
-            _ZEROS[(c, device)] = z
+            _ZEROS[key] = z
     return z
 
 
 # ------------------------------------------------------------------------------------------------ raw launches
-_PACKED = {}       # id(parameter) -> (version, weakref, packed, coutp, winograd-transformed | None): one packing per optimiser step
+_PACKED = {}       # (id(parameter), .., stream) -> (version, weakref, packed, coutp, winograd-transformed | None): one packing per optimiser step and stream
 
 
 _RECORDED = {}     # id(parameter) -> weakref: weights of recorded steps
@@ -142,7 +144,8 @@ def _packed(r, weight, flipped=False, owner=None):
     # ``owner``: the nn.Parameter a reshaped view was taken from (nn.Linear's (cout, cin) weight seen as a 1x1 convolution): the cache
     # is keyed on it -- the view is a new object on every call (it shares the parameter's storage and version counter)
     own = owner if owner is not None else weight
-    key = (id(own), flipped, tuple(weight.shape))
+    # one a stream: on another one the packing may not be written yet, and its memory may be taken again while that one still reads it
+    key = (id(own), flipped, tuple(weight.shape), r.stream().value)
     keep = _may_keep(own)
     ent = _PACKED.get(key) if keep else None
     # ``_version`` does not move for writes through ``.data`` nor for ``module.to(device)`` (which re-points ``.data``): the storage

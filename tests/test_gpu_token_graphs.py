@@ -112,3 +112,31 @@ def test_packings_are_forgotten_on_demand():
         torch.cuda.synchronize()
         T.forget_packings()
         assert all(torch.equal(a, b) for a, b in zip(step(), step(copy.deepcopy(m))))
+
+
+@pytest.mark.parametrize("act8", [False, True])
+def test_a_weight_packed_on_a_busy_stream(monkeypatch, act8):
+    """A layer called on two streams at once: the second call does not take a packing (or zeros) that the first stream has yet to write."""
+    from airv2x_perception_amd.opencood_iface import act8_ops as A8, train_fusion_ops as F, train_ops as T
+    monkeypatch.setattr(A8, "SMALL_PRODUCT", 0)
+    g = torch.Generator().manual_seed(17)
+    x = torch.randn(1, 10, 20, 256, generator=g).cuda()
+    w = torch.nn.Parameter(torch.randn(256, 256, generator=g).cuda())
+    f = (lambda w: A8.linear(x, w)) if act8 else (lambda w: F.linear(x, w))
+    want = f(copy.deepcopy(w)).detach()
+    big = torch.randn(4096, 4096, device="cuda")
+    monkeypatch.setattr(T, "_PACKED", {})
+    monkeypatch.setattr(T, "_ZEROS", {})
+    torch.empty(1 << 22, device="cuda").fill_(float("nan"))          # what freshly taken memory holds
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(one):
+        for _ in range(40):                                          # some 40 ms of work
+            big = (big @ big).clamp_(-1, 1)
+        a = f(w).detach()
+    with torch.cuda.stream(two):
+        b = f(w).detach()
+    two.synchronize()
+    got = b.cpu()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want.cpu()) and torch.equal(a, want)
