@@ -836,9 +836,9 @@ __global__ __launch_bounds__(1024) void bs_scan_kernel(int NB, int G, int rows, 
 // Accumulators: column lane & 31, rows 8 (i / 4) + 4 half + i % 4; a contraction over keys or queries takes such a tile as the B operand as it lies: step s
 // of 16 covers rows 16 s + 4 half + {0..3, 8..11}.
 //
-// fp32 tensors run on the same instructions as two fp16 terms each: a row (queries, dO) or a block (K, V) is brought to the top of fp16's range by a power of two,
-// hi + lo hold it to 22 bits, three products of terms make one product.  Three 16-bit MFMAs take 3 / 16 of the time of the fp32 instruction
-// (backward of 281600 queries x 8 blocks: 597 us, 1204 with v_mfma_f32_32x32x2_f32).
+// fp32 tensors run on the fp32 instruction, 32 x 32 x 2: the eight elements of a piece one after the other, so that nothing of a value's 24 bits or of its range is
+// lost beside another one (an infinity among the values stays one).  Two fp16 terms of values relative to the largest of their block are faster (281600 queries x 8 blocks:
+// forward 206 us against 285, backward 597 against 814) and hold 22 bits, but only of values within 2^-18 of that largest: one huge value took the others' bits.
 template <typename T> struct Op;
 template <> struct Op<__bf16> {
     typedef __bf16 frag __attribute__((ext_vector_type(8)));
@@ -848,20 +848,22 @@ template <> struct Op<_Float16> {
     typedef _Float16 frag __attribute__((ext_vector_type(8)));
     static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
-template <typename T> struct Held {              // how a tensor of T is held in LDS and registers
-    static constexpr bool two = is_f32<T>::value;
-    static constexpr int terms = two ? 2 : 1;
-    typedef typename std::conditional<two, _Float16, T>::type E;
-    typedef typename Op<E>::frag frag;
-    static constexpr bool narrow = std::is_same<E, _Float16>::value;      // P and dS need a common power of two
+template <> struct Op<float> {
+    typedef float frag __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+        return c;
+    }
 };
+template <typename T> constexpr bool kNarrow = std::is_same<T, _Float16>::value;      // P and dS need a common power of two
 
 template <typename T, int D> struct Shape {
     static constexpr int KS = D / 16;                           // k-steps over d
     static constexpr int DT = (D + 31) / 32;                    // 32-wide tiles of d
-    static constexpr int P = D + 8;                             // row pitch of a [row][d] tile: banks
+    static constexpr int P = D + 16 / (int)sizeof(T);           // row pitch of a [row][d] tile: banks
     static constexpr int PT = kKeys + 4;                        // row pitch of a [d][key] tile
-    static constexpr int kRowTile = kKeys * P;                  // of one term
+    static constexpr int kRowTile = kKeys * P;
     static constexpr int kTransTile = DT * 32 * PT;             // d padded to 32 with zeros
 };
 
@@ -872,155 +874,99 @@ __device__ __forceinline__ f32x16 zero16() {
     return z;
 }
 
+// eight elements on a 16-byte address, in pieces of 16 bytes
+template <typename T> __device__ __forceinline__ typename tok_vec<T>::v8 get8(const T* p) {
+    if constexpr (is_f32<T>::value) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+        return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+        return *reinterpret_cast<const typename tok_vec<T>::v8*>(p);
+    }
+}
+template <typename T> __device__ __forceinline__ void put8(T* p, typename tok_vec<T>::v8 x) {
+    if constexpr (is_f32<T>::value) {
+        *reinterpret_cast<f32x4*>(p) = f32x4{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<f32x4*>(p + 4) = f32x4{x[4], x[5], x[6], x[7]};
+    } else {
+        *reinterpret_cast<typename tok_vec<T>::v8*>(p) = x;
+    }
+}
+
 // the power of two that brings m to 2^14 .. 2^15, the top of fp16: values down to 2^-18 of the largest keep 22 bits in two terms, and what is below that is off by
-// 2^-40 of it at most
+// 2^-39 of it at most (half of fp16's last step, 2^-25, beside 2^14)
 __device__ __forceinline__ float pow2_over(float m) {
     return m < INFINITY ? ldexpf(1.0f, max(__builtin_amdgcn_frexp_expf(m) - 15, -126)) : 1.0f;      // (its reciprocal stays finite)
 }
 
-// rows [0, 64) of a block to LDS: [key][d], and [d][key] of DA channels from d0 on.  Keys behind the end or masked are zeros.  Returns the power of two that was taken out (fp32).
+// rows [0, 64) of a block to LDS: [key][d], and [d][key] of DA channels from d0 on.  Keys behind the end or masked are zeros.
 // All 256 threads; ends with the writes, not with a barrier.
 template <typename T, int D, bool ROW, bool TRANS, int DA = D>
-__device__ __forceinline__ float load_block(const T* src, long long st, int t0, unsigned long long seen, typename Held<T>::E* row, typename Held<T>::E* tr, float* red, int d0 = 0) {
+__device__ __forceinline__ void load_block(const T* src, long long st, int t0, unsigned long long seen, T* row, T* tr, int d0 = 0) {
     using S = Shape<T, D>;
-    constexpr int kTrans = Shape<T, DA>::kTransTile;
-    using E = typename Held<T>::E;
     constexpr int CPR = D / 8, N = kKeys * CPR / 256 > 0 ? kKeys * CPR / 256 : 1;
-    typedef T vec __attribute__((ext_vector_type(8)));
-    typedef E evec __attribute__((ext_vector_type(8)));
+    typedef typename tok_vec<T>::v8 vec;
     vec x[N];
-    float m = 0.f, back = 1.0f;
 #pragma unroll
     for (int u = 0; u < N; ++u) {
         const int i = threadIdx.x + u * 256, key = i & 63, c = i >> 6;
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[u][e] = (T)0.f;
-        if (c < CPR && (seen >> key & 1)) {
-            const T* p = src + (long long)(t0 + key) * st + c * 8;
-            if constexpr (Held<T>::two) {
-                const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) { x[u][e] = a[e]; x[u][4 + e] = b[e]; m = fmaxf(m, fmaxf(fabsf(a[e]), fabsf(b[e]))); }
-            } else {
-                x[u] = *reinterpret_cast<const vec*>(p);
-            }
-        }
+        if (c < CPR && (seen >> key & 1)) x[u] = get8(src + (long long)(t0 + key) * st + c * 8);
     }
-    if constexpr (Held<T>::two) {
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-        __syncthreads();
-        back = pow2_over(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-    }
-    const float to = 1.0f / back;
 #pragma unroll
     for (int u = 0; u < N; ++u) {
         const int i = threadIdx.x + u * 256, key = i & 63, c = i >> 6;
         if (c >= CPR) continue;
+        if constexpr (ROW) put8(row + key * S::P + c * 8, x[u]);
+        if constexpr (TRANS) {
+            const int d = c * 8 - d0;
+            if (DA == D || (d >= 0 && d < DA)) {
 #pragma unroll
-        for (int k = 0; k < Held<T>::terms; ++k) {
-            evec y;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if constexpr (Held<T>::two) {
-                    const float v = x[u][e] * to;
-                    const _Float16 h = (_Float16)v;
-                    y[e] = k == 0 ? h : (_Float16)(v - (float)h);
-                } else {
-                    y[e] = x[u][e];
-                }
-            }
-            if constexpr (ROW) *reinterpret_cast<evec*>(row + k * S::kRowTile + key * S::P + c * 8) = y;
-            if constexpr (TRANS) {
-                const int d = c * 8 - d0;
-                if (DA == D || (d >= 0 && d < DA)) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) tr[k * kTrans + (d + e) * S::PT + key] = y[e];
-                }
+                for (int e = 0; e < 8; ++e) tr[(d + e) * S::PT + key] = x[u][e];
             }
         }
     }
     if constexpr (TRANS && D < 32) {
-        for (int i = threadIdx.x; i < (32 - D) * S::PT; i += 256)
-#pragma unroll
-            for (int k = 0; k < Held<T>::terms; ++k) tr[k * kTrans + D * S::PT + i] = (E)0.f;
+        for (int i = threadIdx.x; i < (32 - D) * S::PT; i += 256) tr[D * S::PT + i] = (T)0.f;
     }
-    return back;
 }
 
-// a head vector in pieces of one k-step and its power of two, straight from global memory; the two half waves hold halves of it
-template <typename T, int D> struct RowFrags {
-    typename Held<T>::frag f[Held<T>::terms][Shape<T, D>::KS];
-    float back = 1.0f;
-};
-template <typename T, int D> struct RawRow { typename tok_vec<T>::v8 x[D / 16]; };
-template <typename T, int D> __device__ __forceinline__ RawRow<T, D> load_row(const T* p, bool in, int half) {
-    RawRow<T, D> r;
+// a head vector in pieces of one k-step, straight from global memory; the two half waves hold halves of it
+template <typename T, int D> struct RowFrags { typename Op<T>::frag f[D / 16]; };
+template <typename T, int D> __device__ __forceinline__ RowFrags<T, D> load_row(const T* p, bool in, int half) {
+    RowFrags<T, D> r;
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) r.x[s][e] = (T)0.f;
-        if (in) r.x[s] = *reinterpret_cast<const typename tok_vec<T>::v8*>(p + s * 16 + half * 8);
+        for (int e = 0; e < 8; ++e) r.f[s][e] = (T)0.f;
+        if (in) r.f[s] = get8(p + s * 16 + half * 8);
     }
     return r;
-}
-template <typename T, int D> __device__ __forceinline__ void to_frags(const RawRow<T, D>& w, RowFrags<T, D>& r) {
-    if constexpr (Held<T>::two) {
-        float m = 0.f;
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(w.x[s][e]));
-        m = fmaxf(m, __shfl_xor(m, 32));
-        r.back = pow2_over(m);
-        const float to = 1.0f / r.back;
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float v = w.x[s][e] * to;
-                const _Float16 h = (_Float16)v;
-                r.f[0][s][e] = h;
-                r.f[1][s][e] = (_Float16)(v - (float)h);
-            }
-    } else {
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s) r.f[0][s] = w.x[s];
-    }
 }
 
 // acc += (32 rows of an LDS tile) x (32 row vectors in registers), over d; SWAP: the LDS rows are the columns of the result
 template <typename T, int D, bool SWAP>
-__device__ __forceinline__ f32x16 mma_d(const typename Held<T>::E* tile, int r, int half, const RowFrags<T, D>& q, f32x16 acc) {
+__device__ __forceinline__ f32x16 mma_d(const T* tile, int r, int half, const RowFrags<T, D>& q, f32x16 acc) {
     using S = Shape<T, D>;
-    using O = Op<typename Held<T>::E>;
-    using frag = typename Held<T>::frag;
-    auto mul = [&](frag a, frag b) { acc = SWAP ? O::mma(b, a, acc) : O::mma(a, b, acc); };
 #pragma unroll
     for (int s = 0; s < S::KS; ++s) {
-        const frag hi = *reinterpret_cast<const frag*>(tile + r * S::P + s * 16 + half * 8);
-        if constexpr (Held<T>::two) {
-            const frag lo = *reinterpret_cast<const frag*>(tile + S::kRowTile + r * S::P + s * 16 + half * 8);
-            mul(lo, q.f[0][s]);
-            mul(hi, q.f[1][s]);
-        }
-        mul(hi, q.f[0][s]);
+        const typename Op<T>::frag x = get8(tile + r * S::P + s * 16 + half * 8);
+        acc = SWAP ? Op<T>::mma(q.f[s], x, acc) : Op<T>::mma(x, q.f[s], acc);
     }
     return acc;
 }
 
-// A 32 x 32 tile of P or dS as B operand in two terms: the product then has the precision of fp32 probabilities and the result's own rounding is the only one
-// that counts.  RANGE: the backward's tiles have no largest value to be relative to, and fp16 ends at 2^-24: a column (a lane and the one 32 further, in the
-// operand and in the result) is brought to the top of its range by a power of two, and the product brought back (gradients of a scaled or a small loss keep their
-// precision); bf16 has the range.  The first fp16 term is cut, not rounded (one instruction for two): the second, rounded, holds what it leaves.
+// A 32 x 32 tile of P or dS as B operand: fp32 as it is, for 16-bit tensors in two terms -- the product then has the precision of fp32 probabilities and the result's own
+// rounding is the only one that counts.  RANGE: the backward's tiles have no largest value to be relative to, and fp16 ends at 2^-24: a column (a lane and the one 32
+// further, in the operand and in the result) is brought to the top of its range by a power of two, and the product brought back (gradients of a scaled or a small loss
+// keep their precision); bf16 has the range.  The first fp16 term is cut, not rounded (one instruction for two): the second, rounded, holds what it leaves.
 template <typename T, bool RANGE> struct Split {
-    using E = typename Held<T>::E;
-    typename Held<T>::frag hi[2], lo[2];
+    static constexpr bool two = !is_f32<T>::value, far = RANGE && kNarrow<T>;
+    typename Op<T>::frag hi[2], lo[2];
     float back = 1.0f;
     __device__ __forceinline__ explicit Split(const f32x16& p) {
         float to = 1.0f;
-        if constexpr (RANGE && Held<T>::narrow) {
+        if constexpr (far) {
             float m = 0.f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(p[i]));
@@ -1032,47 +978,39 @@ template <typename T, bool RANGE> struct Split {
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
-                const float x = RANGE && Held<T>::narrow ? p[s * 8 + e] * to : p[s * 8 + e], y = RANGE && Held<T>::narrow ? p[s * 8 + e + 1] * to : p[s * 8 + e + 1];
-                E h, g;
-                if constexpr (Held<T>::narrow) {
+                const float x = far ? p[s * 8 + e] * to : p[s * 8 + e], y = far ? p[s * 8 + e + 1] * to : p[s * 8 + e + 1];
+                T h, g;
+                if constexpr (kNarrow<T>) {
                     const auto c = __builtin_amdgcn_cvt_pkrtz(x, y);
-                    h = (E)c[0];
-                    g = (E)c[1];
+                    h = (T)c[0];
+                    g = (T)c[1];
                 } else {
-                    h = (E)x;
-                    g = (E)y;
+                    h = (T)x;
+                    g = (T)y;
                 }
                 hi[s][e] = h;
                 hi[s][e + 1] = g;
-                lo[s][e] = (E)(x - (float)h);
-                lo[s][e + 1] = (E)(y - (float)g);
+                if constexpr (two) {
+                    lo[s][e] = (T)(x - (float)h);
+                    lo[s][e + 1] = (T)(y - (float)g);
+                }
             }
     }
 };
 
-// acc (d x columns) += A^T (d x 32 rows) p (32 rows x columns): A in LDS as [d][row], its second term `term` elements behind
+// acc (d x columns) += A^T (d x 32 rows) p (32 rows x columns): A in LDS as [d][row]
 template <typename T, bool RANGE>
-__device__ __forceinline__ f32x16 mma_rows(const typename Held<T>::E* a, int pitch, int term, int lane, const Split<T, RANGE>& x, f32x16 acc) {
-    using E = typename Held<T>::E;
-    using O = Op<E>;
-    using frag = typename Held<T>::frag;
-    typedef E v4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x16 mma_rows(const T* a, int pitch, int lane, const Split<T, RANGE>& x, f32x16 acc) {
+    typedef typename tok_vec<T>::v4 v4;
     const int half = lane >> 5, m = lane & 31;
-    constexpr bool far = RANGE && Held<T>::narrow;
+    constexpr bool far = Split<T, RANGE>::far;
     f32x16 t = far ? zero16() : acc;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-        auto get = [&](const E* p) {
-            const v4 u = *reinterpret_cast<const v4*>(p + m * pitch + s * 16 + half * 4), w = *reinterpret_cast<const v4*>(p + m * pitch + s * 16 + half * 4 + 8);
-            frag f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) { f[e] = u[e]; f[4 + e] = w[e]; }
-            return f;
-        };
-        const frag hi = get(a);
-        if constexpr (Held<T>::two) t = O::mma(get(a + term), x.hi[s], t);
-        t = O::mma(hi, x.lo[s], t);
-        t = O::mma(hi, x.hi[s], t);
+        const v4 u = *reinterpret_cast<const v4*>(a + m * pitch + s * 16 + half * 4), w = *reinterpret_cast<const v4*>(a + m * pitch + s * 16 + half * 4 + 8);
+        const typename Op<T>::frag f = __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7);
+        if constexpr (Split<T, RANGE>::two) t = Op<T>::mma(f, x.lo[s], t);
+        t = Op<T>::mma(f, x.hi[s], t);
     }
     if constexpr (far) {
 #pragma unroll
@@ -1126,17 +1064,14 @@ template <int D> struct Record {
     static __device__ __forceinline__ f32x4 get(const char* r, int d) { return *reinterpret_cast<const v4*>(r + 8 + d * 4); }
 };
 
-// 281600 queries x 8 blocks of 32 channels: bf16 197 us, fp32 206 us.  The products take 25 and 48 us at the matrix cores' measured rate, the records 62 us at HBM's; the
-// vector units bound it: about 20 instructions for each score a lane holds (scaling, maximum, exponential, sum, two terms).  The launch bounds keep one more wave
-// on a SIMD than the compiler would (heads of 64 fp32: 136 us against 166, of 128 bf16: 103 against 115).
+// 281600 queries x 8 blocks of 32 channels: bf16 197 us, fp32 285 us.  The products take 25 and 120 us at the matrix cores' measured rates, the records 62 us at HBM's,
+// and neither overlaps well with the vector steps of a score (scaling, maximum, exponential, sum, two terms): a wave goes through them one after the other, and
+// three or four waves a SIMD hide only part of that.  The launch bounds keep one more wave on a SIMD than the compiler would (heads of 128 bf16: 103 us against 115).
 template <typename T, int D>
-__global__ __launch_bounds__(256, (Held<T>::two ? (D <= 32 ? 3 : D == 64 ? 2 : 1) : (D <= 32 ? 4 : D == 64 ? 3 : 2))) void bs_forward_kernel(BsArgs a) {
+__global__ __launch_bounds__(256, (is_f32<T>::value ? (D <= 32 ? 3 : D == 64 ? 2 : 1) : (D <= 32 ? 4 : D == 64 ? 3 : 2))) void bs_forward_kernel(BsArgs a) {
     using S = Shape<T, D>;
-    using E = typename Held<T>::E;
-    constexpr int TERMS = Held<T>::terms;
-    __shared__ __align__(16) E lk[TERMS * S::kRowTile];
-    __shared__ __align__(16) E lv[TERMS * S::kTransTile];
-    __shared__ float red[2][4];
+    __shared__ __align__(16) T lk[S::kRowTile];
+    __shared__ __align__(16) T lv[S::kTransTile];
     const int bh = blockIdx.y, b = bh / a.KV, h = bh % a.KV;
     if ((int)blockIdx.x >= a.n_items[bh]) return;
     const int32_t* it = a.items + ((size_t)bh * a.max_items + blockIdx.x) * 2;
@@ -1149,22 +1084,20 @@ __global__ __launch_bounds__(256, (Held<T>::two ? (D <= 32 ? 3 : D == 64 ? 2 : 1
     const T* qbase = static_cast<const T*>(a.q) + b * a.qb;
     // the first queries are on their way before K and V, the next ones during the work on these
     Row r = row_of(a, list, len, h, first + wave * 32 + (lane & 31));
-    RawRow<T, D> raw = load_row<T, D>(qbase + r.t * a.qt + r.head * a.qh, r.in, half);
+    RowFrags<T, D> raw = load_row<T, D>(qbase + r.t * a.qt + r.head * a.qh, r.in, half);
     const unsigned long long seen = seen_keys(a, b, j);
-    const float kf = load_block<T, D, true, false>(static_cast<const T*>(a.k) + b * a.kb + h * a.kh, a.kt, j * kKeys, seen, lk, nullptr, red[0]);
-    const float vf = load_block<T, D, false, true>(static_cast<const T*>(a.v) + b * a.vb + h * a.vh, a.vt, j * kKeys, seen, nullptr, lv, red[1]);
+    load_block<T, D, true, false>(static_cast<const T*>(a.k) + b * a.kb + h * a.kh, a.kt, j * kKeys, seen, lk, nullptr);
+    load_block<T, D, false, true>(static_cast<const T*>(a.v) + b * a.vb + h * a.vh, a.vt, j * kKeys, seen, nullptr, lv);
     __syncthreads();
-    const float c2 = a.scale * kLog2e * kf;
+    const float c = a.scale * kLog2e;
     Row ahead = row_of(a, list, len, h, first + wave * 32 + 128 + (lane & 31));
     for (int r0 = first + wave * 32; r0 < last; r0 += 128) {
-        RowFrags<T, D> qf;
-        to_frags<T, D>(raw, qf);
+        const RowFrags<T, D> qf = raw;
         const Row next = ahead;
         if (r0 + 128 < last) {
             raw = load_row<T, D>(qbase + next.t * a.qt + next.head * a.qh, next.in, half);
             ahead = row_of(a, list, len, h, r0 + 256 + (lane & 31));
         }
-        const float c = c2 * qf.back;
         f32x16 s[2];
         float m = -INFINITY;
 #pragma unroll
@@ -1177,7 +1110,7 @@ __global__ __launch_bounds__(256, (Held<T>::two ? (D <= 32 ? 3 : D == 64 ? 2 : 1
             for (int i = 0; i < 16; ++i) m = fmaxf(m, s[kt][i]);
         }
         m = fmaxf(m, __shfl_xor(m, 32));
-        constexpr float kTop = Held<T>::narrow ? 15.f : 0.f;               // fp16 terms: from the top of their range as well
+        constexpr float kTop = kNarrow<T> ? 15.f : 0.f;               // fp16 terms: from the top of their range as well
         const float base = m == -INFINITY ? 0.f : m - kTop;
         float l = 0.f;
 #pragma unroll
@@ -1188,14 +1121,14 @@ __global__ __launch_bounds__(256, (Held<T>::two ? (D <= 32 ? 3 : D == 64 ? 2 : 1
                 l += s[kt][i];
             }
         l += __shfl_xor(l, 32);
-        const float inv = l == 0.f ? 0.f : vf / l;
-        if constexpr (Held<T>::narrow) l *= 1.0f / 32768.f;
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        if constexpr (kNarrow<T>) l *= 1.0f / 32768.f;
         char* rec = Record<D>::at(a.part, (((size_t)b * a.T + r.t) * a.H + r.head) * a.n + r.slot);
         const Split<T, false> p0(s[0]), p1(s[1]);
 #pragma unroll
         for (int dt = 0; dt < S::DT; ++dt) {
-            f32x16 o = mma_rows<T>(lv + dt * 32 * S::PT, S::PT, S::kTransTile, lane, p0, zero16());
-            o = mma_rows<T>(lv + dt * 32 * S::PT + 32, S::PT, S::kTransTile, lane, p1, o);
+            f32x16 o = mma_rows<T>(lv + dt * 32 * S::PT, S::PT, lane, p0, zero16());
+            o = mma_rows<T>(lv + dt * 32 * S::PT + 32, S::PT, lane, p1, o);
             if (r.in) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -1345,27 +1278,22 @@ __global__ __launch_bounds__(256) void bs_delta_kernel(const T* __restrict__ out
 
 // One workgroup per work item, four waves of 32 rows.  P and dP are computed twice, as keys x queries for dQ (a lane keeps a query) and as queries x
 // keys for dK, dV (a lane keeps a key): two more products instead of a transpose through LDS.  DA: the part of d whose dK, dV, dQ this workgroup
-// keeps (blockIdx.z-th).  The powers of two of fp32 operands: those of K and V are common to the block and are applied on their own -- in one factor with a
-// query's they would leave fp32's range where both are small --, those of a query's Q and dO go into its dS and P.
-// 281600 queries x 8 blocks of 32 channels, fp32: 597 us; 17600 x 8 of 64, bf16: 81 us.  Seven products (three terms each in fp32: 194 GFLOP, 170 us at the matrix cores'
-// measured rate); the vector units bound it: two exponentials and four splits into terms for every score, at two waves a SIMD (256 registers).
+// keeps (blockIdx.z-th).
+// 281600 queries x 8 blocks of 32 channels, fp32: 814 us; 17600 x 8 of 64, bf16: 76 us.  Seven products: 64.6 GFLOP in fp32, 420 us at the matrix cores' measured rate;
+// two waves a SIMD (205 registers of 256) leave a good part of the two exponentials a score and of the LDS reads uncovered.
 template <typename T, int D, int DA>
 __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsArgs a) {
     using S = Shape<T, D>;
-    using E = typename Held<T>::E;
-    constexpr bool two = Held<T>::two;
-    constexpr int TERMS = Held<T>::terms;
     constexpr int AT = (DA + 31) / 32;                                     // d tiles of this workgroup
-    constexpr int QP = 32 + 4, kWaveTile = AT * 32 * QP;                   // per-wave tile of 32 rows: [d][row], of one term
+    constexpr int QP = 32 + 4, kWaveTile = AT * 32 * QP;                   // per-wave tile of 32 rows: [d][row]
     constexpr int kTrans = Shape<T, DA>::kTransTile;
-    constexpr size_t kTiles = sizeof(E) * TERMS * (2 * S::kRowTile + kTrans + 8 * kWaveTile);
+    constexpr size_t kTiles = sizeof(T) * (2 * S::kRowTile + kTrans + 8 * kWaveTile);
     __shared__ __align__(16) char smem[kTiles > 32768 ? kTiles : 32768];   // the last sums take 32 KB
-    E* lk = reinterpret_cast<E*>(smem);
-    E* lv = lk + TERMS * S::kRowTile;
-    E* lkt = lv + TERMS * S::kRowTile;
-    E* lqs = lkt + TERMS * kTrans;
-    __shared__ __align__(16) f32x4 lld[4][32];
-    __shared__ float red4[2][4];
+    T* lk = reinterpret_cast<T*>(smem);
+    T* lv = lk + S::kRowTile;
+    T* lkt = lv + S::kRowTile;
+    T* lqs = lkt + kTrans;
+    __shared__ __align__(16) f32x2 lld[4][32];
     const int bh = blockIdx.y, b = bh / a.KV, h = bh % a.KV, d0 = blockIdx.z * DA;
     if ((int)blockIdx.x >= a.n_items[bh]) return;
     const int32_t* it = a.items + ((size_t)bh * a.max_items + blockIdx.x) * 2;
@@ -1374,19 +1302,17 @@ __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsA
     const int len = st[1] - st[0];
     const int32_t* list = a.list + (size_t)bh * a.T * a.n + st[0];
     const unsigned long long seen = seen_keys(a, b, j);
-    const float kf = load_block<T, D, true, true, DA>(static_cast<const T*>(a.k) + b * a.kb + h * a.kh, a.kt, j * kKeys, seen, lk, lkt, red4[0], d0);
-    const float vf = load_block<T, D, true, false>(static_cast<const T*>(a.v) + b * a.vb + h * a.vh, a.vt, j * kKeys, seen, lv, nullptr, red4[1]);
+    load_block<T, D, true, true, DA>(static_cast<const T*>(a.k) + b * a.kb + h * a.kh, a.kt, j * kKeys, seen, lk, lkt, d0);
+    load_block<T, D, true, false>(static_cast<const T*>(a.v) + b * a.vb + h * a.vh, a.vt, j * kKeys, seen, lv, nullptr);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    E* lq = lqs + wave * 2 * TERMS * kWaveTile;
-    E* lo = lq + TERMS * kWaveTile;
+    T* lq = lqs + wave * 2 * kWaveTile;
+    T* lo = lq + kWaveTile;
     if constexpr (DA < 32) {                                               // channels behind D: zeros, once
-        for (int i = lane; i < (32 - DA) * QP; i += 64)
-#pragma unroll
-            for (int k = 0; k < TERMS; ++k) lq[k * kWaveTile + DA * QP + i] = lo[k * kWaveTile + DA * QP + i] = (E)0.f;
+        for (int i = lane; i < (32 - DA) * QP; i += 64) lq[DA * QP + i] = lo[DA * QP + i] = (T)0.f;
     }
     __syncthreads();
     const int last = min(first + a.item_rows, len * a.G);
-    const float c2 = a.scale * kLog2e * kf;
+    const float c = a.scale * kLog2e;
     f32x16 dk[AT][2], dv[AT][2];
 #pragma unroll
     for (int t = 0; t < AT; ++t) { dk[t][0] = zero16(); dk[t][1] = zero16(); dv[t][0] = zero16(); dv[t][1] = zero16(); }
@@ -1394,23 +1320,19 @@ __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsA
     for (int r0 = first + wave * 32; r0 < last; r0 += 128) {
         const Row r = ahead;
         const size_t qrow = ((size_t)b * a.T + r.t) * a.H + r.head;
-        RowFrags<T, D> qf, of;
-        to_frags<T, D>(load_row<T, D>(static_cast<const T*>(a.q) + b * a.qb + r.t * a.qt + r.head * a.qh, r.in, half), qf);
-        to_frags<T, D>(load_row<T, D>(static_cast<const T*>(a.dout) + qrow * D, r.in, half), of);
+        const RowFrags<T, D> qf = load_row<T, D>(static_cast<const T*>(a.q) + b * a.qb + r.t * a.qt + r.head * a.qh, r.in, half);
+        const RowFrags<T, D> of = load_row<T, D>(static_cast<const T*>(a.dout) + qrow * D, r.in, half);
         const f32x2 ld = r.in ? a.ld[qrow] : f32x2{INFINITY, 0.f};         // rows that are not there: P = 0
         ahead = row_of(a, list, len, h, r0 + 128 + (lane & 31));
-        if (half == 0) lld[wave][lane & 31] = f32x4{qf.back, ld.x, of.back, ld.y};
+        if (half == 0) lld[wave][lane & 31] = ld;
 #pragma unroll
         for (int s = 0; s < S::KS; ++s)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int d = s * 16 + half * 8 + e - d0;
                 if (DA == D || (d >= 0 && d < DA)) {
-#pragma unroll
-                    for (int k = 0; k < TERMS; ++k) {
-                        lq[k * kWaveTile + d * QP + (lane & 31)] = qf.f[k][s][e];
-                        lo[k * kWaveTile + d * QP + (lane & 31)] = of.f[k][s][e];
-                    }
+                    lq[d * QP + (lane & 31)] = qf.f[s][e];
+                    lo[d * QP + (lane & 31)] = of.f[s][e];
                 }
             }
         __builtin_amdgcn_wave_barrier();
@@ -1422,14 +1344,14 @@ __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsA
             // keys x queries
             f32x16 s = mma_d<T, D, false>(lk, kt * 32 + (lane & 31), half, qf, zero16()), p = mma_d<T, D, false>(lv, kt * 32 + (lane & 31), half, of, zero16());
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = fmaf(s[i] * c2, qf.back, -ld.x);
+            for (int i = 0; i < 16; ++i) s[i] = fmaf(s[i], c, -ld.x);
             if (seen != ~0ull) hide(s, seen, kt, half);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(s[i]) * fmaf(p[i] * vf, of.back, -ld.y);
+            for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(s[i]) * (p[i] - ld.y);
             {
                 const Split<T, true> ds(p);
 #pragma unroll
-                for (int t = 0; t < AT; ++t) dq[t] = mma_rows<T>(lkt + t * 32 * S::PT + kt * 32, S::PT, kTrans, lane, ds, dq[t]);
+                for (int t = 0; t < AT; ++t) dq[t] = mma_rows<T>(lkt + t * 32 * S::PT + kt * 32, S::PT, lane, ds, dq[t]);
             }
             __builtin_amdgcn_sched_barrier(0);                             // one part's registers at a time
             // queries x keys
@@ -1438,21 +1360,20 @@ __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsA
             // (keys that are not visible: their columns are left out at the end)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const f32x4 x = lld[wave][8 * (i / 4) + 4 * half + (i & 3)];
-                const float w = __builtin_amdgcn_exp2f(fmaf(s[i] * c2, x[0], -x[1]));
-                p[i] = w * fmaf(p[i] * vf, x[2], -x[3]) * x[0];
-                s[i] = w * x[2];
+                const f32x2 x = lld[wave][8 * (i / 4) + 4 * half + (i & 3)];
+                s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -x[0]));
+                p[i] = s[i] * (p[i] - x[1]);
             }
             {
                 const Split<T, true> rp(s);
 #pragma unroll
-                for (int t = 0; t < AT; ++t) dv[t][kt] = mma_rows<T>(lo + t * 32 * QP, QP, kWaveTile, lane, rp, dv[t][kt]);
+                for (int t = 0; t < AT; ++t) dv[t][kt] = mma_rows<T>(lo + t * 32 * QP, QP, lane, rp, dv[t][kt]);
             }
             __builtin_amdgcn_sched_barrier(0);
             {
                 const Split<T, true> rs(p);
 #pragma unroll
-                for (int t = 0; t < AT; ++t) dk[t][kt] = mma_rows<T>(lq + t * 32 * QP, QP, kWaveTile, lane, rs, dk[t][kt]);
+                for (int t = 0; t < AT; ++t) dk[t][kt] = mma_rows<T>(lq + t * 32 * QP, QP, lane, rs, dk[t][kt]);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -1464,7 +1385,7 @@ __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsA
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int d = t * 32 + 8 * i + 4 * half;
-                    if (d < DA) *reinterpret_cast<f32x4*>(dst + d) = f32x4{dq[t][4 * i], dq[t][4 * i + 1], dq[t][4 * i + 2], dq[t][4 * i + 3]} * (kf * a.scale);
+                    if (d < DA) *reinterpret_cast<f32x4*>(dst + d) = f32x4{dq[t][4 * i], dq[t][4 * i + 1], dq[t][4 * i + 2], dq[t][4 * i + 3]} * a.scale;
                 }
         }
     }

@@ -23,3 +23,43 @@ def test_outputs_do_not_depend_on_gradients(monkeypatch, few, dt, b, t, n, h, kv
     chosen = A.select_blocks(q.cuda(), A.block_bounds(k.cuda(), seen), blocks)
     out = check(q, k, v, do, chosen.cpu(), mask, dt)              # the bound without any part's rounding
     assert torch.equal(A.block_sparse_attention(q.cuda(), k.cuda(), v.cuda(), chosen, seen), out)
+
+
+@pytest.mark.parametrize("few", [0, 1 << 30])
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+@pytest.mark.parametrize("what", ["value", "key"])
+def test_a_huge_key_or_value_takes_nothing_from_its_block(monkeypatch, few, d, what):
+    """One key of every block that no query gives weight to (score -40 sqrt(d) to -60, or far below) has a value of 1e10, or is itself 1e9 long: the others count in full precision.
+    The bounds are relative to sum p |v| and to the scores that have weight, whatever else the block holds."""
+    from airv2x_perception_amd.opencood_iface import token_attention as A
+    monkeypatch.setattr(A, "FEW_MENTIONS", few)
+    q, k, v, do, _ = make(91 + d, 1, 60, 300, 4, 2, d, F32)
+    q[..., 0] = 8.0
+    k[..., 0] = 0.0
+    k[:, 5::64] = 0.0
+    k[:, 5::64, :, 0] = -1e9 if what == "key" else -8.0 * d ** 0.5
+    if what == "value":
+        v[:, 5::64] *= 1e10
+    blocks = A.select_blocks(q.cuda(), A.block_bounds(k.cuda()), 3)
+    check(q, k, v, do, blocks.cpu(), None, F32)
+
+
+@pytest.mark.parametrize("few", [0, 1 << 30])
+def test_infinities_in_fp32(monkeypatch, few):
+    """As the formula has them: a key of -inf in a channel where the query is positive has no weight; a value of inf with weight gives inf, in its channel alone."""
+    from airv2x_perception_amd.opencood_iface import token_attention as A
+    monkeypatch.setattr(A, "FEW_MENTIONS", few)
+    q, k, v, _, _ = [x.cuda() if x is not None else None for x in make(97, 1, 50, 300, 4, 2, 32, F32)]
+    q[..., 0] = q[..., 0].abs() + 0.1
+    blocks = A.select_blocks(q, A.block_bounds(k), 3)
+    seen = torch.ones(1, 300, dtype=torch.bool, device="cuda")
+    seen[:, 7::64] = False
+    want = A.block_sparse_attention(q, k, v, blocks, seen)
+    k2 = k.clone()
+    k2[:, 7::64, :, 0] = -float("inf")
+    assert torch.equal(A.block_sparse_attention(q, k2, v, blocks), want)
+    v2 = v.clone()
+    v2[:, 9::64, :, 3] = float("inf")
+    out, plain = A.block_sparse_attention(q, k, v2, blocks), A.block_sparse_attention(q, k, v, blocks)
+    rest = torch.arange(32) != 3
+    assert (out[..., 3] == float("inf")).all() and torch.equal(out[..., rest], plain[..., rest])
