@@ -125,3 +125,23 @@ def test_small_layers(act8, b, t, heads, dh):
             assert rel(a, r) <= (0.02 if act8 else 2e-5), (n, rel(a, r))
         else:
             assert float(a.abs().max()) <= 1e-4
+
+
+@pytest.mark.parametrize("act8", [False, True])
+def test_inference_mode(monkeypatch, act8):
+    from airv2x_perception_amd.opencood_iface import act8_ops as A8
+    from tests.test_gpu_token_layer import layer
+    monkeypatch.setattr(A8, "SMALL_PRODUCT", 0)
+    m = layer(14, 256, 4, 2, 32, 2)
+    m.act8 = act8
+    x = torch.randn(2, 70, 256, generator=torch.Generator().manual_seed(14)).cuda()
+    pos = torch.stack([torch.arange(70) // 9, torch.arange(70) % 9], 1).int().cuda()
+    want = m(x, pos).detach()
+    for _ in range(2):
+        with torch.inference_mode():
+            got = m(x, pos)
+            clone = m(x.clone(), pos)
+        assert torch.equal(got, want) and torch.equal(clone, want)
+        with torch.no_grad():
+            m.to_qkv.weight.mul_(1.5)                          # a packing of the old values is not taken
+        want = m(x, pos).detach()
