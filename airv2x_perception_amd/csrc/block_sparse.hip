@@ -347,10 +347,12 @@ __global__ __launch_bounds__(256) void bs_select_kernel(const T* __restrict__ q,
 // the lanes' own maxima, which at least n scores reach -- and only their scores are computed again, exactly, one a lane.  What is above goes to a list of
 // pending entries; sixteen at a time count how many of the kept and of each other are better, which is their place.  Loops, not unrolled
 // code: an unrolled form of this filled the instruction cache (10 000 instructions) and ran at 1490 us.  281600 queries x 2200 blocks of 32 channels, bf16, n = 8:
-// 513 us, 1.2e12 scores a second.  Without the picking it takes two thirds of that, half of which is the bounds' way from L2 (2.5 GB, once for every 32 queries: 8 TB/s);
-// the matrix products are 33 us.  64 queries a workgroup halve those bytes but leave one workgroup a CU, whose scores and picks no longer overlap (568 us against 479
-// under the same clock); the next tiles fetched ahead gained nothing.  n = 1 / 8 / 16: 408 / 478 / 584 us where the kernel above takes 1075 / 1650 / 1812; 35200 queries of 2 x 64 channels x 550 blocks: 78 / 96 / 125 and
-// 178 / 266 / 269; one query x 2200 blocks: 11 / 13 / 21 and 28 / 28 / 28.
+// 520 us, 1.2e12 scores a second.  Counters: vector instructions issue in 57 % of the cycles, the matrix cores are busy in 7 %, and a wave waits two thirds of its time
+// (LDS, L2, barriers; four waves a SIMD, 8 % of the cycles lost to bank conflicts of the picking).  L2 serves 31 million requests of at most 128 bytes (the bounds,
+// once for every 32 queries, and the picking's), 120 us at the 34 TB/s that this path reaches: vector issue and the waits between short phases bound it, not L2.
+// Without the picking it takes two thirds; the matrix products are 33 us.  64 queries a workgroup halve those bytes but leave one workgroup a CU, whose scores and
+// picks no longer overlap (568 us against 479 under the same clock); the next tiles fetched ahead gained nothing.  n = 1 / 8 / 16: 408 / 478 / 584 us where the kernel
+// above takes 1075 / 1650 / 1812; 35200 queries of 2 x 64 channels x 550 blocks: 78 / 96 / 125 and 178 / 266 / 269; one query x 2200 blocks: 11 / 13 / 21 and 28 / 28 / 28.
 template <int R> __device__ __forceinline__ unsigned row_ror(unsigned x) {
     return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + R, 0xf, 0xf, false);
 }
@@ -1046,9 +1048,9 @@ __device__ __forceinline__ Row row_of(const BsArgs& a, const int32_t* list, int 
 }
 
 // Rows (mentions x heads of the group) of a work item: 1024, which reads K and V once for all queries of a block of average fame, down to 512 where that leaves fewer
-// than 1024 items.  Measured (us, forward / with backward, items of 512 | 1024 | 2048): 35200 x 35200, 8 heads of 32, 8 blocks, fp32: 328 / 1020 | 333 / 1008 | 355 / 1067;
-// 4400 x 8789, 4 of 64, bf16: 54 / 158 | 62 / 180 | 69 / 201; 600 x 35189, 8 of 64 over 2, 16 blocks: 50 / 136 | 58 / 160 | 73 / 212; 256 or 128 there cost
-// the backward more slabs than they bring (4400: 164, 189).
+// than 1024 items.  Measured (us, forward / with backward, items of 512 | 1024 | 2048): 35200 x 35200, 8 heads of 32, 8 blocks, fp32: 369 / 1230 | 379 / 1249 | 403 / 1319
+// (512 gains 2 % there, at twice the slabs in the workspace); 4400 x 8789, 4 of 64, bf16: 53 / 152 | 61 / 167 | 77 / 210; 600 x 35189, 8 of 64 over 2, 16 blocks:
+// 49 / 136 | 56 / 155 | 69 / 180; 256 or 128 there cost the backward more slabs than they bring (4400: 164, 189 where 512 took 158).
 constexpr int kItemRows = 1024, kItemLeast = 512;
 
 // ------------------------------------------------------------------------------------------------------------ attention, many queries
@@ -1064,9 +1066,10 @@ template <int D> struct Record {
     static __device__ __forceinline__ f32x4 get(const char* r, int d) { return *reinterpret_cast<const v4*>(r + 8 + d * 4); }
 };
 
-// 281600 queries x 8 blocks of 32 channels: bf16 197 us, fp32 285 us.  The products take 25 and 120 us at the matrix cores' measured rates, the records 62 us at HBM's,
-// and neither overlaps well with the vector steps of a score (scaling, maximum, exponential, sum, two terms): a wave goes through them one after the other, and
-// three or four waves a SIMD hide only part of that.  The launch bounds keep one more wave on a SIMD than the compiler would (heads of 128 bf16: 103 us against 115).
+// 281600 queries x 8 blocks of 32 channels: bf16 197 us, fp32 285 us.  fp32: the matrix cores are busy in 52 % of the cycles (120 us of products at their measured rate),
+// vector instructions issue in 21 %.  bf16: 7 % and 41 %, and a wave waits 60 % of its time, mostly for memory: the records go to places all over the workspace, 306 MB
+// (62 us at the rate of a large copy) as pieces of two or three cache lines each.  The launch bounds keep one more wave on a SIMD than the compiler would (whole call,
+// 17600 queries x 4 heads of 64 fp32: 207 us against 246, 8800 x 4 of 128 bf16: 105 against 116).
 template <typename T, int D>
 __global__ __launch_bounds__(256, (is_f32<T>::value ? (D <= 32 ? 3 : D == 64 ? 2 : 1) : (D <= 32 ? 4 : D == 64 ? 3 : 2))) void bs_forward_kernel(BsArgs a) {
     using S = Shape<T, D>;
@@ -1279,8 +1282,9 @@ __global__ __launch_bounds__(256) void bs_delta_kernel(const T* __restrict__ out
 // One workgroup per work item, four waves of 32 rows.  P and dP are computed twice, as keys x queries for dQ (a lane keeps a query) and as queries x
 // keys for dK, dV (a lane keeps a key): two more products instead of a transpose through LDS.  DA: the part of d whose dK, dV, dQ this workgroup
 // keeps (blockIdx.z-th).
-// 281600 queries x 8 blocks of 32 channels, fp32: 814 us; 17600 x 8 of 64, bf16: 76 us.  Seven products: 64.6 GFLOP in fp32, 420 us at the matrix cores' measured rate;
-// two waves a SIMD (205 registers of 256) leave a good part of the two exponentials a score and of the LDS reads uncovered.
+// 281600 queries x 8 blocks of 32 channels, fp32: 814 us; seven products, 64.6 GFLOP, 420 us at the matrix cores' measured rate: they are busy in 62 % of the cycles, vector
+// instructions issue in 14 %, at two waves a SIMD (205 registers of 256).  17600 x 8 of 64, bf16: 76 us; one wave a SIMD (registers and LDS), which waits for loads and
+// LDS half of its time: matrix cores 8 %, vector issue 22 %.
 template <typename T, int D, int DA>
 __global__ __launch_bounds__(256, (D <= 32 ? 2 : 1)) void bs_backward_kernel(BsArgs a) {
     using S = Shape<T, D>;

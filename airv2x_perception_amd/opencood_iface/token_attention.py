@@ -37,9 +37,10 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 # Few queries: one wave takes each (query, head group, block) mention and reads its block directly.  Many: the mentions are sorted by block and a block is read once
 # for all its queries, which costs four launches and more work items the more blocks there are.  The waves' time goes with heads x channels, so up to this many
 # mentions x heads of a group x max(D, 64) / 64, more by one part in 1536 for every block, the waves are taken.  Measured (us, waves / sorted):
-#   8 heads of 32, bf16          8800 keys: 8192 mentions 19 / 24, 16384: 28 / 25     140800 keys: 16384: 38 / 54, 32768: 64 / 59
-#   8 heads of 64 over 2, bf16   8800 keys: 1024 mentions 23 / 27, 4096: 36 / 34      140800 keys: 4096: 39 / 48, 8192: 64 / 58
-#   4 heads of 128, fp32         8800 keys: 4096 mentions 42 / 43, 8192: 66 / 47      140800 keys: 8192: 77 / 146, 32768: 277 / 251
+#   8 heads of 32, bf16          8800 keys: 8192 mentions 19 / 24, 16384: 28 / 25     140800 keys: 16384: 38 / 48, 32768: 65 / 53
+#   8 heads of 32, fp32          8800 keys: 8192 mentions 24 / 30, 16384: 35 / 33     140800 keys: 16384: 40 / 67, 32768: 68 / 79
+#   8 heads of 64 over 2, bf16   8800 keys: 1024 mentions 23 / 26, 4096: 36 / 34      140800 keys: 4096: 39 / 42, 8192: 64 / 47
+#   4 heads of 128, fp32         8800 keys: 4096 mentions 43 / 47, 8192: 67 / 58      140800 keys: 8192: 76 / 161, 32768: 272 / 257
 FEW_MENTIONS = 12288
 
 
@@ -63,13 +64,13 @@ def _check_token(what, x, dim_axes, name):
 
 def _steps(x):
     """Strides of the axes before the channels; an axis of one element takes no steps, whatever its stride says."""
-    return [s if n > 1 else 0 for s, n in zip(x.stride()[:-1], x.shape[:-1])]
+    steps, shape = x.stride()[:-1], x.shape
+    return steps if 1 not in shape else [s if n > 1 else 0 for s, n in zip(steps, shape)]
 
 
 def _strided(x, elems):
     """x itself where the kernels can read it in pieces of ``elems`` elements, else a contiguous copy."""
-    ok = x.stride(-1) == 1 and x.data_ptr() % (elems * x.element_size()) == 0 and all(s % elems == 0 for s in _steps(x))
-    if ok:
+    if x.stride(-1) == 1 and x.data_ptr() % (elems * x.element_size()) == 0 and all(s % elems == 0 for s in _steps(x)):
         return x
     x = x.contiguous()
     return x if x.data_ptr() % 16 == 0 else x.clone()
