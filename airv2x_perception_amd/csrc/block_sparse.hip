@@ -347,7 +347,7 @@ __global__ __launch_bounds__(256) void bs_select_kernel(const T* __restrict__ q,
 // the lanes' own maxima, which at least n scores reach -- and only their scores are computed again, exactly, one a lane.  What is above goes to a list of
 // pending entries; sixteen at a time count how many of the kept and of each other are better, which is their place.  Loops, not unrolled
 // code: an unrolled form of this filled the instruction cache (10 000 instructions) and ran at 1490 us.  281600 queries x 2200 blocks of 32 channels, bf16, n = 8:
-// 520 us, 1.2e12 scores a second.  Counters: vector instructions issue in 57 % of the cycles, the matrix cores are busy in 7 %, and a wave waits two thirds of its time
+// 520 us, 1.2e12 scores a second.  Counters: vector instructions issue in 60 % of the cycles, the matrix cores are busy in 7 %, and a wave waits two thirds of its time
 // (LDS, L2, barriers; four waves a SIMD, 8 % of the cycles lost to bank conflicts of the picking).  L2 serves 31 million requests of at most 128 bytes (the bounds,
 // once for every 32 queries, and the picking's), 120 us at the 34 TB/s that this path reaches: vector issue and the waits between short phases bound it, not L2.
 // Without the picking it takes two thirds; the matrix products are 33 us.  64 queries a workgroup halve those bytes but leave one workgroup a CU, whose scores and

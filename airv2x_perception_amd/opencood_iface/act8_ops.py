@@ -14,7 +14,8 @@ derivative taken at x8 instead of x:
                   dx = rstd (a - mean(a) - u mean(a u))  dgamma = sum (dY W) u = sum_o W (dY^T u)    dbeta = sum dY W = sum_o W db
     gelu(_linear) dW = dY^T gelu(z8)                     dz = (dY W) gelu'(z8)
 
-A group with an infinity or a NaN has a NaN scale: the gradients show it, as they would without the 8 bits (GradScaler's check works).
+A group with an infinity or a NaN has a NaN scale: the gradients show it, as they would without the 8 bits (GradScaler's check works).  In the products an infinity, split
+into three terms, gives NaN.
 A step can be captured into a HIP graph, while no eager graph of the same leaves is alive (torch's engine would wait for the stream of a leaf's old node); its weights are
 packed on every replay, and in every later eager call (train_ops.forget_packings: for weights that a replay changes without running their layers).
 ``model.act8 = True`` trains Airv2xCoBEVT / Airv2xV2XVit's fusion with these nodes (train_ops.act8_scope).

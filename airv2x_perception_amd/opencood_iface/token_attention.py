@@ -390,7 +390,8 @@ class _BlockSparseAttention(torch.autograd.Function):
 def block_sparse_attention(q, k, v, blocks, mask=None, scale=None):
     """softmax(scale q k^T) v of every query over the visible keys of its blocks: q (B, T, H, D), k, v (B, N, KV, D), blocks int32 (B, T, KV, n) (select_blocks, or any
     choice: indices outside 0 .. ceil(N / 64) - 1 are none, a block named twice counts twice), mask (B, N) bool of visible keys.  A query without a
-    visible key gets zeros, and what stands in masked places is never read.  scale: 1 / sqrt(D).  Differentiable in q, k, v, bit for bit the same every time."""
+    visible key gets zeros, and what stands in masked places is never read.  scale: 1 / sqrt(D).  Differentiable in q, k, v, bit for bit the same every time, with and
+    without gradients.  A visible infinity or NaN gives outputs that are not finite (fp32: those of the formula; 16 bits: NaN, where the formula may have an infinity)."""
     what = "block_sparse_attention"
     for x, name in ((q, "q"), (k, "k"), (v, "v")):
         _check_token(what, x, 4, name)
@@ -416,8 +417,8 @@ def block_sparse_attention(q, k, v, blocks, mask=None, scale=None):
 # ------------------------------------------------------------------------------------------------ the layer
 class BlockSparseAttention(nn.Module):
     """x + to_out(attention(LayerNorm(x))) over all tokens of a sample: x (B, T, dim) fp32, positions int32 (T, axes) or (B, T, axes), mask (B, T) bool of
-    visible tokens -> (B, T, dim).  A global counterpart of the fusions' PreNorm windowed attentions.  Under ``torch.autocast`` (or ``amp = True``) the attention runs in bf16;
-    ``act8 = True`` keeps the Linears' inputs in 8 bits for the backward."""
+    visible tokens -> (B, T, dim); dim 256 or 512 (act8: any multiple of 32 up to 1024), parameters fp32.  A global counterpart of the fusions' PreNorm windowed
+    attentions.  Under ``torch.autocast`` (or ``amp = True``) the attention runs in bf16; ``act8 = True`` keeps the Linears' inputs in 8 bits for the backward."""
 
     def __init__(self, dim, heads=8, dim_head=32, blocks=8, kv_heads=None, axes=2, base=10000.0, eps=1e-6):
         super().__init__()

@@ -1016,7 +1016,8 @@ int av2x_act8_gemm(const float* a, const float* w, const float* bias, const floa
  * av2x_block_lists    the mentions of every block, for the two calls below: av2x_block_lists_bytes bytes of device memory, kept by the caller
  * av2x_block_sparse_attention   out (batch, queries, heads, dim) = softmax(scale q k^T) v over the visible keys of a query's blocks (indices outside
  *                     0 .. NB - 1 are none; one that is named twice counts twice; no key at all: zeros), lse (batch, queries, heads): log-sum-exp to base 2, rest (as out, or
- *                     NULL): out's rounding errors; both for the backward, lse NULL: no backward, 16-bit results of the blocks.  lists NULL: one wave per mention (few queries; at most 2^25 mentions).  strides: HOST {q, k, v} x {batch, token, head}; 16-byte rows.
+ *                     NULL): out's rounding errors; both for the backward, which does not change out.  lists NULL: one wave per mention (few queries; at most 2^25 mentions).
+ *                     strides: HOST {q, k, v} x {batch, token, head}; 16-byte rows.
  * av2x_block_sparse_attention_backward   dq (as out), dk, dv (as k, v but contiguous; NULL: not wanted).  Bit-reproducible.
  * workspace: av2x_block_sparse_workspace_bytes.
  * ------------------------------------------------------------------------------------ */
