@@ -134,7 +134,8 @@ def _may_keep(own):
 
 def forget_packings():
     """Drops all kept packings.  To be called where weights changed in a way that moves neither their version counter nor their storage: after replays of a
-    graph that updates them but does not run their layers (a recorded optimizer step beside eager forward and backward passes)."""
+    graph that updates them but does not run their layers (a recorded optimizer step beside eager forward and backward passes).
+    torch.autograd.graph.increment_version on the weights does as much for them, and for the eval engines."""
     _PACKED.clear()
 
 
