@@ -14,6 +14,9 @@ derivative taken at x8 instead of x:
                   dx = rstd (a - mean(a) - u mean(a u))  dgamma = sum (dY W) u = sum_o W (dY^T u)    dbeta = sum dY W = sum_o W db
     gelu(_linear) dW = dY^T gelu(z8)                     dz = (dY W) gelu'(z8)
 
+The stored values are off by at most scale / 2, 1/254 of the group's largest |x|; LayerNorm's backward sees that error times rstd, so a row whose mean is large beside its
+spread (|mean| = 10 standard deviations: 4 % of one in u) has noisier gradients than the residual stream's centred rows.
+
 A group with an infinity or a NaN has a NaN scale: the gradients show it, as they would without the 8 bits (GradScaler's check works).  In the products an infinity, split
 into three terms, gives NaN.
 A step can be captured into a HIP graph, while no eager graph of the same leaves is alive (torch's engine would wait for the stream of a leaf's old node); its weights are
